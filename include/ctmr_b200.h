@@ -298,7 +298,102 @@ CTMR_API int ctmr_window_finalize(const float* acc, const float* wsum, float* ou
 CTMR_API int ctmr_rflow_step(const float* z, const float* vel, long long n, float guidance, int guided, float dt,
                              const float* dt_device, float* out, void* stream);
 
-/* Device error word (bit set when a bounded wait gave up); optionally cleared.
+/* ---------------------------------------------------------------------------------------------
+ * Packed tokens: several requests (volumes of different extents) in one call. `offsets` are int32
+ * values in device memory, documents + 1 of them, not falling: document d holds the rows
+ * [offsets[d], offsets[d + 1]) of the packed tensor. The host never reads them; the kernels clamp
+ * them into the tensor, and what a clamp changed sets bit 5 of the device error word
+ * (ctmr_get_device_error). The reference runs one request at a time and has no counterpart. */
+
+/* Rotary positions along several axes. A head's first 2 * (section[0] + .. + section[axes - 1])
+ * channels are rotated in pairs, (2c, 2c + 1) when interleaved, (c, c + pairs) otherwise, the rest
+ * copied. Pair c of axis a: angle = positions[token][a] * inv_freq[c] (the product and its reduction
+ * to a turn in 64 bits), (u, v) -> (u cos - v sin, v cos + u sin); inverse: the opposite angle (the
+ * transpose, which carries gradients back). Any strides; y may be x. */
+#define CTMR_MAX_ROTARY_AXES 8
+typedef struct ctmr_rotary_desc {
+  const void* x;                   /* (tokens, heads, head_dim), channels contiguous */
+  void* y;
+  int dtype;                       /* CTMR_DTYPE_F32, _BF16 or _F16 */
+  long long tokens;
+  int heads, head_dim;
+  long long x_token_stride, x_head_stride, y_token_stride, y_head_stride; /* elements */
+  const void* positions;           /* (tokens, axes), rows positions_stride elements apart */
+  int positions_f32;               /* fp32 positions; int32 otherwise */
+  long long positions_stride;
+  const float* inv_freq;           /* one per pair */
+  int axes;                        /* 1 .. CTMR_MAX_ROTARY_AXES */
+  int section[CTMR_MAX_ROTARY_AXES]; /* pairs of each axis */
+  int interleaved;
+  int inverse;
+} ctmr_rotary_desc;
+CTMR_API int ctmr_rotary_axes(const ctmr_rotary_desc* desc, void* stream);
+
+/* A projection shared by all rows and a low-rank adapter for each segment of rows:
+ *   y_i = weight x_i + bias + scale[a] * up[a] (down[a] x_i),  a = index[segment of row i],
+ * without the adapter's term where a is negative or no segment holds the row. 16-bit operands,
+ * fp32 sums; the adapter's inner product (scaled) is rounded once to the operands' type. */
+typedef struct ctmr_adapter_linear_desc {
+  const void* x;                   /* (rows, in_features), rows x_stride elements apart */
+  long long x_stride;              /* a multiple of 8 */
+  int dtype;                       /* CTMR_DTYPE_BF16 or _F16: x, weight, down, up and y */
+  int rows, in_features, out_features; /* in_features a multiple of 8 */
+  const void* weight;              /* (out_features, in_features), rows weight_stride elements apart */
+  long long weight_stride;
+  const void* bias;                /* (out_features) or NULL */
+  int bias_dtype;                  /* CTMR_DTYPE_F32 or dtype */
+  const void* down;                /* (adapters, rank, in_features), dense */
+  const void* up;                  /* (adapters, out_features, rank), dense */
+  const float* scale;              /* (adapters) */
+  int adapters, rank;              /* rank: a multiple of 8 up to 128 */
+  const int* offsets;              /* (segments + 1) */
+  const int* index;                /* (segments): the segment's adapter; negative: none */
+  int segments;                    /* 0: no adapters (the fields above are not read) */
+  void* y;                         /* (rows, out_features), rows y_stride elements apart; not x */
+  long long y_stride;
+} ctmr_adapter_linear_desc;
+CTMR_API size_t ctmr_adapter_linear_workspace_size(const ctmr_adapter_linear_desc* desc);
+CTMR_API int ctmr_adapter_linear(const ctmr_adapter_linear_desc* desc, void* workspace, size_t workspace_bytes,
+                                 void* stream);
+
+/* out_i = sum_j softmax_j(s_ij) v_j over the keys j that query i sees, in its own document:
+ *   s_ij = cap(scale q_i . k_j) - slopes[head] * |p_i - j|,  p_i = i + Lk - Lq,
+ * i and j counted inside the document of Lq queries and Lk keys, cap(x) = cap * tanh(x / cap) (x when
+ * cap is 0). Not causal: every key of the document is seen. Causal: j <= p_i, or j < prefix[document].
+ * A query that sees nothing gets zeros (and lse -infinity). Query head h reads key head
+ * h / (heads / kv_heads). Sums and softmax statistics are fp32; the softmax weights are rounded to
+ * the operands' type for their product with v.
+ *
+ * Two forms. Packed: q_offsets and k_offsets given, q_tokens and k_tokens the packed totals, document
+ * strides unused. Batched: both NULL, each document has q_tokens queries and k_tokens key rows, of
+ * which the first k_lengths[document] are used (all when NULL). Values of keys outside the used ones
+ * are never part of a result, whatever they are; values of used keys must be finite. */
+typedef struct ctmr_attention_desc {
+  const void *q, *k, *v;           /* [document][token][head][head_dim], channels contiguous */
+  void* out;
+  float* lse;                      /* ([document][token][heads]) natural log of the softmax sum, or NULL */
+  int dtype;                       /* CTMR_DTYPE_BF16 or _F16 */
+  int documents, q_tokens, k_tokens;
+  int heads, kv_heads, head_dim;   /* head_dim: a multiple of 8 up to 128 */
+  /* Element strides, multiples of 8; addresses 16-byte aligned. */
+  long long q_doc_stride, q_token_stride, q_head_stride;
+  long long k_doc_stride, k_token_stride, k_head_stride;
+  long long v_doc_stride, v_token_stride, v_head_stride;
+  long long out_doc_stride, out_token_stride, out_head_stride;
+  const int *q_offsets, *k_offsets; /* (documents + 1) each, or both NULL */
+  const int* k_lengths;            /* (documents), batched form only, or NULL */
+  const int* prefix;               /* (documents), causal only, or NULL */
+  const float* slopes;             /* (heads), or NULL */
+  float scale;                     /* positive */
+  float cap;                       /* 0: none */
+  int causal;
+  int max_q;                       /* packed form: no document has more queries (0: not known) */
+} ctmr_attention_desc;
+CTMR_API size_t ctmr_attention_workspace_size(const ctmr_attention_desc* desc);
+CTMR_API int ctmr_attention(const ctmr_attention_desc* desc, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Device error word (bits 0-4 set when a bounded wait gave up or a launch was inconsistent, bit 5 when
+ * offsets, lengths or adapter numbers in device memory were out of range); optionally cleared.
  * Synchronises the current device. */
 CTMR_API int ctmr_get_device_error(unsigned* bits, int clear);
 

@@ -23,6 +23,7 @@
 #include "pack.cuh"
 #include "prepare.cuh"
 #include "launch.cuh"
+#include "capi_internal.cuh"
 
 namespace ctmr {
 int conv_stage_plan(int kc, int bn, bool exact, bool one_cta_per_sm, size_t* smem_bytes);
@@ -511,6 +512,14 @@ bool plan_v2(const ConvPlan& p, const ctmr_conv3d_desc* d, bool with_stats, V2Pl
 }  // namespace
 
 namespace ctmr {
+int api_fail(int status, const char* fmt, ...) {
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(g_last_error, sizeof(g_last_error), fmt, ap);
+  va_end(ap);
+  return status;
+}
+PFN_cuTensorMapEncodeTiled_v12000 api_tensor_map_encoder() { return tensor_map_encoder(); }
 // Records `message` as this thread's ctmr_last_error() and returns `status`.
 int set_last_error(int status, const char* message) { return fail(status, "%s", message); }
 }  // namespace ctmr

@@ -20,6 +20,7 @@ enum : unsigned {
   kErrWaitAcc = 1u << 2,      // epilogue waited too long for the accumulator
   kErrWaitDrain = 1u << 3,    // teardown drain of in-flight copies timed out
   kErrBadLaunch = 1u << 4,    // kernel saw an inconsistent launch configuration
+  kErrBadOffsets = 1u << 5,   // offsets, lengths or adapter numbers in device memory were out of range
 };
 
 // Two seconds: far above any single tile's lifetime, far below a watchdog.

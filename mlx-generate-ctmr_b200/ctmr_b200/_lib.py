@@ -29,6 +29,7 @@ PRECISION_TF32 = 3
 TRANSFORM_COPY = 0
 TRANSFORM_TRILINEAR = 1
 TRANSFORM_AVGPOOL = 2
+MAX_ROTARY_AXES = 8
 CONV_PREPARE = 1
 CONV_GEMM = 2
 
@@ -57,6 +58,11 @@ EXPORTED_SYMBOLS = (
     "ctmr_window_accumulate",
     "ctmr_window_finalize",
     "ctmr_rflow_step",
+    "ctmr_rotary_axes",
+    "ctmr_adapter_linear_workspace_size",
+    "ctmr_adapter_linear",
+    "ctmr_attention_workspace_size",
+    "ctmr_attention",
     "ctmr_get_device_error",
     "ctmr_status_string",
     "ctmr_last_error",
@@ -133,6 +139,98 @@ class TransformDesc(ctypes.Structure):
     ]
 
 
+class RotaryDesc(ctypes.Structure):
+    """``ctmr_rotary_desc``."""
+
+    _fields_ = [
+        ("x", ctypes.c_void_p),
+        ("y", ctypes.c_void_p),
+        ("dtype", ctypes.c_int),
+        ("tokens", ctypes.c_longlong),
+        ("heads", ctypes.c_int),
+        ("head_dim", ctypes.c_int),
+        ("x_token_stride", ctypes.c_longlong),
+        ("x_head_stride", ctypes.c_longlong),
+        ("y_token_stride", ctypes.c_longlong),
+        ("y_head_stride", ctypes.c_longlong),
+        ("positions", ctypes.c_void_p),
+        ("positions_f32", ctypes.c_int),
+        ("positions_stride", ctypes.c_longlong),
+        ("inv_freq", ctypes.c_void_p),
+        ("axes", ctypes.c_int),
+        ("section", ctypes.c_int * MAX_ROTARY_AXES),
+        ("interleaved", ctypes.c_int),
+        ("inverse", ctypes.c_int),
+    ]
+
+
+class AdapterLinearDesc(ctypes.Structure):
+    """``ctmr_adapter_linear_desc``."""
+
+    _fields_ = [
+        ("x", ctypes.c_void_p),
+        ("x_stride", ctypes.c_longlong),
+        ("dtype", ctypes.c_int),
+        ("rows", ctypes.c_int),
+        ("in_features", ctypes.c_int),
+        ("out_features", ctypes.c_int),
+        ("weight", ctypes.c_void_p),
+        ("weight_stride", ctypes.c_longlong),
+        ("bias", ctypes.c_void_p),
+        ("bias_dtype", ctypes.c_int),
+        ("down", ctypes.c_void_p),
+        ("up", ctypes.c_void_p),
+        ("scale", ctypes.c_void_p),
+        ("adapters", ctypes.c_int),
+        ("rank", ctypes.c_int),
+        ("offsets", ctypes.c_void_p),
+        ("index", ctypes.c_void_p),
+        ("segments", ctypes.c_int),
+        ("y", ctypes.c_void_p),
+        ("y_stride", ctypes.c_longlong),
+    ]
+
+
+class AttentionDesc(ctypes.Structure):
+    """``ctmr_attention_desc``."""
+
+    _fields_ = [
+        ("q", ctypes.c_void_p),
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("out", ctypes.c_void_p),
+        ("lse", ctypes.c_void_p),
+        ("dtype", ctypes.c_int),
+        ("documents", ctypes.c_int),
+        ("q_tokens", ctypes.c_int),
+        ("k_tokens", ctypes.c_int),
+        ("heads", ctypes.c_int),
+        ("kv_heads", ctypes.c_int),
+        ("head_dim", ctypes.c_int),
+        ("q_doc_stride", ctypes.c_longlong),
+        ("q_token_stride", ctypes.c_longlong),
+        ("q_head_stride", ctypes.c_longlong),
+        ("k_doc_stride", ctypes.c_longlong),
+        ("k_token_stride", ctypes.c_longlong),
+        ("k_head_stride", ctypes.c_longlong),
+        ("v_doc_stride", ctypes.c_longlong),
+        ("v_token_stride", ctypes.c_longlong),
+        ("v_head_stride", ctypes.c_longlong),
+        ("out_doc_stride", ctypes.c_longlong),
+        ("out_token_stride", ctypes.c_longlong),
+        ("out_head_stride", ctypes.c_longlong),
+        ("q_offsets", ctypes.c_void_p),
+        ("k_offsets", ctypes.c_void_p),
+        ("k_lengths", ctypes.c_void_p),
+        ("prefix", ctypes.c_void_p),
+        ("slopes", ctypes.c_void_p),
+        ("scale", ctypes.c_float),
+        ("cap", ctypes.c_float),
+        ("causal", ctypes.c_int),
+        ("max_q", ctypes.c_int),
+    ]
+
+
 def _load() -> ctypes.CDLL:
     if not LIB_PATH.exists():
         raise ImportError(
@@ -165,6 +263,11 @@ def _load() -> ctypes.CDLL:
         "ctmr_window_accumulate": (i, [Tensor, i, i, i, i, i, i, i, i, i, i, vp, vp, vp, i, f, vp, vp, vp]),
         "ctmr_window_finalize": (i, [vp, vp, vp, i, i, i, i, i, i, i, i, i, i, i, vp]),
         "ctmr_rflow_step": (i, [vp, vp, ll, f, i, f, vp, vp, vp]),
+        "ctmr_rotary_axes": (i, [ctypes.POINTER(RotaryDesc), vp]),
+        "ctmr_adapter_linear_workspace_size": (sz, [ctypes.POINTER(AdapterLinearDesc)]),
+        "ctmr_adapter_linear": (i, [ctypes.POINTER(AdapterLinearDesc), vp, sz, vp]),
+        "ctmr_attention_workspace_size": (sz, [ctypes.POINTER(AttentionDesc)]),
+        "ctmr_attention": (i, [ctypes.POINTER(AttentionDesc), vp, sz, vp]),
         "ctmr_get_device_error": (i, [ctypes.POINTER(ctypes.c_uint), i]),
         "ctmr_status_string": (ctypes.c_char_p, [i]),
         "ctmr_last_error": (ctypes.c_char_p, []),
@@ -197,7 +300,8 @@ def check(status: int, what: str) -> None:
 
 
 def device_error(clear: bool = False) -> int:
-    """Device error word: non-zero when a bounded device wait gave up. Synchronises."""
+    """Device error word: non-zero when a bounded device wait gave up or offsets, lengths or adapter numbers
+    in device memory were out of range. Synchronises."""
     bits = ctypes.c_uint(0)
     check(LIB.ctmr_get_device_error(ctypes.byref(bits), int(clear)), "ctmr_get_device_error")
     return int(bits.value)

@@ -514,6 +514,238 @@ def attention_d32(qkv: torch.Tensor, heads: int, scale: float) -> torch.Tensor:
     return out
 
 
+def _int32_vector(t: torch.Tensor, n: int | None, name: str, like: torch.Tensor) -> torch.Tensor:
+    if t.dtype != torch.int32 or t.dim() != 1 or (n is not None and t.shape[0] != n) or t.device != like.device:
+        raise ValueError(f"{name} must be {'' if n is None else f'{n} '}int32 values on {like.device}; got "
+                         f"{tuple(t.shape)} {t.dtype} on {t.device}")
+    return t.contiguous()
+
+
+def _strides(t: torch.Tensor) -> tuple[int, ...]:
+    """Strides with those of extents of one, which address nothing, set to zero."""
+    return tuple(0 if n <= 1 else st for n, st in zip(t.shape, t.stride()))
+
+
+def axis_frequencies(sections: tuple[int, ...], *, theta: float = 10000.0, device="cuda") -> torch.Tensor:
+    """``inv_freq`` for ``rotary_axes``: pair l of an axis with n pairs turns by ``theta ** (-l / n)`` per unit."""
+    freq = [theta ** (-torch.arange(n, dtype=torch.float64) / max(n, 1)) for n in sections]
+    return torch.cat(freq).to(F32).to(device)
+
+
+def rotary_axes(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, sections: tuple[int, ...], *,
+                interleaved: bool = False, inverse: bool = False, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Rotary positions along several axes (``ctmr_rotary_axes``).
+
+    ``x`` is ``(tokens, heads, head_dim)`` in fp32, bf16 or fp16, any strides over tokens and heads (the query
+    and key heads of a fused projection are one such view); ``positions`` is ``(tokens, axes)`` int32 or fp32;
+    ``sections`` gives the number of pairs of each axis and ``inv_freq`` one fp32 frequency per pair
+    (``axis_frequencies``). Pairs are ``(c, c + pairs)``, or ``(2c, 2c + 1)`` when ``interleaved``; channels past
+    them are copied. ``inverse`` turns back (the transpose: a gradient's direction). ``out`` may be ``x``.
+    """
+    if x.dim() != 3 or x.dtype not in (F32, BF16, torch.float16) or not x.is_cuda:
+        raise ValueError(f"x must be a CUDA (tokens, heads, head_dim) fp32/bf16/fp16 tensor; got {tuple(x.shape)} "
+                         f"{x.dtype} on {x.device}")
+    tokens, heads, dim = x.shape
+    axes, pairs = len(sections), sum(sections)
+    if not 1 <= axes <= _lib.MAX_ROTARY_AXES or min(sections) < 0:
+        raise ValueError(f"sections {sections} must name 1 to {_lib.MAX_ROTARY_AXES} axes")
+    if (positions.dim() != 2 or positions.shape != (tokens, axes) or positions.dtype not in (torch.int32, F32)
+            or positions.device != x.device):
+        raise ValueError(f"positions must be ({tokens}, {axes}) int32 or float32 on {x.device}; got "
+                         f"{tuple(positions.shape)} {positions.dtype} on {positions.device}")
+    if inv_freq.dtype != F32 or inv_freq.shape != (pairs,) or inv_freq.device != x.device:
+        raise ValueError(f"inv_freq must be {pairs} float32 values on {x.device}")
+    if axes > 1 and positions.stride(1) != 1:
+        positions = positions.contiguous()
+    if out is None:
+        out = torch.empty((tokens, heads, dim), dtype=x.dtype, device=x.device)
+    elif out.shape != x.shape or out.dtype != x.dtype or out.device != x.device:
+        raise ValueError(f"out must be like x: {tuple(x.shape)} {x.dtype}")
+    xs, ys = _strides(x), _strides(out)
+    if dim > 1 and (xs[2] != 1 or ys[2] != 1):
+        raise ValueError("the channels of x and out must be contiguous")
+    inv_freq = inv_freq.contiguous()
+    desc = _lib.RotaryDesc(
+        x.data_ptr(), out.data_ptr(), _dtype_code(x.dtype, allow_f16=True), tokens, heads, dim, xs[0], xs[1], ys[0],
+        ys[1], positions.data_ptr(), int(positions.dtype == F32), positions.stride(0), inv_freq.data_ptr(), axes,
+        (ctypes.c_int * _lib.MAX_ROTARY_AXES)(*sections), int(interleaved), int(inverse))
+    _count(1)
+    check(LIB.ctmr_rotary_axes(ctypes.byref(desc), _stream()), "rotary_axes")
+    return out
+
+
+def stack_adapters(adapters, *, dtype: torch.dtype, device="cuda") -> dict[str, torch.Tensor]:
+    """The ``down``, ``up`` and ``scale`` of ``adapter_linear`` for ``(down, up, scale)`` triples of any ranks up
+    to 128: ``down`` ``(rank, in)`` and ``up`` ``(out, rank)``, padded with zeros to the largest rank's next
+    multiple of 8. Done once, where the adapters are loaded."""
+    adapters = list(adapters)
+    if not adapters:
+        raise ValueError("no adapters to stack")
+    inner, outer = int(adapters[0][0].shape[1]), int(adapters[0][1].shape[0])
+    for d, u, _ in adapters:
+        if d.dim() != 2 or u.dim() != 2 or d.shape[1] != inner or u.shape[0] != outer or d.shape[0] != u.shape[1]:
+            raise ValueError(f"adapter of shapes {tuple(d.shape)}, {tuple(u.shape)} beside a ({outer}, {inner}) projection")
+    rank = (max(int(d.shape[0]) for d, _, _ in adapters) + 7) // 8 * 8
+    down = torch.zeros((len(adapters), rank, inner), dtype=dtype, device=device)
+    up = torch.zeros((len(adapters), outer, rank), dtype=dtype, device=device)
+    for i, (d, u, _) in enumerate(adapters):
+        down[i, :d.shape[0]] = d.to(device=device, dtype=dtype)
+        up[i, :, :u.shape[1]] = u.to(device=device, dtype=dtype)
+    scale = torch.tensor([float(s) for _, _, s in adapters], dtype=F32, device=device)
+    return {"down": down, "up": up, "scale": scale}
+
+
+def adapter_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, *,
+                   down: torch.Tensor | None = None, up: torch.Tensor | None = None,
+                   scale: torch.Tensor | None = None, offsets: torch.Tensor | None = None,
+                   index: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """A shared projection with each request's low-rank adapter beside it (``ctmr_adapter_linear``).
+
+    ``x`` ``(rows, in)`` holds the requests' rows one after another, request s at
+    ``offsets[s]:offsets[s + 1]`` (int32, on the device); ``index[s]`` is its adapter, negative for none:
+    ``y = x weight^T + bias + scale[a] * (x down[a]^T) up[a]^T``. 16-bit operands (all of one type; ``bias`` may
+    be fp32), fp32 sums. ``down`` ``(n, rank, in)``, ``up`` ``(n, out, rank)`` and ``scale`` ``(n,)`` come from
+    ``stack_adapters``. Without them it is the plain projection. ``out`` must not overlap ``x``.
+    """
+    if x.dim() != 2 or x.dtype not in (BF16, torch.float16) or not x.is_cuda:
+        raise ValueError(f"x must be a CUDA (rows, in) bf16/fp16 tensor; got {tuple(x.shape)} {x.dtype} on {x.device}")
+    rows, inner = x.shape
+    dtype, device = x.dtype, x.device
+    if weight.dim() != 2 or weight.shape[1] != inner or weight.dtype != dtype or weight.device != device:
+        raise ValueError(f"weight must be (out, {inner}) {dtype} on {device}; got {tuple(weight.shape)} {weight.dtype}")
+    outer = weight.shape[0]
+    if bias is not None and (bias.shape != (outer,) or bias.dtype not in (F32, dtype) or bias.device != device):
+        raise ValueError(f"bias must be {outer} float32 or {dtype} values on {device}")
+    if out is None:
+        out = torch.empty((rows, outer), dtype=dtype, device=device)
+    elif out.shape != (rows, outer) or out.dtype != dtype or out.device != device:
+        raise ValueError(f"out must be ({rows}, {outer}) {dtype} on {device}")
+    for name, t in (("x", x), ("weight", weight), ("out", out)):
+        if t.shape[1] > 1 and t.stride(1) != 1:
+            raise ValueError(f"the columns of {name} must be contiguous")
+    desc = _lib.AdapterLinearDesc()
+    desc.x, desc.x_stride = x.data_ptr(), x.stride(0) if rows > 1 else inner
+    desc.dtype = _dtype_code(dtype, allow_f16=True)
+    desc.rows, desc.in_features, desc.out_features = rows, inner, outer
+    desc.weight, desc.weight_stride = weight.data_ptr(), weight.stride(0) if outer > 1 else inner
+    desc.y, desc.y_stride = out.data_ptr(), out.stride(0) if rows > 1 else outer
+    if bias is not None:
+        bias = bias.contiguous()
+        desc.bias, desc.bias_dtype = bias.data_ptr(), _dtype_code(bias.dtype, allow_f16=True)
+    given = [t is not None for t in (down, up, scale, offsets, index)]
+    if any(given):
+        if not all(given):
+            raise ValueError("down, up, scale, offsets and index come together")
+        n, rank = down.shape[0], down.shape[1] if down.dim() == 3 else 0
+        if down.shape != (n, rank, inner) or up.shape != (n, outer, rank) or scale.shape != (n,):
+            raise ValueError(f"adapters must be (n, rank, {inner}), (n, {outer}, rank) and (n,); got "
+                             f"{tuple(down.shape)}, {tuple(up.shape)}, {tuple(scale.shape)}")
+        if down.dtype != dtype or up.dtype != dtype or scale.dtype != F32 or any(
+                t.device != device for t in (down, up, scale)):
+            raise ValueError(f"down and up must be {dtype}, scale float32, all on {device}")
+        down, up, scale = down.contiguous(), up.contiguous(), scale.contiguous()
+        index = _int32_vector(index, None, "index", x)
+        offsets = _int32_vector(offsets, index.shape[0] + 1, "offsets", x)
+        desc.down, desc.up, desc.scale = down.data_ptr(), up.data_ptr(), scale.data_ptr()
+        desc.adapters, desc.rank = n, rank
+        desc.offsets, desc.index, desc.segments = offsets.data_ptr(), index.data_ptr(), index.shape[0]
+    ws_bytes = LIB.ctmr_adapter_linear_workspace_size(ctypes.byref(desc))
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=device) if ws_bytes else None
+    _count(2 if ws_bytes else 1)
+    check(LIB.ctmr_adapter_linear(ctypes.byref(desc), ws.data_ptr() if ws_bytes else None, ws_bytes, _stream()),
+          "adapter_linear")
+    return out
+
+
+def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, q_offsets: torch.Tensor | None = None,
+              k_offsets: torch.Tensor | None = None, k_lengths: torch.Tensor | None = None, max_q: int = 0,
+              scale: float | None = None, causal: bool = False, prefix: torch.Tensor | None = None, cap: float = 0.0,
+              slopes: torch.Tensor | None = None, out: torch.Tensor | None = None, return_lse: bool = False):
+    """Softmax attention inside documents (``ctmr_attention``); 16-bit, head size a multiple of 8 up to 128.
+
+    Packed: ``q`` ``(q_tokens, heads, head_dim)``, ``k`` and ``v`` ``(k_tokens, kv_heads, head_dim)``; document d is
+    rows ``q_offsets[d]:q_offsets[d + 1]`` and ``k_offsets[d]:k_offsets[d + 1]`` (int32 on the device; ``k_offsets``
+    defaults to ``q_offsets``, no offsets at all to one document). ``max_q``, where known, says that no document has
+    more queries. Batched: ``(batch, tokens, heads, head_dim)``, of each item's keys the first ``k_lengths[b]``.
+
+    ``causal``: query i of Lq sees keys up to i + Lk - Lq, and those before ``prefix[d]``; otherwise all of its
+    document. ``cap`` > 0 caps the scaled scores with a tanh; ``slopes`` ``(heads,)`` then subtracts
+    ``slopes[h] * |i + Lk - Lq - j|``. A query that sees no key gives zeros (log-sum-exp -inf). ``heads`` may be a
+    multiple of ``kv_heads``. Any strides that are multiples of 8. Returns ``out``, or ``(out, lse)`` with the
+    fp32 natural log-sum-exp ``(.., tokens, heads)``.
+    """
+    if q.dim() not in (3, 4) or k.dim() != q.dim() or q.dtype not in (BF16, torch.float16) or not q.is_cuda:
+        raise ValueError(f"q must be a CUDA (tokens, heads, head_dim) or (batch, tokens, heads, head_dim) bf16/fp16 "
+                         f"tensor and k alike; got {tuple(q.shape)} {q.dtype} on {q.device}, {tuple(k.shape)}")
+    dtype, device = q.dtype, q.device
+    heads, dim = q.shape[-2:]
+    kv_heads = k.shape[-2]
+    if k.shape != v.shape or k.shape[-1] != dim or k.shape[:-3] != q.shape[:-3] or kv_heads < 1 or heads % kv_heads:
+        raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not belong together")
+    if k.dtype != dtype or v.dtype != dtype or k.device != device or v.device != device:
+        raise ValueError(f"k and v must be {dtype} on {device}")
+    if out is None:
+        out = torch.empty(q.shape, dtype=dtype, device=device)
+    elif out.shape != q.shape or out.dtype != dtype or out.device != device:
+        raise ValueError(f"out must be {tuple(q.shape)} {dtype} on {device}")
+    desc = _lib.AttentionDesc()
+    if q.dim() == 4:
+        if q_offsets is not None or k_offsets is not None:
+            raise ValueError("offsets belong to packed (tokens, heads, head_dim) tensors")
+        documents = q.shape[0]
+        if k_lengths is not None:
+            k_lengths = _int32_vector(k_lengths, documents, "k_lengths", q)
+            desc.k_lengths = k_lengths.data_ptr()
+    else:
+        if k_lengths is not None:
+            raise ValueError("k_lengths belong to batched (batch, tokens, heads, head_dim) tensors")
+        documents = 1
+        if q_offsets is not None:
+            q_offsets = _int32_vector(q_offsets, None, "q_offsets", q)
+            documents = q_offsets.shape[0] - 1
+            if k_offsets is None and k.shape[0] != q.shape[0]:
+                raise ValueError("k_offsets are needed where k has other tokens than q")
+            k_offsets = q_offsets if k_offsets is None else _int32_vector(k_offsets, documents + 1, "k_offsets", q)
+            desc.q_offsets, desc.k_offsets = q_offsets.data_ptr(), k_offsets.data_ptr()
+        elif k_offsets is not None:
+            raise ValueError("q_offsets and k_offsets come together")
+    if documents == 0:
+        if q.shape[-3] and q.dim() == 3:
+            raise ValueError("offsets name no documents")
+        lse = torch.empty(q.shape[:-1], dtype=F32, device=device)
+        return (out, lse) if return_lse else out
+    if prefix is not None:
+        prefix = _int32_vector(prefix, documents, "prefix", q)
+        desc.prefix = prefix.data_ptr()
+    if slopes is not None:
+        if slopes.dtype != F32 or slopes.shape != (heads,) or slopes.device != device:
+            raise ValueError(f"slopes must be {heads} float32 values on {device}")
+        slopes = slopes.contiguous()
+        desc.slopes = slopes.data_ptr()
+    lse = torch.empty(q.shape[:-1], dtype=F32, device=device) if return_lse else None
+    desc.q, desc.k, desc.v, desc.out = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
+    desc.lse = lse.data_ptr() if return_lse else None
+    desc.dtype = _lib.DTYPE_BF16 if dtype == BF16 else _lib.DTYPE_F16
+    desc.documents, desc.q_tokens, desc.k_tokens = documents, q.shape[-3], k.shape[-3]
+    desc.heads, desc.kv_heads, desc.head_dim = heads, kv_heads, dim
+    for name, t in (("q", q), ("k", k), ("v", v), ("out", out)):
+        st = _strides(t)
+        if st[-1] != 1:
+            raise ValueError(f"the channels of {name} must be contiguous")
+        if len(st) == 4:
+            setattr(desc, name + "_doc_stride", st[0])
+        setattr(desc, name + "_token_stride", st[-3])
+        setattr(desc, name + "_head_stride", st[-2])
+    desc.scale = float(dim) ** -0.5 if scale is None else float(scale)
+    desc.cap, desc.causal, desc.max_q = float(cap), int(causal), int(max_q)
+    ws_bytes = LIB.ctmr_attention_workspace_size(ctypes.byref(desc))
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=device) if ws_bytes else None
+    _count(2 if ws_bytes else 1)
+    check(LIB.ctmr_attention(ctypes.byref(desc), ws.data_ptr() if ws_bytes else None, ws_bytes, _stream()),
+          "attention")
+    return (out, lse) if return_lse else out
+
+
 def transform(
     x: torch.Tensor,
     *,
