@@ -1,89 +1,520 @@
 // Attention over packed documents: softmax over the keys of a query's own document, with causal and
 // prefix masks, capped scores and a bias that falls with distance, grouped heads.
 //   s_ij = cap(scale q_i . k_j) - slope_h |p_i - j|,  p_i = i + Lk - Lq,  cap(x) = c tanh(x / c)
-// First form: one warp per query and head, the online softmax over its keys one by one.
+// Every mask leaves a query the keys [0, lim_i): lim_i = Lk, or min(Lk, max(p_i + 1, prefix)) when causal.
+//
+// One CTA takes 256 queries of a document and head, as two tiles of 128 with a softmax warpgroup each
+// (one query per thread). Keys come in tiles of 128: S = Q K^T (128 x 128 fp32) lands in TMEM, a
+// thread reads its whole row into registers, turns it into base-2 scores, takes the maximum and writes
+// P = 2^(s - m) as 16-bit pairs over S's own columns, and the tensor core reads P from TMEM for
+// O += P V (V is MN-major in shared memory, as loaded). One thread issues
+//   S0 S1 | PV0(j) S0(j + 1) PV1(j) S1(j + 1) | ...
+// so that a tile's products run under the other tile's softmax. O stays in TMEM; it is rescaled (by
+// the softmax threads, which hold m) only where a row's maximum has grown by more than 2^8 since the
+// last time: until then P may exceed one, up to 2^8, which neither 16-bit type minds, and the sum
+// of P is kept in fp32 with the same m.
+#include <cmath>
+
+#include "capi_internal.cuh"
+#include "ctmr_b200.h"
 #include "launch.cuh"
 #include "tokens.cuh"
 
 namespace ctmr {
 namespace {
 
-template <typename T>
-__global__ void attention_warp_kernel(const AttentionParams p) {
+constexpr int kThreads = 384;  // warps 0-3 and 4-7: softmax of tiles 0 and 1; 8: TMA; 9: MMA; 10, 11: none
+// A block of 384 threads starts with 168 registers each (64,512 of the SM's); a softmax thread holds a
+// row of 128 scores and takes 216, the last warpgroup gives back to 72: 256 * 216 + 128 * 72 = 64,512.
+constexpr int kSoftmaxRegs = 216, kOtherRegs = 72;
+constexpr int kTile = 128;     // queries per tile, keys per tile
+constexpr int kBlock = 2 * kTile;
+constexpr uint32_t kChunkBytes = kTile * 128;  // 128 rows of 64 16-bit channels
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kRescale = 8.f;  // log2 of the growth that O and the sum are rescaled for
+
+// NC chunks of 64 channels per row; K and V in rings of kStages tiles.
+template <int NC>
+struct Smem {
+  static constexpr int kStages = NC == 1 ? 4 : 2;
+  static constexpr uint32_t kTileBytes = NC * kChunkBytes;
+  static constexpr uint32_t kOffK = 2 * kTileBytes;
+  static constexpr uint32_t kOffV = kOffK + kStages * kTileBytes;
+  static constexpr uint32_t kOffBar = kOffV + kStages * kTileBytes;
+  static constexpr uint32_t kBytes = kOffBar + 256 + 1024;  // + barriers + alignment slack
+};
+
+struct Maps {
+  CUtensorMap q, k, v;
+};
+
+__device__ __forceinline__ float exp2_unit(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ float rcp_unit(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Pairs of fp32 operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, c, d;\n\t"
+      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+      "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, d;\n\t"
+      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "add.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+
+// 2^x of a pair, x <= 8, on the FMA pipe: x = n + f with n the nearest integer (the low bits of x plus
+// 1.5 * 2^23) and |f| <= 1/2, 2^f by a cubic (least maximum relative error on that interval, 7.5e-5,
+// below a quarter of fp16's half-ulp), n added to the exponent. Clamped at 2^-125.
+__device__ __forceinline__ float2 exp2_poly(float2 x) {
+  x.x = fmaxf(x.x, -125.f), x.y = fmaxf(x.y, -125.f);
+  const float2 magic = make_float2(12582912.f, 12582912.f), back = make_float2(-12582912.f, -12582912.f);
+  const float2 j = add2(x, magic), n = add2(j, back);
+  const float2 f = fma2(n, make_float2(-1.f, -1.f), x);
+  float2 p = fma2(make_float2(0.0551716685295105f, 0.0551716685295105f), f,
+                  make_float2(0.2426111251115799f, 0.2426111251115799f));
+  p = fma2(p, f, make_float2(0.6932609677314758f, 0.6932609677314758f));
+  p = fma2(p, f, make_float2(0.9999280571937561f, 0.9999280571937561f));
+  p.x = __int_as_float(__float_as_int(p.x) + (__float_as_int(j.x) << 23));
+  p.y = __int_as_float(__float_as_int(p.y) + (__float_as_int(j.y) << 23));
+  return p;
+}
+
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if constexpr (BF16) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+
+// The document and rows of one CTA.
+struct Place {
+  int doc, q_row, k_row;  // rows of the TMA maps where the document's queries and keys start
+  int map_doc;            // document coordinate of the maps
+  int q_len, k_len, first;  // first: the CTA's first query inside the document
+  int prefix;
+  long long row0;         // the document's first row of lse
+};
+
+// Keys [0, lim) that query i of the document sees.
+__device__ __forceinline__ int limit_of(const AttentionParams& p, const Place& w, int i) {
+  if (!p.causal) return w.k_len;
+  return min(w.k_len, max(max(i + w.k_len - w.q_len + 1, w.prefix), 0));
+}
+
+__device__ __forceinline__ bool find_place(const AttentionParams& p, int id, int lane, Place& w) {
+  int tile;
+  if (p.q_offsets != nullptr) {
+    w.doc = segment_of_tile(p.q_offsets, p.documents, kBlock, id, lane);
+    int qe, ke;
+    segment_range(p.q_offsets, w.doc, p.q_tokens, w.q_row, qe);
+    segment_range(p.k_offsets, w.doc, p.k_tokens, w.k_row, ke);
+    w.q_len = qe - w.q_row, w.k_len = ke - w.k_row;
+    tile = id - (max(p.q_offsets[w.doc], 0) / kBlock + w.doc);
+    w.map_doc = 0;
+    w.row0 = w.q_row;
+  } else {
+    const int per = (p.q_tokens + kBlock - 1) / kBlock;
+    w.doc = id / per, tile = id - w.doc * per;
+    w.q_row = w.k_row = 0, w.map_doc = w.doc, w.q_len = p.q_tokens, w.k_len = p.k_tokens;
+    if (p.k_lengths != nullptr) {
+      const int n = p.k_lengths[w.doc];
+      w.k_len = min(max(n, 0), p.k_tokens);
+      if (n != w.k_len) flag_error(kErrBadOffsets);
+    }
+    w.row0 = static_cast<long long>(w.doc) * p.q_tokens;
+  }
+  if (w.q_len > p.max_q) flag_error(kErrBadOffsets);
+  const int tiles = (w.q_len + kBlock - 1) / kBlock;
+  if (tile < 0 || tile >= tiles) return false;
+  // Later queries see more keys: the longest tiles of a causal document start first.
+  w.first = (p.causal ? tiles - 1 - tile : tile) * kBlock;
+  w.prefix = p.prefix != nullptr ? p.prefix[w.doc] : 0;
+  return true;
+}
+
+template <int NC, bool CAP, bool BIAS, bool BF16>
+__global__ void __launch_bounds__(kThreads, 1)
+    attention_tile_kernel(const __grid_constant__ Maps maps, const AttentionParams p) {
+  using L = Smem<NC>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bar = reinterpret_cast<uint64_t*>(smem + L::kOffBar);
+  uint64_t* q_full = bar;                  // [2]
+  uint64_t* s_full = bar + 2;              // [2] S of a tile (and every earlier product) is done
+  uint64_t* p_full = bar + 4;              // [2] P of a tile is written and S read
+  uint64_t* k_full = bar + 6;              // [kStages]
+  uint64_t* k_empty = k_full + L::kStages;
+  uint64_t* v_full = k_empty + L::kStages;
+  uint64_t* v_empty = v_full + L::kStages;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(v_empty + L::kStages);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int h = blockIdx.y, hk = h / (p.heads / p.kv_heads);
   griddep_wait();
   griddep_launch_dependents();
-  const int lane = threadIdx.x & 31, h = blockIdx.y, hk = h / (p.heads / p.kv_heads);
-  const int row = blockIdx.x * 4 + (threadIdx.x >> 5);
-  int doc, i, q_len, k_len;
-  long long qo, ko, vo, oo, at;
-  if (p.q_offsets != nullptr) {
-    if (row >= p.q_tokens) return;
-    doc = segment_of_row(p.q_offsets, p.documents, row);
-    if (doc < 0) {
-      flag_error(kErrBadOffsets);
-      return;
+  Place w;
+  if (!find_place(p, blockIdx.x, lane, w)) return;  // the same answer in every warp
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&q_full[i], 1);
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], kTile);
     }
-    int qb, qe, kb, ke;
-    segment_range(p.q_offsets, doc, p.q_tokens, qb, qe);
-    segment_range(p.k_offsets, doc, p.k_tokens, kb, ke);
-    i = row - qb, q_len = qe - qb, k_len = ke - kb;
-    qo = row * p.q_token, oo = row * p.o_token, ko = kb * p.k_token, vo = kb * p.v_token, at = row;
+    for (int i = 0; i < L::kStages; ++i) {
+      mbar_init(&k_full[i], 1);
+      mbar_init(&k_empty[i], 1);
+      mbar_init(&v_full[i], 1);
+      mbar_init(&v_empty[i], 1);
+    }
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 9) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;  // S0 S1 at columns 0, 128 (P over them), O0 O1 at 256, 384
+
+  // Key tiles of each query tile: those that its last query sees.
+  int n[2];
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    const int last = min(w.q_len - 1, w.first + (t + 1) * kTile - 1);
+    n[t] = last < w.first + t * kTile ? 0 : (limit_of(p, w, last) + kTile - 1) / kTile;
+  }
+  const int n_max = max(n[0], n[1]);
+
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+    if (warp == 8) {
+    // ------------------------------------------------------------ TMA producer
+    if (lane == 0 && n_max > 0) {
+      tma_prefetch_desc(&maps.q);
+      tma_prefetch_desc(&maps.k);
+      tma_prefetch_desc(&maps.v);
+      auto load = [&](const CUtensorMap* map, uint32_t off, uint64_t* full, int head, int row) {
+        mbar_arrive_expect_tx(full, L::kTileBytes);
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+          tma_load_4d(smem + off + c * kChunkBytes, map, full, c * 64, head, row, w.map_doc);
+      };
+      int j = 0;
+      for (int t = 0; t < 2; ++t)
+        if (n[t] > 0) load(&maps.q, t * L::kTileBytes, &q_full[t], h, w.q_row + w.first + t * kTile);
+      for (; j < n_max && !*abort_flag; ++j) {
+        const int s = j % L::kStages, use = j / L::kStages;
+        const uint32_t freed = static_cast<uint32_t>(use - 1) & 1u;
+        if (use > 0 && !mbar_wait_bounded(&k_empty[s], freed, kErrWaitEmpty)) break;
+        load(&maps.k, L::kOffK + s * L::kTileBytes, &k_full[s], hk, w.k_row + j * kTile);
+        if (use > 0 && !mbar_wait_bounded(&v_empty[s], freed, kErrWaitEmpty)) {
+          mbar_wait_bounded(&k_full[s], static_cast<uint32_t>(use) & 1u, kErrWaitDrain);
+          break;
+        }
+        load(&maps.v, L::kOffV + s * L::kTileBytes, &v_full[s], hk, w.k_row + j * kTile);
+      }
+      if (j < n_max) *abort_flag = 1;
+      // Drain: every issued load lands before the CTA can exit.
+      for (int t = 0; t < 2; ++t)
+        if (n[t] > 0) mbar_wait_bounded(&q_full[t], 0, kErrWaitDrain);
+      for (int i = max(0, j - L::kStages); i < j; ++i) {
+        const uint32_t phase = static_cast<uint32_t>(i / L::kStages) & 1u;
+        mbar_wait_bounded(&k_full[i % L::kStages], phase, kErrWaitDrain);
+        mbar_wait_bounded(&v_full[i % L::kStages], phase, kErrWaitDrain);
+      }
+    }
+    __syncwarp();
+    } else if (warp == 9) {
+    // ------------------------------------------------------------ MMA issuer (lane 0 issues, all wait)
+    const int dk = (p.dim + 15) / 16;
+    const uint32_t id_s = idesc_f16(BF16, kTile, kTile);
+    const uint32_t id_o = idesc_f16(BF16, kTile, static_cast<uint32_t>(dk) * 16u) | (1u << 16);  // V MN-major
+    bool ok = true;
+    auto issue_s = [&](int t, int j) {
+      if (lane == 0) {
+        const uint32_t a = smem_u32(smem + t * L::kTileBytes);
+        const uint32_t b = smem_u32(smem + L::kOffK + (j % L::kStages) * L::kTileBytes);
+        for (int k = 0; k < dk; ++k) {
+          const uint32_t off = static_cast<uint32_t>(k >> 2) * kChunkBytes + static_cast<uint32_t>(k & 3) * 32u;
+          umma_f16(tmem + t * 128, smem_desc_kmajor(a + off, 128), smem_desc_kmajor(b + off, 128), id_s, k > 0 ? 1u : 0u);
+        }
+        umma_commit(&s_full[t]);
+      }
+    };
+    auto wait_k = [&](int j) {
+      return mbar_wait_bounded(&k_full[j % L::kStages], static_cast<uint32_t>(j / L::kStages) & 1u, kErrWaitFull);
+    };
+    if (n_max > 0) ok = wait_k(0);
+    for (int t = 0; ok && t < 2; ++t)
+      if (n[t] > 0) {
+        ok = mbar_wait_bounded(&q_full[t], 0, kErrWaitFull);
+        tc_fence_after();
+        if (ok) issue_s(t, 0);
+      }
+    if (ok && n_max > 0 && lane == 0) umma_commit(&k_empty[0]);
+    for (int j = 0; ok && j < n_max && !*abort_flag; ++j) {
+      const int s = j % L::kStages;
+      uint8_t* vt = smem + L::kOffV + s * L::kTileBytes;
+      ok = mbar_wait_bounded(&v_full[s], static_cast<uint32_t>(j / L::kStages) & 1u, kErrWaitFull);
+      if (ok && j + 1 < n_max) ok = wait_k(j + 1);
+      const int used = w.k_len - j * kTile;  // the document's keys in this tile
+      if (ok && used < kTile) {
+        // Rows past the document hold another's values, whose product with P = 0 must still be 0.
+        for (int i = lane; i < (kTile - used) * 8; i += 32)
+#pragma unroll
+          for (int c = 0; c < NC; ++c)
+            *reinterpret_cast<uint4*>(vt + c * kChunkBytes + used * 128 + i * 16) = make_uint4(0, 0, 0, 0);
+        fence_proxy_async_shared();
+        __syncwarp();
+      }
+      for (int t = 0; ok && t < 2; ++t) {
+        if (j >= n[t]) continue;
+        ok = mbar_wait_bounded(&p_full[t], static_cast<uint32_t>(j) & 1u, kErrWaitFull);
+        if (!ok) break;
+        tc_fence_after();
+        if (lane == 0) {
+          const uint32_t b = smem_u32(vt);
+#pragma unroll
+          for (int k = 0; k < kTile / 16; ++k)
+            umma_f16_ts(tmem + 256 + t * 128, tmem + t * 128 + k * 8, smem_desc_mnmajor(b + k * 2048u, kChunkBytes), id_o,
+                        j > 0 || k > 0 ? 1u : 0u);
+        }
+        if (j + 1 < n[t]) issue_s(t, j + 1);
+        else if (lane == 0) umma_commit(&s_full[t]);  // the last one: O is complete
+      }
+      if (ok && lane == 0) {
+        umma_commit(&v_empty[s]);
+        if (j + 1 < n_max) umma_commit(&k_empty[(j + 1) % L::kStages]);
+      }
+    }
+    if (!ok) *abort_flag = 1;
+    __syncwarp();
+    }
   } else {
-    if (row >= p.q_tokens * p.documents) return;
-    doc = row / p.q_tokens, i = row - doc * p.q_tokens, q_len = p.q_tokens, k_len = p.k_tokens;
-    if (p.k_lengths != nullptr) {
-      const int n = p.k_lengths[doc];
-      if (n < 0 || n > k_len) flag_error(kErrBadOffsets);
-      k_len = min(max(n, 0), k_len);
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+    // ------------------------------------------------------------ softmax, one query per thread
+    const int t = warp >> 2;
+    const int i = w.first + t * kTile + (warp & 3) * 32 + lane;  // the query inside the document
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t t_s = tmem + lanes + t * 128, t_o = tmem + lanes + 256 + t * 128;
+    const int lim = limit_of(p, w, i), place = i + w.k_len - w.q_len;
+    const float scale = p.scale * kLog2e;
+    const float cap_in = CAP ? 2.f * scale / p.cap : 0.f, cap_out = CAP ? p.cap * kLog2e : 0.f;
+    const float slope = BIAS ? p.slopes[h] * kLog2e : 0.f;
+    const float unit = CAP || BIAS ? 1.f : scale;  // what turns s below into base-2 scores
+    float m = -INFINITY, l = 0.f;                  // m: what P is relative to; the maximum or up to 2^8 below
+    bool ok = true;
+    for (int j = 0; j < n[t]; ++j) {
+      ok = mbar_wait_bounded(&s_full[t], static_cast<uint32_t>(j) & 1u, kErrWaitAcc) && !*abort_flag;
+      if (!ok) break;
+      tc_fence_after();
+      float s[kTile];
+#pragma unroll
+      for (int c = 0; c < kTile; c += 32) tmem_ld32(t_s + c, s + c);
+      tmem_ld_wait();
+#pragma unroll
+      for (int c = 0; c < kTile; c += 32) tmem_ld_fence(s + c);
+      if constexpr (CAP) {
+        // c tanh(x / c) = c - 2 c / (e^(2 x / c) + 1): two units' operations, absolute error c 2^-22.
+#pragma unroll
+        for (int c = 0; c < kTile; ++c) s[c] = fmaf(-2.f * cap_out, rcp_unit(exp2_unit(s[c] * cap_in) + 1.f), cap_out);
+      }
+      if constexpr (BIAS) {
+        const float at = static_cast<float>(place - j * kTile);
+#pragma unroll
+        for (int c = 0; c < kTile; ++c)
+          s[c] = fmaf(-slope, fabsf(at - static_cast<float>(c)), CAP ? s[c] : s[c] * scale);
+      }
+      const int left = lim - j * kTile;
+      if (left < kTile) {
+#pragma unroll
+        for (int c = 0; c < kTile; ++c) s[c] = c < left ? s[c] : -INFINITY;
+      }
+      float mx[8];
+#pragma unroll
+      for (int c = 0; c < 8; ++c) mx[c] = s[c];
+#pragma unroll
+      for (int c = 8; c < kTile; ++c) mx[c & 7] = fmaxf(mx[c & 7], s[c]);
+      const float top = unit * fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])),
+                                     fmaxf(fmaxf(mx[4], mx[5]), fmaxf(mx[6], mx[7])));
+      const bool grow = top > m + kRescale || (m == -INFINITY && top > m);
+      if (__any_sync(0xffffffffu, grow)) {
+        const float f = grow ? exp2_unit(m - top) : 1.f;
+        if (grow) m = top;
+        l *= f;
+        if (j > 0) {  // S(j) was issued after PV(j - 1): O is up to date and nothing writes it now
+          for (int c = 0; c < p.dim; c += 32) {
+            float o[32];
+            tmem_ld32(t_o + c, o);
+            tmem_ld_wait();
+            tmem_ld_fence(o);
+            uint32_t r[32];
+#pragma unroll
+            for (int e = 0; e < 32; ++e) r[e] = __float_as_uint(o[e] * f);
+            tmem_st32(t_o + c, r);
+          }
+        }
+      }
+      const float base = m == -INFINITY ? 0.f : -m;
+      const float2 u2 = make_float2(unit, unit), b2 = make_float2(base, base);
+      float2 sum[4] = {};
+#pragma unroll
+      for (int c = 0; c < kTile; c += 64) {
+        uint32_t r[32];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+          float2 x = fma2(make_float2(s[c + 2 * e], s[c + 2 * e + 1]), u2, b2);
+          // One pair in four on the FMA pipe, the others on the exponential unit (16 a clock per SM,
+          // half of the time of a tile's two products at head size 128 and more below it).
+          if ((e & 3) == 3) x = exp2_poly(x);
+          else x = make_float2(exp2_unit(x.x), exp2_unit(x.y));
+          sum[e & 3] = add2(sum[e & 3], x);
+          r[e] = pack2<BF16>(x.x, x.y);
+        }
+        tmem_st32(t_s + c / 2, r);
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive(&p_full[t]);
+      sum[0] = add2(add2(sum[0], sum[1]), add2(sum[2], sum[3]));
+      l += sum[0].x + sum[0].y;
     }
-    qo = doc * p.q_doc + i * p.q_token, oo = doc * p.o_doc + i * p.o_token;
-    ko = doc * p.k_doc, vo = doc * p.v_doc, at = row;
-  }
-  if (q_len > p.max_q) flag_error(kErrBadOffsets);
-  const int place = i + k_len - q_len;
-  const int prefix = p.prefix != nullptr ? p.prefix[doc] : 0;
-  const int seen = p.causal ? min(k_len, max(place + 1, prefix)) : k_len;
-  const float slope = p.slopes != nullptr ? p.slopes[h] : 0.f;
-  const T* q = static_cast<const T*>(p.q) + qo + h * p.q_head;
-  const T* k = static_cast<const T*>(p.k) + ko + hk * p.k_head;
-  const T* v = static_cast<const T*>(p.v) + vo + hk * p.v_head;
-  float qv[4], acc[4] = {}, m = -INFINITY, l = 0.f;
-#pragma unroll
-  for (int c = 0; c < 4; ++c) qv[c] = lane + 32 * c < p.dim ? to_float(q[lane + 32 * c]) : 0.f;
-  for (int j = 0; j < seen; ++j) {
-    float s = 0.f, vv[4];
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      const bool in = lane + 32 * c < p.dim;
-      s = fmaf(qv[c], in ? to_float(k[j * p.k_token + lane + 32 * c]) : 0.f, s);
-      vv[c] = in ? to_float(v[j * p.v_token + lane + 32 * c]) : 0.f;
+    if (ok && n[t] > 0) {
+      ok = mbar_wait_bounded(&s_full[t], static_cast<uint32_t>(n[t]) & 1u, kErrWaitAcc);
+      tc_fence_after();
     }
+    if (!ok) *abort_flag = 1;
+    const bool some = m != -INFINITY;  // a query that saw nothing gets zeros
+    const float inv = some ? 1.f / l : 0.f;
+    uint16_t* out = static_cast<uint16_t*>(p.out) + w.map_doc * p.o_doc + (w.q_row + i) * p.o_token + h * p.o_head;
+    for (int c = 0; c < p.dim; c += 32) {
+      float o[32];
+      if (n[t] > 0) {
+        tmem_ld32(t_o + c, o);
+        tmem_ld_wait();
+        tmem_ld_fence(o);
+      }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    s *= p.scale;
-    if (p.cap > 0.f) s = p.cap * tanhf(s / p.cap);
-    s -= slope * fabsf(static_cast<float>(place - j));
-    const float m_new = fmaxf(m, s), f = __expf(m - m_new), e = __expf(s - m_new);
-    l = l * f + e;
-#pragma unroll
-    for (int c = 0; c < 4; ++c) acc[c] = acc[c] * f + e * vv[c];
-    m = m_new;
+      for (int e = 0; e < 32; e += 8) {
+        if (c + e >= p.dim || i >= w.q_len) break;
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (some)
+          v = make_uint4(pack2<BF16>(o[e] * inv, o[e + 1] * inv), pack2<BF16>(o[e + 2] * inv, o[e + 3] * inv),
+                         pack2<BF16>(o[e + 4] * inv, o[e + 5] * inv), pack2<BF16>(o[e + 6] * inv, o[e + 7] * inv));
+        *reinterpret_cast<uint4*>(out + c + e) = v;
+      }
+    }
+    if (p.lse != nullptr && i < w.q_len)
+      p.lse[(w.row0 + i) * p.heads + h] = some ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY;
   }
-  T* out = static_cast<T*>(p.out) + oo + h * p.o_head;
-#pragma unroll
-  for (int c = 0; c < 4; ++c)
-    if (lane + 32 * c < p.dim) out[lane + 32 * c] = from_float<T>(l > 0.f ? acc[c] / l : 0.f);
-  if (p.lse != nullptr && lane == 0) p.lse[at * p.heads + h] = l > 0.f ? m + logf(l) : -INFINITY;
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// (channel, head, token, document) view of one operand, a box of 64 channels x 128 tokens.
+int encode(CUtensorMap* map, const void* base, bool bf16, int dim, int heads, long long tokens, long long docs,
+           long long s_head, long long s_token, long long s_doc, const char* what) {
+  auto enc = api_tensor_map_encoder();
+  if (enc == nullptr) return api_fail(CTMR_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
+  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(dim), static_cast<cuuint64_t>(heads),
+                              static_cast<cuuint64_t>(tokens), static_cast<cuuint64_t>(docs)};
+  // A stride that addresses nothing (an extent of one) may be anything the encoder takes.
+  const cuuint64_t strides[3] = {static_cast<cuuint64_t>(heads > 1 ? s_head * 2 : 16),
+                                 static_cast<cuuint64_t>(tokens > 1 ? s_token * 2 : 16),
+                                 static_cast<cuuint64_t>(docs > 1 ? s_doc * 2 : 16)};
+  const cuuint32_t box[4] = {64, 1, kTile, 1}, step[4] = {1, 1, 1, 1};
+  const CUresult r = enc(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+                         const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return api_fail(CTMR_ERR_INVALID, "%s's strides cannot be read by TMA (CUresult %d)", what, int(r));
+  return CTMR_OK;
+}
+
+template <int NC, bool CAP, bool BIAS, bool BF16>
+cudaError_t launch_tiles(const Maps& maps, const AttentionParams& p, dim3 grid, cudaStream_t stream) {
+  auto kern = attention_tile_kernel<NC, CAP, BIAS, BF16>;
+  constexpr int bytes = static_cast<int>(Smem<NC>::kBytes);
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != cudaSuccess) return e;
+  return launch_kernel(kern, grid, dim3(kThreads), bytes, stream, maps, p);
+}
+
+template <int NC, bool BF16>
+cudaError_t launch_variant(const Maps& maps, const AttentionParams& p, dim3 grid, cudaStream_t stream) {
+  if (p.cap > 0.f)
+    return p.slopes != nullptr ? launch_tiles<NC, true, true, BF16>(maps, p, grid, stream)
+                               : launch_tiles<NC, true, false, BF16>(maps, p, grid, stream);
+  return p.slopes != nullptr ? launch_tiles<NC, false, true, BF16>(maps, p, grid, stream)
+                             : launch_tiles<NC, false, false, BF16>(maps, p, grid, stream);
 }
 
 }  // namespace
 
+cudaError_t attention_error_word(unsigned* bits, bool clear) {
+  cudaError_t e = cudaMemcpyFromSymbol(bits, g_device_error, sizeof(*bits));
+  const unsigned zero = 0;
+  if (e == cudaSuccess && clear && *bits != 0) e = cudaMemcpyToSymbol(g_device_error, &zero, sizeof(zero));
+  return e;
+}
+
 size_t attention_packed_workspace(const AttentionParams&) { return 0; }
 
-cudaError_t launch_attention_packed(const AttentionParams& p, bool bf16, cudaStream_t stream) {
-  const int rows = p.q_offsets != nullptr ? p.q_tokens : p.q_tokens * p.documents;
-  auto kern = bf16 ? attention_warp_kernel<__nv_bfloat16> : attention_warp_kernel<__half>;
-  return launch_kernel(kern, dim3((rows + 3) / 4, p.heads), dim3(128), 0, stream, p);
+int launch_attention_packed(const AttentionParams& p, bool bf16, cudaStream_t stream) {
+  const bool packed = p.q_offsets != nullptr;
+  const int docs = packed ? 1 : p.documents;
+  Maps maps;
+  int st = encode(&maps.q, p.q, bf16, p.dim, p.heads, p.q_tokens, docs, p.q_head, p.q_token, p.q_doc, "q");
+  if (st != CTMR_OK) return st;
+  maps.k = maps.v = maps.q;  // not read where there are no keys
+  if (p.k_tokens > 0) {
+    st = encode(&maps.k, p.k, bf16, p.dim, p.kv_heads, p.k_tokens, docs, p.k_head, p.k_token, p.k_doc, "k");
+    if (st != CTMR_OK) return st;
+    st = encode(&maps.v, p.v, bf16, p.dim, p.kv_heads, p.k_tokens, docs, p.v_head, p.v_token, p.v_doc, "v");
+    if (st != CTMR_OK) return st;
+  }
+  const long long blocks = packed ? p.q_tokens / kBlock + static_cast<long long>(p.documents)
+                                  : static_cast<long long>(p.documents) * ((p.q_tokens + kBlock - 1) / kBlock);
+  if (blocks > 0x7fffffffLL) return api_fail(CTMR_ERR_UNSUPPORTED, "too many documents");
+  const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(p.heads));
+  cudaError_t e;
+  if (p.dim <= 64)
+    e = bf16 ? launch_variant<1, true>(maps, p, grid, stream) : launch_variant<1, false>(maps, p, grid, stream);
+  else
+    e = bf16 ? launch_variant<2, true>(maps, p, grid, stream) : launch_variant<2, false>(maps, p, grid, stream);
+  return e == cudaSuccess ? CTMR_OK : api_fail(CTMR_ERR_CUDA, "attention launch: %s", cudaGetErrorString(e));
 }
 
 }  // namespace ctmr

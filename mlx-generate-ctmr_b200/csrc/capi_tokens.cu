@@ -182,8 +182,7 @@ int ctmr_attention(const ctmr_attention_desc* d, void* workspace, size_t workspa
   st = check_workspace(ctmr::attention_packed_workspace(p), workspace, workspace_bytes);
   if (st != CTMR_OK) return st;
   p.workspace = workspace;
-  return finish(ctmr::launch_attention_packed(p, d->dtype == CTMR_DTYPE_BF16, static_cast<cudaStream_t>(stream)),
-                "attention launch");
+  return ctmr::launch_attention_packed(p, d->dtype == CTMR_DTYPE_BF16, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

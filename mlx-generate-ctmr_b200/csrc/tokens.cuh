@@ -58,7 +58,10 @@ cudaError_t launch_rotary(const RotaryParams& p, int dtype, cudaStream_t stream)
 size_t adapter_linear_workspace(const LinearParams& p);
 cudaError_t launch_adapter_linear(const LinearParams& p, bool bf16, cudaStream_t stream);
 size_t attention_packed_workspace(const AttentionParams& p);
-cudaError_t launch_attention_packed(const AttentionParams& p, bool bf16, cudaStream_t stream);
+int launch_attention_packed(const AttentionParams& p, bool bf16, cudaStream_t stream);  // a CTMR_ status
+
+// The attention file's own error word (see ptx.cuh), read and optionally cleared.
+cudaError_t attention_error_word(unsigned* bits, bool clear);
 
 // ---------------------------------------------------------------- ragged rows
 // offsets[s] clamped into [0, total] (a negative or excessive offset never indexes memory) and, with
