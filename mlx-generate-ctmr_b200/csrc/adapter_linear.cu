@@ -1,109 +1,767 @@
 // A projection shared by all rows, beside it a low-rank adapter for each segment of rows:
 //   y_i = W x_i + b + scale_a up_a (down_a x_i),  a = index[segment of i], no adapter where a < 0.
-// First form: a plain tiled product on the FMA pipe; the adapters' inner products are computed by a
-// kernel before it.
+//
+// Two launches. adapter_inner_kernel computes t_i = scale_a down_a x_i (fp32 sums, rounded once to the
+// operands' type: it becomes a tensor-core operand, and its rounding is that of y's own adapter part).
+// The product kernel then computes y^T tiles, 128 (or a CTA pair's 256) outputs as TMEM lanes by a
+// tile of rows as columns: D = W x^T over the input in blocks of 64, and for every segment that
+// meets the tile one or two further blocks of K = rank, up_a t^T, into the same accumulator. An
+// adapter thus costs its own bytes and rank / in of the product, and y is rounded and written once.
+//
+// t is stored by blocks: block tile + segment for each pair of a row tile and a segment that meet (both
+// grow along the rows, so the numbers are distinct and at most tiles + segments - 1), `tile` rows each,
+// zeros in the rows of other segments. A block is a TMA box and needs no mask in the product.
+//
+// The product kernel starts (programmatic launch) while the inner products run: it reads x and W at
+// once, whose producers finished before the inner kernel let it start, and waits only for t.
+//
+// Outputs as lanes: a warp stores 32 adjacent outputs of a row, and few rows (serving) use few
+// columns: the tensor core then streams W at the memory's rate.
+#include <atomic>
+
+#include "capi_internal.cuh"
+#include "ctmr_b200.h"
 #include "launch.cuh"
 #include "tokens.cuh"
 
 namespace ctmr {
 namespace {
 
-constexpr int kTile = 64, kStep = 16;
+constexpr int kK = 64;                     // inputs per block: one 128-byte swizzled row
+constexpr uint32_t kABytes = 128 * 128;    // 128 outputs x 64 inputs
 
-__device__ __forceinline__ int adapter_of_row(const LinearParams& p, int row) {
-  const int s = p.segments > 0 ? segment_of_row(p.offsets, p.segments, row) : -1;
-  if (s < 0) return -1;
+struct LinearMaps {
+  CUtensorMap x, w, up, inner;
+};
+
+// What the two product kernels and the inner kernel have to agree on.
+struct LinearPlan {
+  int tile;      // rows per tile
+  int row_tiles, out_tiles;
+  int split;     // CTAs (a cluster) that share a tile's blocks; 0: CTA pairs of 256 outputs
+  int blocks;    // blocks of t
+  int rank_pad;  // t's row length: rank rounded up to the 16 of one product step
+};
+
+// ---------------------------------------------------------------- segments of a row tile
+// The last s with offsets[s] <= row (0 if none), by a warp.
+__device__ __forceinline__ int segment_at_row(const int* offsets, int segments, int row, int lane) {
+  int lo = 0, n = segments;
+  while (n > 1) {
+    const int step = (n + 31) / 32;
+    const bool ok = lane == 0 || (lane * step < n && offsets[lo + lane * step] <= row);
+    const int last = 31 - __clz(__ballot_sync(0xffffffffu, ok));
+    n = min(step, n - last * step);
+    lo += last * step;
+  }
+  return lo;
+}
+
+// The segments with an adapter that meet rows [r0, r1), in order; used by a whole warp. The first 32 are
+// read at once when the scan begins, ahead of their use.
+struct AdapterScan {
+  int r0, r1, base, lane;
+  unsigned hits;
+  bool more;
+  int my_adapter, my_lo, my_hi;
+
+  __device__ __forceinline__ void fill(const LinearParams& p) {
+    const int s = base + lane;
+    bool hit = false, beyond = true;
+    if (s < p.segments) {
+      const int begin = p.offsets[s], end = min(p.offsets[s + 1], p.rows);
+      my_adapter = p.index[s];
+      my_lo = max(begin, r0), my_hi = min(end, r1);
+      hit = my_lo < my_hi && my_adapter >= 0 && my_adapter < p.adapters;
+      beyond = begin >= r1;
+    }
+    hits = __ballot_sync(0xffffffffu, hit);
+    more = __ballot_sync(0xffffffffu, beyond) == 0;
+  }
+  __device__ __forceinline__ void begin(const LinearParams& p, int row0, int row1, int lane_) {
+    r0 = row0, r1 = row1, lane = lane_, hits = 0, more = false, my_adapter = -1, my_lo = my_hi = 0;
+    if (p.segments == 0) return;
+    base = segment_at_row(p.offsets, p.segments, r0, lane);
+    fill(p);
+  }
+  __device__ __forceinline__ bool next(const LinearParams& p, int& segment, int& adapter, int& lo, int& hi) {
+    while (hits == 0) {
+      if (!more) return false;
+      base += 32;
+      fill(p);
+    }
+    const int src = __ffs(hits) - 1;
+    hits &= hits - 1;
+    segment = base + src;
+    adapter = __shfl_sync(0xffffffffu, my_adapter, src);
+    lo = __shfl_sync(0xffffffffu, my_lo, src);
+    hi = __shfl_sync(0xffffffffu, my_hi, src);
+    return true;
+  }
+};
+
+// ---------------------------------------------------------------- inner products
+template <bool BF16>
+__device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (BF16)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// One CTA: 16 rows of one block of t, all ranks (at most NT * 8). Its eight warps take the input in turn,
+// 32 inputs at a time, and add up in shared memory. Both operands come straight from memory, 16 bytes a
+// thread: a thread's eight inputs are dealt to two product steps, the same way for x and down, which
+// permutes the sum's order and nothing else. Memory-bound (x once, down once per 16 rows from L2);
+// tcgen05 would want 128 rows and a trip through shared memory for the same bytes.
+template <bool BF16, int NT>
+__global__ void __launch_bounds__(256) adapter_inner_kernel(const LinearParams p, const LinearPlan plan) {
+  constexpr int kParts = NT == 16 ? 4 : 8;  // within 48 KB: at 128 ranks the upper four warps go first
+  __shared__ float part[kParts][16][NT * 8 + 1];
+  griddep_wait();
+  griddep_launch_dependents();  // after the wait: what starts now may read all that came before this kernel
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int block = blockIdx.x;
+  const int s = segment_of_tile(p.offsets, p.segments, plan.tile, block, lane);
+  const int tile = block - s, row0 = tile * plan.tile + blockIdx.y * 16;
   int begin, end;
   segment_range(p.offsets, s, p.rows, begin, end);
-  const int a = p.index[s];
-  if (a >= p.adapters) flag_error(kErrBadOffsets);
-  return a >= p.adapters ? -1 : a;
-}
-
-// inner[i][r] = scale_a * sum_c down_a[r][c] x[i][c]: one warp per row.
-template <typename T>
-__global__ void adapter_inner_kernel(const LinearParams p) {
-  griddep_wait();
-  griddep_launch_dependents();
-  const int row = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  if (row >= p.rows) return;
-  const int a = adapter_of_row(p, row);
-  const T* x = static_cast<const T*>(p.x) + row * p.x_stride;
-  for (int r = 0; r < p.rank && a >= 0; ++r) {
-    const T* d = static_cast<const T*>(p.down) + (static_cast<long long>(a) * p.rank + r) * p.in;
-    float sum = 0.f;
-    for (int c = lane; c < p.in; c += 32) sum = fmaf(to_float(d[c]), to_float(x[c]), sum);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane == 0) static_cast<float*>(p.inner)[static_cast<long long>(row) * p.rank + r] = sum * p.scale[a];
+  const int adapter = p.index[s];
+  if (adapter >= p.adapters) flag_error(kErrBadOffsets);
+  const int lo = max(begin, tile * plan.tile), hi = min(end, (tile + 1) * plan.tile);
+  if (tile < 0 || lo >= hi || adapter < 0 || adapter >= p.adapters) return;  // no such block, or none is read
+  uint16_t* inner = static_cast<uint16_t*>(p.inner) +
+                    (static_cast<long long>(block) * plan.tile + blockIdx.y * 16) * plan.rank_pad;
+  const bool mine = row0 < hi && row0 + 16 > lo;
+  if (!mine) {
+    if (plan.split == 0)  // a pair's product takes the whole tile of rows
+      for (int i = threadIdx.x; i < 16 * plan.rank_pad / 8; i += 256)
+        reinterpret_cast<uint4*>(inner)[i] = make_uint4(0, 0, 0, 0);
+    return;
   }
-}
-
-template <typename T>
-__global__ void __launch_bounds__(256) linear_kernel(const LinearParams p) {
-  __shared__ float xs[kStep][kTile + 1], ws[kStep][kTile + 1];
-  griddep_wait();
-  griddep_launch_dependents();
-  const int r0 = blockIdx.y * kTile, o0 = blockIdx.x * kTile;
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  float acc[4][4] = {};
-  for (int c0 = 0; c0 < p.in; c0 += kStep) {
-    for (int i = threadIdx.x; i < kStep * kTile; i += 256) {
-      const int c = i & 15, j = i >> 4;
-      const bool in = c0 + c < p.in;
-      xs[c][j] = in && r0 + j < p.rows
-                     ? to_float(static_cast<const T*>(p.x)[(r0 + j) * p.x_stride + c0 + c]) : 0.f;
-      ws[c][j] = in && o0 + j < p.out
-                     ? to_float(static_cast<const T*>(p.weight)[(o0 + j) * p.weight_stride + c0 + c]) : 0.f;
+  const int g = lane >> 2, c = lane & 3;
+  const uint16_t* x0 = static_cast<const uint16_t*>(p.x) + static_cast<long long>(min(row0 + g, p.rows - 1)) * p.x_stride;
+  const uint16_t* x1 =
+      static_cast<const uint16_t*>(p.x) + static_cast<long long>(min(row0 + g + 8, p.rows - 1)) * p.x_stride;
+  const uint16_t* d = static_cast<const uint16_t*>(p.down) + static_cast<long long>(adapter) * p.rank * p.in;
+  float acc[NT][4] = {};
+  for (int k = warp * 32 + c * 8; k - c * 8 < p.in; k += 256) {
+    const uint4 zero = make_uint4(0, 0, 0, 0);
+    const bool in = k < p.in;
+    const uint4 a0 = in ? *reinterpret_cast<const uint4*>(x0 + k) : zero;
+    const uint4 a1 = in ? *reinterpret_cast<const uint4*>(x1 + k) : zero;
+    uint4 b[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+      b[n] = in && n * 8 + g < p.rank ? *reinterpret_cast<const uint4*>(d + static_cast<long long>(n * 8 + g) * p.in + k)
+                                      : zero;
+    const uint32_t u0[4] = {a0.x, a1.x, a0.y, a1.y}, u1[4] = {a0.z, a1.z, a0.w, a1.w};
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      mma_16816<BF16>(acc[n], u0, b[n].x, b[n].y);
+      mma_16816<BF16>(acc[n], u1, b[n].z, b[n].w);
     }
-    __syncthreads();
-#pragma unroll
-    for (int c = 0; c < kStep; ++c)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(xs[c][ty + 16 * i], ws[c][tx + 16 * j], acc[i][j]);
-    __syncthreads();
   }
-  for (int i = 0; i < 4; ++i) {
-    const int row = r0 + ty + 16 * i;
-    if (row >= p.rows) continue;
-    const int a = adapter_of_row(p, row);
-    for (int j = 0; j < 4; ++j) {
-      const int o = o0 + tx + 16 * j;
-      if (o >= p.out) continue;
-      float v = acc[i][j];
-      if (p.bias != nullptr)
-        v += p.bias_f32 ? static_cast<const float*>(p.bias)[o] : to_float(static_cast<const T*>(p.bias)[o]);
-      if (a >= 0) {
-        const T* u = static_cast<const T*>(p.up) + (static_cast<long long>(a) * p.out + o) * p.rank;
-        const float* t = static_cast<const float*>(p.inner) + static_cast<long long>(row) * p.rank;
-        for (int r = 0; r < p.rank; ++r) v = fmaf(t[r], to_float(u[r]), v);
+  auto put = [&](int w) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      part[w][g][n * 8 + 2 * c] = acc[n][0], part[w][g][n * 8 + 2 * c + 1] = acc[n][1];
+      part[w][g + 8][n * 8 + 2 * c] = acc[n][2], part[w][g + 8][n * 8 + 2 * c + 1] = acc[n][3];
+    }
+  };
+  if (kParts == 4) {
+    if (warp >= 4) put(warp - 4);
+    __syncthreads();
+    if (warp < 4) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        acc[n][0] += part[warp][g][n * 8 + 2 * c], acc[n][1] += part[warp][g][n * 8 + 2 * c + 1];
+        acc[n][2] += part[warp][g + 8][n * 8 + 2 * c], acc[n][3] += part[warp][g + 8][n * 8 + 2 * c + 1];
       }
-      static_cast<T*>(p.y)[row * p.y_stride + o] = from_float<T>(v);
+      put(warp);
     }
+  } else {
+    put(warp);
+  }
+  __syncthreads();
+  const float scale = p.scale[adapter];
+  for (int i = threadIdx.x; i < 16 * plan.rank_pad; i += 256) {
+    const int r = i / plan.rank_pad, n = i - r * plan.rank_pad;
+    float v = 0.f;
+    if (row0 + r >= lo && row0 + r < hi && n < p.rank) {
+#pragma unroll
+      for (int q = 0; q < kParts; ++q) v += part[q][r][n];
+      v *= scale;
+    }
+    if constexpr (BF16) reinterpret_cast<__nv_bfloat16*>(inner)[i] = __float2bfloat16_rn(v);
+    else reinterpret_cast<__half*>(inner)[i] = __float2half_rn(v);
   }
 }
 
-template <typename T>
-cudaError_t launch(const LinearParams& p, cudaStream_t stream) {
-  if (p.segments > 0) {
-    const cudaError_t e =
-        launch_kernel(adapter_inner_kernel<T>, dim3((p.rows + 3) / 4), dim3(128), 0, stream, p);
-    if (e != cudaSuccess) return e;
+// ---------------------------------------------------------------- product, one CTA (or a cluster) per tile
+constexpr int kSmallThreads = 192;  // warp 0 TMA, warp 1 MMA, warps 2-5 epilogue
+
+template <int BN>
+struct SmallSmem {
+  static constexpr uint32_t kBBytes = BN * 128;
+  static constexpr uint32_t kStageBytes = kABytes + kBBytes;
+  static constexpr int kStages = 196608 / kStageBytes > 10 ? 10 : 196608 / kStageBytes;
+  static constexpr uint32_t kOffBar = kStages * kStageBytes;
+  static constexpr uint32_t kBytes = kOffBar + 512 + 1024;  // + barriers + alignment slack
+  static_assert(BN * 512u <= kOffBar, "the partial sums fit in the stages");
+};
+
+// A block as the producer hands it to the MMA thread beside its data: product steps (16 inputs each),
+// first column and columns of the product, and whether it is the last.
+__device__ __forceinline__ uint32_t pack_block(int steps, int col, int cols, bool last) {
+  return static_cast<uint32_t>(steps) | static_cast<uint32_t>(col) << 4 | static_cast<uint32_t>(cols) << 16 |
+         (last ? 1u << 31 : 0u);
+}
+
+__device__ __forceinline__ float bias_of(const LinearParams& p, bool bf16, int o) {
+  if (p.bias == nullptr || o >= p.out) return 0.f;
+  if (p.bias_f32) return static_cast<const float*>(p.bias)[o];
+  return bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(p.bias)[o])
+              : __half2float(static_cast<const __half*>(p.bias)[o]);
+}
+
+template <bool BF16>
+__device__ __forceinline__ void store16(void* y, long long i, float v) {
+  if constexpr (BF16) static_cast<__nv_bfloat16*>(y)[i] = __float2bfloat16_rn(v);
+  else static_cast<__half*>(y)[i] = __float2half_rn(v);
+}
+
+__device__ __forceinline__ float ld_cluster(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+// blockIdx.x = (row tile * out tiles + out tile) * split + rank. Rank r of a cluster takes its share of the
+// input blocks and every split-th adapter block; the partial tiles meet through distributed shared
+// memory, each CTA adding up and writing its share of the columns.
+template <int BN, bool BF16>
+__global__ void __launch_bounds__(kSmallThreads, 1)
+    linear_small_kernel(const __grid_constant__ LinearMaps maps, const LinearParams p, const LinearPlan plan) {
+  using L = SmallSmem<BN>;
+  constexpr int S = L::kStages;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::kOffBar);
+  uint64_t* empty = full + S;
+  uint64_t* done = empty + S;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  volatile uint32_t* info = tmem_slot + 2;  // [S]
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = static_cast<int>(blockIdx.x) % plan.split, unit = static_cast<int>(blockIdx.x) / plan.split;
+  const int row_tile = unit / plan.out_tiles, m0 = (unit - row_tile * plan.out_tiles) * 128, r0 = row_tile * BN;
+  constexpr uint32_t kCols = BN < 32 ? 32 : BN;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < S; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    mbar_init(done, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
   }
-  return launch_kernel(linear_kernel<T>, dim3((p.out + kTile - 1) / kTile, (p.rows + kTile - 1) / kTile), dim3(256), 0,
-                       stream, p);
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, kCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  if (p.segments == 0) griddep_wait();  // otherwise x, W and the segments are complete already
+  griddep_launch_dependents();
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ TMA producer
+    const int kb = (p.in + kK - 1) / kK, k_begin = rank * kb / plan.split, k_end = (rank + 1) * kb / plan.split;
+    int it = 0;
+    bool ok = true;
+    auto stage = [&](int s) {
+      if (it >= S && !mbar_wait_bounded(&empty[s], static_cast<uint32_t>(it / S - 1) & 1u, kErrWaitEmpty)) return false;
+      return *abort_flag == 0;
+    };
+    // Adapter blocks known from the start, so that the last input block knows whether more follow.
+    AdapterScan scan;
+    scan.begin(p, r0, min(r0 + BN, p.rows), lane);
+    int ordinal = 0, seg = 0, adapter = 0, lo = 0, hi = 0;
+    auto next_mine = [&]() {
+      while (scan.next(p, seg, adapter, lo, hi))
+        if (ordinal++ % plan.split == rank) return true;
+      return false;
+    };
+    bool more = next_mine();
+    for (int k = k_begin; ok && k < k_end; ++k, ++it) {
+      const int s = it % S;
+      ok = stage(s);
+      if (ok && lane == 0) {
+        info[s] = pack_block(min(kK, p.in - k * kK + 15) / 16, 0, BN, k + 1 == k_end && !more);
+        mbar_arrive_expect_tx(&full[s], L::kStageBytes);
+        tma_load_2d(smem + s * L::kStageBytes, &maps.w, &full[s], k * kK, m0);
+        tma_load_2d(smem + s * L::kStageBytes + kABytes, &maps.x, &full[s], k * kK, r0);
+      }
+      __syncwarp();
+      if (!ok) break;
+    }
+    // Every CTA waits here, so this grid cannot end before the inner products' does.
+    if (p.segments > 0) griddep_wait();
+    while (ok && more) {
+      const int block = row_tile + seg, a = adapter, c0 = (lo - r0) & ~15, c1 = (hi - r0 + 15) & ~15;
+      more = next_mine();
+      for (int k = 0; ok && k < plan.rank_pad; k += kK, ++it) {
+        const int s = it % S;
+        ok = stage(s);
+        if (ok && lane == 0) {
+          info[s] = pack_block(min(kK, plan.rank_pad - k) / 16, c0, c1 - c0, k + kK >= plan.rank_pad && !more);
+          mbar_arrive_expect_tx(&full[s], L::kStageBytes);
+          tma_load_3d(smem + s * L::kStageBytes, &maps.up, &full[s], k, m0, a);
+          tma_load_2d(smem + s * L::kStageBytes + kABytes, &maps.inner, &full[s], k, block * BN);
+        }
+        __syncwarp();
+        if (!ok) break;
+      }
+    }
+    if (lane == 0) {
+      if (!ok) *abort_flag = 1;
+      for (int i = max(0, it - S); i < it; ++i)  // every issued load lands before the CTA goes on
+        mbar_wait_bounded(&full[i % S], static_cast<uint32_t>(i / S) & 1u, kErrWaitDrain);
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA issuer
+    if (lane == 0) {
+      for (int it = 0;; ++it) {
+        const int s = it % S;
+        if (*abort_flag || !mbar_wait_bounded(&full[s], static_cast<uint32_t>(it / S) & 1u, kErrWaitFull)) {
+          *abort_flag = 1;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t b = info[s];
+        const uint32_t steps = b & 15u, col = (b >> 4) & 0xfffu, cols = (b >> 16) & 0x7fffu;
+        const uint32_t a0 = smem_u32(smem + s * L::kStageBytes);
+        const uint64_t ad = smem_desc_kmajor(a0, 128), bd = smem_desc_kmajor(a0 + kABytes + col * 128u, 128);
+        const uint32_t id = idesc_f16(BF16, 128, cols);
+        for (uint32_t k = 0; k < steps; ++k)
+          umma_f16(tmem + col, desc_advance(ad, k * 32u), desc_advance(bd, k * 32u), id, it > 0 || k > 0 ? 1u : 0u);
+        umma_commit(&empty[s]);
+        if (b >> 31) {
+          umma_commit(done);
+          break;
+        }
+      }
+    }
+    __syncwarp();
+  } else {
+    // ------------------------------------------------------------ epilogue
+    const int quarter = warp & 3, o = m0 + quarter * 32 + lane;
+    const float bias = bias_of(p, BF16, o);
+    const bool ok = mbar_wait_bounded(done, 0, kErrWaitAcc) && !*abort_flag;
+    tc_fence_after();
+    const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
+    for (int c = 0; c < BN; c += 16) {
+      float v[16];
+      tmem_ld16(tmem + lanes + c, v);
+      if (plan.split > 1) {
+        // The stages' data are consumed: they hold the partial tile now, [column][output].
+        float* part = reinterpret_cast<float*>(smem);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) part[(c + e) * 128 + quarter * 32 + lane] = v[e];
+      } else if (ok && o < p.out) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (r0 + c + e < p.rows) store16<BF16>(p.y, static_cast<long long>(r0 + c + e) * p.y_stride + o, v[e] + bias);
+      }
+    }
+    if (!ok) *abort_flag = 1;
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (plan.split > 1) {
+    cluster_sync();
+    if (warp >= 2 && !*abort_flag) {
+      const int f = (warp & 3) * 32 + lane, o = m0 + f;
+      const float bias = bias_of(p, BF16, o);
+      const int c_end = min((rank + 1) * BN / plan.split, p.rows - r0);
+      for (int c = rank * BN / plan.split; c < c_end; ++c) {
+        float v = bias;
+        for (int z = 0; z < plan.split; ++z) v += ld_cluster(cluster_addr(smem, z) + (c * 128 + f) * 4);
+        if (o < p.out) store16<BF16>(p.y, static_cast<long long>(r0 + c) * p.y_stride + o, v);
+      }
+    }
+    cluster_sync();  // no CTA leaves while another reads its partial tile
+  }
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, kCols);
+  }
+}
+
+// ---------------------------------------------------------------- product, CTA pairs
+constexpr int kPairThreads = 320;  // warp 0 TMA, warp 1 MMA (first CTA), warps 2-9 epilogue
+constexpr int kPairRows = 256;
+constexpr int kPairStages = 6;
+constexpr uint32_t kPairStageBytes = 2 * kABytes;  // this CTA's 128 outputs and 128 of the rows
+constexpr uint32_t kPairOffBar = kPairStages * kPairStageBytes;
+constexpr uint32_t kPairBytes = kPairOffBar + 512 + 1024;
+constexpr int kRaster = 8;  // row tiles that are walked together, so that W's and x's tiles meet in L2
+
+// 256 outputs x 256 rows per pair of CTAs (tcgen05.mma.cta_group::2): each CTA loads half of W's rows and
+// half of x's, i.e. 64 bytes per clock and SM at the tensor cores' full rate where one CTA's own
+// 128 x 256 tile would take 96. Two accumulators in TMEM: a tile is written while the next is computed.
+template <bool BF16>
+__global__ void __launch_bounds__(kPairThreads, 1)
+    linear_pair_kernel(const __grid_constant__ LinearMaps maps, const LinearParams p, const LinearPlan plan) {
+  constexpr int S = kPairStages;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + kPairOffBar);
+  uint64_t* empty = full + S;
+  uint64_t* acc_full = empty + S;      // [2]
+  uint64_t* acc_empty = acc_full + 2;  // [2] read out by both CTAs (first CTA's barriers)
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  volatile uint32_t* info = tmem_slot + 2;  // [S]
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const int pair = static_cast<int>(blockIdx.x >> 1), pairs = static_cast<int>(gridDim.x >> 1);
+  const int tiles = plan.row_tiles * plan.out_tiles;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < S; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&acc_full[i], 1);
+      mbar_init(&acc_empty[i], 16);
+    }
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(tmem_slot, 512);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();  // both CTAs' barriers exist before anything crosses the pair
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  if (p.segments == 0) griddep_wait();
+  griddep_launch_dependents();
+
+  auto place = [&](int t, int& row_tile, int& m0) {
+    const int per = kRaster * plan.out_tiles, group = t / per, in_group = t - group * per;
+    const int height = min(kRaster, plan.row_tiles - group * kRaster);
+    row_tile = group * kRaster + in_group % height;
+    m0 = in_group / height * 256;
+  };
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ TMA producer (both CTAs)
+    const int kb = (p.in + kK - 1) / kK;
+    const uint32_t full0 = cluster_addr(full, 0);
+    int it = 0;
+    bool ok = true, waited = p.segments == 0;
+    auto stage = [&](int s) {
+      if (it >= S && !mbar_wait_bounded(&empty[s], static_cast<uint32_t>(it / S - 1) & 1u, kErrWaitEmpty)) return false;
+      return *abort_flag == 0;
+    };
+    for (int t = pair; ok && t < tiles; t += pairs) {
+      int row_tile, m0;
+      place(t, row_tile, m0);
+      const int r0 = row_tile * kPairRows, my_m = m0 + static_cast<int>(rank) * 128;
+      const int my_r = r0 + static_cast<int>(rank) * 128;
+      AdapterScan scan;
+      scan.begin(p, r0, min(r0 + kPairRows, p.rows), lane);
+      int seg, adapter, lo, hi;
+      bool more = scan.next(p, seg, adapter, lo, hi);
+      for (int k = 0; ok && k < kb; ++k) {
+        const int s = it % S;
+        ok = stage(s);
+        if (!ok) break;
+        if (lane == 0) {
+          if (rank == 0) {
+            info[s] = pack_block(min(kK, p.in - k * kK + 15) / 16, 0, kPairRows, k + 1 == kb && !more);
+            mbar_arrive_expect_tx(&full[s], 2u * kPairStageBytes);
+          }
+          tma_load_2d_pair(smem + s * kPairStageBytes, &maps.w, full0 + 8u * s, k * kK, my_m);
+          tma_load_2d_pair(smem + s * kPairStageBytes + kABytes, &maps.x, full0 + 8u * s, k * kK, my_r);
+        }
+        __syncwarp();
+        ++it;
+      }
+      if (!waited) {
+        griddep_wait();
+        waited = true;
+      }
+      while (ok && more) {
+        const int row = (row_tile + seg) * kPairRows + static_cast<int>(rank) * 128, a = adapter;
+        more = scan.next(p, seg, adapter, lo, hi);
+        for (int k = 0; k < plan.rank_pad; k += kK) {
+          const int s = it % S;
+          ok = stage(s);
+          if (!ok) break;
+          if (lane == 0) {
+            if (rank == 0) {
+              info[s] = pack_block(min(kK, plan.rank_pad - k) / 16, 0, kPairRows, k + kK >= plan.rank_pad && !more);
+              mbar_arrive_expect_tx(&full[s], 2u * kPairStageBytes);
+            }
+            tma_load_3d_pair(smem + s * kPairStageBytes, &maps.up, full0 + 8u * s, k, my_m, a);
+            tma_load_2d_pair(smem + s * kPairStageBytes + kABytes, &maps.inner, full0 + 8u * s, k, row);
+          }
+          __syncwarp();
+          ++it;
+        }
+      }
+    }
+    if (!waited) griddep_wait();
+    if (lane == 0) {
+      if (!ok) *abort_flag = 1;
+      // The first CTA's barriers count both CTAs' bytes: all land before the closing cluster barrier.
+      if (rank == 0)
+        for (int i = max(0, it - S); i < it; ++i)
+          if (!mbar_wait_bounded(&full[i % S], static_cast<uint32_t>(i / S) & 1u, kErrWaitDrain)) break;
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA issuer (first CTA)
+    if (lane == 0 && rank == 0) {
+      const uint32_t id = idesc_f16(BF16, 256, kPairRows);
+      int it = 0, lt = 0;
+      bool ok = true;
+      for (int t = pair; ok && t < tiles; t += pairs, ++lt) {
+        const int buf = lt & 1;
+        if (lt >= 2) ok = mbar_wait_bounded(&acc_empty[buf], static_cast<uint32_t>((lt >> 1) - 1) & 1u, kErrWaitAcc);
+        if (!ok) break;
+        bool last = false;
+        for (bool first = true; ok && !last; first = false, ++it) {
+          const int s = it % S;
+          ok = !*abort_flag && mbar_wait_bounded(&full[s], static_cast<uint32_t>(it / S) & 1u, kErrWaitFull);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t b = info[s], steps = b & 15u;
+          last = b >> 31;
+          const uint32_t a0 = smem_u32(smem + s * kPairStageBytes);
+          const uint64_t ad = smem_desc_kmajor(a0, 128), bd = smem_desc_kmajor(a0 + kABytes, 128);
+          for (uint32_t k = 0; k < steps; ++k)
+            umma_f16_pair(tmem + buf * 256, desc_advance(ad, k * 32u), desc_advance(bd, k * 32u), id,
+                          !first || k > 0 ? 1u : 0u);
+          umma_commit_pair(&empty[s]);
+        }
+        if (ok) umma_commit_pair(&acc_full[buf]);
+      }
+      if (!ok) *abort_flag = 1;
+    }
+    __syncwarp();
+  } else {
+    // ------------------------------------------------------------ epilogue (both CTAs)
+    const int quarter = warp & 3, half = (warp - 2) >> 2;
+    const uint32_t lanes = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
+    const uint32_t release0 = cluster_addr(acc_empty, 0);
+    int lt = 0;
+    for (int t = pair; t < tiles; t += pairs, ++lt) {
+      int row_tile, m0;
+      place(t, row_tile, m0);
+      const int o = m0 + static_cast<int>(rank) * 128 + quarter * 32 + lane, buf = lt & 1;
+      const float bias = bias_of(p, BF16, o);
+      if (!mbar_wait_bounded(&acc_full[buf], static_cast<uint32_t>(lt >> 1) & 1u, kErrWaitAcc) || *abort_flag) {
+        *abort_flag = 1;
+        break;
+      }
+      tc_fence_after();
+      for (int c = half * 128; c < half * 128 + 128; c += 32) {
+        float v[32];
+        tmem_ld32(lanes + buf * 256 + c, v);
+        tmem_ld_wait();
+        tmem_ld_fence(v);
+        if (c == half * 128 + 96) {  // all read: the next tile but one may overwrite it
+          tc_fence_before();
+          if (lane == 0) mbar_arrive_cluster(release0 + 8u * buf);
+        }
+        const int row = row_tile * kPairRows + c;
+        if (o < p.out) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if (row + e < p.rows) store16<BF16>(p.y, static_cast<long long>(row + e) * p.y_stride + o, v[e] + bias);
+        }
+        __syncwarp();
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();  // neither CTA exits while the other's products, copies or arrivals may reach it
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem, 512);
+  }
+}
+
+// ---------------------------------------------------------------- host
+// CTA pairs that are resident at once (a GPC with an odd number of SMs leaves one idle), queried once per
+// device: one pair more would run alone after all the others.
+int resident_pairs() {
+  static std::atomic<int> cached[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = 0;
+  int n = cached[dev].load(std::memory_order_relaxed);
+  if (n > 0) return n;
+  auto kern = linear_pair_kernel<true>;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.gridDim = dim3(2 * (device_sm_count() / 2));
+  cfg.blockDim = dim3(kPairThreads);
+  cfg.dynamicSmemBytes = kPairBytes;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kPairBytes)) !=
+          cudaSuccess ||
+      cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess || n < 1) {
+    (void)cudaGetLastError();
+    n = device_sm_count() / 2;
+  }
+  cached[dev].store(n, std::memory_order_relaxed);
+  return n;
+}
+
+int encode(CUtensorMap* map, const void* base, bool bf16, int rank, long long d0, long long d1, long long d2,
+           long long s1, long long s2, int box_rows, const char* what) {
+  auto enc = api_tensor_map_encoder();
+  if (enc == nullptr) return api_fail(CTMR_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
+  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(d0), static_cast<cuuint64_t>(d1), static_cast<cuuint64_t>(d2)};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(s1 * 2), static_cast<cuuint64_t>(s2 * 2)};
+  const cuuint32_t box[3] = {kK, static_cast<cuuint32_t>(box_rows), 1}, step[3] = {1, 1, 1};
+  const CUresult r = enc(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                         static_cast<cuuint32_t>(rank), const_cast<void*>(base), dims, strides, box, step,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return api_fail(CTMR_ERR_INVALID, "%s: tensor map rejected (CUresult %d)", what, int(r));
+  return CTMR_OK;
+}
+
+LinearPlan plan_linear(const LinearParams& p) {
+  LinearPlan plan{};
+  const int sms = device_sm_count();
+  const long long pair_tiles = ((p.out + 255LL) / 256) * ((p.rows + 255LL) / 256);
+  if (pair_tiles * 2 >= sms) {
+    plan.tile = kPairRows, plan.split = 0, plan.out_tiles = (p.out + 255) / 256;
+  } else {
+    plan.tile = p.rows <= 16 ? 16 : (p.rows <= 32 ? 32 : (p.rows <= 64 ? 64 : 128));
+    plan.out_tiles = (p.out + 127) / 128;
+    const long long tiles = static_cast<long long>(plan.out_tiles) * ((p.rows + plan.tile - 1) / plan.tile);
+    const int kb = (p.in + kK - 1) / kK;
+    plan.split = 1;
+    while (plan.split < 8 && tiles * plan.split * 2 <= sms && plan.split * 4 <= kb) plan.split *= 2;
+  }
+  plan.row_tiles = (p.rows + plan.tile - 1) / plan.tile;
+  plan.blocks = p.segments > 0 ? plan.row_tiles + p.segments - 1 : 0;
+  plan.rank_pad = (p.rank + 15) / 16 * 16;
+  return plan;
+}
+
+template <bool BF16, int NT>
+cudaError_t launch_inner(const LinearParams& p, const LinearPlan& plan, cudaStream_t stream) {
+  return launch_kernel(adapter_inner_kernel<BF16, NT>, dim3(plan.blocks, plan.tile / 16), dim3(256), 0, stream, p, plan);
+}
+
+template <typename... KArgs, typename... Args>
+cudaError_t launch_cluster(void (*kern)(KArgs...), unsigned grid, int threads, size_t smem, int cluster,
+                           cudaStream_t stream, Args&&... args) {
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = static_cast<unsigned>(cluster);
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...);
+}
+
+template <bool BF16>
+int launch(const LinearParams& p, const LinearPlan& plan, cudaStream_t stream) {
+  LinearMaps maps;
+  const int box_rows = plan.split == 0 ? 128 : plan.tile;
+  int st = encode(&maps.x, p.x, BF16, 2, p.in, p.rows, 1, p.x_stride, 0, box_rows, "x");
+  if (st == CTMR_OK) st = encode(&maps.w, p.weight, BF16, 2, p.in, p.out, 1, p.weight_stride, 0, 128, "weight");
+  if (st != CTMR_OK) return st;
+  maps.up = maps.inner = maps.w;  // not read without adapters
+  cudaError_t e = cudaSuccess;
+  if (p.segments > 0) {
+    st = encode(&maps.up, p.up, BF16, 3, p.rank, p.out, p.adapters, p.rank, static_cast<long long>(p.rank) * p.out, 128,
+                "up");
+    if (st == CTMR_OK)
+      st = encode(&maps.inner, p.inner, BF16, 2, plan.rank_pad, static_cast<long long>(plan.blocks) * plan.tile, 1,
+                  plan.rank_pad, 0, box_rows, "workspace");
+    if (st != CTMR_OK) return st;
+    if (p.rank <= 16) e = launch_inner<BF16, 2>(p, plan, stream);
+    else if (p.rank <= 32) e = launch_inner<BF16, 4>(p, plan, stream);
+    else if (p.rank <= 64) e = launch_inner<BF16, 8>(p, plan, stream);
+    else e = launch_inner<BF16, 16>(p, plan, stream);
+    if (e != cudaSuccess) return api_fail(CTMR_ERR_CUDA, "adapter_linear launch: %s", cudaGetErrorString(e));
+  }
+  const long long tiles = static_cast<long long>(plan.row_tiles) * plan.out_tiles;
+  if (plan.split == 0) {
+    const long long pairs = resident_pairs();
+    e = launch_cluster(linear_pair_kernel<BF16>, static_cast<unsigned>(2 * (tiles < pairs ? tiles : pairs)),
+                       kPairThreads, kPairBytes, 2, stream, maps, p, plan);
+  } else {
+    const unsigned grid = static_cast<unsigned>(tiles * plan.split);
+    if (plan.tile == 16)
+      e = launch_cluster(linear_small_kernel<16, BF16>, grid, kSmallThreads, SmallSmem<16>::kBytes, plan.split, stream,
+                         maps, p, plan);
+    else if (plan.tile == 32)
+      e = launch_cluster(linear_small_kernel<32, BF16>, grid, kSmallThreads, SmallSmem<32>::kBytes, plan.split, stream,
+                         maps, p, plan);
+    else if (plan.tile == 64)
+      e = launch_cluster(linear_small_kernel<64, BF16>, grid, kSmallThreads, SmallSmem<64>::kBytes, plan.split, stream,
+                         maps, p, plan);
+    else
+      e = launch_cluster(linear_small_kernel<128, BF16>, grid, kSmallThreads, SmallSmem<128>::kBytes, plan.split,
+                         stream, maps, p, plan);
+  }
+  return e == cudaSuccess ? CTMR_OK : api_fail(CTMR_ERR_CUDA, "adapter_linear launch: %s", cudaGetErrorString(e));
 }
 
 }  // namespace
 
 size_t adapter_linear_workspace(const LinearParams& p) {
-  return p.segments > 0 ? static_cast<size_t>(p.rows) * p.rank * sizeof(float) : 0;
+  const LinearPlan plan = plan_linear(p);
+  return static_cast<size_t>(plan.blocks) * plan.tile * plan.rank_pad * 2;
 }
 
-cudaError_t launch_adapter_linear(const LinearParams& p, bool bf16, cudaStream_t stream) {
-  return bf16 ? launch<__nv_bfloat16>(p, stream) : launch<__half>(p, stream);
+int launch_adapter_linear(const LinearParams& p, bool bf16, cudaStream_t stream) {
+  const LinearPlan plan = plan_linear(p);
+  if (plan.blocks > 0x3fffff) return api_fail(CTMR_ERR_UNSUPPORTED, "too many segments");
+  return bf16 ? launch<true>(p, plan, stream) : launch<false>(p, plan, stream);
 }
 
 }  // namespace ctmr

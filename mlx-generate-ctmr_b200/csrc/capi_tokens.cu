@@ -166,8 +166,7 @@ int ctmr_adapter_linear(const ctmr_adapter_linear_desc* d, void* workspace, size
   st = check_workspace(ctmr::adapter_linear_workspace(p), workspace, workspace_bytes);
   if (st != CTMR_OK) return st;
   p.inner = workspace;
-  return finish(ctmr::launch_adapter_linear(p, d->dtype == CTMR_DTYPE_BF16, static_cast<cudaStream_t>(stream)),
-                "adapter_linear launch");
+  return ctmr::launch_adapter_linear(p, d->dtype == CTMR_DTYPE_BF16, static_cast<cudaStream_t>(stream));
 }
 
 size_t ctmr_attention_workspace_size(const ctmr_attention_desc* d) {

@@ -34,7 +34,7 @@ struct LinearParams {
   const float* scale;
   const int *offsets, *index;
   void* y;
-  void* inner;                          // workspace: the adapters' inner products
+  void* inner;                          // workspace: the adapters' inner products, 16-bit
   long long x_stride, weight_stride, y_stride;
   int rows, in, out, rank, adapters, segments;
   int bias_f32;
@@ -56,7 +56,7 @@ struct AttentionParams {
 
 cudaError_t launch_rotary(const RotaryParams& p, int dtype, cudaStream_t stream);
 size_t adapter_linear_workspace(const LinearParams& p);
-cudaError_t launch_adapter_linear(const LinearParams& p, bool bf16, cudaStream_t stream);
+int launch_adapter_linear(const LinearParams& p, bool bf16, cudaStream_t stream);  // a CTMR_ status
 size_t attention_packed_workspace(const AttentionParams& p);
 int launch_attention_packed(const AttentionParams& p, bool bf16, cudaStream_t stream);  // a CTMR_ status
 
@@ -91,17 +91,6 @@ __device__ __forceinline__ int segment_of_tile(const int* offsets, int segments,
     lo += last * step;
   }
   return lo;
-}
-
-// The segment that holds `row`: the last s with offsets[s] <= row; -1 where no segment holds it.
-__device__ __forceinline__ int segment_of_row(const int* offsets, int segments, int row) {
-  int lo = -1, hi = segments;  // offsets[lo] <= row < offsets[hi]
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (offsets[mid] <= row) lo = mid;
-    else hi = mid;
-  }
-  return lo >= 0 && row < offsets[lo + 1] ? lo : -1;
 }
 
 // ---------------------------------------------------------------- 16-bit values

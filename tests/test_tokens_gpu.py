@@ -210,6 +210,11 @@ LINEAR = [  # lengths, index, inner, outer, rank, adapters
     ([1500, 548, 3], [-1, 0, 1], 1024, 768, 32, 2),
     ([0, 2000, 0], [0, 1, 0], 1032, 515, 72, 2),
     (list(range(40)), [(5 * i) % 7 - 1 for i in range(40)], 320, 640, 16, 6),
+    # enough 256 x 256 tiles for the CTA pairs: an adapter border inside a tile, a last tile of two rows,
+    # many short segments, the largest rank over a short sum
+    ([1000, 1, 0, 1305], [2, 0, 1, 1], 136, 2310, 24, 3),
+    ([61] * 39, [(3 * i) % 8 - 1 for i in range(39)], 520, 2500, 8, 7),
+    ([2500, 2500], [1, 0], 64, 1100, 128, 2),
 ]
 
 
@@ -227,11 +232,11 @@ def test_adapter_linear(cuda, case, dtype):
 
 
 @pytest.mark.parametrize("dtype", HALF)
-@pytest.mark.parametrize("rows", [1, 2, 31, 100, 513, 2300])
+@pytest.mark.parametrize("rows", [1, 2, 31, 100, 513, 2300, 10007])
 def test_linear_without_adapters(cuda, rows, dtype):
     from ctmr_b200 import ops
 
-    c = _linear_case(rows, [rows], [-1], 264, 300, 8, 1, dtype)
+    c = _linear_case(rows, [rows], [-1], 264, 300 if rows < 10000 else 601, 8, 1, dtype)
     _within(ops.adapter_linear(c["x"], c["weight"], c["bias"]), *_linear_ref(c))
 
 
