@@ -37,10 +37,6 @@ COMMON_FLAGS = [
 ]
 
 
-# Compiled without relocatable device code, under which the assembler ignores setmaxnreg.
-WHOLE_PROGRAM = {"attention_packed.cu"}
-
-
 def _nvcc() -> str:
     found = shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc"
     if not Path(found).exists():
@@ -71,10 +67,7 @@ def build(verbose: bool = False, force: bool = False) -> Path:
     def compile_one(src: Path, obj: Path) -> None:
         if not force and not _stale(obj, [src, *headers]):
             return
-        flags = COMMON_FLAGS
-        if src.name in WHOLE_PROGRAM:
-            flags = [f for f in COMMON_FLAGS if f != "-rdc=true"] + ["-DCTMR_WHOLE_PROGRAM"]
-        cmd = [nvcc, *ARCH_FLAGS, *flags, "-c", str(src), "-o", str(obj)]
+        cmd = [nvcc, *ARCH_FLAGS, *COMMON_FLAGS, "-c", str(src), "-o", str(obj)]
         if verbose:
             print(" ".join(cmd), file=sys.stderr)
         subprocess.run(cmd, check=True)

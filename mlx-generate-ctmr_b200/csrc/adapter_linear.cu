@@ -151,6 +151,7 @@ __global__ void __launch_bounds__(256) adapter_inner_kernel(const LinearParams p
       static_cast<const uint16_t*>(p.x) + static_cast<long long>(min(row0 + g + 8, p.rows - 1)) * p.x_stride;
   const uint16_t* d = static_cast<const uint16_t*>(p.down) + static_cast<long long>(adapter) * p.rank * p.in;
   float acc[NT][4] = {};
+#pragma unroll (NT <= 4 ? 4 : NT <= 8 ? 2 : 1)
   for (int k = warp * 32 + c * 8; k - c * 8 < p.in; k += 256) {
     const uint4 zero = make_uint4(0, 0, 0, 0);
     const bool in = k < p.in;
@@ -239,7 +240,7 @@ __device__ __forceinline__ void store16(void* y, long long i, float v) {
 
 __device__ __forceinline__ float ld_cluster(uint32_t addr) {
   float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr));  // in order with the barriers
   return v;
 }
 
@@ -341,29 +342,38 @@ __global__ void __launch_bounds__(kSmallThreads, 1)
     }
     __syncwarp();
   } else if (warp == 1) {
-    // ------------------------------------------------------------ MMA issuer
-    if (lane == 0) {
-      for (int it = 0;; ++it) {
-        const int s = it % S;
-        if (*abort_flag || !mbar_wait_bounded(&full[s], static_cast<uint32_t>(it / S) & 1u, kErrWaitFull)) {
-          *abort_flag = 1;
-          break;
+    // ------------------------------------------------------------ MMA issuer: a warp that stays together
+    const uint32_t tm = warp_value(tmem), base = warp_value(smem_u32(smem));
+    const uint64_t d0 = smem_desc_kmajor(base, 128);
+    bool ok = true, last = false;
+    for (int it = 0; ok && !last; ++it) {
+      const int s = it % S;
+      ok = mbar_wait_warp(&full[s], static_cast<uint32_t>(it / S) & 1u, kErrWaitFull) &&
+           __all_sync(0xffffffffu, *abort_flag == 0);
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t b = warp_value(static_cast<uint32_t>(info[s]));
+      const uint32_t steps = b & 15u, col = (b >> 4) & 0xfffu, cols = (b >> 16) & 0x7fffu;
+      last = b >> 31;
+      const uint64_t ad = desc_advance(d0, static_cast<uint32_t>(s) * L::kStageBytes);
+      const uint64_t bd = desc_advance(ad, kABytes + col * 128u);
+      const uint32_t id = idesc_f16(BF16, 128, cols);
+      if (elect_one()) {
+        if (steps == 4) {
+#pragma unroll
+          for (uint32_t k = 0; k < 4; ++k)
+            umma_f16(tm + col, desc_advance(ad, k * 32u), desc_advance(bd, k * 32u), id, it > 0 || k > 0 ? 1u : 0u);
+        } else {
+#pragma unroll 1
+          for (uint32_t k = 0; k < steps; ++k)
+            umma_f16(tm + col, desc_advance(ad, k * 32u), desc_advance(bd, k * 32u), id, it > 0 || k > 0 ? 1u : 0u);
         }
-        tc_fence_after();
-        const uint32_t b = info[s];
-        const uint32_t steps = b & 15u, col = (b >> 4) & 0xfffu, cols = (b >> 16) & 0x7fffu;
-        const uint32_t a0 = smem_u32(smem + s * L::kStageBytes);
-        const uint64_t ad = smem_desc_kmajor(a0, 128), bd = smem_desc_kmajor(a0 + kABytes + col * 128u, 128);
-        const uint32_t id = idesc_f16(BF16, 128, cols);
-        for (uint32_t k = 0; k < steps; ++k)
-          umma_f16(tmem + col, desc_advance(ad, k * 32u), desc_advance(bd, k * 32u), id, it > 0 || k > 0 ? 1u : 0u);
         umma_commit(&empty[s]);
-        if (b >> 31) {
-          umma_commit(done);
-          break;
-        }
+        if (last) umma_commit(done);
       }
+      __syncwarp();
     }
+    if (!ok) *abort_flag = 1;
     __syncwarp();
   } else {
     // ------------------------------------------------------------ epilogue
@@ -397,10 +407,20 @@ __global__ void __launch_bounds__(kSmallThreads, 1)
       const int f = (warp & 3) * 32 + lane, o = m0 + f;
       const float bias = bias_of(p, BF16, o);
       const int c_end = min((rank + 1) * BN / plan.split, p.rows - r0);
-      for (int c = rank * BN / plan.split; c < c_end; ++c) {
-        float v = bias;
-        for (int z = 0; z < plan.split; ++z) v += ld_cluster(cluster_addr(smem, z) + (c * 128 + f) * 4);
-        if (o < p.out) store16<BF16>(p.y, static_cast<long long>(r0 + c) * p.y_stride + o, v);
+      constexpr int kBatch = BN / 8;  // columns read together, at most a rank's share of them
+      for (int c = rank * BN / plan.split; c < c_end; c += kBatch) {
+        float v[kBatch];
+#pragma unroll
+        for (int e = 0; e < kBatch; ++e) v[e] = bias;
+#pragma unroll 4
+        for (int z = 0; z < plan.split; ++z) {
+          const uint32_t at = cluster_addr(smem, z) + (c * 128 + f) * 4;
+#pragma unroll
+          for (int e = 0; e < kBatch; ++e) v[e] += ld_cluster(at + e * 512);
+        }
+#pragma unroll
+        for (int e = 0; e < kBatch; ++e)
+          if (o < p.out && c + e < c_end) store16<BF16>(p.y, static_cast<long long>(r0 + c + e) * p.y_stride + o, v[e]);
       }
     }
     cluster_sync();  // no CTA leaves while another reads its partial tile
@@ -541,31 +561,45 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     }
     __syncwarp();
   } else if (warp == 1) {
-    // ------------------------------------------------------------ MMA issuer (first CTA)
-    if (lane == 0 && rank == 0) {
+    // ------------------------------------------------------------ MMA issuer (first CTA): a warp that stays together
+    if (rank == 0) {
       const uint32_t id = idesc_f16(BF16, 256, kPairRows);
+      const uint32_t tm = warp_value(tmem), base = warp_value(smem_u32(smem));
+      const uint64_t d0 = smem_desc_kmajor(base, 128);
       int it = 0, lt = 0;
       bool ok = true;
       for (int t = pair; ok && t < tiles; t += pairs, ++lt) {
         const int buf = lt & 1;
-        if (lt >= 2) ok = mbar_wait_bounded(&acc_empty[buf], static_cast<uint32_t>((lt >> 1) - 1) & 1u, kErrWaitAcc);
+        if (lt >= 2) ok = mbar_wait_warp(&acc_empty[buf], static_cast<uint32_t>((lt >> 1) - 1) & 1u, kErrWaitAcc);
         if (!ok) break;
         bool last = false;
         for (bool first = true; ok && !last; first = false, ++it) {
           const int s = it % S;
-          ok = !*abort_flag && mbar_wait_bounded(&full[s], static_cast<uint32_t>(it / S) & 1u, kErrWaitFull);
+          ok = mbar_wait_warp(&full[s], static_cast<uint32_t>(it / S) & 1u, kErrWaitFull) &&
+               __all_sync(0xffffffffu, *abort_flag == 0);
           if (!ok) break;
           tc_fence_after();
-          const uint32_t b = info[s], steps = b & 15u;
+          const uint32_t b = warp_value(static_cast<uint32_t>(info[s])), steps = b & 15u;
           last = b >> 31;
-          const uint32_t a0 = smem_u32(smem + s * kPairStageBytes);
-          const uint64_t ad = smem_desc_kmajor(a0, 128), bd = smem_desc_kmajor(a0 + kABytes, 128);
-          for (uint32_t k = 0; k < steps; ++k)
-            umma_f16_pair(tmem + buf * 256, desc_advance(ad, k * 32u), desc_advance(bd, k * 32u), id,
-                          !first || k > 0 ? 1u : 0u);
-          umma_commit_pair(&empty[s]);
+          const uint64_t ad = desc_advance(d0, static_cast<uint32_t>(s) * kPairStageBytes);
+          const uint64_t bd = desc_advance(ad, kABytes);
+          if (elect_one()) {
+            if (steps == 4) {
+#pragma unroll
+              for (uint32_t k = 0; k < 4; ++k)
+                umma_f16_pair(tm + buf * 256, desc_advance(ad, k * 32u), desc_advance(bd, k * 32u), id,
+                              !first || k > 0 ? 1u : 0u);
+            } else {
+#pragma unroll 1
+              for (uint32_t k = 0; k < steps; ++k)
+                umma_f16_pair(tm + buf * 256, desc_advance(ad, k * 32u), desc_advance(bd, k * 32u), id,
+                              !first || k > 0 ? 1u : 0u);
+            }
+            umma_commit_pair(&empty[s]);
+            if (last) umma_commit_pair(&acc_full[buf]);
+          }
+          __syncwarp();
         }
-        if (ok) umma_commit_pair(&acc_full[buf]);
       }
       if (!ok) *abort_flag = 1;
     }

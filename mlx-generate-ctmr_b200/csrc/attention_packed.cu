@@ -4,15 +4,17 @@
 // Every mask leaves a query the keys [0, lim_i): lim_i = Lk, or min(Lk, max(p_i + 1, prefix)) when causal.
 //
 // One CTA takes 256 queries of a document and head, as two tiles of 128 with a softmax warpgroup each
-// (one query per thread). Keys come in tiles of 128: S = Q K^T (128 x 128 fp32) lands in TMEM, a
+// (one query per thread). Keys come in steps of 64: S = Q K^T (128 x 64 fp32) lands in TMEM, a
 // thread reads its whole row into registers, turns it into base-2 scores, takes the maximum and writes
 // P = 2^(s - m) as 16-bit pairs over S's own columns, and the tensor core reads P from TMEM for
-// O += P V (V is MN-major in shared memory, as loaded). One thread issues
-//   S0 S1 | PV0(j) S0(j + 1) PV1(j) S1(j + 1) | ...
-// so that a tile's products run under the other tile's softmax. O stays in TMEM; it is rescaled (by
-// the softmax threads, which hold m) only where a row's maximum has grown by more than 2^8 since the
-// last time: until then P may exceed one, up to 2^8, which neither 16-bit type minds, and the sum
-// of P is kept in fp32 with the same m.
+// O += P V (V is MN-major in shared memory, as loaded). Each tile has two S buffers, S(j + 1) is ready
+// while the threads work on S(j), and one thread issues
+//   S0(0) S1(0) S0(1) S1(1) | PV0(j) S0(j + 2) PV1(j) S1(j + 2) | ...
+// so the softmax never waits for a product: with one buffer of 128 keys to a tile (the same TMEM) it
+// did for half of its time (1,570 of 3,190 clocks a step at head size 32). O stays in TMEM; it is
+// rescaled (by the softmax threads, which hold m) only where a row's maximum has grown by more than 2^8
+// since the last time: until then P may exceed one, up to 2^8, which neither 16-bit type minds, and
+// the sum of P is kept in fp32 with the same m.
 #include <cmath>
 
 #include "capi_internal.cuh"
@@ -23,24 +25,22 @@
 namespace ctmr {
 namespace {
 
-constexpr int kThreads = 384;  // warps 0-3 and 4-7: softmax of tiles 0 and 1; 8: TMA; 9: MMA; 10, 11: none
-// A block of 384 threads starts with 168 registers each (64,512 of the SM's); a softmax thread holds a
-// row of 128 scores and takes 216, the last warpgroup gives back to 72: 256 * 216 + 128 * 72 = 64,512.
-constexpr int kSoftmaxRegs = 216, kOtherRegs = 72;
-constexpr int kTile = 128;     // queries per tile, keys per tile
+constexpr int kThreads = 320;  // warps 0-3 and 4-7: softmax of tiles 0 and 1; 8: TMA; 9: MMA
+constexpr int kTile = 128;     // queries per tile
+constexpr int kStep = 64;      // keys per step
 constexpr int kBlock = 2 * kTile;
-constexpr uint32_t kChunkBytes = kTile * 128;  // 128 rows of 64 16-bit channels
+constexpr uint32_t kQChunk = kTile * 128, kKChunk = kStep * 128;  // rows of 64 16-bit channels
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRescale = 8.f;  // log2 of the growth that O and the sum are rescaled for
 
-// NC chunks of 64 channels per row; K and V in rings of kStages tiles.
+// NC chunks of 64 channels per row; K and V in rings of kStages steps.
 template <int NC>
 struct Smem {
-  static constexpr int kStages = NC == 1 ? 4 : 2;
-  static constexpr uint32_t kTileBytes = NC * kChunkBytes;
-  static constexpr uint32_t kOffK = 2 * kTileBytes;
-  static constexpr uint32_t kOffV = kOffK + kStages * kTileBytes;
-  static constexpr uint32_t kOffBar = kOffV + kStages * kTileBytes;
+  static constexpr int kStages = 4;
+  static constexpr uint32_t kQBytes = NC * kQChunk, kKBytes = NC * kKChunk;
+  static constexpr uint32_t kOffK = 2 * kQBytes;
+  static constexpr uint32_t kOffV = kOffK + kStages * kKBytes;
+  static constexpr uint32_t kOffBar = kOffV + kStages * kKBytes;
   static constexpr uint32_t kBytes = kOffBar + 256 + 1024;  // + barriers + alignment slack
 };
 
@@ -163,13 +163,15 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bar = reinterpret_cast<uint64_t*>(smem + L::kOffBar);
   uint64_t* q_full = bar;                  // [2]
-  uint64_t* s_full = bar + 2;              // [2] S of a tile (and every earlier product) is done
-  uint64_t* p_full = bar + 4;              // [2] P of a tile is written and S read
-  uint64_t* k_full = bar + 6;              // [kStages]
+  // [tile][buffer]: S(j) is done, and with it PV(j - 2); both also for the two steps after the last.
+  uint64_t* s_full = bar + 2;
+  uint64_t* p_full = bar + 6;              // [tile][buffer]: P(j) is written, S(j) read
+  uint64_t* k_full = bar + 10;             // [kStages]
   uint64_t* k_empty = k_full + L::kStages;
   uint64_t* v_full = k_empty + L::kStages;
   uint64_t* v_empty = v_full + L::kStages;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(v_empty + L::kStages);
+  uint64_t* v_fixed = v_empty + L::kStages;  // the last V step has zeros past the document
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(v_fixed + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -180,8 +182,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (!find_place(p, blockIdx.x, lane, w)) return;  // the same answer in every warp
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&q_full[i], 1);
+    for (int i = 0; i < 2; ++i) mbar_init(&q_full[i], 1);
+    for (int i = 0; i < 4; ++i) {
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i], kTile);
     }
@@ -191,6 +193,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&v_full[i], 1);
       mbar_init(&v_empty[i], 1);
     }
+    mbar_init(v_fixed, 1);
     *abort_flag = 0;
     fence_barrier_init();
   }
@@ -201,49 +204,51 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;  // S0 S1 at columns 0, 128 (P over them), O0 O1 at 256, 384
+  const uint32_t tmem = *tmem_slot;  // S0a S0b S1a S1b at columns 0, 64, .. (P over them), O0 O1 at 256, 384
 
-  // Key tiles of each query tile: those that its last query sees.
-  int n[2];
-#pragma unroll
-  for (int t = 0; t < 2; ++t) {
+  // Steps of each query tile: the keys that its last query sees.
+  auto steps_of = [&](int t) {
     const int last = min(w.q_len - 1, w.first + (t + 1) * kTile - 1);
-    n[t] = last < w.first + t * kTile ? 0 : (limit_of(p, w, last) + kTile - 1) / kTile;
-  }
-  const int n_max = max(n[0], n[1]);
+    return last < w.first + t * kTile ? 0 : (limit_of(p, w, last) + kStep - 1) / kStep;
+  };
+  const int n0 = steps_of(0), n1 = steps_of(1), n_max = max(n0, n1);
+  const int tail = w.k_len - (n_max - 1) * kStep;  // the document's keys in the last step, if fewer than 64
 
-  if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
-    if (warp == 8) {
+  if (warp == 8) {
     // ------------------------------------------------------------ TMA producer
     if (lane == 0 && n_max > 0) {
       tma_prefetch_desc(&maps.q);
       tma_prefetch_desc(&maps.k);
       tma_prefetch_desc(&maps.v);
-      auto load = [&](const CUtensorMap* map, uint32_t off, uint64_t* full, int head, int row) {
-        mbar_arrive_expect_tx(full, L::kTileBytes);
+      for (int t = 0; t < 2; ++t) {
+        if ((t == 0 ? n0 : n1) == 0) continue;
+        mbar_arrive_expect_tx(&q_full[t], L::kQBytes);
 #pragma unroll
         for (int c = 0; c < NC; ++c)
-          tma_load_4d(smem + off + c * kChunkBytes, map, full, c * 64, head, row, w.map_doc);
+          tma_load_4d(smem + t * L::kQBytes + c * kQChunk, &maps.q, &q_full[t], c * 64, h, w.q_row + w.first + t * kTile,
+                      w.map_doc);
+      }
+      auto load = [&](const CUtensorMap* map, uint32_t off, uint64_t* full, int row) {
+        mbar_arrive_expect_tx(full, L::kKBytes);
+#pragma unroll
+        for (int c = 0; c < NC; ++c) tma_load_4d(smem + off + c * kKChunk, map, full, c * 64, hk, row, w.map_doc);
       };
       int j = 0;
-      for (int t = 0; t < 2; ++t)
-        if (n[t] > 0) load(&maps.q, t * L::kTileBytes, &q_full[t], h, w.q_row + w.first + t * kTile);
       for (; j < n_max && !*abort_flag; ++j) {
         const int s = j % L::kStages, use = j / L::kStages;
         const uint32_t freed = static_cast<uint32_t>(use - 1) & 1u;
         if (use > 0 && !mbar_wait_bounded(&k_empty[s], freed, kErrWaitEmpty)) break;
-        load(&maps.k, L::kOffK + s * L::kTileBytes, &k_full[s], hk, w.k_row + j * kTile);
+        load(&maps.k, L::kOffK + s * L::kKBytes, &k_full[s], w.k_row + j * kStep);
         if (use > 0 && !mbar_wait_bounded(&v_empty[s], freed, kErrWaitEmpty)) {
           mbar_wait_bounded(&k_full[s], static_cast<uint32_t>(use) & 1u, kErrWaitDrain);
           break;
         }
-        load(&maps.v, L::kOffV + s * L::kTileBytes, &v_full[s], hk, w.k_row + j * kTile);
+        load(&maps.v, L::kOffV + s * L::kKBytes, &v_full[s], w.k_row + j * kStep);
       }
       if (j < n_max) *abort_flag = 1;
       // Drain: every issued load lands before the CTA can exit.
-      for (int t = 0; t < 2; ++t)
-        if (n[t] > 0) mbar_wait_bounded(&q_full[t], 0, kErrWaitDrain);
+      if (n0 > 0) mbar_wait_bounded(&q_full[0], 0, kErrWaitDrain);
+      if (n1 > 0) mbar_wait_bounded(&q_full[1], 0, kErrWaitDrain);
       for (int i = max(0, j - L::kStages); i < j; ++i) {
         const uint32_t phase = static_cast<uint32_t>(i / L::kStages) & 1u;
         mbar_wait_bounded(&k_full[i % L::kStages], phase, kErrWaitDrain);
@@ -251,79 +256,113 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
     __syncwarp();
-    } else if (warp == 9) {
-    // ------------------------------------------------------------ MMA issuer (lane 0 issues, all wait)
-    const int dk = (p.dim + 15) / 16;
-    const uint32_t id_s = idesc_f16(BF16, kTile, kTile);
+    if (n_max > 0 && tail < kStep && !*abort_flag) {
+      // Rows past the document hold another's values, whose product with P = 0 must still be 0.
+      uint8_t* vt = smem + L::kOffV + (n_max - 1) % L::kStages * L::kKBytes;
+      for (int i = lane; i < (kStep - tail) * 8; i += 32)
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+          *reinterpret_cast<uint4*>(vt + c * kKChunk + tail * 128 + i * 16) = make_uint4(0, 0, 0, 0);
+      fence_proxy_async_shared();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(v_fixed);
+    }
+  } else if (warp == 9) {
+    // ------------------------------------------------------------ MMA issuer: a warp that stays together
+    const int dk = warp_value((p.dim + 15) / 16), u0 = warp_value(n0), u1 = warp_value(n1), u_max = max(u0, u1);
+    const bool fix = warp_value(tail) < kStep;
+    const uint32_t tm = warp_value(tmem), base = warp_value(smem_u32(smem));
+    const uint32_t id_s = idesc_f16(BF16, kTile, kStep);
     const uint32_t id_o = idesc_f16(BF16, kTile, static_cast<uint32_t>(dk) * 16u) | (1u << 16);  // V MN-major
+    const uint64_t d_q = smem_desc_kmajor(base, 128);
+    const uint64_t d_k = smem_desc_kmajor(base + L::kOffK, 128);
+    const uint64_t d_v = smem_desc_mnmajor(base + L::kOffV, kKChunk);
     bool ok = true;
+    // S(j) of tile t. The last chunk of channels may have fewer than four products: those are a loop.
     auto issue_s = [&](int t, int j) {
-      if (lane == 0) {
-        const uint32_t a = smem_u32(smem + t * L::kTileBytes);
-        const uint32_t b = smem_u32(smem + L::kOffK + (j % L::kStages) * L::kTileBytes);
-        for (int k = 0; k < dk; ++k) {
-          const uint32_t off = static_cast<uint32_t>(k >> 2) * kChunkBytes + static_cast<uint32_t>(k & 3) * 32u;
-          umma_f16(tmem + t * 128, smem_desc_kmajor(a + off, 128), smem_desc_kmajor(b + off, 128), id_s, k > 0 ? 1u : 0u);
+      const uint64_t a = desc_advance(d_q, static_cast<uint32_t>(t) * L::kQBytes);
+      const uint64_t b = desc_advance(d_k, static_cast<uint32_t>(j % L::kStages) * L::kKBytes);
+      const uint32_t d = tm + t * 128 + (j & 1) * 64;
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        const int steps = dk - c * 4;
+        const uint64_t ac = desc_advance(a, c * kQChunk), bc = desc_advance(b, c * kKChunk);
+        if (steps >= 4) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            umma_f16(d, desc_advance(ac, k * 32u), desc_advance(bc, k * 32u), id_s, c > 0 || k > 0 ? 1u : 0u);
+        } else {
+#pragma unroll 1
+          for (int k = 0; k < steps; ++k)
+            umma_f16(d, desc_advance(ac, k * 32u), desc_advance(bc, k * 32u), id_s, c > 0 || k > 0 ? 1u : 0u);
         }
-        umma_commit(&s_full[t]);
       }
     };
     auto wait_k = [&](int j) {
-      return mbar_wait_bounded(&k_full[j % L::kStages], static_cast<uint32_t>(j / L::kStages) & 1u, kErrWaitFull);
+      return mbar_wait_warp(&k_full[j % L::kStages], static_cast<uint32_t>(j / L::kStages) & 1u, kErrWaitFull);
     };
-    if (n_max > 0) ok = wait_k(0);
-    for (int t = 0; ok && t < 2; ++t)
-      if (n[t] > 0) {
-        ok = mbar_wait_bounded(&q_full[t], 0, kErrWaitFull);
-        tc_fence_after();
-        if (ok) issue_s(t, 0);
+    if (u0 > 0) ok = mbar_wait_warp(&q_full[0], 0, kErrWaitFull);
+    if (ok && u1 > 0) ok = mbar_wait_warp(&q_full[1], 0, kErrWaitFull);
+    for (int j = 0; ok && j < 2 && j < u_max; ++j) {
+      ok = wait_k(j);
+      tc_fence_after();
+      if (!ok) break;
+      if (elect_one()) {
+        if (j < u0) {
+          issue_s(0, j);
+          umma_commit(&s_full[j]);
+        }
+        if (j < u1) {
+          issue_s(1, j);
+          umma_commit(&s_full[2 + j]);
+        }
+        umma_commit(&k_empty[j]);
       }
-    if (ok && n_max > 0 && lane == 0) umma_commit(&k_empty[0]);
-    for (int j = 0; ok && j < n_max && !*abort_flag; ++j) {
+      __syncwarp();
+    }
+    for (int j = 0; ok && j < u_max; ++j) {
       const int s = j % L::kStages;
-      uint8_t* vt = smem + L::kOffV + s * L::kTileBytes;
-      ok = mbar_wait_bounded(&v_full[s], static_cast<uint32_t>(j / L::kStages) & 1u, kErrWaitFull);
-      if (ok && j + 1 < n_max) ok = wait_k(j + 1);
-      const int used = w.k_len - j * kTile;  // the document's keys in this tile
-      if (ok && used < kTile) {
-        // Rows past the document hold another's values, whose product with P = 0 must still be 0.
-        for (int i = lane; i < (kTile - used) * 8; i += 32)
-#pragma unroll
-          for (int c = 0; c < NC; ++c)
-            *reinterpret_cast<uint4*>(vt + c * kChunkBytes + used * 128 + i * 16) = make_uint4(0, 0, 0, 0);
-        fence_proxy_async_shared();
-        __syncwarp();
-      }
+      ok = mbar_wait_warp(&v_full[s], static_cast<uint32_t>(j / L::kStages) & 1u, kErrWaitFull);
+      if (ok && j + 2 < u_max) ok = wait_k(j + 2);
+      if (ok && j + 1 == u_max && fix) ok = mbar_wait_warp(v_fixed, 0, kErrWaitFull);
       for (int t = 0; ok && t < 2; ++t) {
-        if (j >= n[t]) continue;
-        ok = mbar_wait_bounded(&p_full[t], static_cast<uint32_t>(j) & 1u, kErrWaitFull);
+        const int n = t == 0 ? u0 : u1;
+        if (j >= n) continue;
+        ok = mbar_wait_warp(&p_full[t * 2 + (j & 1)], static_cast<uint32_t>(j >> 1) & 1u, kErrWaitFull);
         if (!ok) break;
         tc_fence_after();
-        if (lane == 0) {
-          const uint32_t b = smem_u32(vt);
+        if (elect_one()) {
+          const uint64_t b = desc_advance(d_v, static_cast<uint32_t>(s) * L::kKBytes);
 #pragma unroll
-          for (int k = 0; k < kTile / 16; ++k)
-            umma_f16_ts(tmem + 256 + t * 128, tmem + t * 128 + k * 8, smem_desc_mnmajor(b + k * 2048u, kChunkBytes), id_o,
+          for (int k = 0; k < kStep / 16; ++k)
+            umma_f16_ts(tm + 256 + t * 128, tm + t * 128 + (j & 1) * 64 + k * 8, desc_advance(b, k * 2048u), id_o,
                         j > 0 || k > 0 ? 1u : 0u);
+          if (j + 2 < n) issue_s(t, j + 2);
+          umma_commit(&s_full[t * 2 + (j & 1)]);
         }
-        if (j + 1 < n[t]) issue_s(t, j + 1);
-        else if (lane == 0) umma_commit(&s_full[t]);  // the last one: O is complete
+        __syncwarp();
       }
-      if (ok && lane == 0) {
+      ok = ok && __all_sync(0xffffffffu, *abort_flag == 0);
+      if (ok && elect_one()) {
         umma_commit(&v_empty[s]);
-        if (j + 1 < n_max) umma_commit(&k_empty[(j + 1) % L::kStages]);
+        if (j + 2 < u_max) umma_commit(&k_empty[(j + 2) % L::kStages]);
       }
+      __syncwarp();
     }
     if (!ok) *abort_flag = 1;
     __syncwarp();
-    }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
     // ------------------------------------------------------------ softmax, one query per thread
     const int t = warp >> 2;
     const int i = w.first + t * kTile + (warp & 3) * 32 + lane;  // the query inside the document
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t t_s = tmem + lanes + t * 128, t_o = tmem + lanes + 256 + t * 128;
+    const uint32_t t_o = tmem + lanes + 256 + t * 128;
+    const int n = t == 0 ? n0 : n1;
+    auto wait_s = [&](int j) {
+      const bool ok = mbar_wait_bounded(&s_full[t * 2 + (j & 1)], static_cast<uint32_t>(j >> 1) & 1u, kErrWaitAcc);
+      tc_fence_after();
+      return ok && !*abort_flag;
+    };
     const int lim = limit_of(p, w, i), place = i + w.k_len - w.q_len;
     const float scale = p.scale * kLog2e;
     const float cap_in = CAP ? 2.f * scale / p.cap : 0.f, cap_out = CAP ? p.cap * kLog2e : 0.f;
@@ -331,37 +370,37 @@ __global__ void __launch_bounds__(kThreads, 1)
     const float unit = CAP || BIAS ? 1.f : scale;  // what turns s below into base-2 scores
     float m = -INFINITY, l = 0.f;                  // m: what P is relative to; the maximum or up to 2^8 below
     bool ok = true;
-    for (int j = 0; j < n[t]; ++j) {
-      ok = mbar_wait_bounded(&s_full[t], static_cast<uint32_t>(j) & 1u, kErrWaitAcc) && !*abort_flag;
+    for (int j = 0; j < n; ++j) {
+      ok = wait_s(j);
       if (!ok) break;
-      tc_fence_after();
-      float s[kTile];
+      const uint32_t t_s = tmem + lanes + t * 128 + (j & 1) * 64;
+      float s[kStep];
 #pragma unroll
-      for (int c = 0; c < kTile; c += 32) tmem_ld32(t_s + c, s + c);
+      for (int c = 0; c < kStep; c += 32) tmem_ld32(t_s + c, s + c);
       tmem_ld_wait();
 #pragma unroll
-      for (int c = 0; c < kTile; c += 32) tmem_ld_fence(s + c);
+      for (int c = 0; c < kStep; c += 32) tmem_ld_fence(s + c);
       if constexpr (CAP) {
         // c tanh(x / c) = c - 2 c / (e^(2 x / c) + 1): two units' operations, absolute error c 2^-22.
 #pragma unroll
-        for (int c = 0; c < kTile; ++c) s[c] = fmaf(-2.f * cap_out, rcp_unit(exp2_unit(s[c] * cap_in) + 1.f), cap_out);
+        for (int c = 0; c < kStep; ++c) s[c] = fmaf(-2.f * cap_out, rcp_unit(exp2_unit(s[c] * cap_in) + 1.f), cap_out);
       }
       if constexpr (BIAS) {
-        const float at = static_cast<float>(place - j * kTile);
+        const float at = static_cast<float>(place - j * kStep);
 #pragma unroll
-        for (int c = 0; c < kTile; ++c)
+        for (int c = 0; c < kStep; ++c)
           s[c] = fmaf(-slope, fabsf(at - static_cast<float>(c)), CAP ? s[c] : s[c] * scale);
       }
-      const int left = lim - j * kTile;
-      if (left < kTile) {
+      const int left = lim - j * kStep;
+      if (left < kStep) {
 #pragma unroll
-        for (int c = 0; c < kTile; ++c) s[c] = c < left ? s[c] : -INFINITY;
+        for (int c = 0; c < kStep; ++c) s[c] = c < left ? s[c] : -INFINITY;
       }
       float mx[8];
 #pragma unroll
       for (int c = 0; c < 8; ++c) mx[c] = s[c];
 #pragma unroll
-      for (int c = 8; c < kTile; ++c) mx[c & 7] = fmaxf(mx[c & 7], s[c]);
+      for (int c = 8; c < kStep; ++c) mx[c & 7] = fmaxf(mx[c & 7], s[c]);
       const float top = unit * fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])),
                                      fmaxf(fmaxf(mx[4], mx[5]), fmaxf(mx[6], mx[7])));
       const bool grow = top > m + kRescale || (m == -INFINITY && top > m);
@@ -369,7 +408,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         const float f = grow ? exp2_unit(m - top) : 1.f;
         if (grow) m = top;
         l *= f;
-        if (j > 0) {  // S(j) was issued after PV(j - 1): O is up to date and nothing writes it now
+        if (j > 0) {  // PV(j - 1) has to be done; nothing writes O then until P(j) is handed over
+          ok = wait_s(j + 1);
+          if (!ok) break;
           for (int c = 0; c < p.dim; c += 32) {
             float o[32];
             tmem_ld32(t_o + c, o);
@@ -385,38 +426,32 @@ __global__ void __launch_bounds__(kThreads, 1)
       const float base = m == -INFINITY ? 0.f : -m;
       const float2 u2 = make_float2(unit, unit), b2 = make_float2(base, base);
       float2 sum[4] = {};
+      uint32_t r[kStep / 2];
 #pragma unroll
-      for (int c = 0; c < kTile; c += 64) {
-        uint32_t r[32];
-#pragma unroll
-        for (int e = 0; e < 32; ++e) {
-          float2 x = fma2(make_float2(s[c + 2 * e], s[c + 2 * e + 1]), u2, b2);
-          // One pair in four on the FMA pipe, the others on the exponential unit (16 a clock per SM,
-          // half of the time of a tile's two products at head size 128 and more below it).
-          if ((e & 3) == 3) x = exp2_poly(x);
-          else x = make_float2(exp2_unit(x.x), exp2_unit(x.y));
-          sum[e & 3] = add2(sum[e & 3], x);
-          r[e] = pack2<BF16>(x.x, x.y);
-        }
-        tmem_st32(t_s + c / 2, r);
+      for (int e = 0; e < kStep / 2; ++e) {
+        float2 x = fma2(make_float2(s[2 * e], s[2 * e + 1]), u2, b2);
+        // One pair in four on the FMA pipe, the others on the exponential unit (16 a clock per SM,
+        // half of the time of a step's two products at head size 128 and more below it).
+        if ((e & 3) == 3) x = exp2_poly(x);
+        else x = make_float2(exp2_unit(x.x), exp2_unit(x.y));
+        sum[e & 3] = add2(sum[e & 3], x);
+        r[e] = pack2<BF16>(x.x, x.y);
       }
+      tmem_st32(t_s, r);
       tmem_st_wait();
       tc_fence_before();
-      mbar_arrive(&p_full[t]);
+      mbar_arrive(&p_full[t * 2 + (j & 1)]);
       sum[0] = add2(add2(sum[0], sum[1]), add2(sum[2], sum[3]));
       l += sum[0].x + sum[0].y;
     }
-    if (ok && n[t] > 0) {
-      ok = mbar_wait_bounded(&s_full[t], static_cast<uint32_t>(n[t]) & 1u, kErrWaitAcc);
-      tc_fence_after();
-    }
+    if (ok && n > 0) ok = wait_s(n + 1);  // PV(n - 1)
     if (!ok) *abort_flag = 1;
     const bool some = m != -INFINITY;  // a query that saw nothing gets zeros
     const float inv = some ? 1.f / l : 0.f;
     uint16_t* out = static_cast<uint16_t*>(p.out) + w.map_doc * p.o_doc + (w.q_row + i) * p.o_token + h * p.o_head;
     for (int c = 0; c < p.dim; c += 32) {
       float o[32];
-      if (n[t] > 0) {
+      if (n > 0) {
         tmem_ld32(t_o + c, o);
         tmem_ld_wait();
         tmem_ld_fence(o);
@@ -443,9 +478,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-// (channel, head, token, document) view of one operand, a box of 64 channels x 128 tokens.
+// (channel, head, token, document) view of one operand, a box of 64 channels x box_tokens tokens.
 int encode(CUtensorMap* map, const void* base, bool bf16, int dim, int heads, long long tokens, long long docs,
-           long long s_head, long long s_token, long long s_doc, const char* what) {
+           long long s_head, long long s_token, long long s_doc, int box_tokens, const char* what) {
   auto enc = api_tensor_map_encoder();
   if (enc == nullptr) return api_fail(CTMR_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
   const cuuint64_t dims[4] = {static_cast<cuuint64_t>(dim), static_cast<cuuint64_t>(heads),
@@ -454,7 +489,7 @@ int encode(CUtensorMap* map, const void* base, bool bf16, int dim, int heads, lo
   const cuuint64_t strides[3] = {static_cast<cuuint64_t>(heads > 1 ? s_head * 2 : 16),
                                  static_cast<cuuint64_t>(tokens > 1 ? s_token * 2 : 16),
                                  static_cast<cuuint64_t>(docs > 1 ? s_doc * 2 : 16)};
-  const cuuint32_t box[4] = {64, 1, kTile, 1}, step[4] = {1, 1, 1, 1};
+  const cuuint32_t box[4] = {64, 1, static_cast<cuuint32_t>(box_tokens), 1}, step[4] = {1, 1, 1, 1};
   const CUresult r = enc(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
                          const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
@@ -483,26 +518,19 @@ cudaError_t launch_variant(const Maps& maps, const AttentionParams& p, dim3 grid
 
 }  // namespace
 
-cudaError_t attention_error_word(unsigned* bits, bool clear) {
-  cudaError_t e = cudaMemcpyFromSymbol(bits, g_device_error, sizeof(*bits));
-  const unsigned zero = 0;
-  if (e == cudaSuccess && clear && *bits != 0) e = cudaMemcpyToSymbol(g_device_error, &zero, sizeof(zero));
-  return e;
-}
-
 size_t attention_packed_workspace(const AttentionParams&) { return 0; }
 
 int launch_attention_packed(const AttentionParams& p, bool bf16, cudaStream_t stream) {
   const bool packed = p.q_offsets != nullptr;
   const int docs = packed ? 1 : p.documents;
   Maps maps;
-  int st = encode(&maps.q, p.q, bf16, p.dim, p.heads, p.q_tokens, docs, p.q_head, p.q_token, p.q_doc, "q");
+  int st = encode(&maps.q, p.q, bf16, p.dim, p.heads, p.q_tokens, docs, p.q_head, p.q_token, p.q_doc, kTile, "q");
   if (st != CTMR_OK) return st;
   maps.k = maps.v = maps.q;  // not read where there are no keys
   if (p.k_tokens > 0) {
-    st = encode(&maps.k, p.k, bf16, p.dim, p.kv_heads, p.k_tokens, docs, p.k_head, p.k_token, p.k_doc, "k");
+    st = encode(&maps.k, p.k, bf16, p.dim, p.kv_heads, p.k_tokens, docs, p.k_head, p.k_token, p.k_doc, kStep, "k");
     if (st != CTMR_OK) return st;
-    st = encode(&maps.v, p.v, bf16, p.dim, p.kv_heads, p.k_tokens, docs, p.v_head, p.v_token, p.v_doc, "v");
+    st = encode(&maps.v, p.v, bf16, p.dim, p.kv_heads, p.k_tokens, docs, p.v_head, p.v_token, p.v_doc, kStep, "v");
     if (st != CTMR_OK) return st;
   }
   const long long blocks = packed ? p.q_tokens / kBlock + static_cast<long long>(p.documents)

@@ -24,7 +24,6 @@
 #include "prepare.cuh"
 #include "launch.cuh"
 #include "capi_internal.cuh"
-#include "tokens.cuh"
 
 namespace ctmr {
 int conv_stage_plan(int kc, int bn, bool exact, bool one_cta_per_sm, size_t* smem_bytes);
@@ -1276,10 +1275,7 @@ int ctmr_get_device_error(unsigned* bits, int clear) {
   unsigned v = 0;
   e = cudaMemcpyFromSymbol(&v, ctmr::g_device_error, sizeof(v));
   if (e != cudaSuccess) return cuda_fail(e, "read device error");
-  unsigned other = 0;
-  e = ctmr::attention_error_word(&other, clear != 0);
-  if (e != cudaSuccess) return cuda_fail(e, "read device error");
-  if (bits != nullptr) *bits = v | other;
+  if (bits != nullptr) *bits = v;
   if (clear && v != 0) {
     const unsigned zero = 0;
     e = cudaMemcpyToSymbol(ctmr::g_device_error, &zero, sizeof(zero));

@@ -26,13 +26,7 @@ enum : unsigned {
 // Two seconds: far above any single tile's lifetime, far below a watchdog.
 constexpr uint64_t kWaitLimitNs = 2000000000ull;
 
-// The error word. A file compiled as a whole program (build_ext.py: setmaxnreg, which relocatable device
-// code ignores) cannot refer to the library's and holds one of its own, which ctmr_get_device_error adds.
-#ifdef CTMR_WHOLE_PROGRAM
-static __device__ unsigned int g_device_error;
-#else
 extern __device__ unsigned int g_device_error;
-#endif
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));
@@ -99,6 +93,25 @@ __device__ __forceinline__ bool mbar_wait_bounded(uint64_t* bar, uint32_t parity
       return false;
     }
   }
+}
+
+// ---------------------------------------------------------------- warps that issue as one
+// tcgen05.mma takes its descriptors from registers that a warp shares. A warp that stays together and
+// elects one lane around the instruction alone keeps them there; inside an `if (lane == 0)` each of them is
+// moved over for every product, which takes longer than a small product itself.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
+}
+
+// A value that all lanes hold alike, in a form that the compiler knows to be so.
+__device__ __forceinline__ uint32_t warp_value(uint32_t v) { return __reduce_max_sync(0xffffffffu, v); }
+__device__ __forceinline__ int warp_value(int v) { return __reduce_max_sync(0xffffffffu, v); }
+
+// mbar_wait_bounded by a whole warp, the answer the same for all lanes.
+__device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, unsigned err_bit) {
+  return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, err_bit)) != 0;
 }
 
 // ---------------------------------------------------------------- TMA

@@ -60,9 +60,6 @@ int launch_adapter_linear(const LinearParams& p, bool bf16, cudaStream_t stream)
 size_t attention_packed_workspace(const AttentionParams& p);
 int launch_attention_packed(const AttentionParams& p, bool bf16, cudaStream_t stream);  // a CTMR_ status
 
-// The attention file's own error word (see ptx.cuh), read and optionally cleared.
-cudaError_t attention_error_word(unsigned* bits, bool clear);
-
 // ---------------------------------------------------------------- ragged rows
 // offsets[s] clamped into [0, total] (a negative or excessive offset never indexes memory) and, with
 // it, the end of segment s clamped into [start, total]. A clamp that changed anything sets
