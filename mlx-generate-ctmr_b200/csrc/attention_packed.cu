@@ -8,10 +8,9 @@
 // thread reads its whole row into registers, turns it into base-2 scores, takes the maximum and writes
 // P = 2^(s - m) as 16-bit pairs over S's own columns, and the tensor core reads P from TMEM for
 // O += P V (V is MN-major in shared memory, as loaded). Each tile has two S buffers, S(j + 1) is ready
-// while the threads work on S(j), and one thread issues
-//   S0(0) S1(0) S0(1) S1(1) | PV0(j) S0(j + 2) PV1(j) S1(j + 2) | ...
-// so the softmax never waits for a product: with one buffer of 128 keys to a tile (the same TMEM) it
-// did for half of its time (1,570 of 3,190 clocks a step at head size 32). O stays in TMEM; it is
+// while the threads work on S(j), and a warp for each tile issues
+//   S(0) S(1) | PV(0) S(2) | PV(1) S(3) | ...
+// O stays in TMEM; it is
 // rescaled (by the softmax threads, which hold m) only where a row's maximum has grown by more than 2^8
 // since the last time: until then P may exceed one, up to 2^8, which neither 16-bit type minds, and
 // the sum of P is kept in fp32 with the same m.
@@ -25,7 +24,7 @@
 namespace ctmr {
 namespace {
 
-constexpr int kThreads = 320;  // warps 0-3 and 4-7: softmax of tiles 0 and 1; 8: TMA; 9: MMA
+constexpr int kThreads = 352;  // warps 0-3 and 4-7: softmax of tiles 0 and 1; 8: TMA; 9, 10: their products
 constexpr int kTile = 128;     // queries per tile
 constexpr int kStep = 64;      // keys per step
 constexpr int kBlock = 2 * kTile;
@@ -33,15 +32,17 @@ constexpr uint32_t kQChunk = kTile * 128, kKChunk = kStep * 128;  // rows of 64 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRescale = 8.f;  // log2 of the growth that O and the sum are rescaled for
 
-// NC chunks of 64 channels per row; K and V in rings of kStages steps.
+// NC chunks of 64 channels per row. V in a ring of kStages steps, K, which runs two steps ahead, in one of
+// two more: K(j + 2) then takes the place of K(j - 4), read before step j - 4 freed V's.
 template <int NC>
 struct Smem {
-  static constexpr int kStages = 4;
+  static constexpr int kStages = 4, kKSlots = kStages + 2;
   static constexpr uint32_t kQBytes = NC * kQChunk, kKBytes = NC * kKChunk;
   static constexpr uint32_t kOffK = 2 * kQBytes;
-  static constexpr uint32_t kOffV = kOffK + kStages * kKBytes;
+  static constexpr uint32_t kOffV = kOffK + kKSlots * kKBytes;
   static constexpr uint32_t kOffBar = kOffV + kStages * kKBytes;
   static constexpr uint32_t kBytes = kOffBar + 256 + 1024;  // + barriers + alignment slack
+  static_assert(kBytes <= 227 * 1024, "shared memory of an SM");
 };
 
 struct Maps {
@@ -166,11 +167,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   // [tile][buffer]: S(j) is done, and with it PV(j - 2); both also for the two steps after the last.
   uint64_t* s_full = bar + 2;
   uint64_t* p_full = bar + 6;              // [tile][buffer]: P(j) is written, S(j) read
-  uint64_t* k_full = bar + 10;             // [kStages]
-  uint64_t* k_empty = k_full + L::kStages;
-  uint64_t* v_full = k_empty + L::kStages;
-  uint64_t* v_empty = v_full + L::kStages;
-  uint64_t* v_fixed = v_empty + L::kStages;  // the last V step has zeros past the document
+  uint64_t* k_first = bar + 10;            // [2] K(0), K(1)
+  uint64_t* full = bar + 12;               // [kStages] V(j) and K(j + 2)
+  uint64_t* empty = full + L::kStages;     // [kStages] both read by both tiles
+  uint64_t* v_fixed = empty + L::kStages;  // the last V step has zeros past the document
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(v_fixed + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
@@ -182,16 +182,17 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (!find_place(p, blockIdx.x, lane, w)) return;  // the same answer in every warp
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 2; ++i) mbar_init(&q_full[i], 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&q_full[i], 1);
+      mbar_init(&k_first[i], 1);
+    }
     for (int i = 0; i < 4; ++i) {
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i], kTile);
     }
     for (int i = 0; i < L::kStages; ++i) {
-      mbar_init(&k_full[i], 1);
-      mbar_init(&k_empty[i], 1);
-      mbar_init(&v_full[i], 1);
-      mbar_init(&v_empty[i], 1);
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 2);
     }
     mbar_init(v_fixed, 1);
     *abort_flag = 0;
@@ -228,32 +229,32 @@ __global__ void __launch_bounds__(kThreads, 1)
           tma_load_4d(smem + t * L::kQBytes + c * kQChunk, &maps.q, &q_full[t], c * 64, h, w.q_row + w.first + t * kTile,
                       w.map_doc);
       }
-      auto load = [&](const CUtensorMap* map, uint32_t off, uint64_t* full, int row) {
-        mbar_arrive_expect_tx(full, L::kKBytes);
+      auto load = [&](const CUtensorMap* map, uint32_t off, uint64_t* bar, int j) {
 #pragma unroll
-        for (int c = 0; c < NC; ++c) tma_load_4d(smem + off + c * kKChunk, map, full, c * 64, hk, row, w.map_doc);
+        for (int c = 0; c < NC; ++c)
+          tma_load_4d(smem + off + c * kKChunk, map, bar, c * 64, hk, w.k_row + j * kStep, w.map_doc);
       };
+      const int firsts = min(n_max, 2);
+      for (int j = 0; j < firsts; ++j) {
+        mbar_arrive_expect_tx(&k_first[j], L::kKBytes);
+        load(&maps.k, L::kOffK + j * L::kKBytes, &k_first[j], j);
+      }
       int j = 0;
       for (; j < n_max && !*abort_flag; ++j) {
         const int s = j % L::kStages, use = j / L::kStages;
-        const uint32_t freed = static_cast<uint32_t>(use - 1) & 1u;
-        if (use > 0 && !mbar_wait_bounded(&k_empty[s], freed, kErrWaitEmpty)) break;
-        load(&maps.k, L::kOffK + s * L::kKBytes, &k_full[s], w.k_row + j * kStep);
-        if (use > 0 && !mbar_wait_bounded(&v_empty[s], freed, kErrWaitEmpty)) {
-          mbar_wait_bounded(&k_full[s], static_cast<uint32_t>(use) & 1u, kErrWaitDrain);
-          break;
-        }
-        load(&maps.v, L::kOffV + s * L::kKBytes, &v_full[s], w.k_row + j * kStep);
+        if (use > 0 && !mbar_wait_bounded(&empty[s], static_cast<uint32_t>(use - 1) & 1u, kErrWaitEmpty)) break;
+        const bool more = j + 2 < n_max;
+        mbar_arrive_expect_tx(&full[s], more ? 2 * L::kKBytes : L::kKBytes);
+        load(&maps.v, L::kOffV + s * L::kKBytes, &full[s], j);
+        if (more) load(&maps.k, L::kOffK + (j + 2) % L::kKSlots * L::kKBytes, &full[s], j + 2);
       }
       if (j < n_max) *abort_flag = 1;
       // Drain: every issued load lands before the CTA can exit.
       if (n0 > 0) mbar_wait_bounded(&q_full[0], 0, kErrWaitDrain);
       if (n1 > 0) mbar_wait_bounded(&q_full[1], 0, kErrWaitDrain);
-      for (int i = max(0, j - L::kStages); i < j; ++i) {
-        const uint32_t phase = static_cast<uint32_t>(i / L::kStages) & 1u;
-        mbar_wait_bounded(&k_full[i % L::kStages], phase, kErrWaitDrain);
-        mbar_wait_bounded(&v_full[i % L::kStages], phase, kErrWaitDrain);
-      }
+      for (int i = 0; i < firsts; ++i) mbar_wait_bounded(&k_first[i], 0, kErrWaitDrain);
+      for (int i = max(0, j - L::kStages); i < j; ++i)
+        mbar_wait_bounded(&full[i % L::kStages], static_cast<uint32_t>(i / L::kStages) & 1u, kErrWaitDrain);
     }
     __syncwarp();
     if (n_max > 0 && tail < kStep && !*abort_flag) {
@@ -267,26 +268,27 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(v_fixed);
     }
-  } else if (warp == 9) {
-    // ------------------------------------------------------------ MMA issuer: a warp that stays together
-    const int dk = warp_value((p.dim + 15) / 16), u0 = warp_value(n0), u1 = warp_value(n1), u_max = max(u0, u1);
+  } else if (warp >= 9) {
+    // ------------------------------------------------------------ MMA issuer of tile t: a warp that stays together
+    const int t = warp - 9;
+    const int dk = warp_value((p.dim + 15) / 16), n = warp_value(t == 0 ? n0 : n1), last = warp_value(n_max);
     const bool fix = warp_value(tail) < kStep;
-    const uint32_t tm = warp_value(tmem), base = warp_value(smem_u32(smem));
+    const uint32_t tm_s = warp_value(tmem + t * 128), tm_o = tm_s + 256;
+    const uint32_t base = warp_value(smem_u32(smem));
     const uint32_t id_s = idesc_f16(BF16, kTile, kStep);
     const uint32_t id_o = idesc_f16(BF16, kTile, static_cast<uint32_t>(dk) * 16u) | (1u << 16);  // V MN-major
-    const uint64_t d_q = smem_desc_kmajor(base, 128);
+    const uint64_t d_q = smem_desc_kmajor(base + t * L::kQBytes, 128);
     const uint64_t d_k = smem_desc_kmajor(base + L::kOffK, 128);
     const uint64_t d_v = smem_desc_mnmajor(base + L::kOffV, kKChunk);
     bool ok = true;
-    // S(j) of tile t. The last chunk of channels may have fewer than four products: those are a loop.
-    auto issue_s = [&](int t, int j) {
-      const uint64_t a = desc_advance(d_q, static_cast<uint32_t>(t) * L::kQBytes);
-      const uint64_t b = desc_advance(d_k, static_cast<uint32_t>(j % L::kStages) * L::kKBytes);
-      const uint32_t d = tm + t * 128 + (j & 1) * 64;
+    // S(j). The last chunk of channels may have fewer than four products: those are a loop.
+    auto issue_s = [&](int j) {
+      const uint64_t b = desc_advance(d_k, static_cast<uint32_t>(j % L::kKSlots) * L::kKBytes);
+      const uint32_t d = tm_s + (j & 1) * 64;
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
         const int steps = dk - c * 4;
-        const uint64_t ac = desc_advance(a, c * kQChunk), bc = desc_advance(b, c * kKChunk);
+        const uint64_t ac = desc_advance(d_q, c * kQChunk), bc = desc_advance(b, c * kKChunk);
         if (steps >= 4) {
 #pragma unroll
           for (int k = 0; k < 4; ++k)
@@ -298,55 +300,42 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
     };
-    auto wait_k = [&](int j) {
-      return mbar_wait_warp(&k_full[j % L::kStages], static_cast<uint32_t>(j / L::kStages) & 1u, kErrWaitFull);
-    };
-    if (u0 > 0) ok = mbar_wait_warp(&q_full[0], 0, kErrWaitFull);
-    if (ok && u1 > 0) ok = mbar_wait_warp(&q_full[1], 0, kErrWaitFull);
-    for (int j = 0; ok && j < 2 && j < u_max; ++j) {
-      ok = wait_k(j);
-      tc_fence_after();
+    if (n > 0) ok = mbar_wait_warp(&q_full[t], 0, kErrWaitFull);
+    for (int j = 0; ok && j < 2 && j < n; ++j) {
+      ok = mbar_wait_warp(&k_first[j], 0, kErrWaitFull);
       if (!ok) break;
+      tc_fence_after();
       if (elect_one()) {
-        if (j < u0) {
-          issue_s(0, j);
-          umma_commit(&s_full[j]);
-        }
-        if (j < u1) {
-          issue_s(1, j);
-          umma_commit(&s_full[2 + j]);
-        }
-        umma_commit(&k_empty[j]);
+        issue_s(j);
+        umma_commit(&s_full[t * 2 + j]);
       }
       __syncwarp();
     }
-    for (int j = 0; ok && j < u_max; ++j) {
+    for (int j = 0; ok && j < n; ++j) {
       const int s = j % L::kStages;
-      ok = mbar_wait_warp(&v_full[s], static_cast<uint32_t>(j / L::kStages) & 1u, kErrWaitFull);
-      if (ok && j + 2 < u_max) ok = wait_k(j + 2);
-      if (ok && j + 1 == u_max && fix) ok = mbar_wait_warp(v_fixed, 0, kErrWaitFull);
-      for (int t = 0; ok && t < 2; ++t) {
-        const int n = t == 0 ? u0 : u1;
-        if (j >= n) continue;
-        ok = mbar_wait_warp(&p_full[t * 2 + (j & 1)], static_cast<uint32_t>(j >> 1) & 1u, kErrWaitFull);
-        if (!ok) break;
-        tc_fence_after();
-        if (elect_one()) {
-          const uint64_t b = desc_advance(d_v, static_cast<uint32_t>(s) * L::kKBytes);
+      // One lane to a barrier: V(j) with K(j + 2), P(j), and at the end V's zeros.
+      bool got = true;
+      if (lane == 0) got = mbar_wait_bounded(&full[s], static_cast<uint32_t>(j / L::kStages) & 1u, kErrWaitFull);
+      if (lane == 1) got = mbar_wait_bounded(&p_full[t * 2 + (j & 1)], static_cast<uint32_t>(j >> 1) & 1u, kErrWaitFull);
+      if (lane == 2 && fix && j + 1 == last) got = mbar_wait_bounded(v_fixed, 0, kErrWaitFull);
+      ok = __all_sync(0xffffffffu, got);
+      if (!ok) break;
+      tc_fence_after();
+      if (elect_one()) {
+        const uint64_t b = desc_advance(d_v, static_cast<uint32_t>(s) * L::kKBytes);
 #pragma unroll
-          for (int k = 0; k < kStep / 16; ++k)
-            umma_f16_ts(tm + 256 + t * 128, tm + t * 128 + (j & 1) * 64 + k * 8, desc_advance(b, k * 2048u), id_o,
-                        j > 0 || k > 0 ? 1u : 0u);
-          if (j + 2 < n) issue_s(t, j + 2);
-          umma_commit(&s_full[t * 2 + (j & 1)]);
-        }
-        __syncwarp();
+        for (int k = 0; k < kStep / 16; ++k)
+          umma_f16_ts(tm_o, tm_s + (j & 1) * 64 + k * 8, desc_advance(b, k * 2048u), id_o, j > 0 || k > 0 ? 1u : 0u);
+        if (j + 2 < n) issue_s(j + 2);
+        umma_commit(&s_full[t * 2 + (j & 1)]);
+        umma_commit(&empty[s]);
       }
-      ok = ok && __all_sync(0xffffffffu, *abort_flag == 0);
-      if (ok && elect_one()) {
-        umma_commit(&v_empty[s]);
-        if (j + 2 < u_max) umma_commit(&k_empty[(j + 2) % L::kStages]);
-      }
+      __syncwarp();
+    }
+    // The other tile may see more keys: this one frees their stages as they come.
+    for (int j = n; ok && j < last; ++j) {
+      ok = mbar_wait_warp(&full[j % L::kStages], static_cast<uint32_t>(j / L::kStages) & 1u, kErrWaitFull);
+      if (ok && lane == 0) mbar_arrive(&empty[j % L::kStages]);
       __syncwarp();
     }
     if (!ok) *abort_flag = 1;
@@ -381,15 +370,27 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
       for (int c = 0; c < kStep; c += 32) tmem_ld_fence(s + c);
       if constexpr (CAP) {
-        // c tanh(x / c) = c - 2 c / (e^(2 x / c) + 1): two units' operations, absolute error c 2^-22.
+        // c tanh(x / c) = c - 2 c / (e^(2 x / c) + 1): two operations of the exponential unit, error c 2^-22.
 #pragma unroll
         for (int c = 0; c < kStep; ++c) s[c] = fmaf(-2.f * cap_out, rcp_unit(exp2_unit(s[c] * cap_in) + 1.f), cap_out);
       }
       if constexpr (BIAS) {
-        const float at = static_cast<float>(place - j * kStep);
+        // s - slope |at - c|: away from the query's own place the distance is linear in c.
+        const int at = place - j * kStep;
+        const float2 mul = make_float2(CAP ? 1.f : scale, CAP ? 1.f : scale);
+        if (__all_sync(0xffffffffu, at >= kStep - 1 || at <= 0)) {
+          const float step = at > 0 ? slope : -slope, from = -step * static_cast<float>(at);
+          const float2 step2 = make_float2(step, step), from2 = make_float2(from, from);
 #pragma unroll
-        for (int c = 0; c < kStep; ++c)
-          s[c] = fmaf(-slope, fabsf(at - static_cast<float>(c)), CAP ? s[c] : s[c] * scale);
+          for (int c = 0; c < kStep; c += 2) {
+            const float2 b = fma2(make_float2(static_cast<float>(c), static_cast<float>(c + 1)), step2, from2);
+            const float2 x = fma2(make_float2(s[c], s[c + 1]), mul, b);
+            s[c] = x.x, s[c + 1] = x.y;
+          }
+        } else {
+#pragma unroll
+          for (int c = 0; c < kStep; ++c) s[c] = fmaf(-slope, fabsf(static_cast<float>(at - c)), s[c] * mul.x);
+        }
       }
       const int left = lim - j * kStep;
       if (left < kStep) {
