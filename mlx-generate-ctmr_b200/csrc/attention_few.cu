@@ -1,0 +1,380 @@
+// The attention of attention_packed.cu for documents of few queries (serving: one new token per request
+// over a cache): group x queries rows, at most 32, share each key head's keys. The cache is read once and
+// that read is the time, so all of the GPU has to read at once: the keys of a (document, key head) are split
+// over a cluster of up to 16 CTAs and within a CTA over its eight warps, 16 keys at a time; the partial
+// softmaxes meet in shared memory and, across the cluster, in distributed shared memory, in one launch.
+//
+// The products are mma.sync m16n8k16 straight from global memory, 16 bytes a thread and access: tcgen05 would
+// want 128 rows where there are 1 to 32, and a trip through shared memory. The fragments' order inside a
+// sum is free, so a thread of K's product takes 8 adjacent channels of one key (32 channels make two
+// product steps), and one of V's product 8 adjacent channels of four keys, whose pairs it interleaves
+// by byte permutes: column n of output tile t is channel 8 n + t, which also leaves each thread 16
+// adjacent output channels.
+#include <cooperative_groups.h>
+
+#include "ctmr_b200.h"
+#include "launch.cuh"
+#include "tokens.cuh"
+
+namespace ctmr {
+namespace {
+
+constexpr int kWarps = 8, kThreads = kWarps * 32;
+constexpr int kKeys = 16;  // keys per warp and step
+constexpr float kLog2e = 1.4426950408889634f;
+
+template <bool BF16>
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (BF16)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ float exp2_unit(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if constexpr (BF16) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+
+// The lower (upper) halves of two registers as one.
+__device__ __forceinline__ uint32_t low_halves(uint32_t a, uint32_t b) { return __byte_perm(a, b, 0x5410); }
+__device__ __forceinline__ uint32_t high_halves(uint32_t a, uint32_t b) { return __byte_perm(a, b, 0x7632); }
+
+// MT: row tiles of 16. DC: channel chunks of 64.
+template <int MT, int DC>
+struct FewSmem {
+  static constexpr int kRows = MT * 16, kD = DC * 64, kPitch = kD + 8;  // of Q, 16-bit
+  static constexpr size_t kQ = static_cast<size_t>(kRows) * kPitch * 2;
+  static constexpr size_t kO = static_cast<size_t>(kRows) * kD * 4;     // one warp's (later the CTA's) sums
+  static constexpr size_t kStat = static_cast<size_t>(kRows) * 2 * 4;   // and its (m, l)
+  static constexpr size_t kBytes = kQ + kWarps * (kO + kStat);
+};
+
+template <int MT, int DC, bool BF16>
+__global__ void __launch_bounds__(kThreads) attention_few_kernel(const AttentionParams p, int splits) {
+  using L = FewSmem<MT, DC>;
+  extern __shared__ __align__(16) uint8_t smem[];
+  uint16_t* q_s = reinterpret_cast<uint16_t*>(smem);
+  float* o_s = reinterpret_cast<float*>(smem + L::kQ);                      // [kWarps][kRows][kD]
+  float* stat_s = reinterpret_cast<float*>(smem + L::kQ + kWarps * L::kO);  // [kWarps][kRows][2]
+  griddep_wait();
+  griddep_launch_dependents();
+  const int rank = static_cast<int>(blockIdx.x) % splits, doc = static_cast<int>(blockIdx.x) / splits, hk = blockIdx.y;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+  const int group = p.heads / p.kv_heads;
+
+  // The document's rows. (All threads of the cluster agree on them.)
+  int q_len = p.q_tokens, k_len = p.k_tokens;
+  long long q_at = 0, k_at = 0, v_at = 0, o_at = 0, lse_at = 0;
+  if (p.q_offsets != nullptr) {
+    int qb, qe, kb, ke;
+    segment_range(p.q_offsets, doc, p.q_tokens, qb, qe);
+    segment_range(p.k_offsets, doc, p.k_tokens, kb, ke);
+    q_len = qe - qb, k_len = ke - kb;
+    if (q_len > p.max_q) flag_error(kErrBadOffsets);
+    q_at = qb * p.q_token, o_at = qb * p.o_token, k_at = kb * p.k_token, v_at = kb * p.v_token, lse_at = qb;
+  } else {
+    if (p.k_lengths != nullptr) {
+      const int n = p.k_lengths[doc];
+      k_len = min(max(n, 0), p.k_tokens);
+      if (n != k_len) flag_error(kErrBadOffsets);
+    }
+    q_at = doc * p.q_doc, o_at = doc * p.o_doc, k_at = doc * p.k_doc, v_at = doc * p.v_doc;
+    lse_at = static_cast<long long>(doc) * p.q_tokens;
+  }
+  const int prefix = p.prefix != nullptr ? p.prefix[doc] : 0, shift = k_len - q_len;
+  const int queries = min(q_len, p.max_q), rows = queries * group;  // row r: query r / group, head r % group
+  auto limit_of = [&](int i) { return p.causal ? min(k_len, max(max(i + shift + 1, prefix), 0)) : k_len; };
+  const uint16_t* qp = static_cast<const uint16_t*>(p.q) + q_at;
+  const uint16_t* kp = static_cast<const uint16_t*>(p.k) + k_at + hk * p.k_head;
+  const uint16_t* vp = static_cast<const uint16_t*>(p.v) + v_at + hk * p.v_head;
+
+  // This CTA's keys: a share of those that any row sees, in steps of all warps.
+  const int seen = queries > 0 ? limit_of(queries - 1) : 0;
+  constexpr int kStep = kWarps * kKeys;
+  const int share = (seen + splits * kStep - 1) / (splits * kStep) * kStep;
+  const int k0 = min(rank * share, seen), k1 = min(k0 + share, seen);
+
+  for (int i = threadIdx.x; i < L::kRows * (L::kD / 8); i += kThreads) {
+    const int r = i / (L::kD / 8), d = (i - r * (L::kD / 8)) * 8;
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (r < rows && d < p.dim)
+      v = *reinterpret_cast<const uint4*>(qp + (r / group) * p.q_token + (hk * group + r % group) * p.q_head + d);
+    *reinterpret_cast<uint4*>(q_s + r * L::kPitch + d) = v;
+  }
+  __syncthreads();
+
+  float o[MT][DC * 8][4] = {};
+  float m[MT][2], l[MT][2] = {}, slope[MT][2];
+  int lim[MT][2], place[MT][2];
+#pragma unroll
+  for (int t = 0; t < MT; ++t)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int r = t * 16 + g + 8 * e;
+      m[t][e] = -INFINITY;
+      lim[t][e] = r < rows ? limit_of(r / group) : 0;
+      place[t][e] = r / group + shift;
+      slope[t][e] = p.slopes != nullptr && r < rows ? p.slopes[hk * group + r % group] * kLog2e : 0.f;
+    }
+  const float scale = p.scale * kLog2e;
+  const float cap_in = p.cap > 0.f ? 2.f * scale / p.cap : 0.f, cap_out = p.cap * kLog2e;
+
+  for (int kb = k0 + warp * kKeys; kb < k1; kb += kStep) {
+    // All of the step's loads at once. Keys past this CTA's share are not read and count as zeros.
+    const uint4 zero = make_uint4(0, 0, 0, 0);
+    uint4 kv[2][DC * 2], vv[4][DC];
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      const int key = kb + n * 8 + g;
+      const uint16_t* at = kp + key * p.k_token + c * 8;
+#pragma unroll
+      for (int w = 0; w < DC * 2; ++w)
+        kv[n][w] = key < k1 && w * 32 + c * 8 < p.dim ? __ldg(reinterpret_cast<const uint4*>(at + w * 32)) : zero;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int key = kb + 2 * c + (j & 1) + (j >> 1) * 8;
+      const uint16_t* at = vp + key * p.v_token + g * 8;
+#pragma unroll
+      for (int w = 0; w < DC; ++w)
+        vv[j][w] = key < k1 && w * 64 + g * 8 < p.dim ? __ldg(reinterpret_cast<const uint4*>(at + w * 64)) : zero;
+    }
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+      float s[2][4] = {};
+#pragma unroll
+      for (int w = 0; w < DC * 2; ++w) {
+        if (w * 32 >= p.dim) break;
+        const uint4 a0 = *reinterpret_cast<const uint4*>(q_s + (t * 16 + g) * L::kPitch + w * 32 + c * 8);
+        const uint4 a1 = *reinterpret_cast<const uint4*>(q_s + (t * 16 + g + 8) * L::kPitch + w * 32 + c * 8);
+        const uint32_t u0[4] = {a0.x, a1.x, a0.y, a1.y}, u1[4] = {a0.z, a1.z, a0.w, a1.w};
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          mma<BF16>(s[n], u0, kv[n][w].x, kv[n][w].y);
+          mma<BF16>(s[n], u1, kv[n][w].z, kv[n][w].w);
+        }
+      }
+      // Base-2 scores; s[n][2 e + i] belongs to row g + 8 e and key kb + 8 n + 2 c + i.
+      float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int e = i >> 1, key = kb + n * 8 + 2 * c + (i & 1);
+          float x = p.cap > 0.f ? fmaf(-2.f * cap_out, __frcp_rn(exp2_unit(s[n][i] * cap_in) + 1.f), cap_out)
+                                : s[n][i] * scale;
+          x = fmaf(-slope[t][e], fabsf(static_cast<float>(place[t][e] - key)), x);
+          x = key < lim[t][e] && key < k1 ? x : -INFINITY;
+          s[n][i] = x;
+          top[e] = fmaxf(top[e], x);
+        }
+      float f[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 1));
+        top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 2));
+        top[e] = fmaxf(top[e], m[t][e]);
+        f[e] = m[t][e] == top[e] ? 1.f : exp2_unit(m[t][e] - top[e]);
+        m[t][e] = top[e];
+      }
+      uint32_t a[4];
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float base = m[t][e] == -INFINITY ? 0.f : m[t][e];
+          const float x0 = exp2_unit(s[n][2 * e] - base), x1 = exp2_unit(s[n][2 * e + 1] - base);
+          l[t][e] = n == 0 ? fmaf(l[t][e], f[e], x0 + x1) : l[t][e] + (x0 + x1);
+          a[n * 2 + e] = pack2<BF16>(x0, x1);
+        }
+      if (__any_sync(0xffffffffu, f[0] != 1.f || f[1] != 1.f)) {
+#pragma unroll
+        for (int n = 0; n < DC * 8; ++n)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[t][n][i] *= f[i >> 1];
+      }
+#pragma unroll
+      for (int w = 0; w < DC; ++w) {
+        if (w * 64 >= p.dim) break;
+        const uint32_t* v0 = reinterpret_cast<const uint32_t*>(&vv[0][w]);
+        const uint32_t* v1 = reinterpret_cast<const uint32_t*>(&vv[1][w]);
+        const uint32_t* v2 = reinterpret_cast<const uint32_t*>(&vv[2][w]);
+        const uint32_t* v3 = reinterpret_cast<const uint32_t*>(&vv[3][w]);
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          mma<BF16>(o[t][w * 8 + 2 * n], a, low_halves(v0[n], v1[n]), low_halves(v2[n], v3[n]));
+          mma<BF16>(o[t][w * 8 + 2 * n + 1], a, high_halves(v0[n], v1[n]), high_halves(v2[n], v3[n]));
+        }
+      }
+    }
+  }
+
+  // Each warp's sums to shared memory: thread (g, c) holds channels 16 c .. 16 c + 15 of each chunk.
+#pragma unroll
+  for (int t = 0; t < MT; ++t)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      l[t][e] += __shfl_xor_sync(0xffffffffu, l[t][e], 1);
+      l[t][e] += __shfl_xor_sync(0xffffffffu, l[t][e], 2);
+      const int r = t * 16 + g + 8 * e;
+      if (c == 0) {
+        stat_s[(warp * L::kRows + r) * 2] = m[t][e];
+        stat_s[(warp * L::kRows + r) * 2 + 1] = l[t][e];
+      }
+      float* to = o_s + (static_cast<size_t>(warp) * L::kRows + r) * L::kD + 16 * c;
+#pragma unroll
+      for (int w = 0; w < DC; ++w)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int n = 0; n < 8; n += 4)
+            *reinterpret_cast<float4*>(to + w * 64 + i * 8 + n) =
+                make_float4(o[t][w * 8 + n][2 * e + i], o[t][w * 8 + n + 1][2 * e + i], o[t][w * 8 + n + 2][2 * e + i],
+                            o[t][w * 8 + n + 3][2 * e + i]);
+    }
+  // The warps' sums into the first one's place, for all rows that exist.
+  __syncthreads();
+  auto merge = [&](int r, int d, float& big, float& total) {  // relative to the largest m, 4 channels from d
+    big = -INFINITY, total = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) big = fmaxf(big, stat_s[(w * L::kRows + r) * 2]);
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (big == -INFINITY) return sum;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float f = exp2_unit(stat_s[(w * L::kRows + r) * 2] - big);
+      total = fmaf(f, stat_s[(w * L::kRows + r) * 2 + 1], total);
+      const float4 v = *reinterpret_cast<const float4*>(o_s + (static_cast<size_t>(w) * L::kRows + r) * L::kD + d);
+      sum.x = fmaf(f, v.x, sum.x), sum.y = fmaf(f, v.y, sum.y);
+      sum.z = fmaf(f, v.z, sum.z), sum.w = fmaf(f, v.w, sum.w);
+    }
+    return sum;
+  };
+  auto finish = [&](int r, int d, float4 sum, float big, float total) {
+    const int i = r / group, h = hk * group + r % group;
+    const float inv = total > 0.f ? 1.f / total : 0.f;  // a query that saw nothing gets zeros
+    uint16_t* out = static_cast<uint16_t*>(p.out) + o_at + i * p.o_token + h * p.o_head;
+    *reinterpret_cast<uint2*>(out + d) =
+        make_uint2(pack2<BF16>(sum.x * inv, sum.y * inv), pack2<BF16>(sum.z * inv, sum.w * inv));
+    if (p.lse != nullptr && d == 0)
+      p.lse[(lse_at + i) * p.heads + h] = total > 0.f ? (big + log2f(total)) * 0.6931471805599453f : -INFINITY;
+  };
+  const int quads = p.dim / 4, work = rows * quads;
+  if (splits == 1) {
+    for (int i = threadIdx.x; i < work; i += kThreads) {
+      const int r = i / quads, d = (i - r * quads) * 4;
+      float big, total;
+      const float4 sum = merge(r, d, big, total);
+      finish(r, d, sum, big, total);
+    }
+    return;
+  }
+  // The CTA's sums and statistics take the place of Q and of the first warp's, which only their readers
+  // overwrite: every thread merges into registers first.
+  constexpr int kEach = (L::kRows * L::kD / 4 + kThreads - 1) / kThreads;
+  float4 mine[kEach];
+  float2 st[kEach];
+#pragma unroll
+  for (int n = 0; n < kEach; ++n) {
+    const int i = threadIdx.x + n * kThreads;
+    if (i < work) mine[n] = merge(i / quads, i % quads * 4, st[n].x, st[n].y);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int n = 0; n < kEach; ++n) {
+    const int i = threadIdx.x + n * kThreads;
+    if (i < work) {
+      const int r = i / quads, d = i % quads * 4;
+      *reinterpret_cast<float4*>(o_s + r * L::kD + d) = mine[n];
+      if (d == 0) stat_s[r * 2] = st[n].x, stat_s[r * 2 + 1] = st[n].y;
+    }
+  }
+  cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
+  cluster.sync();
+  for (int i = rank * kThreads + threadIdx.x; i < work; i += splits * kThreads) {
+    const int r = i / quads, d = (i - r * quads) * 4;
+    float big = -INFINITY, total = 0.f;
+    for (int z = 0; z < splits; ++z) big = fmaxf(big, cluster.map_shared_rank(stat_s, z)[r * 2]);
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (big != -INFINITY) {
+#pragma unroll 4
+      for (int z = 0; z < splits; ++z) {
+        const float2 other = *reinterpret_cast<const float2*>(cluster.map_shared_rank(stat_s, z) + r * 2);
+        const float4 v = *reinterpret_cast<const float4*>(cluster.map_shared_rank(o_s, z) + r * L::kD + d);
+        const float f = exp2_unit(other.x - big);
+        total = fmaf(f, other.y, total);
+        sum.x = fmaf(f, v.x, sum.x), sum.y = fmaf(f, v.y, sum.y);
+        sum.z = fmaf(f, v.z, sum.z), sum.w = fmaf(f, v.w, sum.w);
+      }
+    }
+    finish(r, d, sum, big, total);
+  }
+  cluster.sync();  // no CTA leaves while another reads its sums
+}
+
+template <int MT, int DC, bool BF16>
+cudaError_t launch(const AttentionParams& p, int splits, cudaStream_t stream) {
+  auto kern = attention_few_kernel<MT, DC, BF16>;
+  constexpr int bytes = static_cast<int>(FewSmem<MT, DC>::kBytes);
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && splits > 8) e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(p.documents) * static_cast<unsigned>(splits), static_cast<unsigned>(p.kv_heads));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = bytes;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = static_cast<unsigned>(splits);
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = splits > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kern, p, splits);
+}
+
+template <bool BF16>
+cudaError_t launch_type(const AttentionParams& p, int splits, cudaStream_t stream) {
+  const int rows = p.heads / p.kv_heads * p.max_q;
+  if (p.dim <= 64) return rows <= 16 ? launch<1, 1, BF16>(p, splits, stream) : launch<2, 1, BF16>(p, splits, stream);
+  return rows <= 16 ? launch<1, 2, BF16>(p, splits, stream) : launch<2, 2, BF16>(p, splits, stream);
+}
+
+}  // namespace
+
+// At most 32 rows of a key head: two row tiles of the products.
+bool attention_few_takes(const AttentionParams& p) {
+  return static_cast<long long>(p.heads / p.kv_heads) * p.max_q <= 32 && p.documents <= (1 << 24);
+}
+
+cudaError_t launch_attention_few(const AttentionParams& p, bool bf16, cudaStream_t stream) {
+  // Enough CTAs for every SM, as long as each keeps two steps of 128 keys or more.
+  const long long units = static_cast<long long>(p.documents) * p.kv_heads;
+  const int sms = device_sm_count();
+  int splits = 1;
+  while (splits < 16 && units * splits < sms && p.k_tokens >= splits * 2 * 256) splits *= 2;
+  return bf16 ? launch_type<true>(p, splits, stream) : launch_type<false>(p, splits, stream);
+}
+
+}  // namespace ctmr

@@ -522,6 +522,10 @@ cudaError_t launch_variant(const Maps& maps, const AttentionParams& p, dim3 grid
 size_t attention_packed_workspace(const AttentionParams&) { return 0; }
 
 int launch_attention_packed(const AttentionParams& p, bool bf16, cudaStream_t stream) {
+  if (attention_few_takes(p)) {
+    const cudaError_t e = launch_attention_few(p, bf16, stream);
+    return e == cudaSuccess ? CTMR_OK : api_fail(CTMR_ERR_CUDA, "attention launch: %s", cudaGetErrorString(e));
+  }
   const bool packed = p.q_offsets != nullptr;
   const int docs = packed ? 1 : p.documents;
   Maps maps;

@@ -60,6 +60,10 @@ int launch_adapter_linear(const LinearParams& p, bool bf16, cudaStream_t stream)
 size_t attention_packed_workspace(const AttentionParams& p);
 int launch_attention_packed(const AttentionParams& p, bool bf16, cudaStream_t stream);  // a CTMR_ status
 
+// The form for few query rows per key head, and whether it takes the call.
+bool attention_few_takes(const AttentionParams& p);
+cudaError_t launch_attention_few(const AttentionParams& p, bool bf16, cudaStream_t stream);
+
 // ---------------------------------------------------------------- ragged rows
 // offsets[s] clamped into [0, total] (a negative or excessive offset never indexes memory) and, with
 // it, the end of segment s clamped into [start, total]. A clamp that changed anything sets
