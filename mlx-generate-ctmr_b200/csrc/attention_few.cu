@@ -1,15 +1,13 @@
 // The attention of attention_packed.cu for documents of few queries (serving: one new token per request
 // over a cache): group x queries rows, at most 32, share each key head's keys. The cache is read once and
 // that read is the time, so all of the GPU has to read at once: the keys of a (document, key head) are split
-// over a cluster of up to 16 CTAs and within a CTA over its eight warps, 16 keys at a time; the partial
-// softmaxes meet in shared memory and, across the cluster, in distributed shared memory, in one launch.
+// over a cluster of up to 16 CTAs, in steps of 64 that TMA brings into a ring in shared memory (96 KB a CTA, two
+// CTAs an SM: 192 KB in flight); each of four warps takes 16 keys of a step. The partial softmaxes meet in
+// shared memory and, across the cluster, in distributed shared memory, in one launch.
 //
-// The products are mma.sync m16n8k16 straight from global memory, 16 bytes a thread and access: tcgen05 would
-// want 128 rows where there are 1 to 32, and a trip through shared memory. The fragments' order inside a
-// sum is free, so a thread of K's product takes 8 adjacent channels of one key (32 channels make two
-// product steps), and one of V's product 8 adjacent channels of four keys, whose pairs it interleaves
-// by byte permutes: column n of output tile t is channel 8 n + t, which also leaves each thread 16
-// adjacent output channels.
+// The products are mma.sync m16n8k16, whose 16 rows fit: tcgen05 would want 128 where there are 1 to 32. With
+// the loads in registers instead of a ring (eight warps an SM, a step's loads then its products) the same
+// kernel took 72 us for 16 requests of 4,096 to 8,192 keys, four key heads of 128.
 #include <cooperative_groups.h>
 
 #include "ctmr_b200.h"
@@ -19,8 +17,8 @@
 namespace ctmr {
 namespace {
 
-constexpr int kWarps = 8, kThreads = kWarps * 32;
-constexpr int kKeys = 16;  // keys per warp and step
+constexpr int kWarps = 4, kThreads = kWarps * 32 + 32;  // four warps compute, one loads
+constexpr int kKeys = 16, kStep = kWarps * kKeys;         // keys per warp and per step
 constexpr float kLog2e = 1.4426950408889634f;
 
 template <bool BF16>
@@ -54,64 +52,85 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   }
 }
 
-// The lower (upper) halves of two registers as one.
-__device__ __forceinline__ uint32_t low_halves(uint32_t a, uint32_t b) { return __byte_perm(a, b, 0x5410); }
-__device__ __forceinline__ uint32_t high_halves(uint32_t a, uint32_t b) { return __byte_perm(a, b, 0x7632); }
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
+}
+
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
+}
 
 // MT: row tiles of 16. DC: channel chunks of 64.
 template <int MT, int DC>
 struct FewSmem {
-  static constexpr int kRows = MT * 16, kD = DC * 64, kPitch = kD + 8;  // of Q, 16-bit
-  static constexpr size_t kQ = static_cast<size_t>(kRows) * kPitch * 2;
-  static constexpr size_t kO = static_cast<size_t>(kRows) * kD * 4;     // one warp's (later the CTA's) sums
-  static constexpr size_t kStat = static_cast<size_t>(kRows) * 2 * 4;   // and its (m, l)
-  static constexpr size_t kBytes = kQ + kWarps * (kO + kStat);
+  static constexpr int kRows = MT * 16, kD = DC * 64;
+  static constexpr int kStages = 6 / DC;
+  static constexpr uint32_t kChunk = kStep * 128, kStage = 2 * DC * kChunk;  // K then V, chunks of 64 channels
+  static constexpr int kPitch = kD + 8;                                      // of Q, 16-bit
+  static constexpr uint32_t kOffQ = kStages * kStage, kOffBar = kOffQ + kRows * kPitch * 2;
+  static constexpr uint32_t kBytes = kOffBar + 128 + 1024;  // + barriers + alignment slack
+  // After the last step the ring holds the warps' sums: [kWarps][kRows][kD], then their (m, l).
+  static constexpr uint32_t kOffStat = kWarps * kRows * kD * 4;
+  static_assert(kOffStat + kWarps * kRows * 8 <= kOffQ, "the sums fit in the ring");
 };
 
 template <int MT, int DC, bool BF16>
-__global__ void __launch_bounds__(kThreads) attention_few_kernel(const AttentionParams p, int splits) {
+__global__ void __launch_bounds__(kThreads, 2)
+    attention_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                         const AttentionParams p, int splits) {
   using L = FewSmem<MT, DC>;
-  extern __shared__ __align__(16) uint8_t smem[];
-  uint16_t* q_s = reinterpret_cast<uint16_t*>(smem);
-  float* o_s = reinterpret_cast<float*>(smem + L::kQ);                      // [kWarps][kRows][kD]
-  float* stat_s = reinterpret_cast<float*>(smem + L::kQ + kWarps * L::kO);  // [kWarps][kRows][2]
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  uint16_t* q_s = reinterpret_cast<uint16_t*>(smem + L::kOffQ);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::kOffBar);
+  uint64_t* empty = full + L::kStages;
+  float* o_s = reinterpret_cast<float*>(smem);                   // [kWarps][kRows][kD]
+  float* stat_s = reinterpret_cast<float*>(smem + L::kOffStat);  // [kWarps][kRows][2]
   griddep_wait();
   griddep_launch_dependents();
   const int rank = static_cast<int>(blockIdx.x) % splits, doc = static_cast<int>(blockIdx.x) / splits, hk = blockIdx.y;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < L::kStages; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], kWarps);
+    }
+    fence_barrier_init();
+  }
   const int group = p.heads / p.kv_heads;
 
   // The document's rows. (All threads of the cluster agree on them.)
-  int q_len = p.q_tokens, k_len = p.k_tokens;
-  long long q_at = 0, k_at = 0, v_at = 0, o_at = 0, lse_at = 0;
+  int q_len = p.q_tokens, k_len = p.k_tokens, k_row = 0, map_doc = 0;
+  long long q_at = 0, o_at = 0, lse_at = 0;
   if (p.q_offsets != nullptr) {
     int qb, qe, kb, ke;
     segment_range(p.q_offsets, doc, p.q_tokens, qb, qe);
     segment_range(p.k_offsets, doc, p.k_tokens, kb, ke);
     q_len = qe - qb, k_len = ke - kb;
     if (q_len > p.max_q) flag_error(kErrBadOffsets);
-    q_at = qb * p.q_token, o_at = qb * p.o_token, k_at = kb * p.k_token, v_at = kb * p.v_token, lse_at = qb;
+    q_at = qb * p.q_token, o_at = qb * p.o_token, lse_at = qb, k_row = kb;
   } else {
     if (p.k_lengths != nullptr) {
       const int n = p.k_lengths[doc];
       k_len = min(max(n, 0), p.k_tokens);
       if (n != k_len) flag_error(kErrBadOffsets);
     }
-    q_at = doc * p.q_doc, o_at = doc * p.o_doc, k_at = doc * p.k_doc, v_at = doc * p.v_doc;
+    q_at = doc * p.q_doc, o_at = doc * p.o_doc, map_doc = doc;
     lse_at = static_cast<long long>(doc) * p.q_tokens;
   }
   const int prefix = p.prefix != nullptr ? p.prefix[doc] : 0, shift = k_len - q_len;
   const int queries = min(q_len, p.max_q), rows = queries * group;  // row r: query r / group, head r % group
   auto limit_of = [&](int i) { return p.causal ? min(k_len, max(max(i + shift + 1, prefix), 0)) : k_len; };
   const uint16_t* qp = static_cast<const uint16_t*>(p.q) + q_at;
-  const uint16_t* kp = static_cast<const uint16_t*>(p.k) + k_at + hk * p.k_head;
-  const uint16_t* vp = static_cast<const uint16_t*>(p.v) + v_at + hk * p.v_head;
 
-  // This CTA's keys: a share of those that any row sees, in steps of all warps.
+  // This CTA's keys: a share of those that any row sees, in whole steps.
   const int seen = queries > 0 ? limit_of(queries - 1) : 0;
-  constexpr int kStep = kWarps * kKeys;
   const int share = (seen + splits * kStep - 1) / (splits * kStep) * kStep;
-  const int k0 = min(rank * share, seen), k1 = min(k0 + share, seen);
+  const int k0 = min(rank * share, seen), k1 = min(k0 + share, seen), steps = (k1 - k0 + kStep - 1) / kStep;
 
   for (int i = threadIdx.x; i < L::kRows * (L::kD / 8); i += kThreads) {
     const int r = i / (L::kD / 8), d = (i - r * (L::kD / 8)) * 8;
@@ -123,135 +142,150 @@ __global__ void __launch_bounds__(kThreads) attention_few_kernel(const Attention
   __syncthreads();
 
   float o[MT][DC * 8][4] = {};
-  float m[MT][2], l[MT][2] = {}, slope[MT][2];
-  int lim[MT][2], place[MT][2];
+  float m[MT][2], l[MT][2] = {};
+  if (warp == kWarps) {
+    // ------------------------------------------------------------ TMA producer
+    if (lane == 0) {
+      for (int j = 0; j < steps; ++j) {
+        const int st = j % L::kStages, use = j / L::kStages;
+        if (use > 0 && !mbar_wait_bounded(&empty[st], static_cast<uint32_t>(use - 1) & 1u, kErrWaitEmpty)) {
+          for (int i = max(0, j - L::kStages); i < j; ++i)  // what is in flight lands before anything else
+            mbar_wait_bounded(&full[i % L::kStages], static_cast<uint32_t>(i / L::kStages) & 1u, kErrWaitDrain);
+          break;
+        }
+        mbar_arrive_expect_tx(&full[st], L::kStage);
 #pragma unroll
-  for (int t = 0; t < MT; ++t)
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int r = t * 16 + g + 8 * e;
-      m[t][e] = -INFINITY;
-      lim[t][e] = r < rows ? limit_of(r / group) : 0;
-      place[t][e] = r / group + shift;
-      slope[t][e] = p.slopes != nullptr && r < rows ? p.slopes[hk * group + r % group] * kLog2e : 0.f;
-    }
-  const float scale = p.scale * kLog2e;
-  const float cap_in = p.cap > 0.f ? 2.f * scale / p.cap : 0.f, cap_out = p.cap * kLog2e;
-
-  for (int kb = k0 + warp * kKeys; kb < k1; kb += kStep) {
-    // All of the step's loads at once. Keys past this CTA's share are not read and count as zeros.
-    const uint4 zero = make_uint4(0, 0, 0, 0);
-    uint4 kv[2][DC * 2], vv[4][DC];
-#pragma unroll
-    for (int n = 0; n < 2; ++n) {
-      const int key = kb + n * 8 + g;
-      const uint16_t* at = kp + key * p.k_token + c * 8;
-#pragma unroll
-      for (int w = 0; w < DC * 2; ++w)
-        kv[n][w] = key < k1 && w * 32 + c * 8 < p.dim ? __ldg(reinterpret_cast<const uint4*>(at + w * 32)) : zero;
-    }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int key = kb + 2 * c + (j & 1) + (j >> 1) * 8;
-      const uint16_t* at = vp + key * p.v_token + g * 8;
-#pragma unroll
-      for (int w = 0; w < DC; ++w)
-        vv[j][w] = key < k1 && w * 64 + g * 8 < p.dim ? __ldg(reinterpret_cast<const uint4*>(at + w * 64)) : zero;
-    }
-#pragma unroll
-    for (int t = 0; t < MT; ++t) {
-      float s[2][4] = {};
-#pragma unroll
-      for (int w = 0; w < DC * 2; ++w) {
-        if (w * 32 >= p.dim) break;
-        const uint4 a0 = *reinterpret_cast<const uint4*>(q_s + (t * 16 + g) * L::kPitch + w * 32 + c * 8);
-        const uint4 a1 = *reinterpret_cast<const uint4*>(q_s + (t * 16 + g + 8) * L::kPitch + w * 32 + c * 8);
-        const uint32_t u0[4] = {a0.x, a1.x, a0.y, a1.y}, u1[4] = {a0.z, a1.z, a0.w, a1.w};
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-          mma<BF16>(s[n], u0, kv[n][w].x, kv[n][w].y);
-          mma<BF16>(s[n], u1, kv[n][w].z, kv[n][w].w);
+        for (int w = 0; w < DC; ++w) {
+          uint8_t* to = smem + st * L::kStage + w * L::kChunk;
+          tma_load_4d(to, &map_k, &full[st], w * 64, hk, k_row + k0 + j * kStep, map_doc);
+          tma_load_4d(to + DC * L::kChunk, &map_v, &full[st], w * 64, hk, k_row + k0 + j * kStep, map_doc);
         }
       }
-      // Base-2 scores; s[n][2 e + i] belongs to row g + 8 e and key kb + 8 n + 2 c + i.
-      float top[2] = {-INFINITY, -INFINITY};
+    }
+    __syncwarp();
+  } else {
+    // ------------------------------------------------------------ 16 keys of each step
+    float slope[MT][2];
+    int lim[MT][2], place[MT][2];
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int e = i >> 1, key = kb + n * 8 + 2 * c + (i & 1);
-          float x = p.cap > 0.f ? fmaf(-2.f * cap_out, __frcp_rn(exp2_unit(s[n][i] * cap_in) + 1.f), cap_out)
-                                : s[n][i] * scale;
-          x = fmaf(-slope[t][e], fabsf(static_cast<float>(place[t][e] - key)), x);
-          x = key < lim[t][e] && key < k1 ? x : -INFINITY;
-          s[n][i] = x;
-          top[e] = fmaxf(top[e], x);
-        }
-      float f[2];
+    for (int t = 0; t < MT; ++t)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 1));
-        top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 2));
-        top[e] = fmaxf(top[e], m[t][e]);
-        f[e] = m[t][e] == top[e] ? 1.f : exp2_unit(m[t][e] - top[e]);
-        m[t][e] = top[e];
+        const int r = t * 16 + g + 8 * e;
+        m[t][e] = -INFINITY;
+        lim[t][e] = r < rows ? min(limit_of(r / group), k1) : 0;
+        place[t][e] = r / group + shift;
+        slope[t][e] = p.slopes != nullptr && r < rows ? p.slopes[hk * group + r % group] * kLog2e : 0.f;
       }
-      uint32_t a[4];
+    const float scale = p.scale * kLog2e;
+    const float cap_in = p.cap > 0.f ? 2.f * scale / p.cap : 0.f, cap_out = p.cap * kLog2e;
+    // ldmatrix rows: lanes 8 i .. 8 i + 7 give the rows of matrix i. K: four 16-byte units of 8 keys; V: the
+    // warp's keys 0-7 and 8-15 of one unit, then of the next; Q: rows 0-7 and 8-15 of one unit, then the next.
+    const int mat = lane >> 3, in = lane & 7;
+    const uint32_t ring = smem_u32(smem);
+    const uint32_t k_lane = (warp * kKeys + in) * 128, v_lane = (warp * kKeys + (mat & 1) * 8 + in) * 128;
+    const uint32_t q_lane = smem_u32(q_s) + (((mat & 1) * 8 + in) * L::kPitch + (mat >> 1) * 8) * 2;
+
+    for (int j = 0; j < steps; ++j) {
+      const int st = j % L::kStages, kb = k0 + j * kStep + warp * kKeys;
+      if (!mbar_wait_warp(&full[st], static_cast<uint32_t>(j / L::kStages) & 1u, kErrWaitFull)) break;
+      const uint32_t k_at = ring + st * L::kStage + k_lane, v_at = ring + st * L::kStage + DC * L::kChunk + v_lane;
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
+      for (int t = 0; t < MT; ++t) {
+        float s[2][4] = {};
+#pragma unroll
+        for (int w = 0; w < DC * 2; ++w) {  // 32 channels: two product steps
+          if (w * 32 >= p.dim) break;
+          uint32_t a0[4], a1[4];
+          ldmatrix4(a0, q_lane + (t * 16 * L::kPitch + w * 32) * 2);
+          ldmatrix4(a1, q_lane + (t * 16 * L::kPitch + w * 32 + 16) * 2);
+#pragma unroll
+          for (int n = 0; n < 2; ++n) {
+            uint32_t b[4];
+            ldmatrix4(b, k_at + (w >> 1) * L::kChunk + n * 8 * 128 + (((w & 1) * 4 + mat) ^ in) * 16);
+            mma<BF16>(s[n], a0, b[0], b[1]);
+            mma<BF16>(s[n], a1, b[2], b[3]);
+          }
+        }
+        // Base-2 scores; s[n][2 e + i] belongs to row g + 8 e and key kb + 8 n + 2 c + i.
+        float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int e = i >> 1, key = kb + n * 8 + 2 * c + (i & 1);
+            float x = p.cap > 0.f ? fmaf(-2.f * cap_out, __frcp_rn(exp2_unit(s[n][i] * cap_in) + 1.f), cap_out)
+                                  : s[n][i] * scale;
+            x = fmaf(-slope[t][e], fabsf(static_cast<float>(place[t][e] - key)), x);
+            x = key < lim[t][e] ? x : -INFINITY;
+            s[n][i] = x;
+            top[e] = fmaxf(top[e], x);
+          }
+        float f[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const float base = m[t][e] == -INFINITY ? 0.f : m[t][e];
-          const float x0 = exp2_unit(s[n][2 * e] - base), x1 = exp2_unit(s[n][2 * e + 1] - base);
-          l[t][e] = n == 0 ? fmaf(l[t][e], f[e], x0 + x1) : l[t][e] + (x0 + x1);
-          a[n * 2 + e] = pack2<BF16>(x0, x1);
+          top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 1));
+          top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 2));
+          top[e] = fmaxf(top[e], m[t][e]);
+          f[e] = m[t][e] == top[e] ? 1.f : exp2_unit(m[t][e] - top[e]);
+          m[t][e] = top[e];
         }
-      if (__any_sync(0xffffffffu, f[0] != 1.f || f[1] != 1.f)) {
+        uint32_t a[4];
 #pragma unroll
-        for (int n = 0; n < DC * 8; ++n)
+        for (int n = 0; n < 2; ++n)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) o[t][n][i] *= f[i >> 1];
-      }
+          for (int e = 0; e < 2; ++e) {
+            const float base = m[t][e] == -INFINITY ? 0.f : m[t][e];
+            const float x0 = exp2_unit(s[n][2 * e] - base), x1 = exp2_unit(s[n][2 * e + 1] - base);
+            l[t][e] = n == 0 ? fmaf(l[t][e], f[e], x0 + x1) : l[t][e] + (x0 + x1);
+            a[n * 2 + e] = pack2<BF16>(x0, x1);
+          }
+        if (__any_sync(0xffffffffu, f[0] != 1.f || f[1] != 1.f)) {
 #pragma unroll
-      for (int w = 0; w < DC; ++w) {
-        if (w * 64 >= p.dim) break;
-        const uint32_t* v0 = reinterpret_cast<const uint32_t*>(&vv[0][w]);
-        const uint32_t* v1 = reinterpret_cast<const uint32_t*>(&vv[1][w]);
-        const uint32_t* v2 = reinterpret_cast<const uint32_t*>(&vv[2][w]);
-        const uint32_t* v3 = reinterpret_cast<const uint32_t*>(&vv[3][w]);
+          for (int n = 0; n < DC * 8; ++n)
 #pragma unroll
-        for (int n = 0; n < 4; ++n) {
-          mma<BF16>(o[t][w * 8 + 2 * n], a, low_halves(v0[n], v1[n]), low_halves(v2[n], v3[n]));
-          mma<BF16>(o[t][w * 8 + 2 * n + 1], a, high_halves(v0[n], v1[n]), high_halves(v2[n], v3[n]));
+            for (int i = 0; i < 4; ++i) o[t][n][i] *= f[i >> 1];
+        }
+#pragma unroll
+        for (int u = 0; u < DC * 8; u += 2) {  // 16 channels: two output tiles
+          if (u * 8 >= p.dim) break;
+          uint32_t b[4];
+          ldmatrix4_trans(b, v_at + (u >> 3) * L::kChunk + (((u & 7) + (mat >> 1)) ^ in) * 16);
+          if (kb + kKeys > k1) {  // keys that are not this document's or this CTA's: anything at all, so zeros
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int key = kb + (i & 1) * 8 + 2 * c;
+              b[i] &= (key < k1 ? 0xffffu : 0u) | (key + 1 < k1 ? 0xffff0000u : 0u);
+            }
+          }
+          mma<BF16>(o[t][u], a, b[0], b[1]);
+          mma<BF16>(o[t][u + 1], a, b[2], b[3]);
         }
       }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty[st]);
     }
   }
 
-  // Each warp's sums to shared memory: thread (g, c) holds channels 16 c .. 16 c + 15 of each chunk.
+  // Each warp's sums to shared memory, where the ring was: every step has been read.
+  __syncthreads();
+  if (warp < kWarps) {
 #pragma unroll
-  for (int t = 0; t < MT; ++t)
+    for (int t = 0; t < MT; ++t)
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      l[t][e] += __shfl_xor_sync(0xffffffffu, l[t][e], 1);
-      l[t][e] += __shfl_xor_sync(0xffffffffu, l[t][e], 2);
-      const int r = t * 16 + g + 8 * e;
-      if (c == 0) {
-        stat_s[(warp * L::kRows + r) * 2] = m[t][e];
-        stat_s[(warp * L::kRows + r) * 2 + 1] = l[t][e];
+      for (int e = 0; e < 2; ++e) {
+        l[t][e] += __shfl_xor_sync(0xffffffffu, l[t][e], 1);
+        l[t][e] += __shfl_xor_sync(0xffffffffu, l[t][e], 2);
+        const int r = t * 16 + g + 8 * e;
+        if (c == 0) {
+          stat_s[(warp * L::kRows + r) * 2] = m[t][e];
+          stat_s[(warp * L::kRows + r) * 2 + 1] = l[t][e];
+        }
+        float* to = o_s + (warp * L::kRows + r) * L::kD + 2 * c;
+#pragma unroll
+        for (int u = 0; u < DC * 8; ++u) *reinterpret_cast<float2*>(to + u * 8) = make_float2(o[t][u][2 * e], o[t][u][2 * e + 1]);
       }
-      float* to = o_s + (static_cast<size_t>(warp) * L::kRows + r) * L::kD + 16 * c;
-#pragma unroll
-      for (int w = 0; w < DC; ++w)
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int n = 0; n < 8; n += 4)
-            *reinterpret_cast<float4*>(to + w * 64 + i * 8 + n) =
-                make_float4(o[t][w * 8 + n][2 * e + i], o[t][w * 8 + n + 1][2 * e + i], o[t][w * 8 + n + 2][2 * e + i],
-                            o[t][w * 8 + n + 3][2 * e + i]);
-    }
-  // The warps' sums into the first one's place, for all rows that exist.
+  }
   __syncthreads();
   auto merge = [&](int r, int d, float& big, float& total) {  // relative to the largest m, 4 channels from d
     big = -INFINITY, total = 0.f;
@@ -263,7 +297,7 @@ __global__ void __launch_bounds__(kThreads) attention_few_kernel(const Attention
     for (int w = 0; w < kWarps; ++w) {
       const float f = exp2_unit(stat_s[(w * L::kRows + r) * 2] - big);
       total = fmaf(f, stat_s[(w * L::kRows + r) * 2 + 1], total);
-      const float4 v = *reinterpret_cast<const float4*>(o_s + (static_cast<size_t>(w) * L::kRows + r) * L::kD + d);
+      const float4 v = *reinterpret_cast<const float4*>(o_s + (w * L::kRows + r) * L::kD + d);
       sum.x = fmaf(f, v.x, sum.x), sum.y = fmaf(f, v.y, sum.y);
       sum.z = fmaf(f, v.z, sum.z), sum.w = fmaf(f, v.w, sum.w);
     }
@@ -288,8 +322,7 @@ __global__ void __launch_bounds__(kThreads) attention_few_kernel(const Attention
     }
     return;
   }
-  // The CTA's sums and statistics take the place of Q and of the first warp's, which only their readers
-  // overwrite: every thread merges into registers first.
+  // The CTA's sums take the first warp's place: every thread merges into registers first.
   constexpr int kEach = (L::kRows * L::kD / 4 + kThreads - 1) / kThreads;
   float4 mine[kEach];
   float2 st[kEach];
@@ -332,7 +365,7 @@ __global__ void __launch_bounds__(kThreads) attention_few_kernel(const Attention
 }
 
 template <int MT, int DC, bool BF16>
-cudaError_t launch(const AttentionParams& p, int splits, cudaStream_t stream) {
+cudaError_t launch(const CUtensorMap& k, const CUtensorMap& v, const AttentionParams& p, int splits, cudaStream_t stream) {
   auto kern = attention_few_kernel<MT, DC, BF16>;
   constexpr int bytes = static_cast<int>(FewSmem<MT, DC>::kBytes);
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
@@ -351,14 +384,15 @@ cudaError_t launch(const AttentionParams& p, int splits, cudaStream_t stream) {
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = splits > 1 ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, kern, p, splits);
+  return cudaLaunchKernelEx(&cfg, kern, k, v, p, splits);
 }
 
 template <bool BF16>
-cudaError_t launch_type(const AttentionParams& p, int splits, cudaStream_t stream) {
+cudaError_t launch_type(const CUtensorMap& k, const CUtensorMap& v, const AttentionParams& p, int splits,
+                        cudaStream_t stream) {
   const int rows = p.heads / p.kv_heads * p.max_q;
-  if (p.dim <= 64) return rows <= 16 ? launch<1, 1, BF16>(p, splits, stream) : launch<2, 1, BF16>(p, splits, stream);
-  return rows <= 16 ? launch<1, 2, BF16>(p, splits, stream) : launch<2, 2, BF16>(p, splits, stream);
+  if (p.dim <= 64) return rows <= 16 ? launch<1, 1, BF16>(k, v, p, splits, stream) : launch<2, 1, BF16>(k, v, p, splits, stream);
+  return rows <= 16 ? launch<1, 2, BF16>(k, v, p, splits, stream) : launch<2, 2, BF16>(k, v, p, splits, stream);
 }
 
 }  // namespace
@@ -368,13 +402,14 @@ bool attention_few_takes(const AttentionParams& p) {
   return static_cast<long long>(p.heads / p.kv_heads) * p.max_q <= 32 && p.documents <= (1 << 24);
 }
 
-cudaError_t launch_attention_few(const AttentionParams& p, bool bf16, cudaStream_t stream) {
-  // Enough CTAs for every SM, as long as each keeps two steps of 128 keys or more.
+cudaError_t launch_attention_few(const CUtensorMap& k, const CUtensorMap& v, const AttentionParams& p, bool bf16,
+                                 cudaStream_t stream) {
+  // Up to two CTAs for every SM, as long as each keeps two steps or more.
   const long long units = static_cast<long long>(p.documents) * p.kv_heads;
   const int sms = device_sm_count();
   int splits = 1;
-  while (splits < 16 && units * splits < sms && p.k_tokens >= splits * 2 * 256) splits *= 2;
-  return bf16 ? launch_type<true>(p, splits, stream) : launch_type<false>(p, splits, stream);
+  while (splits < 16 && units * splits <= sms && p.k_tokens >= splits * 2 * 2 * kStep) splits *= 2;
+  return bf16 ? launch_type<true>(k, v, p, splits, stream) : launch_type<false>(k, v, p, splits, stream);
 }
 
 }  // namespace ctmr

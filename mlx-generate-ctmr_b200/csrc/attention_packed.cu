@@ -479,26 +479,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-// (channel, head, token, document) view of one operand, a box of 64 channels x box_tokens tokens.
-int encode(CUtensorMap* map, const void* base, bool bf16, int dim, int heads, long long tokens, long long docs,
-           long long s_head, long long s_token, long long s_doc, int box_tokens, const char* what) {
-  auto enc = api_tensor_map_encoder();
-  if (enc == nullptr) return api_fail(CTMR_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
-  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(dim), static_cast<cuuint64_t>(heads),
-                              static_cast<cuuint64_t>(tokens), static_cast<cuuint64_t>(docs)};
-  // A stride that addresses nothing (an extent of one) may be anything the encoder takes.
-  const cuuint64_t strides[3] = {static_cast<cuuint64_t>(heads > 1 ? s_head * 2 : 16),
-                                 static_cast<cuuint64_t>(tokens > 1 ? s_token * 2 : 16),
-                                 static_cast<cuuint64_t>(docs > 1 ? s_doc * 2 : 16)};
-  const cuuint32_t box[4] = {64, 1, static_cast<cuuint32_t>(box_tokens), 1}, step[4] = {1, 1, 1, 1};
-  const CUresult r = enc(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
-                         const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) return api_fail(CTMR_ERR_INVALID, "%s's strides cannot be read by TMA (CUresult %d)", what, int(r));
-  return CTMR_OK;
-}
-
 template <int NC, bool CAP, bool BIAS, bool BF16>
 cudaError_t launch_tiles(const Maps& maps, const AttentionParams& p, dim3 grid, cudaStream_t stream) {
   auto kern = attention_tile_kernel<NC, CAP, BIAS, BF16>;
@@ -519,34 +499,56 @@ cudaError_t launch_variant(const Maps& maps, const AttentionParams& p, dim3 grid
 
 }  // namespace
 
+// (channel, head, token, document) view of one operand, a box of 64 channels x box_tokens tokens.
+int encode_tokens_map(CUtensorMap* map, const void* base, bool bf16, int dim, int heads, long long tokens, long long docs,
+           long long s_head, long long s_token, long long s_doc, int box_tokens, const char* what) {
+  auto enc = api_tensor_map_encoder();
+  if (enc == nullptr) return api_fail(CTMR_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
+  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(dim), static_cast<cuuint64_t>(heads),
+                              static_cast<cuuint64_t>(tokens), static_cast<cuuint64_t>(docs)};
+  // A stride that addresses nothing (an extent of one) may be anything the encoder takes.
+  const cuuint64_t strides[3] = {static_cast<cuuint64_t>(heads > 1 ? s_head * 2 : 16),
+                                 static_cast<cuuint64_t>(tokens > 1 ? s_token * 2 : 16),
+                                 static_cast<cuuint64_t>(docs > 1 ? s_doc * 2 : 16)};
+  const cuuint32_t box[4] = {64, 1, static_cast<cuuint32_t>(box_tokens), 1}, step[4] = {1, 1, 1, 1};
+  const CUresult r = enc(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+                         const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return api_fail(CTMR_ERR_INVALID, "%s's strides cannot be read by TMA (CUresult %d)", what, int(r));
+  return CTMR_OK;
+}
+
 size_t attention_packed_workspace(const AttentionParams&) { return 0; }
 
 int launch_attention_packed(const AttentionParams& p, bool bf16, cudaStream_t stream) {
-  if (attention_few_takes(p)) {
-    const cudaError_t e = launch_attention_few(p, bf16, stream);
-    return e == cudaSuccess ? CTMR_OK : api_fail(CTMR_ERR_CUDA, "attention launch: %s", cudaGetErrorString(e));
-  }
   const bool packed = p.q_offsets != nullptr;
   const int docs = packed ? 1 : p.documents;
-  Maps maps;
-  int st = encode(&maps.q, p.q, bf16, p.dim, p.heads, p.q_tokens, docs, p.q_head, p.q_token, p.q_doc, kTile, "q");
+  Maps maps{};
+  int st = CTMR_OK;
+  const bool few = attention_few_takes(p);
+  if (!few)
+    st = encode_tokens_map(&maps.q, p.q, bf16, p.dim, p.heads, p.q_tokens, docs, p.q_head, p.q_token, p.q_doc, kTile, "q");
+  if (st == CTMR_OK && p.k_tokens > 0)  // not read where there are no keys
+    st = encode_tokens_map(&maps.k, p.k, bf16, p.dim, p.kv_heads, p.k_tokens, docs, p.k_head, p.k_token, p.k_doc, kStep,
+                           "k");
+  if (st == CTMR_OK && p.k_tokens > 0)
+    st = encode_tokens_map(&maps.v, p.v, bf16, p.dim, p.kv_heads, p.k_tokens, docs, p.v_head, p.v_token, p.v_doc, kStep,
+                           "v");
   if (st != CTMR_OK) return st;
-  maps.k = maps.v = maps.q;  // not read where there are no keys
-  if (p.k_tokens > 0) {
-    st = encode(&maps.k, p.k, bf16, p.dim, p.kv_heads, p.k_tokens, docs, p.k_head, p.k_token, p.k_doc, kStep, "k");
-    if (st != CTMR_OK) return st;
-    st = encode(&maps.v, p.v, bf16, p.dim, p.kv_heads, p.k_tokens, docs, p.v_head, p.v_token, p.v_doc, kStep, "v");
-    if (st != CTMR_OK) return st;
-  }
-  const long long blocks = packed ? p.q_tokens / kBlock + static_cast<long long>(p.documents)
-                                  : static_cast<long long>(p.documents) * ((p.q_tokens + kBlock - 1) / kBlock);
-  if (blocks > 0x7fffffffLL) return api_fail(CTMR_ERR_UNSUPPORTED, "too many documents");
-  const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(p.heads));
   cudaError_t e;
-  if (p.dim <= 64)
-    e = bf16 ? launch_variant<1, true>(maps, p, grid, stream) : launch_variant<1, false>(maps, p, grid, stream);
-  else
-    e = bf16 ? launch_variant<2, true>(maps, p, grid, stream) : launch_variant<2, false>(maps, p, grid, stream);
+  if (few) {
+    e = launch_attention_few(maps.k, maps.v, p, bf16, stream);
+  } else {
+    const long long blocks = packed ? p.q_tokens / kBlock + static_cast<long long>(p.documents)
+                                    : static_cast<long long>(p.documents) * ((p.q_tokens + kBlock - 1) / kBlock);
+    if (blocks > 0x7fffffffLL) return api_fail(CTMR_ERR_UNSUPPORTED, "too many documents");
+    const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(p.heads));
+    if (p.dim <= 64)
+      e = bf16 ? launch_variant<1, true>(maps, p, grid, stream) : launch_variant<1, false>(maps, p, grid, stream);
+    else
+      e = bf16 ? launch_variant<2, true>(maps, p, grid, stream) : launch_variant<2, false>(maps, p, grid, stream);
+  }
   return e == cudaSuccess ? CTMR_OK : api_fail(CTMR_ERR_CUDA, "attention launch: %s", cudaGetErrorString(e));
 }
 

@@ -62,7 +62,13 @@ int launch_attention_packed(const AttentionParams& p, bool bf16, cudaStream_t st
 
 // The form for few query rows per key head, and whether it takes the call.
 bool attention_few_takes(const AttentionParams& p);
-cudaError_t launch_attention_few(const AttentionParams& p, bool bf16, cudaStream_t stream);
+cudaError_t launch_attention_few(const CUtensorMap& k, const CUtensorMap& v, const AttentionParams& p, bool bf16,
+                                 cudaStream_t stream);
+// A (channel, head, token, document) view of an attention operand in boxes of 64 channels x box_tokens
+// tokens, 128-byte swizzled; a CTMR_ status.
+int encode_tokens_map(CUtensorMap* map, const void* base, bool bf16, int dim, int heads, long long tokens,
+                      long long docs, long long s_head, long long s_token, long long s_doc, int box_tokens,
+                      const char* what);
 
 // ---------------------------------------------------------------- ragged rows
 // offsets[s] clamped into [0, total] (a negative or excessive offset never indexes memory) and, with
