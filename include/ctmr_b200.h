@@ -389,8 +389,7 @@ typedef struct ctmr_attention_desc {
   int causal;
   int max_q;                       /* packed form: no document has more queries (0: not known) */
 } ctmr_attention_desc;
-CTMR_API size_t ctmr_attention_workspace_size(const ctmr_attention_desc* desc);
-CTMR_API int ctmr_attention(const ctmr_attention_desc* desc, void* workspace, size_t workspace_bytes, void* stream);
+CTMR_API int ctmr_attention(const ctmr_attention_desc* desc, void* stream);
 
 /* Device error word (bits 0-4 set when a bounded wait gave up or a launch was inconsistent, bit 5 when
  * offsets, lengths or adapter numbers in device memory were out of range); optionally cleared.

@@ -115,14 +115,17 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4],
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// One CTA: 16 rows of one block of t, all ranks (at most NT * 8). Its eight warps take the input in turn,
+// One CTA: 16 rows of one block of t, all ranks (at most NT * 8). Its sixteen warps take the input in turn,
 // 32 inputs at a time, and add up in shared memory. Both operands come straight from memory, 16 bytes a
 // thread: a thread's eight inputs are dealt to two product steps, the same way for x and down, which
-// permutes the sum's order and nothing else. Memory-bound (x once, down once per 16 rows from L2);
+// permutes the sum's order and nothing else. Memory-bound (x once, down once per 16 rows from L2), and
+// for few rows bound by latency, which is why so many warps share a sum;
 // tcgen05 would want 128 rows and a trip through shared memory for the same bytes.
+constexpr int kInnerWarps = 16;
+
 template <bool BF16, int NT>
-__global__ void __launch_bounds__(256) adapter_inner_kernel(const LinearParams p, const LinearPlan plan) {
-  constexpr int kParts = NT == 16 ? 4 : 8;  // within 48 KB: at 128 ranks the upper four warps go first
+__global__ void __launch_bounds__(kInnerWarps * 32) adapter_inner_kernel(const LinearParams p, const LinearPlan plan) {
+  constexpr int kParts = NT <= 4 ? 16 : (NT == 8 ? 8 : 4);  // sums held at once, within 48 KB
   __shared__ float part[kParts][16][NT * 8 + 1];
   griddep_wait();
   griddep_launch_dependents();  // after the wait: what starts now may read all that came before this kernel
@@ -138,64 +141,64 @@ __global__ void __launch_bounds__(256) adapter_inner_kernel(const LinearParams p
   if (tile < 0 || lo >= hi || adapter < 0 || adapter >= p.adapters) return;  // no such block, or none is read
   uint16_t* inner = static_cast<uint16_t*>(p.inner) +
                     (static_cast<long long>(block) * plan.tile + blockIdx.y * 16) * plan.rank_pad;
-  const bool mine = row0 < hi && row0 + 16 > lo;
-  if (!mine) {
+  if (row0 >= hi || row0 + 16 <= lo) {
     if (plan.split == 0)  // a pair's product takes the whole tile of rows
-      for (int i = threadIdx.x; i < 16 * plan.rank_pad / 8; i += 256)
+      for (int i = threadIdx.x; i < 16 * plan.rank_pad / 8; i += kInnerWarps * 32)
         reinterpret_cast<uint4*>(inner)[i] = make_uint4(0, 0, 0, 0);
     return;
   }
   const int g = lane >> 2, c = lane & 3;
-  const uint16_t* x0 = static_cast<const uint16_t*>(p.x) + static_cast<long long>(min(row0 + g, p.rows - 1)) * p.x_stride;
-  const uint16_t* x1 =
-      static_cast<const uint16_t*>(p.x) + static_cast<long long>(min(row0 + g + 8, p.rows - 1)) * p.x_stride;
+  const bool in0 = row0 + g >= lo && row0 + g < hi, in1 = row0 + g + 8 >= lo && row0 + g + 8 < hi;
+  const uint16_t* x0 = static_cast<const uint16_t*>(p.x) + (row0 + g) * p.x_stride;
+  const uint16_t* x1 = x0 + 8 * p.x_stride;
   const uint16_t* d = static_cast<const uint16_t*>(p.down) + static_cast<long long>(adapter) * p.rank * p.in;
   float acc[NT][4] = {};
-#pragma unroll (NT <= 4 ? 4 : NT <= 8 ? 2 : 1)
-  for (int k = warp * 32 + c * 8; k - c * 8 < p.in; k += 256) {
-    const uint4 zero = make_uint4(0, 0, 0, 0);
-    const bool in = k < p.in;
-    const uint4 a0 = in ? *reinterpret_cast<const uint4*>(x0 + k) : zero;
-    const uint4 a1 = in ? *reinterpret_cast<const uint4*>(x1 + k) : zero;
-    uint4 b[NT];
+  // Loads of kDepth turns are started before the first one's products.
+  constexpr int kDepth = NT <= 2 ? 4 : (NT <= 4 ? 2 : 1), kTurn = kInnerWarps * 32;
+  for (int k0 = warp * 32; k0 < p.in; k0 += kTurn * kDepth) {
+    uint4 a0[kDepth], a1[kDepth], b[kDepth][NT];
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
-      b[n] = in && n * 8 + g < p.rank ? *reinterpret_cast<const uint4*>(d + static_cast<long long>(n * 8 + g) * p.in + k)
-                                      : zero;
-    const uint32_t u0[4] = {a0.x, a1.x, a0.y, a1.y}, u1[4] = {a0.z, a1.z, a0.w, a1.w};
+    for (int i = 0; i < kDepth; ++i) {
+      const int k = k0 + i * kTurn + c * 8;
+      const bool in = k < p.in;
+      const uint4 zero = make_uint4(0, 0, 0, 0);
+      a0[i] = in && in0 ? __ldg(reinterpret_cast<const uint4*>(x0 + k)) : zero;
+      a1[i] = in && in1 ? __ldg(reinterpret_cast<const uint4*>(x1 + k)) : zero;
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      mma_16816<BF16>(acc[n], u0, b[n].x, b[n].y);
-      mma_16816<BF16>(acc[n], u1, b[n].z, b[n].w);
+      for (int n = 0; n < NT; ++n)
+        b[i][n] = in && n * 8 + g < p.rank
+                      ? __ldg(reinterpret_cast<const uint4*>(d + static_cast<long long>(n * 8 + g) * p.in + k)) : zero;
     }
-  }
-  auto put = [&](int w) {
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      part[w][g][n * 8 + 2 * c] = acc[n][0], part[w][g][n * 8 + 2 * c + 1] = acc[n][1];
-      part[w][g + 8][n * 8 + 2 * c] = acc[n][2], part[w][g + 8][n * 8 + 2 * c + 1] = acc[n][3];
-    }
-  };
-  if (kParts == 4) {
-    if (warp >= 4) put(warp - 4);
-    __syncthreads();
-    if (warp < 4) {
+    for (int i = 0; i < kDepth; ++i) {
+      const uint32_t u0[4] = {a0[i].x, a1[i].x, a0[i].y, a1[i].y}, u1[4] = {a0[i].z, a1[i].z, a0[i].w, a1[i].w};
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        acc[n][0] += part[warp][g][n * 8 + 2 * c], acc[n][1] += part[warp][g][n * 8 + 2 * c + 1];
-        acc[n][2] += part[warp][g + 8][n * 8 + 2 * c], acc[n][3] += part[warp][g + 8][n * 8 + 2 * c + 1];
+        mma_16816<BF16>(acc[n], u0, b[i][n].x, b[i][n].y);
+        mma_16816<BF16>(acc[n], u1, b[i][n].z, b[i][n].w);
       }
-      put(warp);
     }
-  } else {
-    put(warp);
   }
-  __syncthreads();
+  // Groups of kParts warps, the last first: each adds what the one after it left in its place.
+#pragma unroll
+  for (int turn = kInnerWarps / kParts - 1; turn >= 0; --turn) {
+    if (warp / kParts == turn) {
+      float(*mine)[NT * 8 + 1] = part[warp % kParts];
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float& at = mine[g + (i >> 1) * 8][n * 8 + 2 * c + (i & 1)];
+          at = turn == kInnerWarps / kParts - 1 ? acc[n][i] : at + acc[n][i];
+        }
+    }
+    __syncthreads();
+  }
   const float scale = p.scale[adapter];
-  for (int i = threadIdx.x; i < 16 * plan.rank_pad; i += 256) {
+  for (int i = threadIdx.x; i < 16 * plan.rank_pad; i += kInnerWarps * 32) {
     const int r = i / plan.rank_pad, n = i - r * plan.rank_pad;
     float v = 0.f;
-    if (row0 + r >= lo && row0 + r < hi && n < p.rank) {
+    if (n < p.rank) {
 #pragma unroll
       for (int q = 0; q < kParts; ++q) v += part[q][r][n];
       v *= scale;
@@ -716,13 +719,14 @@ LinearPlan plan_linear(const LinearParams& p) {
 
 template <bool BF16, int NT>
 cudaError_t launch_inner(const LinearParams& p, const LinearPlan& plan, cudaStream_t stream) {
-  return launch_kernel(adapter_inner_kernel<BF16, NT>, dim3(plan.blocks, plan.tile / 16), dim3(256), 0, stream, p, plan);
+  return launch_kernel(adapter_inner_kernel<BF16, NT>, dim3(plan.blocks, plan.tile / 16), dim3(kInnerWarps * 32),
+                       0, stream, p, plan);
 }
 
 template <typename... KArgs, typename... Args>
-cudaError_t launch_cluster(void (*kern)(KArgs...), unsigned grid, int threads, size_t smem, int cluster,
+cudaError_t launch_cluster(SharedMemoryGrant& grant, void (*kern)(KArgs...), unsigned grid, int threads, size_t smem, int cluster,
                            cudaStream_t stream, Args&&... args) {
-  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  cudaError_t e = grant.ensure(kern, smem);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid);
@@ -738,6 +742,14 @@ cudaError_t launch_cluster(void (*kern)(KArgs...), unsigned grid, int threads, s
   cfg.attrs = attr;
   cfg.numAttrs = cluster > 1 ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...);
+}
+
+template <int BN, bool BF16>
+cudaError_t launch_small(const LinearMaps& maps, const LinearParams& p, const LinearPlan& plan, unsigned grid,
+                         cudaStream_t stream) {
+  static SharedMemoryGrant grant;
+  return launch_cluster(grant, linear_small_kernel<BN, BF16>, grid, kSmallThreads, SmallSmem<BN>::kBytes, plan.split,
+                        stream, maps, p, plan);
 }
 
 template <bool BF16>
@@ -765,22 +777,15 @@ int launch(const LinearParams& p, const LinearPlan& plan, cudaStream_t stream) {
   const long long tiles = static_cast<long long>(plan.row_tiles) * plan.out_tiles;
   if (plan.split == 0) {
     const long long pairs = resident_pairs();
-    e = launch_cluster(linear_pair_kernel<BF16>, static_cast<unsigned>(2 * (tiles < pairs ? tiles : pairs)),
+    static SharedMemoryGrant grant;
+    e = launch_cluster(grant, linear_pair_kernel<BF16>, static_cast<unsigned>(2 * (tiles < pairs ? tiles : pairs)),
                        kPairThreads, kPairBytes, 2, stream, maps, p, plan);
   } else {
     const unsigned grid = static_cast<unsigned>(tiles * plan.split);
-    if (plan.tile == 16)
-      e = launch_cluster(linear_small_kernel<16, BF16>, grid, kSmallThreads, SmallSmem<16>::kBytes, plan.split, stream,
-                         maps, p, plan);
-    else if (plan.tile == 32)
-      e = launch_cluster(linear_small_kernel<32, BF16>, grid, kSmallThreads, SmallSmem<32>::kBytes, plan.split, stream,
-                         maps, p, plan);
-    else if (plan.tile == 64)
-      e = launch_cluster(linear_small_kernel<64, BF16>, grid, kSmallThreads, SmallSmem<64>::kBytes, plan.split, stream,
-                         maps, p, plan);
-    else
-      e = launch_cluster(linear_small_kernel<128, BF16>, grid, kSmallThreads, SmallSmem<128>::kBytes, plan.split,
-                         stream, maps, p, plan);
+    if (plan.tile == 16) e = launch_small<16, BF16>(maps, p, plan, grid, stream);
+    else if (plan.tile == 32) e = launch_small<32, BF16>(maps, p, plan, grid, stream);
+    else if (plan.tile == 64) e = launch_small<64, BF16>(maps, p, plan, grid, stream);
+    else e = launch_small<128, BF16>(maps, p, plan, grid, stream);
   }
   return e == cudaSuccess ? CTMR_OK : api_fail(CTMR_ERR_CUDA, "adapter_linear launch: %s", cudaGetErrorString(e));
 }

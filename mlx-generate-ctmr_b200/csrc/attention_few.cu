@@ -283,7 +283,8 @@ __global__ void __launch_bounds__(kThreads, 2)
         }
         float* to = o_s + (warp * L::kRows + r) * L::kD + 2 * c;
 #pragma unroll
-        for (int u = 0; u < DC * 8; ++u) *reinterpret_cast<float2*>(to + u * 8) = make_float2(o[t][u][2 * e], o[t][u][2 * e + 1]);
+        for (int u = 0; u < DC * 8; ++u)
+          *reinterpret_cast<float2*>(to + u * 8) = make_float2(o[t][u][2 * e], o[t][u][2 * e + 1]);
       }
   }
   __syncthreads();
@@ -365,14 +366,15 @@ __global__ void __launch_bounds__(kThreads, 2)
 }
 
 template <int MT, int DC, bool BF16>
-cudaError_t launch(const CUtensorMap& k, const CUtensorMap& v, const AttentionParams& p, int splits, cudaStream_t stream) {
+cudaError_t launch(const CUtensorMap& k, const CUtensorMap& v, const AttentionParams& p, int splits,
+                   cudaStream_t stream) {
   auto kern = attention_few_kernel<MT, DC, BF16>;
   constexpr int bytes = static_cast<int>(FewSmem<MT, DC>::kBytes);
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (e == cudaSuccess && splits > 8) e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  static SharedMemoryGrant grant;
+  const cudaError_t e = grant.ensure(kern, bytes, true);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(p.documents) * static_cast<unsigned>(splits), static_cast<unsigned>(p.kv_heads));
+  cfg.gridDim = dim3(static_cast<unsigned>(p.documents) * splits, static_cast<unsigned>(p.kv_heads));
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = bytes;
   cfg.stream = stream;
@@ -391,7 +393,8 @@ template <bool BF16>
 cudaError_t launch_type(const CUtensorMap& k, const CUtensorMap& v, const AttentionParams& p, int splits,
                         cudaStream_t stream) {
   const int rows = p.heads / p.kv_heads * p.max_q;
-  if (p.dim <= 64) return rows <= 16 ? launch<1, 1, BF16>(k, v, p, splits, stream) : launch<2, 1, BF16>(k, v, p, splits, stream);
+  if (p.dim <= 64)
+    return rows <= 16 ? launch<1, 1, BF16>(k, v, p, splits, stream) : launch<2, 1, BF16>(k, v, p, splits, stream);
   return rows <= 16 ? launch<1, 2, BF16>(k, v, p, splits, stream) : launch<2, 2, BF16>(k, v, p, splits, stream);
 }
 

@@ -483,7 +483,8 @@ template <int NC, bool CAP, bool BIAS, bool BF16>
 cudaError_t launch_tiles(const Maps& maps, const AttentionParams& p, dim3 grid, cudaStream_t stream) {
   auto kern = attention_tile_kernel<NC, CAP, BIAS, BF16>;
   constexpr int bytes = static_cast<int>(Smem<NC>::kBytes);
-  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  static SharedMemoryGrant grant;
+  const cudaError_t e = grant.ensure(kern, bytes);
   if (e != cudaSuccess) return e;
   return launch_kernel(kern, grid, dim3(kThreads), bytes, stream, maps, p);
 }
@@ -518,8 +519,6 @@ int encode_tokens_map(CUtensorMap* map, const void* base, bool bf16, int dim, in
   if (r != CUDA_SUCCESS) return api_fail(CTMR_ERR_INVALID, "%s's strides cannot be read by TMA (CUresult %d)", what, int(r));
   return CTMR_OK;
 }
-
-size_t attention_packed_workspace(const AttentionParams&) { return 0; }
 
 int launch_attention_packed(const AttentionParams& p, bool bf16, cudaStream_t stream) {
   const bool packed = p.q_offsets != nullptr;

@@ -169,18 +169,10 @@ int ctmr_adapter_linear(const ctmr_adapter_linear_desc* d, void* workspace, size
   return ctmr::launch_adapter_linear(p, d->dtype == CTMR_DTYPE_BF16, static_cast<cudaStream_t>(stream));
 }
 
-size_t ctmr_attention_workspace_size(const ctmr_attention_desc* d) {
+int ctmr_attention(const ctmr_attention_desc* d, void* stream) {
   ctmr::AttentionParams p;
-  return attention_params(d, p) == CTMR_OK && p.q_tokens > 0 ? ctmr::attention_packed_workspace(p) : 0;
-}
-
-int ctmr_attention(const ctmr_attention_desc* d, void* workspace, size_t workspace_bytes, void* stream) {
-  ctmr::AttentionParams p;
-  int st = attention_params(d, p);
+  const int st = attention_params(d, p);
   if (st != CTMR_OK || p.q_tokens == 0) return st;
-  st = check_workspace(ctmr::attention_packed_workspace(p), workspace, workspace_bytes);
-  if (st != CTMR_OK) return st;
-  p.workspace = workspace;
   return ctmr::launch_attention_packed(p, d->dtype == CTMR_DTYPE_BF16, static_cast<cudaStream_t>(stream));
 }
 

@@ -44,6 +44,27 @@ inline bool pdl_enabled() {
   return on;
 }
 
+// A kernel's opt-in to more than 48 KB of shared memory (and, where asked, to clusters of 16), requested
+// once per device: the request takes longer than a small kernel's launch. One static object per kernel.
+class SharedMemoryGrant {
+ public:
+  template <typename Kernel>
+  cudaError_t ensure(Kernel kern, size_t bytes, bool large_clusters = false) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev < 64 && (done_.load(std::memory_order_acquire) >> dev & 1)) return cudaSuccess;
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
+    if (e == cudaSuccess && large_clusters)
+      e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e == cudaSuccess && dev < 64) done_.fetch_or(1ull << dev, std::memory_order_release);
+    return e;
+  }
+
+ private:
+  std::atomic<unsigned long long> done_{0};
+};
+
 template <typename... KArgs, typename... Args>
 cudaError_t launch_kernel(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
                           Args&&... args) {

@@ -51,13 +51,11 @@ struct AttentionParams {
   int heads, kv_heads, dim;
   int causal, max_q;                    // max_q: no document has more queries
   float scale, cap;
-  void* workspace;
 };
 
 cudaError_t launch_rotary(const RotaryParams& p, int dtype, cudaStream_t stream);
 size_t adapter_linear_workspace(const LinearParams& p);
 int launch_adapter_linear(const LinearParams& p, bool bf16, cudaStream_t stream);  // a CTMR_ status
-size_t attention_packed_workspace(const AttentionParams& p);
 int launch_attention_packed(const AttentionParams& p, bool bf16, cudaStream_t stream);  // a CTMR_ status
 
 // The form for few query rows per key head, and whether it takes the call.

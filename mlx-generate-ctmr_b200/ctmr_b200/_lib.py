@@ -61,7 +61,6 @@ EXPORTED_SYMBOLS = (
     "ctmr_rotary_axes",
     "ctmr_adapter_linear_workspace_size",
     "ctmr_adapter_linear",
-    "ctmr_attention_workspace_size",
     "ctmr_attention",
     "ctmr_get_device_error",
     "ctmr_status_string",
@@ -266,8 +265,7 @@ def _load() -> ctypes.CDLL:
         "ctmr_rotary_axes": (i, [ctypes.POINTER(RotaryDesc), vp]),
         "ctmr_adapter_linear_workspace_size": (sz, [ctypes.POINTER(AdapterLinearDesc)]),
         "ctmr_adapter_linear": (i, [ctypes.POINTER(AdapterLinearDesc), vp, sz, vp]),
-        "ctmr_attention_workspace_size": (sz, [ctypes.POINTER(AttentionDesc)]),
-        "ctmr_attention": (i, [ctypes.POINTER(AttentionDesc), vp, sz, vp]),
+        "ctmr_attention": (i, [ctypes.POINTER(AttentionDesc), vp]),
         "ctmr_get_device_error": (i, [ctypes.POINTER(ctypes.c_uint), i]),
         "ctmr_status_string": (ctypes.c_char_p, [i]),
         "ctmr_last_error": (ctypes.c_char_p, []),

@@ -514,16 +514,24 @@ def attention_d32(qkv: torch.Tensor, heads: int, scale: float) -> torch.Tensor:
     return out
 
 
-def _int32_vector(t: torch.Tensor, n: int | None, name: str, like: torch.Tensor) -> torch.Tensor:
-    if t.dtype != torch.int32 or t.dim() != 1 or (n is not None and t.shape[0] != n) or t.device != like.device:
-        raise ValueError(f"{name} must be {'' if n is None else f'{n} '}int32 values on {like.device}; got "
+_HALF_CODES = {BF16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16}
+_FLOAT_CODES = {F32: _lib.DTYPE_F32, **_HALF_CODES}
+
+
+def _device_stream(t: torch.Tensor, name: str) -> tuple[int, int]:
+    """Index of the CUDA device that holds ``t``, which must be the current one, and its current stream.
+    (The raw calls: a small kernel is over before ``torch.cuda.current_stream()`` returns.)"""
+    dev = t.get_device()
+    if dev < 0 or dev != torch._C._cuda_getDevice():
+        raise ValueError(f"{name} must be on the current CUDA device; it is on {t.device}")
+    return dev, torch._C._cuda_getCurrentRawStream(dev)
+
+
+def _int32_vector(t: torch.Tensor, n: int | None, name: str, dev: int) -> torch.Tensor:
+    if t.dtype != torch.int32 or t.dim() != 1 or (n is not None and t.shape[0] != n) or t.get_device() != dev:
+        raise ValueError(f"{name} must be {'' if n is None else f'{n} '}int32 values on cuda:{dev}; got "
                          f"{tuple(t.shape)} {t.dtype} on {t.device}")
-    return t.contiguous()
-
-
-def _strides(t: torch.Tensor) -> tuple[int, ...]:
-    """Strides with those of extents of one, which address nothing, set to zero."""
-    return tuple(0 if n <= 1 else st for n, st in zip(t.shape, t.stride()))
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def axis_frequencies(sections: tuple[int, ...], *, theta: float = 10000.0, device="cuda") -> torch.Tensor:
@@ -542,35 +550,44 @@ def rotary_axes(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor
     (``axis_frequencies``). Pairs are ``(c, c + pairs)``, or ``(2c, 2c + 1)`` when ``interleaved``; channels past
     them are copied. ``inverse`` turns back (the transpose: a gradient's direction). ``out`` may be ``x``.
     """
-    if x.dim() != 3 or x.dtype not in (F32, BF16, torch.float16) or not x.is_cuda:
-        raise ValueError(f"x must be a CUDA (tokens, heads, head_dim) fp32/bf16/fp16 tensor; got {tuple(x.shape)} "
-                         f"{x.dtype} on {x.device}")
-    tokens, heads, dim = x.shape
+    code = _FLOAT_CODES.get(x.dtype)
+    if x.dim() != 3 or code is None:
+        raise ValueError(f"x must be a (tokens, heads, head_dim) fp32/bf16/fp16 tensor; got {tuple(x.shape)} {x.dtype}")
+    dev, stream = _device_stream(x, "x")
+    shape = x.shape
+    tokens, heads, dim = shape
     axes, pairs = len(sections), sum(sections)
     if not 1 <= axes <= _lib.MAX_ROTARY_AXES or min(sections) < 0:
         raise ValueError(f"sections {sections} must name 1 to {_lib.MAX_ROTARY_AXES} axes")
-    if (positions.dim() != 2 or positions.shape != (tokens, axes) or positions.dtype not in (torch.int32, F32)
-            or positions.device != x.device):
-        raise ValueError(f"positions must be ({tokens}, {axes}) int32 or float32 on {x.device}; got "
+    fractional = positions.dtype == F32
+    if (positions.shape != (tokens, axes) or not (fractional or positions.dtype == torch.int32)
+            or positions.get_device() != dev):
+        raise ValueError(f"positions must be ({tokens}, {axes}) int32 or float32 on cuda:{dev}; got "
                          f"{tuple(positions.shape)} {positions.dtype} on {positions.device}")
-    if inv_freq.dtype != F32 or inv_freq.shape != (pairs,) or inv_freq.device != x.device:
-        raise ValueError(f"inv_freq must be {pairs} float32 values on {x.device}")
+    if inv_freq.dtype != F32 or inv_freq.shape != (pairs,) or inv_freq.get_device() != dev:
+        raise ValueError(f"inv_freq must be {pairs} float32 values on cuda:{dev}")
     if axes > 1 and positions.stride(1) != 1:
         positions = positions.contiguous()
     if out is None:
-        out = torch.empty((tokens, heads, dim), dtype=x.dtype, device=x.device)
-    elif out.shape != x.shape or out.dtype != x.dtype or out.device != x.device:
-        raise ValueError(f"out must be like x: {tuple(x.shape)} {x.dtype}")
-    xs, ys = _strides(x), _strides(out)
-    if dim > 1 and (xs[2] != 1 or ys[2] != 1):
+        out = torch.empty(shape, dtype=x.dtype, device=x.device)
+    elif out.shape != shape or out.dtype != x.dtype or out.get_device() != dev:
+        raise ValueError(f"out must be like x: {tuple(shape)} {x.dtype}")
+    xt, xh, xc = x.stride()
+    yt, yh, yc = out.stride()
+    if dim > 1 and (xc != 1 or yc != 1):
         raise ValueError("the channels of x and out must be contiguous")
+    if heads == 1:  # a stride that addresses nothing must not narrow the accesses
+        xh = yh = 0
+    if tokens == 1:
+        xt = yt = 0
     inv_freq = inv_freq.contiguous()
-    desc = _lib.RotaryDesc(
-        x.data_ptr(), out.data_ptr(), _dtype_code(x.dtype, allow_f16=True), tokens, heads, dim, xs[0], xs[1], ys[0],
-        ys[1], positions.data_ptr(), int(positions.dtype == F32), positions.stride(0), inv_freq.data_ptr(), axes,
-        (ctypes.c_int * _lib.MAX_ROTARY_AXES)(*sections), int(interleaved), int(inverse))
-    _count(1)
-    check(LIB.ctmr_rotary_axes(ctypes.byref(desc), _stream()), "rotary_axes")
+    desc = _lib.RotaryDesc(x.data_ptr(), out.data_ptr(), code, tokens, heads, dim, xt, xh, yt, yh,
+                           positions.data_ptr(), fractional, positions.stride(0), inv_freq.data_ptr(), axes,
+                           (*sections, *(0,) * (_lib.MAX_ROTARY_AXES - axes)), interleaved, inverse)
+    LAUNCHES[0] += 1
+    status = LIB.ctmr_rotary_axes(ctypes.byref(desc), stream)
+    if status:
+        check(status, "rotary_axes")
     return out
 
 
@@ -607,53 +624,62 @@ def adapter_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | N
     be fp32), fp32 sums. ``down`` ``(n, rank, in)``, ``up`` ``(n, out, rank)`` and ``scale`` ``(n,)`` come from
     ``stack_adapters``. Without them it is the plain projection. ``out`` must not overlap ``x``.
     """
-    if x.dim() != 2 or x.dtype not in (BF16, torch.float16) or not x.is_cuda:
-        raise ValueError(f"x must be a CUDA (rows, in) bf16/fp16 tensor; got {tuple(x.shape)} {x.dtype} on {x.device}")
+    dtype = x.dtype
+    code = _HALF_CODES.get(dtype)
+    if x.dim() != 2 or code is None:
+        raise ValueError(f"x must be a (rows, in) bf16/fp16 tensor; got {tuple(x.shape)} {dtype}")
+    dev, stream = _device_stream(x, "x")
     rows, inner = x.shape
-    dtype, device = x.dtype, x.device
-    if weight.dim() != 2 or weight.shape[1] != inner or weight.dtype != dtype or weight.device != device:
-        raise ValueError(f"weight must be (out, {inner}) {dtype} on {device}; got {tuple(weight.shape)} {weight.dtype}")
+    if weight.dim() != 2 or weight.shape[1] != inner or weight.dtype != dtype or weight.get_device() != dev:
+        raise ValueError(f"weight must be (out, {inner}) {dtype} on cuda:{dev}; got {tuple(weight.shape)} {weight.dtype}")
     outer = weight.shape[0]
-    if bias is not None and (bias.shape != (outer,) or bias.dtype not in (F32, dtype) or bias.device != device):
-        raise ValueError(f"bias must be {outer} float32 or {dtype} values on {device}")
-    if out is None:
-        out = torch.empty((rows, outer), dtype=dtype, device=device)
-    elif out.shape != (rows, outer) or out.dtype != dtype or out.device != device:
-        raise ValueError(f"out must be ({rows}, {outer}) {dtype} on {device}")
-    for name, t in (("x", x), ("weight", weight), ("out", out)):
-        if t.shape[1] > 1 and t.stride(1) != 1:
-            raise ValueError(f"the columns of {name} must be contiguous")
-    desc = _lib.AdapterLinearDesc()
-    desc.x, desc.x_stride = x.data_ptr(), x.stride(0) if rows > 1 else inner
-    desc.dtype = _dtype_code(dtype, allow_f16=True)
-    desc.rows, desc.in_features, desc.out_features = rows, inner, outer
-    desc.weight, desc.weight_stride = weight.data_ptr(), weight.stride(0) if outer > 1 else inner
-    desc.y, desc.y_stride = out.data_ptr(), out.stride(0) if rows > 1 else outer
+    bias_at, bias_code = None, 0
     if bias is not None:
+        if bias.shape != (outer,) or bias.dtype not in (F32, dtype) or bias.get_device() != dev:
+            raise ValueError(f"bias must be {outer} float32 or {dtype} values on cuda:{dev}")
         bias = bias.contiguous()
-        desc.bias, desc.bias_dtype = bias.data_ptr(), _dtype_code(bias.dtype, allow_f16=True)
-    given = [t is not None for t in (down, up, scale, offsets, index)]
-    if any(given):
-        if not all(given):
+        bias_at, bias_code = bias.data_ptr(), _FLOAT_CODES[bias.dtype]
+    if out is None:
+        out = torch.empty((rows, outer), dtype=dtype, device=x.device)
+    elif out.shape != (rows, outer) or out.dtype != dtype or out.get_device() != dev:
+        raise ValueError(f"out must be ({rows}, {outer}) {dtype} on cuda:{dev}")
+    (xs, xc), (ws, wc), (ys, yc) = x.stride(), weight.stride(), out.stride()
+    if (inner > 1 and (xc != 1 or wc != 1)) or (outer > 1 and yc != 1):
+        raise ValueError("the columns of x, weight and out must be contiguous")
+    adapted = (None, None, None, 0, 0, None, None, 0)
+    if down is None:
+        if up is not None or scale is not None or offsets is not None or index is not None:
+            raise ValueError("down, up, scale, offsets and index come together")
+    else:
+        if up is None or scale is None or offsets is None or index is None:
             raise ValueError("down, up, scale, offsets and index come together")
         n, rank = down.shape[0], down.shape[1] if down.dim() == 3 else 0
         if down.shape != (n, rank, inner) or up.shape != (n, outer, rank) or scale.shape != (n,):
             raise ValueError(f"adapters must be (n, rank, {inner}), (n, {outer}, rank) and (n,); got "
                              f"{tuple(down.shape)}, {tuple(up.shape)}, {tuple(scale.shape)}")
-        if down.dtype != dtype or up.dtype != dtype or scale.dtype != F32 or any(
-                t.device != device for t in (down, up, scale)):
-            raise ValueError(f"down and up must be {dtype}, scale float32, all on {device}")
+        if (down.dtype != dtype or up.dtype != dtype or scale.dtype != F32 or down.get_device() != dev
+                or up.get_device() != dev or scale.get_device() != dev):
+            raise ValueError(f"down and up must be {dtype}, scale float32, all on cuda:{dev}")
         down, up, scale = down.contiguous(), up.contiguous(), scale.contiguous()
-        index = _int32_vector(index, None, "index", x)
-        offsets = _int32_vector(offsets, index.shape[0] + 1, "offsets", x)
-        desc.down, desc.up, desc.scale = down.data_ptr(), up.data_ptr(), scale.data_ptr()
-        desc.adapters, desc.rank = n, rank
-        desc.offsets, desc.index, desc.segments = offsets.data_ptr(), index.data_ptr(), index.shape[0]
-    ws_bytes = LIB.ctmr_adapter_linear_workspace_size(ctypes.byref(desc))
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=device) if ws_bytes else None
-    _count(2 if ws_bytes else 1)
-    check(LIB.ctmr_adapter_linear(ctypes.byref(desc), ws.data_ptr() if ws_bytes else None, ws_bytes, _stream()),
-          "adapter_linear")
+        index = _int32_vector(index, None, "index", dev)
+        segments = index.shape[0]
+        offsets = _int32_vector(offsets, segments + 1, "offsets", dev)
+        adapted = (down.data_ptr(), up.data_ptr(), scale.data_ptr(), n, rank, offsets.data_ptr(), index.data_ptr(),
+                   segments)
+    desc = _lib.AdapterLinearDesc(
+        x.data_ptr(), xs if rows > 1 else inner, code, rows, inner, outer, weight.data_ptr(),
+        ws if outer > 1 else inner, bias_at, bias_code, *adapted, out.data_ptr(), ys if rows > 1 else outer)
+    ref = ctypes.byref(desc)
+    ws_bytes = LIB.ctmr_adapter_linear_workspace_size(ref)
+    if ws_bytes:
+        workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device)
+        LAUNCHES[0] += 2
+        status = LIB.ctmr_adapter_linear(ref, workspace.data_ptr(), ws_bytes, stream)
+    else:
+        LAUNCHES[0] += 1
+        status = LIB.ctmr_adapter_linear(ref, None, 0, stream)
+    if status:
+        check(status, "adapter_linear")
     return out
 
 
@@ -674,75 +700,79 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, q_offsets: t
     multiple of ``kv_heads``. Any strides that are multiples of 8. Returns ``out``, or ``(out, lse)`` with the
     fp32 natural log-sum-exp ``(.., tokens, heads)``.
     """
-    if q.dim() not in (3, 4) or k.dim() != q.dim() or q.dtype not in (BF16, torch.float16) or not q.is_cuda:
-        raise ValueError(f"q must be a CUDA (tokens, heads, head_dim) or (batch, tokens, heads, head_dim) bf16/fp16 "
-                         f"tensor and k alike; got {tuple(q.shape)} {q.dtype} on {q.device}, {tuple(k.shape)}")
-    dtype, device = q.dtype, q.device
-    heads, dim = q.shape[-2:]
-    kv_heads = k.shape[-2]
-    if k.shape != v.shape or k.shape[-1] != dim or k.shape[:-3] != q.shape[:-3] or kv_heads < 1 or heads % kv_heads:
-        raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not belong together")
-    if k.dtype != dtype or v.dtype != dtype or k.device != device or v.device != device:
-        raise ValueError(f"k and v must be {dtype} on {device}")
+    dtype, dims = q.dtype, q.dim()
+    code = _HALF_CODES.get(dtype)
+    if dims not in (3, 4) or code is None:
+        raise ValueError(f"q must be a (tokens, heads, head_dim) or (batch, tokens, heads, head_dim) bf16/fp16 tensor; "
+                         f"got {tuple(q.shape)} {dtype}")
+    dev, stream = _device_stream(q, "q")
+    shape, k_shape = q.shape, k.shape
+    heads, dim, kv_heads = shape[-2], shape[-1], k_shape[-2]
+    if (len(k_shape) != dims or v.shape != k_shape or k_shape[-1] != dim or k_shape[:-3] != shape[:-3] or kv_heads < 1
+            or heads % kv_heads):
+        raise ValueError(f"q {tuple(shape)}, k {tuple(k_shape)} and v {tuple(v.shape)} do not belong together")
+    if k.dtype != dtype or v.dtype != dtype or k.get_device() != dev or v.get_device() != dev:
+        raise ValueError(f"k and v must be {dtype} on cuda:{dev}")
     if out is None:
-        out = torch.empty(q.shape, dtype=dtype, device=device)
-    elif out.shape != q.shape or out.dtype != dtype or out.device != device:
-        raise ValueError(f"out must be {tuple(q.shape)} {dtype} on {device}")
-    desc = _lib.AttentionDesc()
-    if q.dim() == 4:
+        out = torch.empty(shape, dtype=dtype, device=q.device)
+    elif out.shape != shape or out.dtype != dtype or out.get_device() != dev:
+        raise ValueError(f"out must be {tuple(shape)} {dtype} on cuda:{dev}")
+    qo = ko = kl = None
+    documents = 1
+    if dims == 4:
         if q_offsets is not None or k_offsets is not None:
             raise ValueError("offsets belong to packed (tokens, heads, head_dim) tensors")
-        documents = q.shape[0]
+        documents = shape[0]
         if k_lengths is not None:
-            k_lengths = _int32_vector(k_lengths, documents, "k_lengths", q)
-            desc.k_lengths = k_lengths.data_ptr()
-    else:
-        if k_lengths is not None:
-            raise ValueError("k_lengths belong to batched (batch, tokens, heads, head_dim) tensors")
-        documents = 1
-        if q_offsets is not None:
-            q_offsets = _int32_vector(q_offsets, None, "q_offsets", q)
-            documents = q_offsets.shape[0] - 1
-            if k_offsets is None and k.shape[0] != q.shape[0]:
-                raise ValueError("k_offsets are needed where k has other tokens than q")
-            k_offsets = q_offsets if k_offsets is None else _int32_vector(k_offsets, documents + 1, "k_offsets", q)
-            desc.q_offsets, desc.k_offsets = q_offsets.data_ptr(), k_offsets.data_ptr()
-        elif k_offsets is not None:
-            raise ValueError("q_offsets and k_offsets come together")
-    if documents == 0:
-        if q.shape[-3] and q.dim() == 3:
-            raise ValueError("offsets name no documents")
-        lse = torch.empty(q.shape[:-1], dtype=F32, device=device)
-        return (out, lse) if return_lse else out
+            k_lengths = _int32_vector(k_lengths, documents, "k_lengths", dev)
+            kl = k_lengths.data_ptr()
+    elif k_lengths is not None:
+        raise ValueError("k_lengths belong to batched (batch, tokens, heads, head_dim) tensors")
+    elif q_offsets is not None:
+        q_offsets = _int32_vector(q_offsets, None, "q_offsets", dev)
+        documents = q_offsets.shape[0] - 1
+        if k_offsets is None and k_shape[0] != shape[0]:
+            raise ValueError("k_offsets are needed where k has other tokens than q")
+        k_offsets = q_offsets if k_offsets is None else _int32_vector(k_offsets, documents + 1, "k_offsets", dev)
+        qo, ko = q_offsets.data_ptr(), k_offsets.data_ptr()
+    elif k_offsets is not None:
+        raise ValueError("q_offsets and k_offsets come together")
+    if documents < 1:
+        if dims == 3:
+            raise ValueError("q_offsets name no document")
+        return (out, torch.empty(shape[:-1], dtype=F32, device=q.device)) if return_lse else out
+    prefix_at = slopes_at = lse = lse_at = None
     if prefix is not None:
-        prefix = _int32_vector(prefix, documents, "prefix", q)
-        desc.prefix = prefix.data_ptr()
+        prefix = _int32_vector(prefix, documents, "prefix", dev)
+        prefix_at = prefix.data_ptr()
     if slopes is not None:
-        if slopes.dtype != F32 or slopes.shape != (heads,) or slopes.device != device:
-            raise ValueError(f"slopes must be {heads} float32 values on {device}")
+        if slopes.dtype != F32 or slopes.shape != (heads,) or slopes.get_device() != dev:
+            raise ValueError(f"slopes must be {heads} float32 values on cuda:{dev}")
         slopes = slopes.contiguous()
-        desc.slopes = slopes.data_ptr()
-    lse = torch.empty(q.shape[:-1], dtype=F32, device=device) if return_lse else None
-    desc.q, desc.k, desc.v, desc.out = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
-    desc.lse = lse.data_ptr() if return_lse else None
-    desc.dtype = _lib.DTYPE_BF16 if dtype == BF16 else _lib.DTYPE_F16
-    desc.documents, desc.q_tokens, desc.k_tokens = documents, q.shape[-3], k.shape[-3]
-    desc.heads, desc.kv_heads, desc.head_dim = heads, kv_heads, dim
-    for name, t in (("q", q), ("k", k), ("v", v), ("out", out)):
-        st = _strides(t)
-        if st[-1] != 1:
-            raise ValueError(f"the channels of {name} must be contiguous")
-        if len(st) == 4:
-            setattr(desc, name + "_doc_stride", st[0])
-        setattr(desc, name + "_token_stride", st[-3])
-        setattr(desc, name + "_head_stride", st[-2])
-    desc.scale = float(dim) ** -0.5 if scale is None else float(scale)
-    desc.cap, desc.causal, desc.max_q = float(cap), int(causal), int(max_q)
-    ws_bytes = LIB.ctmr_attention_workspace_size(ctypes.byref(desc))
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=device) if ws_bytes else None
-    _count(2 if ws_bytes else 1)
-    check(LIB.ctmr_attention(ctypes.byref(desc), ws.data_ptr() if ws_bytes else None, ws_bytes, _stream()),
-          "attention")
+        slopes_at = slopes.data_ptr()
+    if return_lse:
+        lse = torch.empty(shape[:-1], dtype=F32, device=q.device)
+        lse_at = lse.data_ptr()
+    qs, ks, vs, ys = q.stride(), k.stride(), v.stride(), out.stride()
+    if qs[-1] != 1 or ks[-1] != 1 or vs[-1] != 1 or ys[-1] != 1:
+        raise ValueError("the channels of q, k, v and out must be contiguous")
+    if dims == 3:
+        qs, ks, vs, ys = (0, *qs), (0, *ks), (0, *vs), (0, *ys)
+    if documents == 1 or heads == 1 or kv_heads == 1 or shape[-3] <= 1 or k_shape[-3] <= 1:
+        # a stride over an extent of one addresses nothing, whatever torch calls it
+        def cut(st, tokens, n):
+            return (st[0] if documents > 1 else 0, st[1] if tokens > 1 else 0, st[2] if n > 1 else 0)
+
+        qs, ys = cut(qs, shape[-3], heads), cut(ys, shape[-3], heads)
+        ks, vs = cut(ks, k_shape[-3], kv_heads), cut(vs, k_shape[-3], kv_heads)
+    desc = _lib.AttentionDesc(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse_at, code, documents, shape[-3], k_shape[-3], heads,
+        kv_heads, dim, *qs[:3], *ks[:3], *vs[:3], *ys[:3], qo, ko, kl, prefix_at, slopes_at,
+        dim ** -0.5 if scale is None else scale, cap, causal, max_q)
+    LAUNCHES[0] += 1
+    status = LIB.ctmr_attention(ctypes.byref(desc), stream)
+    if status:
+        check(status, "attention")
     return (out, lse) if return_lse else out
 
 

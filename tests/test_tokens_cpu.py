@@ -113,7 +113,6 @@ def _attention(**kw):
 ])
 def test_attention_validation(change, status):
     d = _attention(**change)
-    assert LIB.ctmr_attention(ctypes.byref(d), None, 0, None) == status
+    assert LIB.ctmr_attention(ctypes.byref(d), None) == status
     if status != _lib.CTMR_OK:
         assert LIB.ctmr_last_error()
-        assert LIB.ctmr_attention_workspace_size(ctypes.byref(d)) == 0
