@@ -27,8 +27,10 @@
 namespace ctmr {
 namespace {
 
-constexpr int kK = 64;                     // inputs per block: one 128-byte swizzled row
-constexpr uint32_t kABytes = 128 * 128;    // 128 outputs x 64 inputs
+// Inputs per block: two halves of one 128-byte swizzled row each. (With one half to a block the issuing
+// warp's own instructions, some 600 clocks a block, took longer than a pair's products, 512.)
+constexpr int kHalf = 64, kK = 2 * kHalf;
+constexpr uint32_t kAHalf = 128 * 128;     // 128 outputs x 64 inputs
 
 struct LinearMaps {
   CUtensorMap x, w, up, inner;
@@ -128,14 +130,29 @@ __global__ void __launch_bounds__(kInnerWarps * 32) adapter_inner_kernel(const L
   constexpr int kParts = NT <= 4 ? 16 : (NT == 8 ? 8 : 4);  // sums held at once, within 48 KB
   __shared__ float part[kParts][16][NT * 8 + 1];
   griddep_wait();
-  griddep_launch_dependents();  // after the wait: what starts now may read all that came before this kernel
+  // From here on the product kernel may start: after the wait, so that it may read all that came before this
+  // kernel. A large product hides all of this; a small one is kept from filling the memory's queues with
+  // W before this kernel's own loads are back (32 rows with 24 adapters of 4,096 x 4,096: 26 us when it starts
+  // at once, see below for after).
+  if (plan.split == 0) griddep_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int block = blockIdx.x;
-  const int s = segment_of_tile(p.offsets, p.segments, plan.tile, block, lane);
+  int s, begin, end, adapter;
+  if (p.segments <= 32) {  // all of them in one round of loads
+    const bool is = lane < p.segments;
+    const int a = is ? p.offsets[lane] : 0, b = is ? p.offsets[lane + 1] : 0, mine = is ? p.index[lane] : -1;
+    const bool ok = lane == 0 || (is && max(a, 0) / plan.tile + lane <= block);
+    s = 31 - __clz(__ballot_sync(0xffffffffu, ok));
+    const int a_s = __shfl_sync(0xffffffffu, a, s), b_s = __shfl_sync(0xffffffffu, b, s);
+    adapter = __shfl_sync(0xffffffffu, mine, s);
+    begin = min(max(a_s, 0), p.rows), end = min(max(b_s, begin), p.rows);
+    if (begin != a_s || end != b_s) flag_error(kErrBadOffsets);
+  } else {
+    s = segment_of_tile(p.offsets, p.segments, plan.tile, block, lane);
+    segment_range(p.offsets, s, p.rows, begin, end);
+    adapter = p.index[s];
+  }
   const int tile = block - s, row0 = tile * plan.tile + blockIdx.y * 16;
-  int begin, end;
-  segment_range(p.offsets, s, p.rows, begin, end);
-  const int adapter = p.index[s];
   if (adapter >= p.adapters) flag_error(kErrBadOffsets);
   const int lo = max(begin, tile * plan.tile), hi = min(end, (tile + 1) * plan.tile);
   if (tile < 0 || lo >= hi || adapter < 0 || adapter >= p.adapters) return;  // no such block, or none is read
@@ -152,9 +169,10 @@ __global__ void __launch_bounds__(kInnerWarps * 32) adapter_inner_kernel(const L
   const uint16_t* x0 = static_cast<const uint16_t*>(p.x) + (row0 + g) * p.x_stride;
   const uint16_t* x1 = x0 + 8 * p.x_stride;
   const uint16_t* d = static_cast<const uint16_t*>(p.down) + static_cast<long long>(adapter) * p.rank * p.in;
+  const float scale = p.scale[adapter];
   float acc[NT][4] = {};
   // Loads of kDepth turns are started before the first one's products.
-  constexpr int kDepth = NT <= 2 ? 4 : (NT <= 4 ? 2 : 1), kTurn = kInnerWarps * 32;
+  constexpr int kDepth = NT <= 2 ? 5 : (NT <= 4 ? 2 : 1), kTurn = kInnerWarps * 32;
   for (int k0 = warp * 32; k0 < p.in; k0 += kTurn * kDepth) {
     uint4 a0[kDepth], a1[kDepth], b[kDepth][NT];
 #pragma unroll
@@ -179,6 +197,7 @@ __global__ void __launch_bounds__(kInnerWarps * 32) adapter_inner_kernel(const L
       }
     }
   }
+  griddep_launch_dependents();
   // Groups of kParts warps, the last first: each adds what the one after it left in its place.
 #pragma unroll
   for (int turn = kInnerWarps / kParts - 1; turn >= 0; --turn) {
@@ -194,7 +213,6 @@ __global__ void __launch_bounds__(kInnerWarps * 32) adapter_inner_kernel(const L
     }
     __syncthreads();
   }
-  const float scale = p.scale[adapter];
   for (int i = threadIdx.x; i < 16 * plan.rank_pad; i += kInnerWarps * 32) {
     const int r = i / plan.rank_pad, n = i - r * plan.rank_pad;
     float v = 0.f;
@@ -213,9 +231,9 @@ constexpr int kSmallThreads = 192;  // warp 0 TMA, warp 1 MMA, warps 2-5 epilogu
 
 template <int BN>
 struct SmallSmem {
-  static constexpr uint32_t kBBytes = BN * 128;
-  static constexpr uint32_t kStageBytes = kABytes + kBBytes;
-  static constexpr int kStages = 196608 / kStageBytes > 10 ? 10 : 196608 / kStageBytes;
+  static constexpr uint32_t kBHalf = BN * 128, kOffB = 2 * kAHalf;
+  static constexpr uint32_t kStageBytes = kOffB + 2 * kBHalf;
+  static constexpr int kStages = 196608 / kStageBytes;
   static constexpr uint32_t kOffBar = kStages * kStageBytes;
   static constexpr uint32_t kBytes = kOffBar + 512 + 1024;  // + barriers + alignment slack
   static_assert(BN * 512u <= kOffBar, "the partial sums fit in the stages");
@@ -241,9 +259,11 @@ __device__ __forceinline__ void store16(void* y, long long i, float v) {
   else static_cast<__half*>(y)[i] = __float2half_rn(v);
 }
 
-__device__ __forceinline__ float ld_cluster(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr));  // in order with the barriers
+__device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"  // volatile: in order with the barriers
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr));
   return v;
 }
 
@@ -289,14 +309,13 @@ __global__ void __launch_bounds__(kSmallThreads, 1)
   if (p.segments == 0) griddep_wait();  // otherwise x, W and the segments are complete already
   griddep_launch_dependents();
 
+  const int kb = (p.in + kK - 1) / kK, k_begin = rank * kb / plan.split, k_end = (rank + 1) * kb / plan.split;
   if (warp == 0) {
     // ------------------------------------------------------------ TMA producer
-    const int kb = (p.in + kK - 1) / kK, k_begin = rank * kb / plan.split, k_end = (rank + 1) * kb / plan.split;
     int it = 0;
     bool ok = true;
     auto stage = [&](int s) {
-      if (it >= S && !mbar_wait_bounded(&empty[s], static_cast<uint32_t>(it / S - 1) & 1u, kErrWaitEmpty)) return false;
-      return *abort_flag == 0;
+      return it < S || mbar_wait_warp(&empty[s], static_cast<uint32_t>(it / S - 1) & 1u, kErrWaitEmpty);
     };
     // Adapter blocks known from the start, so that the last input block knows whether more follow.
     AdapterScan scan;
@@ -309,35 +328,53 @@ __global__ void __launch_bounds__(kSmallThreads, 1)
     };
     bool more = next_mine();
     for (int k = k_begin; ok && k < k_end; ++k, ++it) {
-      const int s = it % S;
+      const int s = it % S, left = p.in - k * kK, halves = left > kHalf ? 2 : 1;
       ok = stage(s);
       if (ok && lane == 0) {
-        info[s] = pack_block(min(kK, p.in - k * kK + 15) / 16, 0, BN, k + 1 == k_end && !more);
-        mbar_arrive_expect_tx(&full[s], L::kStageBytes);
-        tma_load_2d(smem + s * L::kStageBytes, &maps.w, &full[s], k * kK, m0);
-        tma_load_2d(smem + s * L::kStageBytes + kABytes, &maps.x, &full[s], k * kK, r0);
+        uint8_t* at = smem + s * L::kStageBytes;
+        info[s] = pack_block(min(kK, left + 15) / 16, 0, BN, k + 1 == k_end && !more);
+        mbar_arrive_expect_tx(&full[s], halves * (kAHalf + L::kBHalf));
+        for (int h = 0; h < halves; ++h) {
+          tma_load_2d(at + h * kAHalf, &maps.w, &full[s], k * kK + h * kHalf, m0);
+          tma_load_2d(at + L::kOffB + h * L::kBHalf, &maps.x, &full[s], k * kK + h * kHalf, r0);
+        }
       }
       __syncwarp();
-      if (!ok) break;
     }
-    // Every CTA waits here, so this grid cannot end before the inner products' does.
-    if (p.segments > 0) griddep_wait();
+    // Adapter blocks, up to a ring of them at a time: up's part at once, t's after the inner products. Every
+    // CTA waits for those, adapters or not, so this grid cannot end before theirs does.
+    const int halves = plan.rank_pad > kHalf ? 2 : 1;
+    bool waited = p.segments == 0;
     while (ok && more) {
-      const int block = row_tile + seg, a = adapter, c0 = (lo - r0) & ~15, c1 = (hi - r0 + 15) & ~15;
-      more = next_mine();
-      for (int k = 0; ok && k < plan.rank_pad; k += kK, ++it) {
+      const int first = it;
+      int my_block = 0;  // lane i: the block of t of stage first + i
+      while (ok && more && it < first + S) {
         const int s = it % S;
         ok = stage(s);
-        if (ok && lane == 0) {
-          info[s] = pack_block(min(kK, plan.rank_pad - k) / 16, c0, c1 - c0, k + kK >= plan.rank_pad && !more);
-          mbar_arrive_expect_tx(&full[s], L::kStageBytes);
-          tma_load_3d(smem + s * L::kStageBytes, &maps.up, &full[s], k, m0, a);
-          tma_load_2d(smem + s * L::kStageBytes + kABytes, &maps.inner, &full[s], k, block * BN);
+        if (!ok) break;
+        if (lane == it - first) my_block = row_tile + seg;
+        const int a = adapter, c0 = (lo - r0) & ~15, c1 = (hi - r0 + 15) & ~15;
+        more = next_mine();
+        if (lane == 0) {
+          info[s] = pack_block(plan.rank_pad / 16, c0, c1 - c0, !more);
+          mbar_arrive_expect_tx(&full[s], halves * (kAHalf + L::kBHalf));
+          for (int h = 0; h < halves; ++h)
+            tma_load_3d(smem + s * L::kStageBytes + h * kAHalf, &maps.up, &full[s], h * kHalf, m0, a);
         }
         __syncwarp();
-        if (!ok) break;
+        ++it;
+      }
+      if (!waited) griddep_wait();
+      waited = true;
+      for (int i = first; i < it; ++i) {
+        const int block = __shfl_sync(0xffffffffu, my_block, i - first), s = i % S;
+        if (lane == 0)
+          for (int h = 0; h < halves; ++h)
+            tma_load_2d(smem + s * L::kStageBytes + L::kOffB + h * L::kBHalf, &maps.inner, &full[s], h * kHalf, block * BN);
+        __syncwarp();
       }
     }
+    if (!waited) griddep_wait();
     if (lane == 0) {
       if (!ok) *abort_flag = 1;
       for (int i = max(0, it - S); i < it; ++i)  // every issued load lands before the CTA goes on
@@ -348,28 +385,32 @@ __global__ void __launch_bounds__(kSmallThreads, 1)
     // ------------------------------------------------------------ MMA issuer: a warp that stays together
     const uint32_t tm = warp_value(tmem), base = warp_value(smem_u32(smem));
     const uint64_t d0 = smem_desc_kmajor(base, 128);
+    const int plain = warp_value(k_end - k_begin) - 1;  // whole blocks that need no word from the producer
     bool ok = true, last = false;
     for (int it = 0; ok && !last; ++it) {
       const int s = it % S;
-      ok = mbar_wait_warp(&full[s], static_cast<uint32_t>(it / S) & 1u, kErrWaitFull) &&
-           __all_sync(0xffffffffu, *abort_flag == 0);
+      ok = mbar_wait_warp(&full[s], static_cast<uint32_t>(it / S) & 1u, kErrWaitFull);
       if (!ok) break;
       tc_fence_after();
-      const uint32_t b = warp_value(static_cast<uint32_t>(info[s]));
-      const uint32_t steps = b & 15u, col = (b >> 4) & 0xfffu, cols = (b >> 16) & 0x7fffu;
-      last = b >> 31;
+      uint32_t steps = 8, col = 0, cols = BN;
+      if (it >= plain) {
+        const uint32_t b = warp_value(static_cast<uint32_t>(info[s]));
+        steps = b & 15u, col = (b >> 4) & 0xfffu, cols = (b >> 16) & 0x7fffu, last = b >> 31;
+      }
       const uint64_t ad = desc_advance(d0, static_cast<uint32_t>(s) * L::kStageBytes);
-      const uint64_t bd = desc_advance(ad, kABytes + col * 128u);
+      const uint64_t bd = desc_advance(ad, L::kOffB + col * 128u);
       const uint32_t id = idesc_f16(BF16, 128, cols);
       if (elect_one()) {
-        if (steps == 4) {
+        if (steps == 8) {
 #pragma unroll
-          for (uint32_t k = 0; k < 4; ++k)
-            umma_f16(tm + col, desc_advance(ad, k * 32u), desc_advance(bd, k * 32u), id, it > 0 || k > 0 ? 1u : 0u);
+          for (uint32_t k = 0; k < 8; ++k)
+            umma_f16(tm + col, desc_advance(ad, (k >> 2) * kAHalf + (k & 3) * 32u),
+                     desc_advance(bd, (k >> 2) * L::kBHalf + (k & 3) * 32u), id, it > 0 || k > 0 ? 1u : 0u);
         } else {
 #pragma unroll 1
           for (uint32_t k = 0; k < steps; ++k)
-            umma_f16(tm + col, desc_advance(ad, k * 32u), desc_advance(bd, k * 32u), id, it > 0 || k > 0 ? 1u : 0u);
+            umma_f16(tm + col, desc_advance(ad, (k >> 2) * kAHalf + (k & 3) * 32u),
+                     desc_advance(bd, (k >> 2) * L::kBHalf + (k & 3) * 32u), id, it > 0 || k > 0 ? 1u : 0u);
         }
         umma_commit(&empty[s]);
         if (last) umma_commit(done);
@@ -407,23 +448,48 @@ __global__ void __launch_bounds__(kSmallThreads, 1)
   if (plan.split > 1) {
     cluster_sync();
     if (warp >= 2 && !*abort_flag) {
-      const int f = (warp & 3) * 32 + lane, o = m0 + f;
-      const float bias = bias_of(p, BF16, o);
-      const int c_end = min((rank + 1) * BN / plan.split, p.rows - r0);
-      constexpr int kBatch = BN / 8;  // columns read together, at most a rank's share of them
-      for (int c = rank * BN / plan.split; c < c_end; c += kBatch) {
-        float v[kBatch];
+      // Four outputs a thread, a column a warp.
+      const int o = m0 + lane * 4;
+      float bias[4];
 #pragma unroll
-        for (int e = 0; e < kBatch; ++e) v[e] = bias;
+      for (int e = 0; e < 4; ++e) bias[e] = bias_of(p, BF16, o + e);
+      const bool wide = o + 4 <= p.out && p.y_stride % 4 == 0 && reinterpret_cast<uintptr_t>(p.y) % 8 == 0;
+      const int c_end = min((rank + 1) * BN / plan.split, p.rows - r0);
+      constexpr int kBatch = BN < 64 ? 1 : BN / 32;  // columns read together
+      for (int c = rank * BN / plan.split + warp - 2; c < c_end; c += 4 * kBatch) {
+        float4 v[kBatch];
+#pragma unroll
+        for (int e = 0; e < kBatch; ++e) v[e] = make_float4(bias[0], bias[1], bias[2], bias[3]);
 #pragma unroll 4
         for (int z = 0; z < plan.split; ++z) {
-          const uint32_t at = cluster_addr(smem, z) + (c * 128 + f) * 4;
+          const uint32_t at = cluster_addr(smem, z) + (c * 128 + lane * 4) * 4;
 #pragma unroll
-          for (int e = 0; e < kBatch; ++e) v[e] += ld_cluster(at + e * 512);
+          for (int e = 0; e < kBatch; ++e) {
+            const float4 t = ld_cluster4(at + e * 4 * 512);  // past the share: still inside the tile
+            v[e].x += t.x, v[e].y += t.y, v[e].z += t.z, v[e].w += t.w;
+          }
         }
 #pragma unroll
-        for (int e = 0; e < kBatch; ++e)
-          if (o < p.out && c + e < c_end) store16<BF16>(p.y, static_cast<long long>(r0 + c + e) * p.y_stride + o, v[e]);
+        for (int e = 0; e < kBatch; ++e) {
+          if (c + 4 * e >= c_end) break;
+          const long long at = static_cast<long long>(r0 + c + 4 * e) * p.y_stride + o;
+          if (wide) {
+            uint2 h;
+            if constexpr (BF16) {
+              const __nv_bfloat162 h0 = __floats2bfloat162_rn(v[e].x, v[e].y), h1 = __floats2bfloat162_rn(v[e].z, v[e].w);
+              h = make_uint2(*reinterpret_cast<const uint32_t*>(&h0), *reinterpret_cast<const uint32_t*>(&h1));
+            } else {
+              const __half2 h0 = __floats2half2_rn(v[e].x, v[e].y), h1 = __floats2half2_rn(v[e].z, v[e].w);
+              h = make_uint2(*reinterpret_cast<const uint32_t*>(&h0), *reinterpret_cast<const uint32_t*>(&h1));
+            }
+            *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.y) + at) = h;
+          } else {
+            const float u[4] = {v[e].x, v[e].y, v[e].z, v[e].w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (o + i < p.out) store16<BF16>(p.y, at + i, u[i]);
+          }
+        }
       }
     }
     cluster_sync();  // no CTA leaves while another reads its partial tile
@@ -437,8 +503,8 @@ __global__ void __launch_bounds__(kSmallThreads, 1)
 // ---------------------------------------------------------------- product, CTA pairs
 constexpr int kPairThreads = 320;  // warp 0 TMA, warp 1 MMA (first CTA), warps 2-9 epilogue
 constexpr int kPairRows = 256;
-constexpr int kPairStages = 6;
-constexpr uint32_t kPairStageBytes = 2 * kABytes;  // this CTA's 128 outputs and 128 of the rows
+constexpr int kPairStages = 3;
+constexpr uint32_t kPairOffB = 2 * kAHalf, kPairStageBytes = 4 * kAHalf;  // this CTA's 128 outputs and 128 rows
 constexpr uint32_t kPairOffBar = kPairStages * kPairStageBytes;
 constexpr uint32_t kPairBytes = kPairOffBar + 512 + 1024;
 constexpr int kRaster = 8;  // row tiles that are walked together, so that W's and x's tiles meet in L2
@@ -496,16 +562,16 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     m0 = in_group / height * 256;
   };
 
+  const int kb = (p.in + kK - 1) / kK;
   if (warp == 0) {
     // ------------------------------------------------------------ TMA producer (both CTAs)
-    const int kb = (p.in + kK - 1) / kK;
     const uint32_t full0 = cluster_addr(full, 0);
     int it = 0;
     bool ok = true, waited = p.segments == 0;
     auto stage = [&](int s) {
-      if (it >= S && !mbar_wait_bounded(&empty[s], static_cast<uint32_t>(it / S - 1) & 1u, kErrWaitEmpty)) return false;
-      return *abort_flag == 0;
+      return it < S || mbar_wait_warp(&empty[s], static_cast<uint32_t>(it / S - 1) & 1u, kErrWaitEmpty);
     };
+    const int rank_halves = plan.rank_pad > kHalf ? 2 : 1;
     for (int t = pair; ok && t < tiles; t += pairs) {
       int row_tile, m0;
       place(t, row_tile, m0);
@@ -515,43 +581,43 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       scan.begin(p, r0, min(r0 + kPairRows, p.rows), lane);
       int seg, adapter, lo, hi;
       bool more = scan.next(p, seg, adapter, lo, hi);
-      for (int k = 0; ok && k < kb; ++k) {
-        const int s = it % S;
+      for (int k = 0; ok && k < kb; ++k, ++it) {
+        const int s = it % S, left = p.in - k * kK, halves = left > kHalf ? 2 : 1;
         ok = stage(s);
-        if (!ok) break;
-        if (lane == 0) {
+        if (ok && lane == 0) {
+          uint8_t* at = smem + s * kPairStageBytes;
           if (rank == 0) {
-            info[s] = pack_block(min(kK, p.in - k * kK + 15) / 16, 0, kPairRows, k + 1 == kb && !more);
-            mbar_arrive_expect_tx(&full[s], 2u * kPairStageBytes);
+            info[s] = pack_block(min(kK, left + 15) / 16, 0, kPairRows, k + 1 == kb && !more);
+            mbar_arrive_expect_tx(&full[s], halves * 4u * kAHalf);
           }
-          tma_load_2d_pair(smem + s * kPairStageBytes, &maps.w, full0 + 8u * s, k * kK, my_m);
-          tma_load_2d_pair(smem + s * kPairStageBytes + kABytes, &maps.x, full0 + 8u * s, k * kK, my_r);
+          for (int h = 0; h < halves; ++h) {
+            tma_load_2d_pair(at + h * kAHalf, &maps.w, full0 + 8u * s, k * kK + h * kHalf, my_m);
+            tma_load_2d_pair(at + kPairOffB + h * kAHalf, &maps.x, full0 + 8u * s, k * kK + h * kHalf, my_r);
+          }
         }
         __syncwarp();
-        ++it;
       }
       if (!waited) {
         griddep_wait();
         waited = true;
       }
       while (ok && more) {
-        const int row = (row_tile + seg) * kPairRows + static_cast<int>(rank) * 128, a = adapter;
+        const int row = (row_tile + seg) * kPairRows + static_cast<int>(rank) * 128, a = adapter, s = it % S;
         more = scan.next(p, seg, adapter, lo, hi);
-        for (int k = 0; k < plan.rank_pad; k += kK) {
-          const int s = it % S;
-          ok = stage(s);
-          if (!ok) break;
-          if (lane == 0) {
-            if (rank == 0) {
-              info[s] = pack_block(min(kK, plan.rank_pad - k) / 16, 0, kPairRows, k + kK >= plan.rank_pad && !more);
-              mbar_arrive_expect_tx(&full[s], 2u * kPairStageBytes);
-            }
-            tma_load_3d_pair(smem + s * kPairStageBytes, &maps.up, full0 + 8u * s, k, my_m, a);
-            tma_load_2d_pair(smem + s * kPairStageBytes + kABytes, &maps.inner, full0 + 8u * s, k, row);
+        ok = stage(s);
+        if (ok && lane == 0) {
+          uint8_t* at = smem + s * kPairStageBytes;
+          if (rank == 0) {
+            info[s] = pack_block(plan.rank_pad / 16, 0, kPairRows, !more);
+            mbar_arrive_expect_tx(&full[s], rank_halves * 4u * kAHalf);
           }
-          __syncwarp();
-          ++it;
+          for (int h = 0; h < rank_halves; ++h) {
+            tma_load_3d_pair(at + h * kAHalf, &maps.up, full0 + 8u * s, h * kHalf, my_m, a);
+            tma_load_2d_pair(at + kPairOffB + h * kAHalf, &maps.inner, full0 + 8u * s, h * kHalf, row);
+          }
         }
+        __syncwarp();
+        ++it;
       }
     }
     if (!waited) griddep_wait();
@@ -569,34 +635,36 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       const uint32_t id = idesc_f16(BF16, 256, kPairRows);
       const uint32_t tm = warp_value(tmem), base = warp_value(smem_u32(smem));
       const uint64_t d0 = smem_desc_kmajor(base, 128);
+      const int plain = warp_value(kb) - 1;  // whole blocks that need no word from the producer
       int it = 0, lt = 0;
       bool ok = true;
       for (int t = pair; ok && t < tiles; t += pairs, ++lt) {
         const int buf = lt & 1;
         if (lt >= 2) ok = mbar_wait_warp(&acc_empty[buf], static_cast<uint32_t>((lt >> 1) - 1) & 1u, kErrWaitAcc);
-        if (!ok) break;
         bool last = false;
-        for (bool first = true; ok && !last; first = false, ++it) {
+        for (int k = 0; ok && !last; ++k, ++it) {
           const int s = it % S;
-          ok = mbar_wait_warp(&full[s], static_cast<uint32_t>(it / S) & 1u, kErrWaitFull) &&
-               __all_sync(0xffffffffu, *abort_flag == 0);
+          ok = mbar_wait_warp(&full[s], static_cast<uint32_t>(it / S) & 1u, kErrWaitFull);
           if (!ok) break;
           tc_fence_after();
-          const uint32_t b = warp_value(static_cast<uint32_t>(info[s])), steps = b & 15u;
-          last = b >> 31;
+          uint32_t steps = 8;
+          if (k >= plain) {
+            const uint32_t b = warp_value(static_cast<uint32_t>(info[s]));
+            steps = b & 15u, last = b >> 31;
+          }
           const uint64_t ad = desc_advance(d0, static_cast<uint32_t>(s) * kPairStageBytes);
-          const uint64_t bd = desc_advance(ad, kABytes);
+          const uint64_t bd = desc_advance(ad, kPairOffB);
           if (elect_one()) {
-            if (steps == 4) {
+            if (steps == 8) {
 #pragma unroll
-              for (uint32_t k = 0; k < 4; ++k)
-                umma_f16_pair(tm + buf * 256, desc_advance(ad, k * 32u), desc_advance(bd, k * 32u), id,
-                              !first || k > 0 ? 1u : 0u);
+              for (uint32_t i = 0; i < 8; ++i)
+                umma_f16_pair(tm + buf * 256, desc_advance(ad, (i >> 2) * kAHalf + (i & 3) * 32u),
+                              desc_advance(bd, (i >> 2) * kAHalf + (i & 3) * 32u), id, k > 0 || i > 0 ? 1u : 0u);
             } else {
 #pragma unroll 1
-              for (uint32_t k = 0; k < steps; ++k)
-                umma_f16_pair(tm + buf * 256, desc_advance(ad, k * 32u), desc_advance(bd, k * 32u), id,
-                              !first || k > 0 ? 1u : 0u);
+              for (uint32_t i = 0; i < steps; ++i)
+                umma_f16_pair(tm + buf * 256, desc_advance(ad, (i >> 2) * kAHalf + (i & 3) * 32u),
+                              desc_advance(bd, (i >> 2) * kAHalf + (i & 3) * 32u), id, k > 0 || i > 0 ? 1u : 0u);
             }
             umma_commit_pair(&empty[s]);
             if (last) umma_commit_pair(&acc_full[buf]);
@@ -688,7 +756,7 @@ int encode(CUtensorMap* map, const void* base, bool bf16, int rank, long long d0
   if (enc == nullptr) return api_fail(CTMR_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
   const cuuint64_t dims[3] = {static_cast<cuuint64_t>(d0), static_cast<cuuint64_t>(d1), static_cast<cuuint64_t>(d2)};
   const cuuint64_t strides[2] = {static_cast<cuuint64_t>(s1 * 2), static_cast<cuuint64_t>(s2 * 2)};
-  const cuuint32_t box[3] = {kK, static_cast<cuuint32_t>(box_rows), 1}, step[3] = {1, 1, 1};
+  const cuuint32_t box[3] = {kHalf, static_cast<cuuint32_t>(box_rows), 1}, step[3] = {1, 1, 1};
   const CUresult r = enc(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
                          static_cast<cuuint32_t>(rank), const_cast<void*>(base), dims, strides, box, step,
                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
@@ -701,7 +769,9 @@ LinearPlan plan_linear(const LinearParams& p) {
   LinearPlan plan{};
   const int sms = device_sm_count();
   const long long pair_tiles = ((p.out + 255LL) / 256) * ((p.rows + 255LL) / 256);
-  if (pair_tiles * 2 >= sms) {
+  const long long small_tiles = ((p.out + 127LL) / 128) * ((p.rows + 127LL) / 128);
+  const long long waves = (pair_tiles + sms / 2 - 1) / (sms / 2);
+  if (small_tiles >= 128 * waves) {
     plan.tile = kPairRows, plan.split = 0, plan.out_tiles = (p.out + 255) / 256;
   } else {
     plan.tile = p.rows <= 16 ? 16 : (p.rows <= 32 ? 32 : (p.rows <= 64 ? 64 : 128));
@@ -709,7 +779,7 @@ LinearPlan plan_linear(const LinearParams& p) {
     const long long tiles = static_cast<long long>(plan.out_tiles) * ((p.rows + plan.tile - 1) / plan.tile);
     const int kb = (p.in + kK - 1) / kK;
     plan.split = 1;
-    while (plan.split < 8 && tiles * plan.split * 2 <= sms && plan.split * 4 <= kb) plan.split *= 2;
+    while (plan.split < 8 && tiles * plan.split * 2 <= sms && plan.split * 2 <= kb) plan.split *= 2;
   }
   plan.row_tiles = (p.rows + plan.tile - 1) / plan.tile;
   plan.blocks = p.segments > 0 ? plan.row_tiles + p.segments - 1 : 0;
