@@ -130,11 +130,7 @@ __global__ void __launch_bounds__(kInnerWarps * 32) adapter_inner_kernel(const L
   constexpr int kParts = NT <= 4 ? 16 : (NT == 8 ? 8 : 4);  // sums held at once, within 48 KB
   __shared__ float part[kParts][16][NT * 8 + 1];
   griddep_wait();
-  // From here on the product kernel may start: after the wait, so that it may read all that came before this
-  // kernel. A large product hides all of this; a small one is kept from filling the memory's queues with
-  // W before this kernel's own loads are back (32 rows with 24 adapters of 4,096 x 4,096: 26 us when it starts
-  // at once, see below for after).
-  if (plan.split == 0) griddep_launch_dependents();
+  griddep_launch_dependents();  // after the wait: what starts now may read all that came before this kernel
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int block = blockIdx.x;
   int s, begin, end, adapter;
@@ -197,7 +193,6 @@ __global__ void __launch_bounds__(kInnerWarps * 32) adapter_inner_kernel(const L
       }
     }
   }
-  griddep_launch_dependents();
   // Groups of kParts warps, the last first: each adds what the one after it left in its place.
 #pragma unroll
   for (int turn = kInnerWarps / kParts - 1; turn >= 0; --turn) {
@@ -455,7 +450,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1)
       for (int e = 0; e < 4; ++e) bias[e] = bias_of(p, BF16, o + e);
       const bool wide = o + 4 <= p.out && p.y_stride % 4 == 0 && reinterpret_cast<uintptr_t>(p.y) % 8 == 0;
       const int c_end = min((rank + 1) * BN / plan.split, p.rows - r0);
-      constexpr int kBatch = BN < 64 ? 1 : BN / 32;  // columns read together
+      constexpr int kBatch = BN / 16;  // columns read together, a warp's share of them at a split of four
       for (int c = rank * BN / plan.split + warp - 2; c < c_end; c += 4 * kBatch) {
         float4 v[kBatch];
 #pragma unroll
