@@ -3,10 +3,11 @@
 //   s_ij = cap(scale q_i . k_j) - slope_h |p_i - j|,  p_i = i + Lk - Lq,  cap(x) = c tanh(x / c)
 // Every mask leaves a query the keys [0, lim_i): lim_i = Lk, or min(Lk, max(p_i + 1, prefix)) when causal.
 //
-// One CTA takes 256 queries of a document and head, as two tiles of 128 with a softmax warpgroup each
-// (one query per thread). Keys come in steps of 64: S = Q K^T (128 x 64 fp32) lands in TMEM, a
-// thread reads its whole row into registers, turns it into base-2 scores, takes the maximum and writes
-// P = 2^(s - m) as 16-bit pairs over S's own columns, and the tensor core reads P from TMEM for
+// One CTA takes 256 queries of a document and head, as two tiles of 128 with two softmax warpgroups each:
+// a query has two threads, of 32 keys a step each (with one thread of 64 keys the schedulers had two warps
+// to choose from and issued in 47 % of the clocks). Keys come in steps of 64: S = Q K^T (128 x 64 fp32)
+// lands in TMEM, a thread reads its half row into registers, turns it into base-2 scores, takes the maximum,
+// exchanges it with the other half's through shared memory, and writes P = 2^(s - m) as 16-bit pairs over S's own columns, and the tensor core reads P from TMEM for
 // O += P V (V is MN-major in shared memory, as loaded). Each tile has two S buffers, S(j + 1) is ready
 // while the threads work on S(j), and a warp for each tile issues
 //   S(0) S(1) | PV(0) S(2) | PV(1) S(3) | ...
@@ -24,24 +25,28 @@
 namespace ctmr {
 namespace {
 
-constexpr int kThreads = 352;  // warps 0-3 and 4-7: softmax of tiles 0 and 1; 8: TMA; 9, 10: their products
+// Warps 0-15: softmax, in groups of four: tile 0's lower and upper halves of the keys, tile 1's; 16: TMA; 17 and
+// 18: the tiles' products.
+constexpr int kThreads = 608, kTmaWarp = 16;
 constexpr int kTile = 128;     // queries per tile
 constexpr int kStep = 64;      // keys per step
+constexpr int kPart = 32;      // of them per softmax thread
 constexpr int kBlock = 2 * kTile;
 constexpr uint32_t kQChunk = kTile * 128, kKChunk = kStep * 128;  // rows of 64 16-bit channels
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRescale = 8.f;  // log2 of the growth that O and the sum are rescaled for
 
-// NC chunks of 64 channels per row. V in a ring of kStages steps, K, which runs two steps ahead, in one of
-// two more: K(j + 2) then takes the place of K(j - 4), read before step j - 4 freed V's.
+// NC chunks of 64 channels per row. V in a ring of four steps, K, which runs two steps ahead, in one of five:
+// K(j + 2) takes the place of K(j - 3), V(j) of V(j - 4); both are read when step j - 3 is done.
 template <int NC>
 struct Smem {
-  static constexpr int kStages = 4, kKSlots = kStages + 2;
+  static constexpr int kStages = 4, kKSlots = 5;
   static constexpr uint32_t kQBytes = NC * kQChunk, kKBytes = NC * kKChunk;
   static constexpr uint32_t kOffK = 2 * kQBytes;
   static constexpr uint32_t kOffV = kOffK + kKSlots * kKBytes;
   static constexpr uint32_t kOffBar = kOffV + kStages * kKBytes;
-  static constexpr uint32_t kBytes = kOffBar + 256 + 1024;  // + barriers + alignment slack
+  static constexpr uint32_t kOffMax = kOffBar + 256;        // [step parity][tile][half][query] maxima
+  static constexpr uint32_t kBytes = kOffMax + 4096 + 1024;  // + alignment slack
   static_assert(kBytes <= 227 * 1024, "shared memory of an SM");
 };
 
@@ -188,7 +193,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int i = 0; i < 4; ++i) {
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], kTile);
+      mbar_init(&p_full[i], 2 * kTile);
     }
     for (int i = 0; i < L::kStages; ++i) {
       mbar_init(&full[i], 1);
@@ -198,7 +203,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     *abort_flag = 0;
     fence_barrier_init();
   }
-  if (warp == 9) {
+  if (warp == kTmaWarp + 1) {
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
@@ -215,7 +220,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int n0 = steps_of(0), n1 = steps_of(1), n_max = max(n0, n1);
   const int tail = w.k_len - (n_max - 1) * kStep;  // the document's keys in the last step, if fewer than 64
 
-  if (warp == 8) {
+  if (warp == kTmaWarp) {
     // ------------------------------------------------------------ TMA producer
     if (lane == 0 && n_max > 0) {
       tma_prefetch_desc(&maps.q);
@@ -241,8 +246,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       int j = 0;
       for (; j < n_max && !*abort_flag; ++j) {
-        const int s = j % L::kStages, use = j / L::kStages;
-        if (use > 0 && !mbar_wait_bounded(&empty[s], static_cast<uint32_t>(use - 1) & 1u, kErrWaitEmpty)) break;
+        const int s = j % L::kStages, done = j - 3;
+        if (done >= 0 && !mbar_wait_bounded(&empty[done % L::kStages], static_cast<uint32_t>(done / L::kStages) & 1u,
+                                            kErrWaitEmpty))
+          break;
         const bool more = j + 2 < n_max;
         mbar_arrive_expect_tx(&full[s], more ? 2 * L::kKBytes : L::kKBytes);
         load(&maps.v, L::kOffV + s * L::kKBytes, &full[s], j);
@@ -268,9 +275,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(v_fixed);
     }
-  } else if (warp >= 9) {
+  } else if (warp > kTmaWarp) {
     // ------------------------------------------------------------ MMA issuer of tile t: a warp that stays together
-    const int t = warp - 9;
+    const int t = warp - kTmaWarp - 1;
     const int dk = warp_value((p.dim + 15) / 16), n = warp_value(t == 0 ? n0 : n1), last = warp_value(n_max);
     const bool fix = warp_value(tail) < kStep;
     const uint32_t tm_s = warp_value(tmem + t * 128), tm_o = tm_s + 256;
@@ -341,78 +348,75 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (!ok) *abort_flag = 1;
     __syncwarp();
   } else {
-    // ------------------------------------------------------------ softmax, one query per thread
-    const int t = warp >> 2;
-    const int i = w.first + t * kTile + (warp & 3) * 32 + lane;  // the query inside the document
+    // ------------------------------------------------------------ softmax, two threads per query
+    const int t = warp >> 3, half = (warp >> 2) & 1;
+    const int row = (warp & 3) * 32 + lane, i = w.first + t * kTile + row;  // the query inside the document
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t t_o = tmem + lanes + 256 + t * 128;
     const int n = t == 0 ? n0 : n1;
+    float* maxima = reinterpret_cast<float*>(smem + L::kOffMax) + t * 2 * kTile + row;  // + parity * 512 + half * 128
+    const int pair_bar = 1 + t * 4 + (warp & 3);  // the two warps of these queries
+    auto meet = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(pair_bar) : "memory"); };
     auto wait_s = [&](int j) {
       const bool ok = mbar_wait_bounded(&s_full[t * 2 + (j & 1)], static_cast<uint32_t>(j >> 1) & 1u, kErrWaitAcc);
       tc_fence_after();
-      return ok && !*abort_flag;
+      return ok;
     };
-    const int lim = limit_of(p, w, i), place = i + w.k_len - w.q_len;
+    const int lim = limit_of(p, w, i) - half * kPart, place = i + w.k_len - w.q_len - half * kPart;
     const float scale = p.scale * kLog2e;
     const float cap_in = CAP ? 2.f * scale / p.cap : 0.f, cap_out = CAP ? p.cap * kLog2e : 0.f;
     const float slope = BIAS ? p.slopes[h] * kLog2e : 0.f;
     const float unit = CAP || BIAS ? 1.f : scale;  // what turns s below into base-2 scores
-    float m = -INFINITY, l = 0.f;                  // m: what P is relative to; the maximum or up to 2^8 below
+    float m = -INFINITY, l = 0.f;  // m: what P is relative to; the maximum or up to 2^8 below; l: of this half
     bool ok = true;
     for (int j = 0; j < n; ++j) {
-      ok = wait_s(j);
-      if (!ok) break;
+      ok = ok && wait_s(j);  // (on a failure the loop goes on without waiting: the other half meets here)
       const uint32_t t_s = tmem + lanes + t * 128 + (j & 1) * 64;
-      float s[kStep];
-#pragma unroll
-      for (int c = 0; c < kStep; c += 32) tmem_ld32(t_s + c, s + c);
+      float s[kPart];
+      tmem_ld32(t_s + half * kPart, s);
       tmem_ld_wait();
-#pragma unroll
-      for (int c = 0; c < kStep; c += 32) tmem_ld_fence(s + c);
+      tmem_ld_fence(s);
       if constexpr (CAP) {
         // c tanh(x / c) = c - 2 c / (e^(2 x / c) + 1): two operations of the exponential unit, error c 2^-22.
 #pragma unroll
-        for (int c = 0; c < kStep; ++c) s[c] = fmaf(-2.f * cap_out, rcp_unit(exp2_unit(s[c] * cap_in) + 1.f), cap_out);
+        for (int c = 0; c < kPart; ++c) s[c] = fmaf(-2.f * cap_out, rcp_unit(exp2_unit(s[c] * cap_in) + 1.f), cap_out);
       }
       if constexpr (BIAS) {
         // s - slope |at - c|: away from the query's own place the distance is linear in c.
         const int at = place - j * kStep;
-        const float2 mul = make_float2(CAP ? 1.f : scale, CAP ? 1.f : scale);
-        if (__all_sync(0xffffffffu, at >= kStep - 1 || at <= 0)) {
+        const float mul = CAP ? 1.f : scale;
+        if (__all_sync(0xffffffffu, at >= kPart - 1 || at <= 0)) {
           const float step = at > 0 ? slope : -slope, from = -step * static_cast<float>(at);
-          const float2 step2 = make_float2(step, step), from2 = make_float2(from, from);
 #pragma unroll
-          for (int c = 0; c < kStep; c += 2) {
-            const float2 b = fma2(make_float2(static_cast<float>(c), static_cast<float>(c + 1)), step2, from2);
-            const float2 x = fma2(make_float2(s[c], s[c + 1]), mul, b);
-            s[c] = x.x, s[c + 1] = x.y;
-          }
+          for (int c = 0; c < kPart; ++c) s[c] = fmaf(s[c], mul, fmaf(static_cast<float>(c), step, from));
         } else {
 #pragma unroll
-          for (int c = 0; c < kStep; ++c) s[c] = fmaf(-slope, fabsf(static_cast<float>(at - c)), s[c] * mul.x);
+          for (int c = 0; c < kPart; ++c) s[c] = fmaf(-slope, fabsf(static_cast<float>(at - c)), s[c] * mul);
         }
       }
       const int left = lim - j * kStep;
-      if (left < kStep) {
+      if (left < kPart) {
 #pragma unroll
-        for (int c = 0; c < kStep; ++c) s[c] = c < left ? s[c] : -INFINITY;
+        for (int c = 0; c < kPart; ++c) s[c] = c < left ? s[c] : -INFINITY;
       }
-      float mx[8];
+      float mx[4];
 #pragma unroll
-      for (int c = 0; c < 8; ++c) mx[c] = s[c];
+      for (int c = 0; c < 4; ++c) mx[c] = s[c];
 #pragma unroll
-      for (int c = 8; c < kStep; ++c) mx[c & 7] = fmaxf(mx[c & 7], s[c]);
-      const float top = unit * fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])),
-                                     fmaxf(fmaxf(mx[4], mx[5]), fmaxf(mx[6], mx[7])));
+      for (int c = 4; c < kPart; ++c) mx[c & 3] = fmaxf(mx[c & 3], s[c]);
+      const float mine = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+      // The halves meet: the maximum of both, and P may take the place of S, which both have read.
+      maxima[(j & 1) * 512 + half * kTile] = mine;
+      meet();
+      const float top = unit * fmaxf(mine, maxima[(j & 1) * 512 + (half ^ 1) * kTile]);
       const bool grow = top > m + kRescale || (m == -INFINITY && top > m);
       if (__any_sync(0xffffffffu, grow)) {
         const float f = grow ? exp2_unit(m - top) : 1.f;
         if (grow) m = top;
         l *= f;
         if (j > 0) {  // PV(j - 1) has to be done; nothing writes O then until P(j) is handed over
-          ok = wait_s(j + 1);
-          if (!ok) break;
-          for (int c = 0; c < p.dim; c += 32) {
+          ok = ok && wait_s(j + 1);
+          for (int c = half * 32; c < p.dim; c += 64) {
             float o[32];
             tmem_ld32(t_o + c, o);
             tmem_ld_wait();
@@ -426,31 +430,36 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       const float base = m == -INFINITY ? 0.f : -m;
       const float2 u2 = make_float2(unit, unit), b2 = make_float2(base, base);
-      float2 sum[4] = {};
-      uint32_t r[kStep / 2];
+      float2 sum[2] = {};
+      uint32_t r[kPart / 2];
 #pragma unroll
-      for (int e = 0; e < kStep / 2; ++e) {
+      for (int e = 0; e < kPart / 2; ++e) {
         float2 x = fma2(make_float2(s[2 * e], s[2 * e + 1]), u2, b2);
         // One pair in four on the FMA pipe, the others on the exponential unit (16 a clock per SM,
         // half of the time of a step's two products at head size 128 and more below it).
         if ((e & 3) == 3) x = exp2_poly(x);
         else x = make_float2(exp2_unit(x.x), exp2_unit(x.y));
-        sum[e & 3] = add2(sum[e & 3], x);
+        sum[e & 1] = add2(sum[e & 1], x);
         r[e] = pack2<BF16>(x.x, x.y);
       }
-      tmem_st32(t_s, r);
+      tmem_st16(t_s + half * (kPart / 2), r);
       tmem_st_wait();
       tc_fence_before();
       mbar_arrive(&p_full[t * 2 + (j & 1)]);
-      sum[0] = add2(add2(sum[0], sum[1]), add2(sum[2], sum[3]));
+      sum[0] = add2(sum[0], sum[1]);
       l += sum[0].x + sum[0].y;
     }
-    if (ok && n > 0) ok = wait_s(n + 1);  // PV(n - 1)
+    if (n > 0) {
+      ok = ok && wait_s(n + 1);  // PV(n - 1)
+      maxima[(n & 1) * 512 + half * kTile] = l;
+      meet();
+      l += maxima[(n & 1) * 512 + (half ^ 1) * kTile];
+    }
     if (!ok) *abort_flag = 1;
     const bool some = m != -INFINITY;  // a query that saw nothing gets zeros
     const float inv = some ? 1.f / l : 0.f;
     uint16_t* out = static_cast<uint16_t*>(p.out) + w.map_doc * p.o_doc + (w.q_row + i) * p.o_token + h * p.o_head;
-    for (int c = 0; c < p.dim; c += 32) {
+    for (int c = half * 32; c < p.dim; c += 64) {
       float o[32];
       if (n > 0) {
         tmem_ld32(t_o + c, o);
@@ -467,13 +476,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         *reinterpret_cast<uint4*>(out + c + e) = v;
       }
     }
-    if (p.lse != nullptr && i < w.q_len)
+    if (p.lse != nullptr && half == 0 && i < w.q_len)
       p.lse[(w.row0 + i) * p.heads + h] = some ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY;
   }
 
   tc_fence_before();
   __syncthreads();
-  if (warp == 9) {
+  if (warp == kTmaWarp + 1) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
