@@ -3,18 +3,24 @@
 //   s_ij = cap(scale q_i . k_j) - slope_h |p_i - j|,  p_i = i + Lk - Lq,  cap(x) = c tanh(x / c)
 // Every mask leaves a query the keys [0, lim_i): lim_i = Lk, or min(Lk, max(p_i + 1, prefix)) when causal.
 //
-// One CTA takes 256 queries of a document and head, as two tiles of 128 with two softmax warpgroups each:
-// a query has two threads, of 32 keys a step each (with one thread of 64 keys the schedulers had two warps
-// to choose from and issued in 47 % of the clocks). Keys come in steps of 64: S = Q K^T (128 x 64 fp32)
+// Queries come in tiles of 128 of a document and head. Head sizes up to 64: a CTA takes one tile and two CTAs
+// share an SM; above: a CTA takes two tiles, which share its K and V in shared memory. A query has two
+// softmax threads of 32 keys a step each (with one thread of 64 keys the schedulers had two warps to choose
+// from and issued in 47 % of the clocks). Keys come in steps of 64: S = Q K^T (128 x 64 fp32)
 // lands in TMEM, a thread reads its half row into registers, turns it into base-2 scores, takes the maximum,
-// exchanges it with the other half's through shared memory, and writes P = 2^(s - m) as 16-bit pairs over S's own columns, and the tensor core reads P from TMEM for
-// O += P V (V is MN-major in shared memory, as loaded). Each tile has two S buffers, S(j + 1) is ready
-// while the threads work on S(j), and a warp for each tile issues
+// exchanges it with the other half's through shared memory, and writes P = 2^(s - m) as 16-bit pairs over S's
+// own columns, and the tensor core reads P from TMEM for O += P V (V is MN-major in shared memory, as
+// loaded). Each tile has two S buffers, S(j + 1) is ready while the threads work on S(j), and a warp for each
+// tile issues
 //   S(0) S(1) | PV(0) S(2) | PV(1) S(3) | ...
 // O stays in TMEM; it is
 // rescaled (by the softmax threads, which hold m) only where a row's maximum has grown by more than 2^8
 // since the last time: until then P may exceed one, up to 2^8, which neither 16-bit type minds, and
 // the sum of P is kept in fp32 with the same m.
+//
+// With a distance bias the steps are visited from the queries' own place outwards, first towards the first
+// key, then towards the last: in order of keys the maximum grew with every step that came nearer, and the
+// tiles at the end of 8,192 tokens took 205 us where those at the start took 131.
 #include <cmath>
 
 #include "capi_internal.cuh"
@@ -25,29 +31,31 @@
 namespace ctmr {
 namespace {
 
-// Warps 0-15: softmax, in groups of four: tile 0's lower and upper halves of the keys, tile 1's; 16: TMA; 17 and
-// 18: the tiles' products.
-constexpr int kThreads = 608, kTmaWarp = 16;
 constexpr int kTile = 128;     // queries per tile
 constexpr int kStep = 64;      // keys per step
 constexpr int kPart = 32;      // of them per softmax thread
-constexpr int kBlock = 2 * kTile;
 constexpr uint32_t kQChunk = kTile * 128, kKChunk = kStep * 128;  // rows of 64 16-bit channels
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRescale = 8.f;  // log2 of the growth that O and the sum are rescaled for
 
-// NC chunks of 64 channels per row. V in a ring of four steps, K, which runs two steps ahead, in one of five:
-// K(j + 2) takes the place of K(j - 3), V(j) of V(j - 4); both are read when step j - 3 is done.
+// NC chunks of 64 channels per row (two above 64 channels), as many query tiles. V in a ring of four steps, K,
+// which runs two steps ahead, in one of five: K(j + 2) takes the place of K(j - 3), V(j) of V(j - 4); both are
+// read when step j - 3 is done.
 template <int NC>
-struct Smem {
+struct Layout {
+  static constexpr int kTiles = NC, kBlock = kTiles * kTile;
+  // Softmax warps by tile, half of the keys and quarter of the queries; then TMA; then each tile's products.
+  static constexpr int kTmaWarp = 8 * kTiles, kThreads = (kTmaWarp + 1 + kTiles) * 32;
+  static constexpr int kCtas = NC == 1 ? 2 : 1;              // per SM
+  static constexpr uint32_t kTmem = 256 * kTiles, kTmemO = 128 * kTiles;  // S of each tile, then O of each
   static constexpr int kStages = 4, kKSlots = 5;
   static constexpr uint32_t kQBytes = NC * kQChunk, kKBytes = NC * kKChunk;
-  static constexpr uint32_t kOffK = 2 * kQBytes;
+  static constexpr uint32_t kOffK = kTiles * kQBytes;
   static constexpr uint32_t kOffV = kOffK + kKSlots * kKBytes;
   static constexpr uint32_t kOffBar = kOffV + kStages * kKBytes;
-  static constexpr uint32_t kOffMax = kOffBar + 256;        // [step parity][tile][half][query] maxima
-  static constexpr uint32_t kBytes = kOffMax + 4096 + 1024;  // + alignment slack
-  static_assert(kBytes <= 227 * 1024, "shared memory of an SM");
+  static constexpr uint32_t kOffMax = kOffBar + 256;  // [step parity][tile][half][query] maxima
+  static constexpr uint32_t kBytes = kOffMax + 2048 * kTiles + 1024;  // + alignment slack
+  static_assert(kCtas * (kBytes + 1024) <= 228 * 1024, "shared memory of an SM");
 };
 
 struct Maps {
@@ -104,6 +112,34 @@ __device__ __forceinline__ float2 exp2_poly(float2 x) {
   return p;
 }
 
+// c tanh(x / c) of 32 scores. Scores that stay below 3/4 of the cap take an odd polynomial (x / c times a quintic
+// in its square, least maximum relative error on [0, 3/4], 9e-9, 1.5e-7 with fp32's roundings); where
+// any lane's is larger, c - 2 c / (e^(2 x / c) + 1), two operations of the exponential unit each. (Four sequences
+// with a cap of 30: 118 us with the latter alone.)
+__device__ __forceinline__ void cap_scores(float (&s)[32], float in, float out) {
+  float big = 0.f;
+#pragma unroll
+  for (int c = 0; c < 32; ++c) big = fmaxf(big, fabsf(s[c]));
+  if (__all_sync(0xffffffffu, big * in <= 0.75f)) {
+    const float2 zero = make_float2(0.f, 0.f), in2 = make_float2(in, in), out2 = make_float2(out, out);
+#pragma unroll
+    for (int c = 0; c < 32; c += 2) {
+      const float2 x = fma2(make_float2(s[c], s[c + 1]), in2, zero), u = fma2(x, x, zero);
+      float2 q = fma2(make_float2(-0.004565585377374933f, -0.004565585377374933f), u,
+                      make_float2(0.01937127571384739f, 0.01937127571384739f));
+      q = fma2(q, u, make_float2(-0.05324007003342396f, -0.05324007003342396f));
+      q = fma2(q, u, make_float2(0.13323310160326868f, 0.13323310160326868f));
+      q = fma2(q, u, make_float2(-0.33332824343712386f, -0.33332824343712386f));
+      q = fma2(q, u, make_float2(0.9999999911877767f, 0.9999999911877767f));
+      q = fma2(q, fma2(x, out2, zero), zero);
+      s[c] = q.x, s[c + 1] = q.y;
+    }
+  } else {
+#pragma unroll
+    for (int c = 0; c < 32; ++c) s[c] = fmaf(-2.f * out, rcp_unit(exp2_unit(2.f * kLog2e * in * s[c]) + 1.f), out);
+  }
+}
+
 template <bool BF16>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
   if constexpr (BF16) {
@@ -130,6 +166,7 @@ __device__ __forceinline__ int limit_of(const AttentionParams& p, const Place& w
   return min(w.k_len, max(max(i + w.k_len - w.q_len + 1, w.prefix), 0));
 }
 
+template <int kBlock>
 __device__ __forceinline__ bool find_place(const AttentionParams& p, int id, int lane, Place& w) {
   int tile;
   if (p.q_offsets != nullptr) {
@@ -162,9 +199,10 @@ __device__ __forceinline__ bool find_place(const AttentionParams& p, int id, int
 }
 
 template <int NC, bool CAP, bool BIAS, bool BF16>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(Layout<NC>::kThreads, Layout<NC>::kCtas)
     attention_tile_kernel(const __grid_constant__ Maps maps, const AttentionParams p) {
-  using L = Smem<NC>;
+  using L = Layout<NC>;
+  constexpr int kTiles = L::kTiles, kTmaWarp = L::kTmaWarp;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bar = reinterpret_cast<uint64_t*>(smem + L::kOffBar);
@@ -177,110 +215,128 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* empty = full + L::kStages;     // [kStages] both read by both tiles
   uint64_t* v_fixed = empty + L::kStages;  // the last V step has zeros past the document
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(v_fixed + 1);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int h = blockIdx.y, hk = h / (p.heads / p.kv_heads);
   griddep_wait();
   griddep_launch_dependents();
   Place w;
-  if (!find_place(p, blockIdx.x, lane, w)) return;  // the same answer in every warp
+  if (!find_place<L::kBlock>(p, blockIdx.x, lane, w)) return;  // the same answer in every warp
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&q_full[i], 1);
       mbar_init(&k_first[i], 1);
     }
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 2 * kTiles; ++i) {
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i], 2 * kTile);
     }
     for (int i = 0; i < L::kStages; ++i) {
       mbar_init(&full[i], 1);
-      mbar_init(&empty[i], 2);
+      mbar_init(&empty[i], kTiles);
     }
     mbar_init(v_fixed, 1);
-    *abort_flag = 0;
     fence_barrier_init();
   }
   if (warp == kTmaWarp + 1) {
-    tmem_alloc(tmem_slot, 512);
+    tmem_alloc(tmem_slot, L::kTmem);
     tmem_relinquish();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;  // S0a S0b S1a S1b at columns 0, 64, .. (P over them), O0 O1 at 256, 384
+  const uint32_t tmem = *tmem_slot;  // tile t: S at columns 128 t and 128 t + 64 (P over them), O at kTmemO + 128 t
 
-  // Steps of each query tile: the keys that its last query sees.
+  // Steps of each query tile: the keys that its last query sees. (With a bias all take the longest's, and
+  // find the rest masked: the order below starts at the far end of it.)
   auto steps_of = [&](int t) {
     const int last = min(w.q_len - 1, w.first + (t + 1) * kTile - 1);
     return last < w.first + t * kTile ? 0 : (limit_of(p, w, last) + kStep - 1) / kStep;
   };
-  const int n0 = steps_of(0), n1 = steps_of(1), n_max = max(n0, n1);
-  const int tail = w.k_len - (n_max - 1) * kStep;  // the document's keys in the last step, if fewer than 64
+  int n0 = steps_of(0), n1 = kTiles == 2 ? steps_of(1) : 0;
+  const int n_max = max(n0, n1);
+  if (BIAS) n0 = n_max, n1 = n1 > 0 ? n_max : 0;
+  // The step of keys that is visited as the j-th.
+  const int own = (w.first + min(L::kBlock, w.q_len - w.first) / 2 + w.k_len - w.q_len) / kStep;
+  const int centre = BIAS ? min(max(own, 0), max(n_max - 1, 0)) : 0;
+  auto step_at = [&](int j) { return !BIAS || j > centre ? j : centre - j; };
+  // The document's keys in its last step, if fewer than 64, and when that is visited.
+  const int tail = w.k_len - (n_max - 1) * kStep, tail_at = BIAS && centre == n_max - 1 ? 0 : n_max - 1;
 
   if (warp == kTmaWarp) {
-    // ------------------------------------------------------------ TMA producer
-    if (lane == 0 && n_max > 0) {
-      tma_prefetch_desc(&maps.q);
-      tma_prefetch_desc(&maps.k);
-      tma_prefetch_desc(&maps.v);
-      for (int t = 0; t < 2; ++t) {
-        if ((t == 0 ? n0 : n1) == 0) continue;
-        mbar_arrive_expect_tx(&q_full[t], L::kQBytes);
+    // ------------------------------------------------------------ TMA producer: lane 0 issues
+    if (n_max > 0) {
+      if (lane == 0) {
+        tma_prefetch_desc(&maps.q);
+        tma_prefetch_desc(&maps.k);
+        tma_prefetch_desc(&maps.v);
+        for (int t = 0; t < kTiles; ++t) {
+          if ((t == 0 ? n0 : n1) == 0) continue;
+          mbar_arrive_expect_tx(&q_full[t], L::kQBytes);
 #pragma unroll
-        for (int c = 0; c < NC; ++c)
-          tma_load_4d(smem + t * L::kQBytes + c * kQChunk, &maps.q, &q_full[t], c * 64, h, w.q_row + w.first + t * kTile,
-                      w.map_doc);
+          for (int c = 0; c < NC; ++c)
+            tma_load_4d(smem + t * L::kQBytes + c * kQChunk, &maps.q, &q_full[t], c * 64, h,
+                        w.q_row + w.first + t * kTile, w.map_doc);
+        }
       }
       auto load = [&](const CUtensorMap* map, uint32_t off, uint64_t* bar, int j) {
 #pragma unroll
         for (int c = 0; c < NC; ++c)
-          tma_load_4d(smem + off + c * kKChunk, map, bar, c * 64, hk, w.k_row + j * kStep, w.map_doc);
+          tma_load_4d(smem + off + c * kKChunk, map, bar, c * 64, hk, w.k_row + step_at(j) * kStep, w.map_doc);
       };
       const int firsts = min(n_max, 2);
-      for (int j = 0; j < firsts; ++j) {
-        mbar_arrive_expect_tx(&k_first[j], L::kKBytes);
-        load(&maps.k, L::kOffK + j * L::kKBytes, &k_first[j], j);
-      }
-      int j = 0;
-      for (; j < n_max && !*abort_flag; ++j) {
-        const int s = j % L::kStages, done = j - 3;
-        if (done >= 0 && !mbar_wait_bounded(&empty[done % L::kStages], static_cast<uint32_t>(done / L::kStages) & 1u,
-                                            kErrWaitEmpty))
-          break;
-        const bool more = j + 2 < n_max;
-        mbar_arrive_expect_tx(&full[s], more ? 2 * L::kKBytes : L::kKBytes);
-        load(&maps.v, L::kOffV + s * L::kKBytes, &full[s], j);
-        if (more) load(&maps.k, L::kOffK + (j + 2) % L::kKSlots * L::kKBytes, &full[s], j + 2);
-      }
-      if (j < n_max) *abort_flag = 1;
-      // Drain: every issued load lands before the CTA can exit.
-      if (n0 > 0) mbar_wait_bounded(&q_full[0], 0, kErrWaitDrain);
-      if (n1 > 0) mbar_wait_bounded(&q_full[1], 0, kErrWaitDrain);
-      for (int i = 0; i < firsts; ++i) mbar_wait_bounded(&k_first[i], 0, kErrWaitDrain);
-      for (int i = max(0, j - L::kStages); i < j; ++i)
-        mbar_wait_bounded(&full[i % L::kStages], static_cast<uint32_t>(i / L::kStages) & 1u, kErrWaitDrain);
-    }
-    __syncwarp();
-    if (n_max > 0 && tail < kStep && !*abort_flag) {
-      // Rows past the document hold another's values, whose product with P = 0 must still be 0.
-      uint8_t* vt = smem + L::kOffV + (n_max - 1) % L::kStages * L::kKBytes;
-      for (int i = lane; i < (kStep - tail) * 8; i += 32)
-#pragma unroll
-        for (int c = 0; c < NC; ++c)
-          *reinterpret_cast<uint4*>(vt + c * kKChunk + tail * 128 + i * 16) = make_uint4(0, 0, 0, 0);
-      fence_proxy_async_shared();
+      if (lane == 0)
+        for (int j = 0; j < firsts; ++j) {
+          mbar_arrive_expect_tx(&k_first[j], L::kKBytes);
+          load(&maps.k, L::kOffK + j * L::kKBytes, &k_first[j], j);
+        }
       __syncwarp();
-      if (lane == 0) mbar_arrive(v_fixed);
+      int j = 0;
+      for (; j < n_max; ++j) {
+        const int s = j % L::kStages, done = j - 3;
+        if (done >= 0 && !mbar_wait_warp(&empty[done % L::kStages], static_cast<uint32_t>(done / L::kStages) & 1u,
+                                         kErrWaitEmpty))
+          break;
+        if (lane == 0) {
+          const bool more = j + 2 < n_max;
+          mbar_arrive_expect_tx(&full[s], more ? 2 * L::kKBytes : L::kKBytes);
+          load(&maps.v, L::kOffV + s * L::kKBytes, &full[s], j);
+          if (more) load(&maps.k, L::kOffK + (j + 2) % L::kKSlots * L::kKBytes, &full[s], j + 2);
+        }
+        __syncwarp();
+        if (j == tail_at && tail < kStep) {
+          // Rows past the document hold another's values, whose product with P = 0 must still be 0.
+          if (!mbar_wait_warp(&full[s], static_cast<uint32_t>(j / L::kStages) & 1u, kErrWaitFull)) {
+            ++j;
+            break;
+          }
+          uint8_t* vt = smem + L::kOffV + s * L::kKBytes;
+          for (int i = lane; i < (kStep - tail) * 8; i += 32)
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+              *reinterpret_cast<uint4*>(vt + c * kKChunk + tail * 128 + i * 16) = make_uint4(0, 0, 0, 0);
+          fence_proxy_async_shared();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(v_fixed);
+        }
+      }
+      if (lane == 0) {
+        // Drain: every issued load lands before the CTA can exit.
+        if (n0 > 0) mbar_wait_bounded(&q_full[0], 0, kErrWaitDrain);
+        if (n1 > 0) mbar_wait_bounded(&q_full[1], 0, kErrWaitDrain);
+        for (int i = 0; i < firsts; ++i) mbar_wait_bounded(&k_first[i], 0, kErrWaitDrain);
+        for (int i = max(0, j - L::kStages); i < j; ++i)
+          mbar_wait_bounded(&full[i % L::kStages], static_cast<uint32_t>(i / L::kStages) & 1u, kErrWaitDrain);
+      }
+      __syncwarp();
     }
   } else if (warp > kTmaWarp) {
     // ------------------------------------------------------------ MMA issuer of tile t: a warp that stays together
     const int t = warp - kTmaWarp - 1;
     const int dk = warp_value((p.dim + 15) / 16), n = warp_value(t == 0 ? n0 : n1), last = warp_value(n_max);
-    const bool fix = warp_value(tail) < kStep;
-    const uint32_t tm_s = warp_value(tmem + t * 128), tm_o = tm_s + 256;
+    const int fix_at = warp_value(tail < kStep ? tail_at : -1);
+    const uint32_t tm_s = warp_value(tmem + t * 128), tm_o = tm_s + L::kTmemO;
     const uint32_t base = warp_value(smem_u32(smem));
     const uint32_t id_s = idesc_f16(BF16, kTile, kStep);
     const uint32_t id_o = idesc_f16(BF16, kTile, static_cast<uint32_t>(dk) * 16u) | (1u << 16);  // V MN-major
@@ -320,11 +376,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int j = 0; ok && j < n; ++j) {
       const int s = j % L::kStages;
-      // One lane to a barrier: V(j) with K(j + 2), P(j), and at the end V's zeros.
+      // One lane to a barrier: V(j) with K(j + 2), P(j), and where there are any V's zeros.
       bool got = true;
       if (lane == 0) got = mbar_wait_bounded(&full[s], static_cast<uint32_t>(j / L::kStages) & 1u, kErrWaitFull);
-      if (lane == 1) got = mbar_wait_bounded(&p_full[t * 2 + (j & 1)], static_cast<uint32_t>(j >> 1) & 1u, kErrWaitFull);
-      if (lane == 2 && fix && j + 1 == last) got = mbar_wait_bounded(v_fixed, 0, kErrWaitFull);
+      if (lane == 1)
+        got = mbar_wait_bounded(&p_full[t * 2 + (j & 1)], static_cast<uint32_t>(j >> 1) & 1u, kErrWaitFull);
+      if (lane == 2 && j == fix_at) got = mbar_wait_bounded(v_fixed, 0, kErrWaitFull);
       ok = __all_sync(0xffffffffu, got);
       if (!ok) break;
       tc_fence_after();
@@ -345,16 +402,16 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (ok && lane == 0) mbar_arrive(&empty[j % L::kStages]);
       __syncwarp();
     }
-    if (!ok) *abort_flag = 1;
     __syncwarp();
   } else {
     // ------------------------------------------------------------ softmax, two threads per query
     const int t = warp >> 3, half = (warp >> 2) & 1;
     const int row = (warp & 3) * 32 + lane, i = w.first + t * kTile + row;  // the query inside the document
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t t_o = tmem + lanes + 256 + t * 128;
+    const uint32_t t_o = tmem + lanes + L::kTmemO + t * 128;
     const int n = t == 0 ? n0 : n1;
-    float* maxima = reinterpret_cast<float*>(smem + L::kOffMax) + t * 2 * kTile + row;  // + parity * 512 + half * 128
+    constexpr int kParity = kTiles * 2 * kTile;
+    float* maxima = reinterpret_cast<float*>(smem + L::kOffMax) + t * 2 * kTile + row;  // + parity, + half * 128
     const int pair_bar = 1 + t * 4 + (warp & 3);  // the two warps of these queries
     auto meet = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(pair_bar) : "memory"); };
     auto wait_s = [&](int j) {
@@ -364,7 +421,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     };
     const int lim = limit_of(p, w, i) - half * kPart, place = i + w.k_len - w.q_len - half * kPart;
     const float scale = p.scale * kLog2e;
-    const float cap_in = CAP ? 2.f * scale / p.cap : 0.f, cap_out = CAP ? p.cap * kLog2e : 0.f;
+    const float cap_in = CAP ? p.scale / p.cap : 0.f, cap_out = CAP ? p.cap * kLog2e : 0.f;
     const float slope = BIAS ? p.slopes[h] * kLog2e : 0.f;
     const float unit = CAP || BIAS ? 1.f : scale;  // what turns s below into base-2 scores
     float m = -INFINITY, l = 0.f;  // m: what P is relative to; the maximum or up to 2^8 below; l: of this half
@@ -372,18 +429,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int j = 0; j < n; ++j) {
       ok = ok && wait_s(j);  // (on a failure the loop goes on without waiting: the other half meets here)
       const uint32_t t_s = tmem + lanes + t * 128 + (j & 1) * 64;
+      const int key0 = step_at(j) * kStep;
       float s[kPart];
       tmem_ld32(t_s + half * kPart, s);
       tmem_ld_wait();
       tmem_ld_fence(s);
-      if constexpr (CAP) {
-        // c tanh(x / c) = c - 2 c / (e^(2 x / c) + 1): two operations of the exponential unit, error c 2^-22.
-#pragma unroll
-        for (int c = 0; c < kPart; ++c) s[c] = fmaf(-2.f * cap_out, rcp_unit(exp2_unit(s[c] * cap_in) + 1.f), cap_out);
-      }
+      if constexpr (CAP) cap_scores(s, cap_in, cap_out);
       if constexpr (BIAS) {
         // s - slope |at - c|: away from the query's own place the distance is linear in c.
-        const int at = place - j * kStep;
+        const int at = place - key0;
         const float mul = CAP ? 1.f : scale;
         if (__all_sync(0xffffffffu, at >= kPart - 1 || at <= 0)) {
           const float step = at > 0 ? slope : -slope, from = -step * static_cast<float>(at);
@@ -394,7 +448,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int c = 0; c < kPart; ++c) s[c] = fmaf(-slope, fabsf(static_cast<float>(at - c)), s[c] * mul);
         }
       }
-      const int left = lim - j * kStep;
+      const int left = lim - key0;
       if (left < kPart) {
 #pragma unroll
         for (int c = 0; c < kPart; ++c) s[c] = c < left ? s[c] : -INFINITY;
@@ -406,9 +460,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int c = 4; c < kPart; ++c) mx[c & 3] = fmaxf(mx[c & 3], s[c]);
       const float mine = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
       // The halves meet: the maximum of both, and P may take the place of S, which both have read.
-      maxima[(j & 1) * 512 + half * kTile] = mine;
+      maxima[(j & 1) * kParity + half * kTile] = mine;
       meet();
-      const float top = unit * fmaxf(mine, maxima[(j & 1) * 512 + (half ^ 1) * kTile]);
+      const float top = unit * fmaxf(mine, maxima[(j & 1) * kParity + (half ^ 1) * kTile]);
       const bool grow = top > m + kRescale || (m == -INFINITY && top > m);
       if (__any_sync(0xffffffffu, grow)) {
         const float f = grow ? exp2_unit(m - top) : 1.f;
@@ -451,11 +505,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     if (n > 0) {
       ok = ok && wait_s(n + 1);  // PV(n - 1)
-      maxima[(n & 1) * 512 + half * kTile] = l;
+      maxima[(n & 1) * kParity + half * kTile] = l;
       meet();
-      l += maxima[(n & 1) * 512 + (half ^ 1) * kTile];
+      l += maxima[(n & 1) * kParity + (half ^ 1) * kTile];
     }
-    if (!ok) *abort_flag = 1;
     const bool some = m != -INFINITY;  // a query that saw nothing gets zeros
     const float inv = some ? 1.f / l : 0.f;
     uint16_t* out = static_cast<uint16_t*>(p.out) + w.map_doc * p.o_doc + (w.q_row + i) * p.o_token + h * p.o_head;
@@ -484,18 +537,18 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   if (warp == kTmaWarp + 1) {
     tc_fence_after();
-    tmem_dealloc(tmem, 512);
+    tmem_dealloc(tmem, L::kTmem);
   }
 }
 
 template <int NC, bool CAP, bool BIAS, bool BF16>
 cudaError_t launch_tiles(const Maps& maps, const AttentionParams& p, dim3 grid, cudaStream_t stream) {
   auto kern = attention_tile_kernel<NC, CAP, BIAS, BF16>;
-  constexpr int bytes = static_cast<int>(Smem<NC>::kBytes);
+  constexpr int bytes = static_cast<int>(Layout<NC>::kBytes);
   static SharedMemoryGrant grant;
   const cudaError_t e = grant.ensure(kern, bytes);
   if (e != cudaSuccess) return e;
-  return launch_kernel(kern, grid, dim3(kThreads), bytes, stream, maps, p);
+  return launch_kernel(kern, grid, dim3(Layout<NC>::kThreads), bytes, stream, maps, p);
 }
 
 template <int NC, bool BF16>
@@ -510,8 +563,9 @@ cudaError_t launch_variant(const Maps& maps, const AttentionParams& p, dim3 grid
 }  // namespace
 
 // (channel, head, token, document) view of one operand, a box of 64 channels x box_tokens tokens.
-int encode_tokens_map(CUtensorMap* map, const void* base, bool bf16, int dim, int heads, long long tokens, long long docs,
-           long long s_head, long long s_token, long long s_doc, int box_tokens, const char* what) {
+int encode_tokens_map(CUtensorMap* map, const void* base, bool bf16, int dim, int heads, long long tokens,
+                      long long docs, long long s_head, long long s_token, long long s_doc, int box_tokens,
+                      const char* what) {
   auto enc = api_tensor_map_encoder();
   if (enc == nullptr) return api_fail(CTMR_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
   const cuuint64_t dims[4] = {static_cast<cuuint64_t>(dim), static_cast<cuuint64_t>(heads),
@@ -525,7 +579,8 @@ int encode_tokens_map(CUtensorMap* map, const void* base, bool bf16, int dim, in
                          const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) return api_fail(CTMR_ERR_INVALID, "%s's strides cannot be read by TMA (CUresult %d)", what, int(r));
+  if (r != CUDA_SUCCESS)
+    return api_fail(CTMR_ERR_INVALID, "%s's strides cannot be read by TMA (CUresult %d)", what, int(r));
   return CTMR_OK;
 }
 
@@ -536,7 +591,8 @@ int launch_attention_packed(const AttentionParams& p, bool bf16, cudaStream_t st
   int st = CTMR_OK;
   const bool few = attention_few_takes(p);
   if (!few)
-    st = encode_tokens_map(&maps.q, p.q, bf16, p.dim, p.heads, p.q_tokens, docs, p.q_head, p.q_token, p.q_doc, kTile, "q");
+    st = encode_tokens_map(&maps.q, p.q, bf16, p.dim, p.heads, p.q_tokens, docs, p.q_head, p.q_token, p.q_doc, kTile,
+                           "q");
   if (st == CTMR_OK && p.k_tokens > 0)  // not read where there are no keys
     st = encode_tokens_map(&maps.k, p.k, bf16, p.dim, p.kv_heads, p.k_tokens, docs, p.k_head, p.k_token, p.k_doc, kStep,
                            "k");
@@ -548,8 +604,9 @@ int launch_attention_packed(const AttentionParams& p, bool bf16, cudaStream_t st
   if (few) {
     e = launch_attention_few(maps.k, maps.v, p, bf16, stream);
   } else {
-    const long long blocks = packed ? p.q_tokens / kBlock + static_cast<long long>(p.documents)
-                                    : static_cast<long long>(p.documents) * ((p.q_tokens + kBlock - 1) / kBlock);
+    const int block = p.dim <= 64 ? Layout<1>::kBlock : Layout<2>::kBlock;
+    const long long blocks = packed ? p.q_tokens / block + static_cast<long long>(p.documents)
+                                    : static_cast<long long>(p.documents) * ((p.q_tokens + block - 1) / block);
     if (blocks > 0x7fffffffLL) return api_fail(CTMR_ERR_UNSUPPORTED, "too many documents");
     const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(p.heads));
     if (p.dim <= 64)
