@@ -569,7 +569,7 @@ def rotary_axes(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor
     if axes > 1 and positions.stride(1) != 1:
         positions = positions.contiguous()
     if out is None:
-        out = torch.empty(shape, dtype=x.dtype, device=x.device)
+        out = x.new_empty(shape)
     elif out.shape != shape or out.dtype != x.dtype or out.get_device() != dev:
         raise ValueError(f"out must be like x: {tuple(shape)} {x.dtype}")
     xt, xh, xc = x.stride()
@@ -640,7 +640,7 @@ def adapter_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | N
         bias = bias.contiguous()
         bias_at, bias_code = bias.data_ptr(), _FLOAT_CODES[bias.dtype]
     if out is None:
-        out = torch.empty((rows, outer), dtype=dtype, device=x.device)
+        out = x.new_empty((rows, outer))
     elif out.shape != (rows, outer) or out.dtype != dtype or out.get_device() != dev:
         raise ValueError(f"out must be ({rows}, {outer}) {dtype} on cuda:{dev}")
     (xs, xc), (ws, wc), (ys, yc) = x.stride(), weight.stride(), out.stride()
@@ -714,7 +714,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, q_offsets: t
     if k.dtype != dtype or v.dtype != dtype or k.get_device() != dev or v.get_device() != dev:
         raise ValueError(f"k and v must be {dtype} on cuda:{dev}")
     if out is None:
-        out = torch.empty(shape, dtype=dtype, device=q.device)
+        out = q.new_empty(shape)
     elif out.shape != shape or out.dtype != dtype or out.get_device() != dev:
         raise ValueError(f"out must be {tuple(shape)} {dtype} on cuda:{dev}")
     qo = ko = kl = None
