@@ -552,6 +552,23 @@ def test_attention_batched_strides_streams_and_max_q(cuda):
     assert (few.float() - more.float()).abs().max() <= 4e-3 and few.shape == out[:, 0].shape
 
 
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("cap", [0.0, 20.0])
+def test_attention_log_sum_exp_is_fp32(cuda, cap, dtype):
+    """The log-sum-exp is a sum of fp32 terms, not of the 16-bit softmax weights: exponentials good to 3e-6, a
+    quarter of them with an error of either sign (0.7e-6 of the sum at worst), scores of size S < 8 (with the
+    cap's 2e-7 S) rounded by 2^-22 S, and the logarithm's own 2^-23."""
+    from ctmr_b200 import ops
+
+    q, k, v, qo, ko = _packed(8, [700, 333], None, 4, 2, 96, dtype)
+    _, lse = ops.attention(q, k, v, q_offsets=qo, cap=cap, return_lse=True)
+    heads = torch.arange(4, device="cuda") // 2
+    for a, b in ((0, 700), (700, 1033)):
+        _, ref, _, size = _document_ref(q[a:b].double(), k[a:b].double()[:, heads], v[a:b].double()[:, heads],
+                                        96 ** -0.5, cap, None, False, 0)
+        _within(lse[a:b], ref, 1e-6 + (2.0 ** -22 + 2e-7) * size + 2.0 ** -22 * ref.abs())
+
+
 def test_attention_bad_offsets_are_reported(cuda):
     """Offsets and lengths out of range are clamped into the tensors and reported, never followed."""
     from ctmr_b200 import _lib, ops
