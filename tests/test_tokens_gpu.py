@@ -569,6 +569,43 @@ def test_attention_log_sum_exp_is_fp32(cuda, cap, dtype):
         _within(lse[a:b], ref, 1e-6 + (2.0 ** -22 + 2e-7) * size + 2.0 ** -22 * ref.abs())
 
 
+@pytest.mark.parametrize("lq", [1, 150])
+def test_attention_offsets_past_32_bits(cuda, lq):
+    """Keys and values more than 2^31 elements into their tensor (the last tokens of the second request of a
+    cache whose token rows are 16 KB apart)."""
+    from ctmr_b200 import ops
+
+    gen, tokens, used = _gen(31), 140_000, 300
+    store = torch.empty((2, tokens, 64, 128), device="cuda", dtype=torch.bfloat16)  # 4.6 GB, two heads of 64 used
+    assert store[1, tokens - used].data_ptr() - store.data_ptr() > 2 * 2 ** 31
+    k, v = store[:, :, :1], store[:, :, 63:]
+    part = store[:, tokens - used:]
+    part[:, :, :1] = _randn(gen, 2, used, 1, 128, dtype=torch.bfloat16)
+    part[:, :, 63:] = _randn(gen, 2, used, 1, 128, dtype=torch.bfloat16)
+    q = _randn(gen, 2, lq, 1, 128, dtype=torch.bfloat16)
+    out = ops.attention(q, k[:, tokens - used:], v[:, tokens - used:])
+    rows = ops.attention(q[1], store.view(-1, 64, 128)[:, :1], store.view(-1, 64, 128)[:, 63:],
+                         q_offsets=_offsets([0, lq]), k_offsets=torch.tensor([0, 2 * tokens - used, 2 * tokens],
+                                                                             device="cuda", dtype=torch.int32))
+    for b in range(2):
+        ref = _document_ref(q[b].double(), part[b, :, :1].double(), part[b, :, 63:].double(), 128 ** -0.5, 0.0, None,
+                            False, 0)
+        _check_attention(out[b], None, [(out[b], None, ref)], torch.bfloat16)
+    _check_attention(rows, None, [(rows, None, ref)], torch.bfloat16)
+    _no_device_error()
+
+
+def test_adapter_linear_offsets_past_32_bits(cuda):
+    """Rows more than 2^31 elements into x and y."""
+    from ctmr_b200 import ops
+
+    c = _linear_case(6, [64, 36], [1, 0], 64, 72, 8, 2, torch.float16)
+    wide = torch.empty((100, 24_000_000), device="cuda", dtype=torch.float16)  # 4.8 GB
+    wide[:, :64] = c["x"]
+    out = ops.adapter_linear(**{**c, "x": wide[:, :64]}, out=wide[:, 100:172])
+    _within(out, *_linear_ref(c))
+
+
 def test_attention_bad_offsets_are_reported(cuda):
     """Offsets and lengths out of range are clamped into the tensors and reported, never followed."""
     from ctmr_b200 import _lib, ops
