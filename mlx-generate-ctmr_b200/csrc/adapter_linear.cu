@@ -4,8 +4,8 @@
 // Two launches. adapter_inner_kernel computes t_i = scale_a down_a x_i (fp32 sums, rounded once to the
 // operands' type: it becomes a tensor-core operand, and its rounding is that of y's own adapter part).
 // The product kernel then computes y^T tiles, 128 (or a CTA pair's 256) outputs as TMEM lanes by a
-// tile of rows as columns: D = W x^T over the input in blocks of 64, and for every segment that
-// meets the tile one or two further blocks of K = rank, up_a t^T, into the same accumulator. An
+// tile of rows as columns: D = W x^T over the input in blocks of 128, and for every segment that
+// meets the tile one further block of K = rank, up_a t^T, into the same accumulator. An
 // adapter thus costs its own bytes and rank / in of the product, and y is rounded and written once.
 //
 // t is stored by blocks: block tile + segment for each pair of a row tile and a segment that meet (both
@@ -764,7 +764,7 @@ int encode(CUtensorMap* map, const void* base, bool bf16, int rank, long long d0
 }
 
 // Which kernel, tile and split: the least of these estimates (microseconds), fitted to runs of 1 to 1,300 rows
-// with 256 to 4,096 inputs and outputs, which they meet within 15 %. One CTA per tile: a wave of them takes
+// with 256 to 4,096 inputs and outputs, which they meet within some 20 %. One CTA per tile: a wave of them takes
 // 2.8 + 0.032 tile, plus 0.8 + 0.01 tile where a cluster splits the input, plus 0.32 + 0.0011 tile per block of 128
 // inputs. CTA pairs of 256 x 256, which overlap a tile's stores with the next one's products: 8 in all and 0.62 per
 // block. (617 rows of 512 -> 1,536: tiles of 64 rows 6.0, of 128 8.2, of 32 9.1, pairs 10.6; 617 rows of

@@ -672,7 +672,7 @@ def adapter_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | N
     ref = ctypes.byref(desc)
     ws_bytes = LIB.ctmr_adapter_linear_workspace_size(ref)
     if ws_bytes:
-        workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device)
+        workspace = x.new_empty(ws_bytes, dtype=torch.uint8)
         LAUNCHES[0] += 2
         status = LIB.ctmr_adapter_linear(ref, workspace.data_ptr(), ws_bytes, stream)
     else:
@@ -751,7 +751,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, q_offsets: t
         slopes = slopes.contiguous()
         slopes_at = slopes.data_ptr()
     if return_lse:
-        lse = torch.empty(shape[:-1], dtype=F32, device=q.device)
+        lse = q.new_empty(shape[:-1], dtype=F32)
         lse_at = lse.data_ptr()
     qs, ks, vs, ys = q.stride(), k.stride(), v.stride(), out.stride()
     if qs[-1] != 1 or ks[-1] != 1 or vs[-1] != 1 or ys[-1] != 1:
