@@ -601,7 +601,8 @@ def stack_adapters(adapters, *, dtype: torch.dtype, device="cuda") -> dict[str, 
     inner, outer = int(adapters[0][0].shape[1]), int(adapters[0][1].shape[0])
     for d, u, _ in adapters:
         if d.dim() != 2 or u.dim() != 2 or d.shape[1] != inner or u.shape[0] != outer or d.shape[0] != u.shape[1]:
-            raise ValueError(f"adapter of shapes {tuple(d.shape)}, {tuple(u.shape)} beside a ({outer}, {inner}) projection")
+            raise ValueError(f"adapter of shapes {tuple(d.shape)}, {tuple(u.shape)} beside a ({outer}, {inner}) "
+                             "projection")
     rank = (max(int(d.shape[0]) for d, _, _ in adapters) + 7) // 8 * 8
     down = torch.zeros((len(adapters), rank, inner), dtype=dtype, device=device)
     up = torch.zeros((len(adapters), outer, rank), dtype=dtype, device=device)
@@ -692,7 +693,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, q_offsets: t
     Packed: ``q`` ``(q_tokens, heads, head_dim)``, ``k`` and ``v`` ``(k_tokens, kv_heads, head_dim)``; document d is
     rows ``q_offsets[d]:q_offsets[d + 1]`` and ``k_offsets[d]:k_offsets[d + 1]`` (int32 on the device; ``k_offsets``
     defaults to ``q_offsets``, no offsets at all to one document). ``max_q``, where known, says that no document has
-    more queries (up to 32 query rows to a key head, the keys are split over the GPU instead). Batched: ``(batch, tokens, heads, head_dim)``, of each item's keys the first ``k_lengths[b]``.
+    more queries (up to 32 query rows to a key head, the keys are split over the GPU instead). Batched:
+    ``(batch, tokens, heads, head_dim)``, of each item's keys the first ``k_lengths[b]``.
 
     ``causal``: query i of Lq sees keys up to i + Lk - Lq, and those before ``prefix[d]``; otherwise all of its
     document. ``cap`` > 0 caps the scaled scores with a tanh; ``slopes`` ``(heads,)`` then subtracts
