@@ -1,11 +1,11 @@
 // The attention of attention_packed.cu for documents of few queries (serving: one new token per request
-// over a cache): group x queries rows, at most 32, share each key head's keys. The cache is read once and
+// over a cache): group x queries rows share each key head's keys, up to 32 to a CTA. The cache is read once and
 // that read is the time, so all of the GPU has to read at once: the keys of a (document, key head) are split
 // over a cluster of up to 16 CTAs, in steps of 64 that TMA brings into a ring in shared memory (96 KB a CTA, two
 // CTAs an SM: 192 KB in flight); each of four warps takes 16 keys of a step. The partial softmaxes meet in
 // shared memory and, across the cluster, in distributed shared memory, in one launch.
 //
-// The products are mma.sync m16n8k16, whose 16 rows fit: tcgen05 would want 128 where there are 1 to 32. With
+// The products are mma.sync m16n8k16, whose 16 rows fit: tcgen05 would want 128 where there are few. With
 // the loads in registers instead of a ring (eight warps an SM, a step's loads then its products) the same
 // kernel took 72 us for 16 requests of 4,096 to 8,192 keys, four key heads of 128.
 #include <cooperative_groups.h>
@@ -123,12 +123,15 @@ __global__ void __launch_bounds__(kThreads, 2)
     lse_at = static_cast<long long>(doc) * p.q_tokens;
   }
   const int prefix = p.prefix != nullptr ? p.prefix[doc] : 0, shift = k_len - q_len;
-  const int queries = min(q_len, p.max_q), rows = queries * group;  // row r: query r / group, head r % group
+  // Row base + r of the key head's: query (base + r) / group, head (base + r) % group. Calls of more rows than a
+  // CTA holds read the keys again for each further kRows of them (blockIdx.z).
+  const int queries = min(q_len, p.max_q), base = blockIdx.z * L::kRows;
+  const int rows = min(max(queries * group - base, 0), L::kRows);
   auto limit_of = [&](int i) { return p.causal ? min(k_len, max(max(i + shift + 1, prefix), 0)) : k_len; };
   const uint16_t* qp = static_cast<const uint16_t*>(p.q) + q_at;
 
   // This CTA's keys: a share of those that any row sees, in whole steps.
-  const int seen = queries > 0 ? limit_of(queries - 1) : 0;
+  const int seen = rows > 0 ? limit_of((base + rows - 1) / group) : 0;
   const int share = (seen + splits * kStep - 1) / (splits * kStep) * kStep;
   const int k0 = min(rank * share, seen), k1 = min(k0 + share, seen), steps = (k1 - k0 + kStep - 1) / kStep;
 
@@ -136,7 +139,8 @@ __global__ void __launch_bounds__(kThreads, 2)
     const int r = i / (L::kD / 8), d = (i - r * (L::kD / 8)) * 8;
     uint4 v = make_uint4(0, 0, 0, 0);
     if (r < rows && d < p.dim)
-      v = *reinterpret_cast<const uint4*>(qp + (r / group) * p.q_token + (hk * group + r % group) * p.q_head + d);
+      v = *reinterpret_cast<const uint4*>(qp + ((base + r) / group) * p.q_token +
+                                          (hk * group + (base + r) % group) * p.q_head + d);
     *reinterpret_cast<uint4*>(q_s + r * L::kPitch + d) = v;
   }
   __syncthreads();
@@ -173,9 +177,9 @@ __global__ void __launch_bounds__(kThreads, 2)
       for (int e = 0; e < 2; ++e) {
         const int r = t * 16 + g + 8 * e;
         m[t][e] = -INFINITY;
-        lim[t][e] = r < rows ? min(limit_of(r / group), k1) : 0;
-        place[t][e] = r / group + shift;
-        slope[t][e] = p.slopes != nullptr && r < rows ? p.slopes[hk * group + r % group] * kLog2e : 0.f;
+        lim[t][e] = r < rows ? min(limit_of((base + r) / group), k1) : 0;
+        place[t][e] = (base + r) / group + shift;
+        slope[t][e] = p.slopes != nullptr && r < rows ? p.slopes[hk * group + (base + r) % group] * kLog2e : 0.f;
       }
     const float scale = p.scale * kLog2e;
     const float cap_in = p.cap > 0.f ? 2.f * scale / p.cap : 0.f, cap_out = p.cap * kLog2e;
@@ -235,8 +239,8 @@ __global__ void __launch_bounds__(kThreads, 2)
         for (int n = 0; n < 2; ++n)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const float base = m[t][e] == -INFINITY ? 0.f : m[t][e];
-            const float x0 = exp2_unit(s[n][2 * e] - base), x1 = exp2_unit(s[n][2 * e + 1] - base);
+            const float from = m[t][e] == -INFINITY ? 0.f : m[t][e];
+            const float x0 = exp2_unit(s[n][2 * e] - from), x1 = exp2_unit(s[n][2 * e + 1] - from);
             l[t][e] = n == 0 ? fmaf(l[t][e], f[e], x0 + x1) : l[t][e] + (x0 + x1);
             a[n * 2 + e] = pack2<BF16>(x0, x1);
           }
@@ -305,7 +309,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     return sum;
   };
   auto finish = [&](int r, int d, float4 sum, float big, float total) {
-    const int i = r / group, h = hk * group + r % group;
+    const int i = (base + r) / group, h = hk * group + (base + r) % group;
     const float inv = total > 0.f ? 1.f / total : 0.f;  // a query that saw nothing gets zeros
     uint16_t* out = static_cast<uint16_t*>(p.out) + o_at + i * p.o_token + h * p.o_head;
     *reinterpret_cast<uint2*>(out + d) =
@@ -374,7 +378,9 @@ cudaError_t launch(const CUtensorMap& k, const CUtensorMap& v, const AttentionPa
   const cudaError_t e = grant.ensure(kern, bytes, true);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(p.documents) * splits, static_cast<unsigned>(p.kv_heads));
+  const int rows = p.heads / p.kv_heads * p.max_q;
+  cfg.gridDim = dim3(static_cast<unsigned>(p.documents) * splits, static_cast<unsigned>(p.kv_heads),
+                     static_cast<unsigned>((rows + MT * 16 - 1) / (MT * 16)));
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = bytes;
   cfg.stream = stream;
@@ -400,18 +406,40 @@ cudaError_t launch_type(const CUtensorMap& k, const CUtensorMap& v, const Attent
 
 }  // namespace
 
-// At most 32 rows of a key head: two row tiles of the products.
+// How many CTAs share the keys of a unit (document, key head, group of rows): up to two CTAs for every SM, as
+// long as each keeps two steps or more.
+static int few_splits(long long units, int keys) {
+  int splits = 1;
+  while (splits < 16 && units * splits <= device_sm_count() && keys >= splits * 2 * 2 * kStep) splits *= 2;
+  return splits;
+}
+
+// Whether this form takes the call: up to 128 rows of a key head, where the lesser of two estimates (microseconds,
+// fitted to 1 to 32 requests of 5 to 128 queries over 256 to 16,000 keys). This one: 6 for 16 rows, 10 for more, and
+// per step of 64 keys of a CTA 0.8 to 1.2 (head sizes to 64, above), 1.4 to 2.8. The tile kernel's CTAs take all
+// keys of one head's queries: 3.5 a wave and 0.57 to 0.65 a step. (16 heads on 2 of
+// 128: 5 queries of one request over 16,000 keys 43 us here and 170 there, 16 queries of 8 over 2,000 35 and 26.)
 bool attention_few_takes(const AttentionParams& p) {
-  return static_cast<long long>(p.heads / p.kv_heads) * p.max_q <= 32 && p.documents <= (1 << 24);
+  const long long rows = static_cast<long long>(p.heads / p.kv_heads) * p.max_q;
+  if (rows > 128 || p.documents > (1 << 24)) return false;
+  const int keys = p.q_offsets != nullptr ? p.k_tokens / p.documents : p.k_tokens, sms = device_sm_count();
+  const bool wide = p.dim > 64, many = rows > 16;
+  const long long units = static_cast<long long>(p.documents) * p.kv_heads * ((rows + 31) / 32);
+  const int splits = few_splits(units, keys);
+  auto waves = [](long long n, long long at_once) { return static_cast<float>((n + at_once - 1) / at_once); };
+  const float steps = static_cast<float>((keys + kStep - 1) / kStep);
+  const float few = (many ? 10.f : 6.f) + waves(units * splits, 2 * sms) * steps / splits *
+                                              (many ? (wide ? 2.8f : 1.4f) : (wide ? 1.2f : 0.8f));
+  const float tiles = 3.f + waves(static_cast<long long>(p.documents) * p.heads, wide ? sms : 2 * sms) *
+                                (3.5f + steps * (wide ? 0.65f : 0.57f));
+  return few <= tiles;
 }
 
 cudaError_t launch_attention_few(const CUtensorMap& k, const CUtensorMap& v, const AttentionParams& p, bool bf16,
                                  cudaStream_t stream) {
-  // Up to two CTAs for every SM, as long as each keeps two steps or more.
-  const long long units = static_cast<long long>(p.documents) * p.kv_heads;
-  const int sms = device_sm_count();
-  int splits = 1;
-  while (splits < 16 && units * splits <= sms && p.k_tokens >= splits * 2 * 2 * kStep) splits *= 2;
+  const int rows = p.heads / p.kv_heads * p.max_q;
+  const int splits = few_splits(static_cast<long long>(p.documents) * p.kv_heads * ((rows + 31) / 32),
+                                p.q_offsets != nullptr ? p.k_tokens / p.documents : p.k_tokens);
   return bf16 ? launch_type<true>(k, v, p, splits, stream) : launch_type<false>(k, v, p, splits, stream);
 }
 

@@ -693,7 +693,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, q_offsets: t
     Packed: ``q`` ``(q_tokens, heads, head_dim)``, ``k`` and ``v`` ``(k_tokens, kv_heads, head_dim)``; document d is
     rows ``q_offsets[d]:q_offsets[d + 1]`` and ``k_offsets[d]:k_offsets[d + 1]`` (int32 on the device; ``k_offsets``
     defaults to ``q_offsets``, no offsets at all to one document). ``max_q``, where known, says that no document has
-    more queries (up to 32 query rows to a key head, the keys are split over the GPU instead). Batched:
+    more queries (few query rows to a key head: the keys are split over the GPU instead). Batched:
     ``(batch, tokens, heads, head_dim)``, of each item's keys the first ``k_lengths[b]``.
 
     ``causal``: query i of Lq sees keys up to i + Lk - Lq, and those before ``prefix[d]``; otherwise all of its
