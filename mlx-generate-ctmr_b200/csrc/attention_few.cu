@@ -12,14 +12,13 @@
 
 #include "ctmr_b200.h"
 #include "launch.cuh"
-#include "tokens.cuh"
+#include "softmax.cuh"
 
 namespace ctmr {
 namespace {
 
 constexpr int kWarps = 4, kThreads = kWarps * 32 + 32;  // four warps compute, one loads
 constexpr int kKeys = 16, kStep = kWarps * kKeys;         // keys per warp and per step
-constexpr float kLog2e = 1.4426950408889634f;
 
 template <bool BF16>
 __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -33,23 +32,6 @@ __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint3
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-__device__ __forceinline__ float exp2_unit(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-template <bool BF16>
-__device__ __forceinline__ uint32_t pack2(float a, float b) {
-  if constexpr (BF16) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&h);
-  } else {
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&h);
-  }
 }
 
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
@@ -182,7 +164,8 @@ __global__ void __launch_bounds__(kThreads, 2)
         slope[t][e] = p.slopes != nullptr && r < rows ? p.slopes[hk * group + (base + r) % group] * kLog2e : 0.f;
       }
     const float scale = p.scale * kLog2e;
-    const float cap_in = p.cap > 0.f ? 2.f * scale / p.cap : 0.f, cap_out = p.cap * kLog2e;
+    const bool capped = p.cap > 0.f;
+    const ScoreCap cap = capped ? score_cap(p.scale, p.cap) : ScoreCap{};
     // ldmatrix rows: lanes 8 i .. 8 i + 7 give the rows of matrix i. K: four 16-byte units of 8 keys; V: the
     // warp's keys 0-7 and 8-15 of one unit, then of the next; Q: rows 0-7 and 8-15 of one unit, then the next.
     const int mat = lane >> 3, in = lane & 7;
@@ -211,6 +194,7 @@ __global__ void __launch_bounds__(kThreads, 2)
             mma<BF16>(s[n], a1, b[2], b[3]);
           }
         }
+        if (capped) cap_scores(reinterpret_cast<float(&)[8]>(s), cap);
         // Base-2 scores; s[n][2 e + i] belongs to row g + 8 e and key kb + 8 n + 2 c + i.
         float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
@@ -218,8 +202,7 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int e = i >> 1, key = kb + n * 8 + 2 * c + (i & 1);
-            float x = p.cap > 0.f ? fmaf(-2.f * cap_out, __frcp_rn(exp2_unit(s[n][i] * cap_in) + 1.f), cap_out)
-                                  : s[n][i] * scale;
+            float x = capped ? s[n][i] : s[n][i] * scale;
             x = fmaf(-slope[t][e], fabsf(static_cast<float>(place[t][e] - key)), x);
             x = key < lim[t][e] ? x : -INFINITY;
             s[n][i] = x;

@@ -26,7 +26,7 @@
 #include "capi_internal.cuh"
 #include "ctmr_b200.h"
 #include "launch.cuh"
-#include "tokens.cuh"
+#include "softmax.cuh"
 
 namespace ctmr {
 namespace {
@@ -35,7 +35,6 @@ constexpr int kTile = 128;     // queries per tile
 constexpr int kStep = 64;      // keys per step
 constexpr int kPart = 32;      // of them per softmax thread
 constexpr uint32_t kQChunk = kTile * 128, kKChunk = kStep * 128;  // rows of 64 16-bit channels
-constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRescale = 8.f;  // log2 of the growth that O and the sum are rescaled for
 
 // NC chunks of 64 channels per row (two above 64 channels), as many query tiles. V in a ring of four steps, K,
@@ -62,39 +61,6 @@ struct Maps {
   CUtensorMap q, k, v;
 };
 
-__device__ __forceinline__ float exp2_unit(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-__device__ __forceinline__ float rcp_unit(float x) {
-  float y;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-// Pairs of fp32 operations in one instruction.
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-  float2 d;
-  asm("{\n\t.reg .b64 a, b, c, d;\n\t"
-      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
-      "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
-      : "=f"(d.x), "=f"(d.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-  return d;
-}
-
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-  float2 d;
-  asm("{\n\t.reg .b64 a, b, d;\n\t"
-      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
-      "add.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
-      : "=f"(d.x), "=f"(d.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return d;
-}
-
 // 2^x of a pair, x <= 8, on the FMA pipe: x = n + f with n the nearest integer (the low bits of x plus
 // 1.5 * 2^23) and |f| <= 1/2, 2^f by a quartic (least maximum relative error on that interval, 2.6e-6, mean
 // error 4e-8: far below P's rounding, and small enough for the log-sum-exp, whose sum it enters; a cubic's
@@ -112,61 +78,6 @@ __device__ __forceinline__ float2 exp2_poly(float2 x) {
   p.x = __int_as_float(__float_as_int(p.x) + (__float_as_int(j.x) << 23));
   p.y = __int_as_float(__float_as_int(p.y) + (__float_as_int(j.y) << 23));
   return p;
-}
-
-// c tanh(x / c) of 32 scores, by how near the largest of any lane comes to the cap:
-//   below 0.3 of it  an odd polynomial (x / c times a cubic in its square, maximum relative error 1e-8), with
-//                    the powers of the scale in its coefficients: five operations to a pair of scores;
-//   below 0.6        x / c times a quartic, 6e-8 (1.7e-7 with fp32's roundings): eight to a pair;
-//   else             c - 2 c / (e^(2 x / c) + 1): two operations of the exponential unit to a score.
-// (8 heads of 8,192 tokens of 128, cap 30: 376 us with the quartic, 341 us with the cubic; 248 us uncapped. With
-// the exponentials alone, four sequences of 1 to 2,300 tokens took 118 us where the quartic took 101.)
-__device__ __forceinline__ void cap_scores(float (&s)[32], float in, float out) {
-  float big = 0.f;
-#pragma unroll
-  for (int c = 0; c < 32; ++c) big = fmaxf(big, fabsf(s[c]));
-  const float2 zero = make_float2(0.f, 0.f);
-  if (__all_sync(0xffffffffu, big * in <= 0.3f && in >= 1e-4f)) {  // (in^7 stays a normal number)
-    const float in2 = in * in, c0 = 0.9999999896019268f * in * out, c1 = -0.3333296267971552f * in2 * in * out;
-    const float c2 = 0.1331259723418185f * in2 * in2 * in * out;
-    const float c3 = -0.050222438703983206f * in2 * in2 * in2 * in * out;
-#pragma unroll
-    for (int c = 0; c < 32; c += 2) {
-      const float2 v = make_float2(s[c], s[c + 1]), u = fma2(v, v, zero);
-      float2 q = fma2(make_float2(c3, c3), u, make_float2(c2, c2));
-      q = fma2(q, u, make_float2(c1, c1));
-      q = fma2(q, u, make_float2(c0, c0));
-      q = fma2(q, v, zero);
-      s[c] = q.x, s[c + 1] = q.y;
-    }
-  } else if (__all_sync(0xffffffffu, big * in <= 0.6f)) {
-    const float2 in2 = make_float2(in, in), all2 = make_float2(in * out, in * out);
-#pragma unroll
-    for (int c = 0; c < 32; c += 2) {
-      const float2 v = make_float2(s[c], s[c + 1]), x = fma2(v, in2, zero), u = fma2(x, x, zero);
-      float2 q = fma2(make_float2(0.015414500613641403f, 0.015414500613641403f), u,
-                      make_float2(-0.052054543053197115f, -0.052054543053197115f));
-      q = fma2(q, u, make_float2(0.13309036526297813f, 0.13309036526297813f));
-      q = fma2(q, u, make_float2(-0.3333222964170574f, -0.3333222964170574f));
-      q = fma2(q, u, make_float2(0.9999999342091528f, 0.9999999342091528f));
-      q = fma2(q, fma2(v, all2, zero), zero);
-      s[c] = q.x, s[c + 1] = q.y;
-    }
-  } else {
-#pragma unroll
-    for (int c = 0; c < 32; ++c) s[c] = fmaf(-2.f * out, rcp_unit(exp2_unit(2.f * kLog2e * in * s[c]) + 1.f), out);
-  }
-}
-
-template <bool BF16>
-__device__ __forceinline__ uint32_t pack2(float a, float b) {
-  if constexpr (BF16) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&h);
-  } else {
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&h);
-  }
 }
 
 // The document and rows of one CTA.
@@ -473,7 +384,7 @@ __global__ void __launch_bounds__(Layout<NC>::kThreads, Layout<NC>::kCtas)
     };
     const int lim = limit_of(p, w, i) - half * kPart, place = i + w.k_len - w.q_len - half * kPart;
     const float scale = p.scale * kLog2e;
-    const float cap_in = CAP ? p.scale / p.cap : 0.f, cap_out = CAP ? p.cap * kLog2e : 0.f;
+    const ScoreCap cap = CAP ? score_cap(p.scale, p.cap) : ScoreCap{};
     const float slope = BIAS ? p.slopes[h] * kLog2e : 0.f;
     const float unit = CAP || BIAS ? 1.f : scale;  // what turns s below into base-2 scores
     float m = -INFINITY, l = 0.f;  // m: what P is relative to; the maximum or up to 2^8 below; l: of this half
@@ -486,7 +397,7 @@ __global__ void __launch_bounds__(Layout<NC>::kThreads, Layout<NC>::kCtas)
       tmem_ld32(t_s + half * kPart, s);
       tmem_ld_wait();
       tmem_ld_fence(s);
-      if constexpr (CAP) cap_scores(s, cap_in, cap_out);
+      if constexpr (CAP) cap_scores(s, cap);
       if constexpr (BIAS) {
         // s - slope |at - c|: away from the query's own place the distance is linear in c.
         const int at = place - key0;

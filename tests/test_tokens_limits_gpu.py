@@ -1,0 +1,88 @@
+"""The packed-token operators at the edges of what they accept, against plain implementations in 64 bits: extreme caps,
+queries that are not numbers, the lowest values in masked places, poisoned adapters, rows outside every document,
+bad offsets, the forms for 17 to 128 rows of a key head, head-major and expanded layouts.
+
+Tolerances. Outputs as in test_tokens_gpu. The log-sum-exp is a sum of fp32 terms: with scores of size S (per query),
+exponentials good to 2^-22 (one pair in four of the tile form 2.6e-6 of either sign, 0.7e-6 of the sum at worst), a
+chain of at most 32 additions (2^-24 each, 1.9e-6), scores rounded by 2^-22 S and the cap good to 2e-7 S, and the
+logarithm's own 2^-22: ``3e-6 + (2^-22 + 2e-7) S + 2^-22 |lse|``.
+"""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+from test_tokens_gpu import HALF, U, _gen, _linear_case, _linear_ref, _no_device_error, _offsets, _randn, _within
+
+pytestmark = pytest.mark.gpu
+
+
+def _rows_ref(q, k, v, *, scale=None, cap=0.0, slopes=None, causal=False, prefix=0):
+    """One document: q (Lq, H, D), k and v (Lk, Hk, D) -> out, lse, sum of softmax |v|, size of the scores, each in
+    64 bits and per query and head; queries that see nothing get zeros and -inf."""
+    heads = torch.arange(q.shape[1], device=q.device) // (q.shape[1] // k.shape[1])
+    q, k, v = q.double(), k.double()[:, heads], v.double()[:, heads]
+    lq, lk = q.shape[0], k.shape[0]
+    s = torch.einsum("ihd,jhd->hij", q, k) * (q.shape[-1] ** -0.5 if scale is None else scale)
+    if cap:
+        s = cap * torch.tanh(s / cap)
+    place, key = torch.arange(lq, device=q.device)[:, None] + lk - lq, torch.arange(lk, device=q.device)[None]
+    if slopes is not None:
+        s = s - slopes.double()[:, None, None] * (place - key).abs()
+    seen = (key <= place) | (key < prefix) if causal else torch.ones((lq, lk), dtype=torch.bool, device=q.device)
+    size = s.masked_fill(~seen, 0.0).abs().amax(-1).T if lk else torch.zeros(q.shape[:2], device=q.device)
+    s = s.masked_fill(~seen, -math.inf)
+    lse = torch.logsumexp(s, -1).T if lk else torch.full(q.shape[:2], -math.inf, dtype=torch.float64, device=q.device)
+    p = torch.where(torch.isneginf(lse).T[..., None], 0.0, torch.exp(s - lse.T[..., None]))
+    v = torch.where(seen.any(0)[:, None, None], v, 0.0)
+    return torch.einsum("hij,jhd->ihd", p, v), lse, torch.einsum("hij,jhd->ihd", p, v.abs()), size
+
+
+def _check(out, lse, ref, dtype):
+    o, m, mag, size = ref
+    _within(out, o, U[dtype] * o.abs() + (1.25 * U[dtype] + 2e-5 + 2.0 ** -21 * size[..., None]) * mag + 2.0 ** -25)
+    if lse is not None:
+        empty = torch.isneginf(m)
+        assert torch.equal(torch.isneginf(lse), empty) and (out[empty] == 0).all()
+        _within(lse[~empty], m[~empty], (3e-6 + (2.0 ** -22 + 2e-7) * size + 2.0 ** -22 * m.abs())[~empty])
+
+
+def _kernels(call):
+    """Names of the kernels that a call launches."""
+    from torch.profiler import ProfilerActivity, profile
+
+    call()
+    torch.cuda.synchronize()
+    with profile(activities=[ProfilerActivity.CUDA]) as prof:
+        call()
+        torch.cuda.synchronize()
+    return " ".join(e.key for e in prof.key_averages())
+
+
+# Each form's cases: query tokens, key tokens, heads, key heads, head size.
+TILES = [(150, 200, 2, 2, 40), (140, 300, 4, 2, 96)]
+FEW = [(1, 1500, 4, 1, 64), (2, 2000, 16, 2, 128), (1, 300, 2, 2, 72)]
+FORMS = [("attention_tile_kernel", c) for c in TILES] + [("attention_few_kernel", c) for c in FEW]
+
+
+def _operands(seed, lq, lk, heads, kv_heads, dim, dtype):
+    gen = _gen(seed)
+    return _randn(gen, lq, heads, dim, dtype=dtype), *(_randn(gen, lk, kv_heads, dim, dtype=dtype) for _ in range(2))
+
+
+# ---------------------------------------------------------------------------------------------- caps
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("cap", [1e-3, 2.0, 50.0, 1e3, 1e4, 1e6, 1e30, 3e38])
+@pytest.mark.parametrize(("form", "case"), FORMS)
+def test_attention_caps_of_any_size(cuda, form, case, cap, dtype):
+    """A cap far above the scores leaves them as they are, one far below makes them its sign."""
+    from ctmr_b200 import ops
+
+    q, k, v = _operands(3, *case, dtype)
+    call = lambda: ops.attention(q, k, v, cap=cap, causal=True, return_lse=True)  # noqa: E731
+    _check(*call(), _rows_ref(q, k, v, cap=cap, causal=True), dtype)
+    if cap == 50.0:
+        assert form in _kernels(call)
+    _no_device_error()
