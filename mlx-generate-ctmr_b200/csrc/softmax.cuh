@@ -56,8 +56,9 @@ __device__ __forceinline__ ScoreCap score_cap(float scale, float cap) {
 //   below 0.3 of it  an odd polynomial (x / c times a cubic in its square, maximum relative error 1e-8), with
 //                    the powers of the scale in its coefficients: five operations to a pair of scores;
 //   below 0.6        x / c times a quartic, 1e-7 (2e-7 with fp32's roundings): eight to a pair;
-//   else             c - 2 c / (e^(2 x / c) + 1): two operations of the exponential unit to a score. Its absolute
-//                    error is 2e-7 c.
+//   else             that for the scores below 0.6 and c - 2 c / (e^(2 x / c) + 1) for the others: two operations
+//                    of the exponential unit to a score. Its absolute error is 2e-7 c, which a small score under a
+//                    large cap would feel (a score of 1 under a cap of 1e6 by 0.1).
 // So a lane's scores may be capped by one polynomial or the other, 1e-7 apart, as its neighbours' are large or not.
 // (8 heads of 8,192 tokens of 128, cap 30: 376 us with the quartic, 341 us with the cubic; 248 us uncapped. With
 // the exponentials alone, four sequences of 1 to 2,300 tokens took 118 us where the quartic took 101.)
@@ -98,8 +99,13 @@ __device__ __forceinline__ void cap_scores(float (&s)[N], const ScoreCap& cap) {
     }
   } else {
 #pragma unroll
-    for (int c = 0; c < N; ++c)
-      s[c] = fmaf(-2.f * cap.out, rcp_unit(exp2_unit(2.f * kLog2e * in * s[c]) + 1.f), cap.out);
+    for (int c = 0; c < N; c += 2) {
+      const float2 v = make_float2(s[c], s[c + 1]), x = fma2(v, make_float2(in, in), zero), q = quartic(v, x);
+      auto far = [&](float x) {
+        return fmaf(-2.f * cap.out, rcp_unit(exp2_unit(2.f * kLog2e * x) + 1.f), cap.out);
+      };
+      s[c] = fabsf(x.x) <= 0.6f ? q.x : far(x.x), s[c + 1] = fabsf(x.y) <= 0.6f ? q.y : far(x.y);
+    }
   }
 }
 

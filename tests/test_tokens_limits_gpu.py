@@ -86,3 +86,15 @@ def test_attention_caps_of_any_size(cuda, form, case, cap, dtype):
     if cap == 50.0:
         assert form in _kernels(call)
     _no_device_error()
+
+
+@pytest.mark.parametrize("cap", [1e2, 1e4, 1e6])
+@pytest.mark.parametrize(("form", "case"), FORMS)
+def test_attention_caps_beside_large_scores(cuda, form, case, cap):
+    """Scores near the cap in some rows do not coarsen those of the others."""
+    from ctmr_b200 import ops
+
+    q, k, v = _operands(4, *case, torch.bfloat16)
+    q[::2, ::2] *= cap
+    out, lse = ops.attention(q, k, v, cap=cap, return_lse=True)
+    _check(out, lse, _rows_ref(q, k, v, cap=cap), torch.bfloat16)
