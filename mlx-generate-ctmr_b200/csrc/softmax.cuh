@@ -43,13 +43,13 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
 
 // How scores (products of q and k, before their scale) become capped base-2 scores.
 struct ScoreCap {
-  float in;    // scale / cap
+  float in;    // scale / cap, at most 1e38 so that a zero score stays zero
   float unit;  // scale * log2(e)
   float out;   // cap * log2(e)
 };
 
 __device__ __forceinline__ ScoreCap score_cap(float scale, float cap) {
-  return {scale / cap, scale * kLog2e, cap * kLog2e};
+  return {fminf(scale / cap, 1e38f), scale * kLog2e, cap * kLog2e};
 }
 
 // c tanh(x / c) of N scores, by how near the largest of any lane comes to the cap:
@@ -78,7 +78,8 @@ __device__ __forceinline__ void cap_scores(float (&s)[N], const ScoreCap& cap) {
     q = fma2(q, u, make_float2(0.9999999342091528f, 0.9999999342091528f));
     return fma2(q, fma2(v, make_float2(unit, unit), zero), zero);
   };
-  if (__all_sync(0xffffffffu, big * in <= 0.3f && in >= 1e-4f)) {  // (in^6 stays a normal number)
+  // (in^6 stays a normal number, and no coefficient grows past the scale itself)
+  if (__all_sync(0xffffffffu, big * in <= 0.3f && in >= 1e-4f && in <= 1.f)) {
     const float in2 = in * in, c0 = 0.9999999896019268f * unit, c1 = -0.3333296267971552f * in2 * unit;
     const float c2 = 0.1331259723418185f * in2 * in2 * unit;
     const float c3 = -0.050222438703983206f * in2 * in2 * in2 * unit;

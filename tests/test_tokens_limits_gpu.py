@@ -98,3 +98,17 @@ def test_attention_caps_beside_large_scores(cuda, form, case, cap):
     q[::2, ::2] *= cap
     out, lse = ops.attention(q, k, v, cap=cap, return_lse=True)
     _check(out, lse, _rows_ref(q, k, v, cap=cap), torch.bfloat16)
+
+
+@pytest.mark.parametrize("cap", [1e-5, 1e-7, 1e-30, 1e-40])
+@pytest.mark.parametrize(("form", "case"), FORMS)
+def test_attention_tiny_caps_of_zero_scores(cuda, form, case, cap):
+    """Queries of zeros see every key alike, however small the cap; others see its sign."""
+    from ctmr_b200 import ops
+
+    q, k, v = _operands(5, *case, torch.float16)
+    for rows in (slice(None), slice(None, None, 2)):  # then every other head only
+        some = q.clone()
+        some[:, rows] = 0
+        out, lse = ops.attention(some, k, v, cap=cap, return_lse=True)
+        _check(out, lse, _rows_ref(some, k, v, cap=cap), torch.float16)
