@@ -280,10 +280,10 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) big = fmaxf(big, stat_s[(w * L::kRows + r) * 2]);
     float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (big == -INFINITY) return sum;
+    const float from = big == -INFINITY ? 0.f : big;  // no maximum: nothing was seen, or NaN, which the sums hold
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-      const float f = exp2_unit(stat_s[(w * L::kRows + r) * 2] - big);
+      const float f = exp2_unit(stat_s[(w * L::kRows + r) * 2] - from);
       total = fmaf(f, stat_s[(w * L::kRows + r) * 2 + 1], total);
       const float4 v = *reinterpret_cast<const float4*>(o_s + (w * L::kRows + r) * L::kD + d);
       sum.x = fmaf(f, v.x, sum.x), sum.y = fmaf(f, v.y, sum.y);
@@ -293,12 +293,13 @@ __global__ void __launch_bounds__(kThreads, 2)
   };
   auto finish = [&](int r, int d, float4 sum, float big, float total) {
     const int i = (base + r) / group, h = hk * group + (base + r) % group;
-    const float inv = total > 0.f ? 1.f / total : 0.f;  // a query that saw nothing gets zeros
+    if (total == 0.f) sum = make_float4(0.f, 0.f, 0.f, 0.f);  // a query that saw nothing gets zeros
+    const float inv = total == 0.f ? 0.f : 1.f / total;
     uint16_t* out = static_cast<uint16_t*>(p.out) + o_at + i * p.o_token + h * p.o_head;
     *reinterpret_cast<uint2*>(out + d) =
         make_uint2(pack2<BF16>(sum.x * inv, sum.y * inv), pack2<BF16>(sum.z * inv, sum.w * inv));
     if (p.lse != nullptr && d == 0)
-      p.lse[(lse_at + i) * p.heads + h] = total > 0.f ? (big + log2f(total)) * 0.6931471805599453f : -INFINITY;
+      p.lse[(lse_at + i) * p.heads + h] = total == 0.f ? -INFINITY : (big + log2f(total)) * 0.6931471805599453f;
   };
   const int quads = p.dim / 4, work = rows * quads;
   if (splits == 1) {
@@ -336,16 +337,15 @@ __global__ void __launch_bounds__(kThreads, 2)
     float big = -INFINITY, total = 0.f;
     for (int z = 0; z < splits; ++z) big = fmaxf(big, cluster.map_shared_rank(stat_s, z)[r * 2]);
     float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (big != -INFINITY) {
+    const float from = big == -INFINITY ? 0.f : big;
 #pragma unroll 4
-      for (int z = 0; z < splits; ++z) {
-        const float2 other = *reinterpret_cast<const float2*>(cluster.map_shared_rank(stat_s, z) + r * 2);
-        const float4 v = *reinterpret_cast<const float4*>(cluster.map_shared_rank(o_s, z) + r * L::kD + d);
-        const float f = exp2_unit(other.x - big);
-        total = fmaf(f, other.y, total);
-        sum.x = fmaf(f, v.x, sum.x), sum.y = fmaf(f, v.y, sum.y);
-        sum.z = fmaf(f, v.z, sum.z), sum.w = fmaf(f, v.w, sum.w);
-      }
+    for (int z = 0; z < splits; ++z) {
+      const float2 other = *reinterpret_cast<const float2*>(cluster.map_shared_rank(stat_s, z) + r * 2);
+      const float4 v = *reinterpret_cast<const float4*>(cluster.map_shared_rank(o_s, z) + r * L::kD + d);
+      const float f = exp2_unit(other.x - from);
+      total = fmaf(f, other.y, total);
+      sum.x = fmaf(f, v.x, sum.x), sum.y = fmaf(f, v.y, sum.y);
+      sum.z = fmaf(f, v.z, sum.z), sum.w = fmaf(f, v.w, sum.w);
     }
     finish(r, d, sum, big, total);
   }

@@ -472,7 +472,8 @@ __global__ void __launch_bounds__(Layout<NC>::kThreads, Layout<NC>::kCtas)
       meet();
       l += maxima[(n & 1) * kParity + (half ^ 1) * kTile];
     }
-    const bool some = m != -INFINITY;  // a query that saw nothing gets zeros
+    // A query that saw nothing gets zeros; one whose scores are NaN has no maximum either, but NaN for a sum.
+    const bool some = m != -INFINITY || l != l;
     const float inv = some ? 1.f / l : 0.f;
     uint16_t* out = static_cast<uint16_t*>(p.out) + w.map_doc * p.o_doc + (w.q_row + i) * p.o_token + h * p.o_head;
     for (int c = half * 32; c < p.dim; c += 64) {

@@ -112,3 +112,21 @@ def test_attention_tiny_caps_of_zero_scores(cuda, form, case, cap):
         some[:, rows] = 0
         out, lse = ops.attention(some, k, v, cap=cap, return_lse=True)
         _check(out, lse, _rows_ref(some, k, v, cap=cap), torch.float16)
+
+
+# ---------------------------------------------------------------------------------------------- not numbers
+@pytest.mark.parametrize("kw", [dict(), dict(causal=True), dict(cap=5.0), dict(causal=True, slopes=True)])
+@pytest.mark.parametrize(("form", "case"), FORMS)
+def test_attention_of_nan_queries_is_nan(cuda, form, case, kw):
+    """A query that is not a number gives an output that is not one (and no zeros), and no other row notices."""
+    from ctmr_b200 import ops
+
+    q, k, v = _operands(6, *case, torch.float16)
+    kw = {**kw, **({"slopes": torch.full((q.shape[1],), 0.1, device="cuda")} if "slopes" in kw else {})}
+    out, lse = ops.attention(q, k, v, return_lse=True, **kw)
+    bad = q.clone()
+    bad[-1, 1, 0] = math.nan
+    got, got_lse = ops.attention(bad, k, v, return_lse=True, **kw)
+    assert torch.isnan(got[-1, 1]).all() and torch.isnan(got_lse[-1, 1])
+    got[-1, 1], got_lse[-1, 1] = out[-1, 1], lse[-1, 1]
+    assert torch.equal(got, out) and torch.equal(got_lse, lse)
