@@ -64,9 +64,10 @@ struct Maps {
 // 2^x of a pair, x <= 8, on the FMA pipe: x = n + f with n the nearest integer (the low bits of x plus
 // 1.5 * 2^23) and |f| <= 1/2, 2^f by a quartic (least maximum relative error on that interval, 2.6e-6, mean
 // error 4e-8: far below P's rounding, and small enough for the log-sum-exp, whose sum it enters; a cubic's
-// 7.5e-5 would show there), n added to the exponent. Clamped at 2^-125.
+// 7.5e-5 would show there), n added to the exponent. Zero below 2^-127, where that leaves no positive bits: a clamp
+// at 2^-125 gave masked keys that weight, and with values near bf16's lowest a share of the output.
 __device__ __forceinline__ float2 exp2_poly(float2 x) {
-  x.x = fmaxf(x.x, -125.f), x.y = fmaxf(x.y, -125.f);
+  x.x = fmaxf(x.x, -250.f), x.y = fmaxf(x.y, -250.f);  // (n fits the nine bits above the mantissa)
   const float2 magic = make_float2(12582912.f, 12582912.f), back = make_float2(-12582912.f, -12582912.f);
   const float2 j = add2(x, magic), n = add2(j, back);
   const float2 f = fma2(n, make_float2(-1.f, -1.f), x);
@@ -75,8 +76,8 @@ __device__ __forceinline__ float2 exp2_poly(float2 x) {
   p = fma2(p, f, make_float2(0.24024836877206313f, 0.24024836877206313f));
   p = fma2(p, f, make_float2(0.6931217761894134f, 0.6931217761894134f));
   p = fma2(p, f, make_float2(0.9999991951706715f, 0.9999991951706715f));
-  p.x = __int_as_float(__float_as_int(p.x) + (__float_as_int(j.x) << 23));
-  p.y = __int_as_float(__float_as_int(p.y) + (__float_as_int(j.y) << 23));
+  p.x = __int_as_float(__viaddmax_s32(__float_as_int(p.x), __float_as_int(j.x) << 23, 0));
+  p.y = __int_as_float(__viaddmax_s32(__float_as_int(p.y), __float_as_int(j.y) << 23, 0));
   return p;
 }
 

@@ -130,3 +130,21 @@ def test_attention_of_nan_queries_is_nan(cuda, form, case, kw):
     assert torch.isnan(got[-1, 1]).all() and torch.isnan(got_lse[-1, 1])
     got[-1, 1], got_lse[-1, 1] = out[-1, 1], lse[-1, 1]
     assert torch.equal(got, out) and torch.equal(got_lse, lse)
+
+
+@pytest.mark.parametrize("lowest", [True, False])
+@pytest.mark.parametrize(("form", "case"), FORMS)
+def test_attention_lowest_values_in_masked_places(cuda, form, case, lowest):
+    """Values that no query sees (causal), or that a score far below the others' leaves without weight, are the
+    type's lowest: they count for nothing."""
+    from ctmr_b200 import ops
+
+    q, k, v = _operands(8, *case, torch.bfloat16)
+    v[-8:] = torch.finfo(torch.bfloat16).min if lowest else torch.finfo(torch.bfloat16).max
+    if q.shape[0] > 8:  # the last eight keys belong to the last eight queries
+        out, lse = ops.attention(q, k, v, causal=True, return_lse=True)
+        _check(out[:-8], lse[:-8], _rows_ref(q[:-8], k[:-8], v[:-8], causal=True), torch.bfloat16)
+    k[:, :, 0], q[:, :, 0] = 0.0, 8.0
+    k[-8:, :, 0] = -1e4  # scores of about -4e4
+    out, lse = ops.attention(q, k, v, scale=0.5, return_lse=True)
+    _check(out, lse, _rows_ref(q, k[:-8], v[:-8], scale=0.5), torch.bfloat16)
