@@ -61,13 +61,21 @@ struct Maps {
   CUtensorMap q, k, v;
 };
 
+// The larger, NaN if either is: a NaN score must not become a weight of zero (the integer addition below makes it the
+// largest number, which is infinity to the product).
+__device__ __forceinline__ float max_or_nan(float a, float b) {
+  float c;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(c) : "f"(a), "f"(b));
+  return c;
+}
+
 // 2^x of a pair, x <= 8, on the FMA pipe: x = n + f with n the nearest integer (the low bits of x plus
 // 1.5 * 2^23) and |f| <= 1/2, 2^f by a quartic (least maximum relative error on that interval, 2.6e-6, mean
 // error 4e-8: far below P's rounding, and small enough for the log-sum-exp, whose sum it enters; a cubic's
 // 7.5e-5 would show there), n added to the exponent. Zero below 2^-127, where that leaves no positive bits: a clamp
 // at 2^-125 gave masked keys that weight, and with values near bf16's lowest a share of the output.
 __device__ __forceinline__ float2 exp2_poly(float2 x) {
-  x.x = fmaxf(x.x, -250.f), x.y = fmaxf(x.y, -250.f);  // (n fits the nine bits above the mantissa)
+  x.x = max_or_nan(x.x, -250.f), x.y = max_or_nan(x.y, -250.f);  // (n fits the nine bits above the mantissa)
   const float2 magic = make_float2(12582912.f, 12582912.f), back = make_float2(-12582912.f, -12582912.f);
   const float2 j = add2(x, magic), n = add2(j, back);
   const float2 f = fma2(n, make_float2(-1.f, -1.f), x);

@@ -148,3 +148,15 @@ def test_attention_lowest_values_in_masked_places(cuda, form, case, lowest):
     k[-8:, :, 0] = -1e4  # scores of about -4e4
     out, lse = ops.attention(q, k, v, scale=0.5, return_lse=True)
     _check(out, lse, _rows_ref(q, k[:-8], v[:-8], scale=0.5), torch.bfloat16)
+
+
+@pytest.mark.parametrize("key", range(24, 32))
+@pytest.mark.parametrize(("form", "case"), FORMS)
+def test_attention_of_a_nan_key_is_not_finite(cuda, form, case, key):
+    """Used keys have to be finite; one that is not leaves no plausible result behind."""
+    from ctmr_b200 import ops
+
+    q, k, v = _operands(7, *case, torch.float16)
+    k[key] = math.nan
+    out = ops.attention(q, k, v)
+    assert not torch.isfinite(out).any()
