@@ -332,7 +332,9 @@ CTMR_API int ctmr_rotary_axes(const ctmr_rotary_desc* desc, void* stream);
 /* A projection shared by all rows and a low-rank adapter for each segment of rows:
  *   y_i = weight x_i + bias + scale[a] * up[a] (down[a] x_i),  a = index[segment of row i],
  * without the adapter's term where a is negative or no segment holds the row. 16-bit operands,
- * fp32 sums; the adapter's inner product (scaled) is rounded once to the operands' type. */
+ * fp32 sums; the adapter's inner product (scaled) is rounded once to the operands' type, whose range it must
+ * not leave (fp16: 65,504). Infinities and NaN stay in the rows and outputs that the formula gives them to:
+ * an adapter that holds some does not touch the rows of other segments. */
 typedef struct ctmr_adapter_linear_desc {
   const void* x;                   /* (rows, in_features), rows x_stride elements apart */
   long long x_stride;              /* a multiple of 8 */

@@ -211,7 +211,7 @@ __global__ void __launch_bounds__(kInnerWarps * 32) adapter_inner_kernel(const L
   for (int i = threadIdx.x; i < 16 * plan.rank_pad; i += kInnerWarps * 32) {
     const int r = i / plan.rank_pad, n = i - r * plan.rank_pad;
     float v = 0.f;
-    if (n < p.rank) {
+    if (n < p.rank && row0 + r >= lo && row0 + r < hi) {  // zeros elsewhere, whatever this adapter makes of a zero
 #pragma unroll
       for (int q = 0; q < kParts; ++q) v += part[q][r][n];
       v *= scale;
@@ -254,6 +254,68 @@ __device__ __forceinline__ void store16(void* y, long long i, float v) {
   else static_cast<__half*>(y)[i] = __float2half_rn(v);
 }
 
+// ---------------------------------------------------------------- outputs that are not finite
+// An adapter's block meets every row of its tile, with t = 0 in those of other segments, and zero times an
+// infinity in `up` is NaN: one request's broken adapter would spoil its neighbours. So an accumulator that is not
+// finite is not taken at its word: that output is computed by itself, from its own row and its own adapter.
+// (Finite calls pay one operation an output for the test: 617 rows of 512 -> 1,536 went from 9.9 to 10.3 us. 8,192
+// rows of 4,096 -> 4,096, 203 us: 11 ms beside one row whose adapter is all NaN, 77 ms with all of W NaN.)
+template <bool BF16>
+__device__ __forceinline__ float dot8(const void* a, const void* b) {
+  const uint4 ua = *static_cast<const uint4*>(a), ub = *static_cast<const uint4*>(b);
+  float sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t wa = (&ua.x)[i], wb = (&ub.x)[i];
+    float2 fa, fb;
+    if constexpr (BF16) {
+      fa = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&wa));
+      fb = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&wb));
+    } else {
+      fa = __half22float2(*reinterpret_cast<const __half2*>(&wa));
+      fb = __half22float2(*reinterpret_cast<const __half2*>(&wb));
+    }
+    sum = fmaf(fa.x, fb.x, sum), sum = fmaf(fa.y, fb.y, sum);
+  }
+  return sum;
+}
+
+// By a whole warp: bit e of a lane's `bad` names row row0 + e / OUTS * step and output o + e % OUTS of this lane.
+template <bool BF16, int OUTS>
+__device__ __noinline__ void alone(const LinearParams& p, const LinearPlan& plan, unsigned bad, int row0, int step, int o) {
+  griddep_wait();  // t is complete
+  const int lane = threadIdx.x & 31;
+  const uint16_t *x = static_cast<const uint16_t*>(p.x), *w = static_cast<const uint16_t*>(p.weight);
+  const uint16_t *up = static_cast<const uint16_t*>(p.up), *inner = static_cast<const uint16_t*>(p.inner);
+  while (const unsigned who = __ballot_sync(0xffffffffu, bad != 0)) {
+    const int src = __ffs(who) - 1, e = __ffs(__shfl_sync(0xffffffffu, bad, src)) - 1;
+    const int row = row0 + e / OUTS * step, out = __shfl_sync(0xffffffffu, o, src) + e % OUTS;
+    float sum = 0.f;
+    for (int k = lane * 8; k < p.in; k += 256) sum += dot8<BF16>(x + row * p.x_stride + k, w + out * p.weight_stride + k);
+    const int s = segment_at_row(p.offsets, p.segments, row, lane), a = p.index[s];
+    if (row >= p.offsets[s] && row < p.offsets[s + 1] && a >= 0 && a < p.adapters && lane * 8 < p.rank) {
+      const long long t = static_cast<long long>(row / plan.tile + s) * plan.tile + row % plan.tile;
+      sum += dot8<BF16>(inner + t * plan.rank_pad + lane * 8, up + (static_cast<long long>(a) * p.out + out) * p.rank + lane * 8);
+    }
+#pragma unroll
+    for (int i = 16; i > 0; i /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, i);
+    if (lane == src) {
+      store16<BF16>(p.y, row * p.y_stride + out, sum + bias_of(p, BF16, out));
+      bad &= bad - 1;
+    }
+  }
+}
+
+// z, zero, as long as all of the values are finite; NaN once one is not.
+template <int N>
+__device__ __forceinline__ float test_finite(const float (&v)[N], float z) {
+#pragma unroll
+  for (int e = 0; e < N; ++e) z = fmaf(v[e], 0.f, z);
+  return z;
+}
+
+__device__ __forceinline__ bool is_finite(float v) { return fabsf(v) <= 3.402823466e38f; }
+
 __device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
   float4 v;
   asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"  // volatile: in order with the barriers
@@ -267,7 +329,8 @@ __device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
 // memory, each CTA adding up and writing its share of the columns.
 template <int BN, bool BF16>
 __global__ void __launch_bounds__(kSmallThreads, 1)
-    linear_small_kernel(const __grid_constant__ LinearMaps maps, const LinearParams p, const LinearPlan plan) {
+    linear_small_kernel(const __grid_constant__ LinearMaps maps, const __grid_constant__ LinearParams p,
+                        const __grid_constant__ LinearPlan plan) {
   using L = SmallSmem<BN>;
   constexpr int S = L::kStages;
   extern __shared__ uint8_t smem_raw[];
@@ -419,9 +482,10 @@ __global__ void __launch_bounds__(kSmallThreads, 1)
     // ------------------------------------------------------------ epilogue
     const int quarter = warp & 3, o = m0 + quarter * 32 + lane;
     const float bias = bias_of(p, BF16, o);
-    const bool ok = mbar_wait_bounded(done, 0, kErrWaitAcc) && !*abort_flag;
+    const bool ok = mbar_wait_warp(done, 0, kErrWaitAcc) && __all_sync(0xffffffffu, !*abort_flag);
     tc_fence_after();
     const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
+    float z = 0.f;
     for (int c = 0; c < BN; c += 16) {
       float v[16];
       tmem_ld16(tmem + lanes + c, v);
@@ -434,6 +498,18 @@ __global__ void __launch_bounds__(kSmallThreads, 1)
 #pragma unroll
         for (int e = 0; e < 16; ++e)
           if (r0 + c + e < p.rows) store16<BF16>(p.y, static_cast<long long>(r0 + c + e) * p.y_stride + o, v[e] + bias);
+      }
+      z = test_finite(v, z);
+    }
+    if (plan.split == 1 && ok && p.segments > 0 && __any_sync(0xffffffffu, z != 0.f)) {
+      for (int c = 0; c < BN; c += 16) {
+        float v[16];
+        tmem_ld16(tmem + lanes + c, v);
+        unsigned bad = 0;
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (o < p.out && r0 + c + e < p.rows && !is_finite(v[e])) bad |= 1u << e;
+        alone<BF16, 1>(p, plan, bad, r0 + c, 1, o);
       }
     }
     if (!ok) *abort_flag = 1;
@@ -487,6 +563,22 @@ __global__ void __launch_bounds__(kSmallThreads, 1)
               if (o + i < p.out) store16<BF16>(p.y, at + i, u[i]);
           }
         }
+        if (p.segments > 0) {
+          float z = 0.f;
+#pragma unroll
+          for (int e = 0; e < kBatch; ++e) z = fmaf(v[e].x, 0.f, fmaf(v[e].y, 0.f, fmaf(v[e].z, 0.f, fmaf(v[e].w, 0.f, z))));
+          if (__any_sync(0xffffffffu, z != 0.f)) {
+            unsigned bad = 0;
+#pragma unroll
+            for (int e = 0; e < kBatch; ++e) {
+              const float u[4] = {v[e].x, v[e].y, v[e].z, v[e].w};
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                if (c + 4 * e < c_end && o + i < p.out && !is_finite(u[i])) bad |= 1u << (e * 4 + i);
+            }
+            alone<BF16, 4>(p, plan, bad, r0 + c, 4, o);
+          }
+        }
       }
     }
     cluster_sync();  // no CTA leaves while another reads its partial tile
@@ -511,7 +603,8 @@ constexpr int kRaster = 8;  // row tiles that are walked together, so that W's a
 // 128 x 256 tile would take 96. Two accumulators in TMEM: a tile is written while the next is computed.
 template <bool BF16>
 __global__ void __launch_bounds__(kPairThreads, 1)
-    linear_pair_kernel(const __grid_constant__ LinearMaps maps, const LinearParams p, const LinearPlan plan) {
+    linear_pair_kernel(const __grid_constant__ LinearMaps maps, const __grid_constant__ LinearParams p,
+                       const __grid_constant__ LinearPlan plan) {
   constexpr int S = kPairStages;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
@@ -703,6 +796,13 @@ __global__ void __launch_bounds__(kPairThreads, 1)
 #pragma unroll
           for (int e = 0; e < 32; ++e, at += p.y_stride)
             if (row + e < p.rows) store16<BF16>(p.y, at, v[e] + bias);
+        }
+        if (p.segments > 0 && __any_sync(0xffffffffu, test_finite(v, 0.f) != 0.f)) {
+          unsigned bad = 0;
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if (o < p.out && row + e < p.rows && !is_finite(v[e])) bad |= 1u << e;
+          alone<BF16, 1>(p, plan, bad, row, 1, o);
         }
         __syncwarp();
       }

@@ -623,7 +623,9 @@ def adapter_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | N
     ``offsets[s]:offsets[s + 1]`` (int32, on the device); ``index[s]`` is its adapter, negative for none:
     ``y = x weight^T + bias + scale[a] * (x down[a]^T) up[a]^T``. 16-bit operands (all of one type; ``bias`` may
     be fp32), fp32 sums. ``down`` ``(n, rank, in)``, ``up`` ``(n, out, rank)`` and ``scale`` ``(n,)`` come from
-    ``stack_adapters``. Without them it is the plain projection. ``out`` must not overlap ``x``.
+    ``stack_adapters``. Without them it is the plain projection. ``out`` must not overlap ``x``. The adapter's inner
+    product ``scale * x down^T`` is rounded to the operands' type and must stay in its range; an adapter that is not
+    finite spoils its own requests' rows only.
     """
     dtype = x.dtype
     code = _HALF_CODES.get(dtype)

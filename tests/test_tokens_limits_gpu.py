@@ -160,3 +160,38 @@ def test_attention_of_a_nan_key_is_not_finite(cuda, form, case, key):
     k[key] = math.nan
     out = ops.attention(q, k, v)
     assert not torch.isfinite(out).any()
+
+
+# ---------------------------------------------------------------------------------------------- adapters
+POISONED = [  # lengths, adapters by segment, inner, outer, rank: tiles of 16 to 128 rows, splits, CTA pairs
+    ([1] * 20, [i % 4 - 1 for i in range(20)], 512, 384, 16),
+    ([5, 3, 40, 2, 17], [0, 1, -1, 2, 1], 136, 257, 8),
+    ([100, 9, 150, 41], [2, 1, 0, -1], 4096, 512, 128),
+    ([300, 77, 1, 222], [0, 1, 2, -1], 520, 1000, 24),
+    ([1000, 1, 0, 1305], [2, 0, 1, 1], 136, 2310, 24),
+    ([2500, 31, 2500], [1, -1, 0], 64, 1100, 72),
+]
+
+
+@pytest.mark.parametrize("where", ["up", "down", "scale"])
+@pytest.mark.parametrize("value", [math.inf, math.nan])
+@pytest.mark.parametrize("case", range(len(POISONED)))
+def test_poisoned_adapters_stay_in_their_rows(cuda, case, value, where):
+    """An adapter that is not finite spoils the rows of its own segments, where the formula says so, and no others:
+    not those beside them in a tile, with other adapters or with none."""
+    from ctmr_b200 import ops
+
+    lengths, index, inner, outer, rank = POISONED[case]
+    c = _linear_case(case, lengths, index, inner, outer, rank, 3, torch.float16)
+    if where == "up":
+        c["up"][1, ::3, rank - 1] = value
+    elif where == "down":
+        c["down"][1, 0, 5] = value
+    else:
+        c["scale"][1] = value
+    y = ops.adapter_linear(**c)
+    ref, tol = _linear_ref(c)
+    fine = torch.isfinite(ref)
+    assert torch.equal(torch.isfinite(y), fine) and fine.any() and not fine.all()
+    _within(y[fine], ref[fine], tol[fine])
+    _no_device_error()
