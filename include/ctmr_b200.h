@@ -367,7 +367,8 @@ CTMR_API int ctmr_adapter_linear(const ctmr_adapter_linear_desc* desc, void* wor
  * the operands' type for their product with v.
  *
  * Two forms. Packed: q_offsets and k_offsets given, q_tokens and k_tokens the packed totals, document
- * strides unused. Batched: both NULL, each document has q_tokens queries and k_tokens key rows, of
+ * strides unused; rows of q before the first document or past the last give zeros (and lse -infinity).
+ * Batched: both NULL, each document has q_tokens queries and k_tokens key rows, of
  * which the first k_lengths[document] are used (all when NULL). Values of keys outside the used ones
  * are never part of a result, whatever they are; values of used keys must be finite. */
 typedef struct ctmr_attention_desc {

@@ -190,9 +190,13 @@ __global__ void __launch_bounds__(Layout<NC>::kThreads, Layout<NC>::kCtas)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   griddep_wait();
   griddep_launch_dependents();
+  int first = 0, last = p.q_tokens;
+  if (p.q_offsets != nullptr) first = p.q_offsets[0], last = p.q_offsets[p.documents];
   Place w;
   int h;
-  if (!find_place<L::kBlock>(p, blockIdx.x, lane, w, h)) return;  // the same answer in every warp
+  const bool mine = find_place<L::kBlock>(p, blockIdx.x, lane, w, h);  // the same answer in every warp
+  clear_outside(p, first, last, blockIdx.x, gridDim.x);
+  if (!mine) return;
   const int hk = h / (p.heads / p.kv_heads);
 
   if (threadIdx.x == 0) {

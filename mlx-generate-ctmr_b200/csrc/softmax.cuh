@@ -2,6 +2,8 @@
 // operations, capped scores, 16-bit pairs.
 #pragma once
 
+#include <cmath>
+
 #include "tokens.cuh"
 
 namespace ctmr {
@@ -118,6 +120,24 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   } else {
     const __half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+
+// Rows of a packed output before the first document and past the last (q_offsets' ends): zeros, and a log-sum-exp
+// of -infinity. Every block of the grid takes its share.
+__device__ __forceinline__ void clear_outside(const AttentionParams& p, int first, int last, long long block,
+                                              long long blocks) {
+  first = min(max(first, 0), p.q_tokens), last = min(max(last, 0), p.q_tokens);
+  const int rows = first + p.q_tokens - last, units = p.heads * (p.dim / 8);
+  if (rows == 0 || last < first) return;
+  const long long step = blocks * blockDim.x, n = static_cast<long long>(rows) * units;
+  for (long long i = block * blockDim.x + threadIdx.x; i < n; i += step) {
+    const int r = static_cast<int>(i / units), u = static_cast<int>(i - static_cast<long long>(r) * units);
+    const int h = u / (p.dim / 8), d = u - h * (p.dim / 8);
+    const long long row = r < first ? r : last + (r - first);
+    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + row * p.o_token + h * p.o_head + d * 8) =
+        make_uint4(0, 0, 0, 0);
+    if (p.lse != nullptr && d == 0) p.lse[row * p.heads + h] = -INFINITY;
   }
 }
 

@@ -700,10 +700,10 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, q_offsets: t
 
     ``causal``: query i of Lq sees keys up to i + Lk - Lq, and those before ``prefix[d]``; otherwise all of its
     document. ``cap`` > 0 caps the scaled scores with a tanh; ``slopes`` ``(heads,)`` then subtracts
-    ``slopes[h] * |i + Lk - Lq - j|``. A query that sees no key gives zeros (log-sum-exp -inf). ``heads`` may be a
-    multiple of ``kv_heads``. Any strides that are multiples of 8. Keys outside a document or past its length may
-    hold anything; those inside must be finite. Returns ``out``, or ``(out, lse)`` with the
-    fp32 natural log-sum-exp ``(.., tokens, heads)``.
+    ``slopes[h] * |i + Lk - Lq - j|``. A query that sees no key gives zeros (log-sum-exp -inf), and so does a
+    row of ``q`` before the first document or past the last. ``heads`` may be a multiple of ``kv_heads``. Any
+    strides that are multiples of 8. Keys outside a document or past its length may hold anything; those inside must
+    be finite. Returns ``out``, or ``(out, lse)`` with the fp32 natural log-sum-exp ``(.., tokens, heads)``.
     """
     dtype, dims = q.dtype, q.dim()
     code = _HALF_CODES.get(dtype)

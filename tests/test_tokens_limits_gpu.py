@@ -195,3 +195,30 @@ def test_poisoned_adapters_stay_in_their_rows(cuda, case, value, where):
     assert torch.equal(torch.isfinite(y), fine) and fine.any() and not fine.all()
     _within(y[fine], ref[fine], tol[fine])
     _no_device_error()
+
+
+# ---------------------------------------------------------------------------------------------- offsets
+@pytest.mark.parametrize("max_q", [0, 2])
+@pytest.mark.parametrize("documents", [1, 3, 40])
+def test_attention_rows_outside_every_document(cuda, documents, max_q):
+    """Rows before the first document and past the last (a call padded to a fixed number of rows) get zeros, and a
+    log-sum-exp of -inf."""
+    from ctmr_b200 import ops
+
+    gen, lead, trail, each = _gen(documents), 33, 150, 2 if max_q else 45
+    used = documents * each
+    rows, heads, dim = lead + used + trail, 4, 72
+    q, k, v = (_randn(gen, rows, heads, dim) for _ in range(3))
+    offsets = torch.arange(documents + 1, device="cuda", dtype=torch.int32) * each + lead
+    wide = torch.full((rows, heads, 96), 7.0, device="cuda", dtype=torch.float16)
+    out, lse = ops.attention(q, k, v, q_offsets=offsets, max_q=max_q, out=wide[..., 8:80], return_lse=True)
+    for part in (slice(0, lead), slice(lead + used, rows)):
+        assert (out[part] == 0).all() and torch.isneginf(lse[part]).all()
+    assert (wide[..., :8] == 7).all() and (wide[..., 80:] == 7).all()
+    for d in range(documents):
+        at = slice(lead + d * each, lead + (d + 1) * each)
+        _check(out[at], lse[at], _rows_ref(q[at], k[at], v[at]), torch.float16)
+    empty = torch.full_like(offsets, 5)  # no document has a row
+    out, lse = ops.attention(q, k, v, q_offsets=empty, max_q=max_q, out=torch.full_like(q, 7.0), return_lse=True)
+    assert (out == 0).all() and torch.isneginf(lse).all()
+    _no_device_error()
