@@ -133,6 +133,13 @@ __global__ void __launch_bounds__(kInnerWarps * 32) adapter_inner_kernel(const L
   griddep_launch_dependents();  // after the wait: what starts now may read all that came before this kernel
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int block = blockIdx.x;
+  if (block == plan.blocks) {  // one more than there are
+    if (blockIdx.y > 0) return;
+    report_offsets(p.offsets, p.segments, p.rows);
+    for (int i = threadIdx.x; i < p.segments; i += blockDim.x)
+      if (p.index[i] >= p.adapters) flag_error(kErrBadOffsets);
+    return;
+  }
   int s, begin, end, adapter;
   if (p.segments <= 32) {  // all of them in one round of loads
     const bool is = lane < p.segments;
@@ -142,14 +149,12 @@ __global__ void __launch_bounds__(kInnerWarps * 32) adapter_inner_kernel(const L
     const int a_s = __shfl_sync(0xffffffffu, a, s), b_s = __shfl_sync(0xffffffffu, b, s);
     adapter = __shfl_sync(0xffffffffu, mine, s);
     begin = min(max(a_s, 0), p.rows), end = min(max(b_s, begin), p.rows);
-    if (begin != a_s || end != b_s) flag_error(kErrBadOffsets);
   } else {
     s = segment_of_tile(p.offsets, p.segments, plan.tile, block, lane);
     segment_range(p.offsets, s, p.rows, begin, end);
     adapter = p.index[s];
   }
   const int tile = block - s, row0 = tile * plan.tile + blockIdx.y * 16;
-  if (adapter >= p.adapters) flag_error(kErrBadOffsets);
   const int lo = max(begin, tile * plan.tile), hi = min(end, (tile + 1) * plan.tile);
   if (tile < 0 || lo >= hi || adapter < 0 || adapter >= p.adapters) return;  // no such block, or none is read
   uint16_t* inner = static_cast<uint16_t*>(p.inner) +
@@ -894,7 +899,7 @@ LinearPlan plan_linear(const LinearParams& p) {
 
 template <bool BF16, int NT>
 cudaError_t launch_inner(const LinearParams& p, const LinearPlan& plan, cudaStream_t stream) {
-  return launch_kernel(adapter_inner_kernel<BF16, NT>, dim3(plan.blocks, plan.tile / 16), dim3(kInnerWarps * 32),
+  return launch_kernel(adapter_inner_kernel<BF16, NT>, dim3(plan.blocks + 1, plan.tile / 16), dim3(kInnerWarps * 32),
                        0, stream, p, plan);
 }
 

@@ -194,6 +194,12 @@ __global__ void __launch_bounds__(Layout<NC>::kThreads, Layout<NC>::kCtas)
   if (p.q_offsets != nullptr) first = p.q_offsets[0], last = p.q_offsets[p.documents];
   Place w;
   int h;
+  if (p.q_offsets != nullptr && blockIdx.x == gridDim.x - 1) {  // one block more than the tiles may need
+    report_offsets(p.q_offsets, p.documents, p.q_tokens);
+    report_offsets(p.k_offsets, p.documents, p.k_tokens);
+    clear_outside(p, first, last, blockIdx.x, gridDim.x);
+    return;
+  }
   const bool mine = find_place<L::kBlock>(p, blockIdx.x, lane, w, h);  // the same answer in every warp
   clear_outside(p, first, last, blockIdx.x, gridDim.x);
   if (!mine) return;
@@ -584,8 +590,8 @@ int launch_attention_packed(const AttentionParams& p, bool bf16, cudaStream_t st
     const int block = p.dim <= 64 ? Layout<1>::kBlock : Layout<2>::kBlock;
     const long long tiles = packed ? p.q_tokens / block + static_cast<long long>(p.documents)
                                    : static_cast<long long>(p.documents) * ((p.q_tokens + block - 1) / block);
-    if (tiles * p.heads > 0x7fffffffLL) return api_fail(CTMR_ERR_UNSUPPORTED, "too many documents and heads");
-    const dim3 grid(static_cast<unsigned>(tiles * p.heads));
+    if (tiles * p.heads >= 0x7fffffffLL) return api_fail(CTMR_ERR_UNSUPPORTED, "too many documents and heads");
+    const dim3 grid(static_cast<unsigned>(tiles * p.heads + packed));
     if (p.dim <= 64)
       e = bf16 ? launch_variant<1, true>(maps, p, grid, stream) : launch_variant<1, false>(maps, p, grid, stream);
     else

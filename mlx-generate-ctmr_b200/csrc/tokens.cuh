@@ -79,6 +79,15 @@ __device__ __forceinline__ void segment_range(const int* offsets, int s, int tot
   if (begin != a || end != b) flag_error(kErrBadOffsets);
 }
 
+// Reports every offset that segment_range would clamp, whether or not a block of the kernel comes to read it (a
+// segment whose offsets make it empty may own no block). By one block.
+__device__ __forceinline__ void report_offsets(const int* offsets, int segments, int total) {
+  for (int s = threadIdx.x; s < segments; s += blockDim.x) {
+    int begin, end;
+    segment_range(offsets, s, total, begin, end);
+  }
+}
+
 // Tiles of `tile` rows that start afresh in each segment, without a table of them: segment s owns the
 // numbers [f(s), f(s + 1)), f(s) = offsets[s] / tile + s, which are at least as many as its tiles
 // (floor(b / t) - floor(a / t) + 1 >= ceil((b - a) / t)), so a grid of total / tile + segments + 1

@@ -222,3 +222,42 @@ def test_attention_rows_outside_every_document(cuda, documents, max_q):
     out, lse = ops.attention(q, k, v, q_offsets=empty, max_q=max_q, out=torch.full_like(q, 7.0), return_lse=True)
     assert (out == 0).all() and torch.isneginf(lse).all()
     _no_device_error()
+
+
+@pytest.mark.parametrize(("q_off", "k_off"), [
+    ([0, 100, 200], [0, 100, 100]), ([0, 100, 100], [0, 100, 200]), ([0, 100, 100], [0, 100, 99]),
+    ([0, 100, 100], [0, -3, 100]), ([0, 60, 40], [0, 50, 100]), ([-1, 60, 100], [0, 50, 100]),
+    ([101, 101, 101], [0, 50, 100]), ([0, 60, 40, 100], [0, 30, 60, 100]),
+])
+@pytest.mark.parametrize("documents", [0, 40])
+def test_attention_reports_every_bad_offset(cuda, documents, q_off, k_off):
+    """Offsets that fall or leave the tensor are reported whether or not their document has queries (with up to 32
+    documents and with more)."""
+    from ctmr_b200 import _lib, ops
+
+    q, k, v = _operands(9, 100, 100, 2, 2, 64, torch.float16)
+    more = [0] * (documents if q_off[0] == 0 else 0)
+    tensors = [torch.tensor([*more, *o], device="cuda", dtype=torch.int32) for o in (q_off, k_off)]
+    ops.attention(q, k, v, q_offsets=tensors[0], k_offsets=tensors[1])
+    assert _lib.device_error(clear=True) == 32
+
+
+@pytest.mark.parametrize("more", [0, 40])
+@pytest.mark.parametrize("rows", [96, 128, 2304])
+def test_adapter_linear_reports_every_bad_number(cuda, rows, more):
+    from ctmr_b200 import _lib, ops
+
+    c = _linear_case(2, [rows], [0], 64, 2310, 8, 2, torch.float16)
+    good = [0] * more
+
+    def call(offsets, index):
+        c["offsets"] = torch.tensor([*good, *offsets], device="cuda", dtype=torch.int32)
+        c["index"] = torch.tensor([*[-1] * len(good), *index], device="cuda", dtype=torch.int32)
+        ops.adapter_linear(**c)
+        return _lib.device_error(clear=True)
+
+    assert call([0, rows, rows], [0, -1]) == 0
+    assert call([0, rows, rows + 200], [0, -1]) == 32   # the last segment begins where the rows end
+    assert call([0, rows, rows - 1], [0, -1]) == 32
+    assert call([0, rows, rows], [0, 2]) == 32          # a segment without rows, an adapter that is not there
+    assert call([0, rows, rows], [2, -1]) == 32
