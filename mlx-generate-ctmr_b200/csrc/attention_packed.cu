@@ -189,7 +189,6 @@ __global__ void __launch_bounds__(Layout<NC>::kThreads, Layout<NC>::kCtas)
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   griddep_wait();
-  griddep_launch_dependents();
   int first = 0, last = p.q_tokens;
   if (p.q_offsets != nullptr) first = p.q_offsets[0], last = p.q_offsets[p.documents];
   Place w;
@@ -228,6 +227,9 @@ __global__ void __launch_bounds__(Layout<NC>::kThreads, Layout<NC>::kCtas)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  // Dependents are released once this block holds its columns: one that allocates ahead of its own wait could take
+  // them otherwise. (A block without a tile releases them by its end.)
+  griddep_launch_dependents();
   const uint32_t tmem = *tmem_slot;  // tile t: S at columns 128 t and 128 t + 64 (P over them), O at kTmemO + 128 t
 
   // Steps of each query tile: the keys that its last query sees. (With a bias all take the longest's, and
