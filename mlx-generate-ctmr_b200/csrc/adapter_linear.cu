@@ -781,7 +781,8 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       place(t, row_tile, m0);
       const int o = m0 + static_cast<int>(rank) * 128 + quarter * 32 + lane, buf = lt & 1;
       const float bias = bias_of(p, BF16, o);
-      if (!mbar_wait_bounded(&acc_full[buf], static_cast<uint32_t>(lt >> 1) & 1u, kErrWaitAcc) || *abort_flag) {
+      if (!mbar_wait_warp(&acc_full[buf], static_cast<uint32_t>(lt >> 1) & 1u, kErrWaitAcc) ||
+          __any_sync(0xffffffffu, *abort_flag)) {
         *abort_flag = 1;
         break;
       }

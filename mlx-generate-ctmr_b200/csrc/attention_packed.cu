@@ -398,10 +398,14 @@ __global__ void __launch_bounds__(Layout<NC>::kThreads, Layout<NC>::kCtas)
     float* maxima = reinterpret_cast<float*>(smem + L::kOffMax) + t * 2 * kTile + row;  // + parity, + half * 128
     const int pair_bar = 1 + t * 4 + (warp & 3);  // the two warps of these queries
     auto meet = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(pair_bar) : "memory"); };
-    auto wait_s = [&](int j) {
-      const bool ok = mbar_wait_bounded(&s_full[t * 2 + (j & 1)], static_cast<uint32_t>(j >> 1) & 1u, kErrWaitAcc);
+    bool ok = true;
+    auto wait_s = [&](int j) {  // (after a failure without waiting: the other half meets here)
+      // By the whole warp: tcgen05.ld wants its lanes together, and each would leave a wait by itself. (One try ahead
+      // of the loop, 8,192 tokens of 8 heads of 32 and 128: 224 and 233 us; the loop alone: 228 and 256.)
+      uint64_t* bar = &s_full[t * 2 + (j & 1)];
+      const uint32_t parity = static_cast<uint32_t>(j >> 1) & 1u;
+      if (!__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) ok = ok && mbar_wait_warp(bar, parity, kErrWaitAcc);
       tc_fence_after();
-      return ok;
     };
     const int lim = limit_of(p, w, i) - half * kPart, place = i + w.k_len - w.q_len - half * kPart;
     const float scale = p.scale * kLog2e;
@@ -409,9 +413,8 @@ __global__ void __launch_bounds__(Layout<NC>::kThreads, Layout<NC>::kCtas)
     const float slope = BIAS ? p.slopes[h] * kLog2e : 0.f;
     const float unit = CAP || BIAS ? 1.f : scale;  // what turns s below into base-2 scores
     float m = -INFINITY, l = 0.f;  // m: what P is relative to; the maximum or up to 2^8 below; l: of this half
-    bool ok = true;
     for (int j = 0; j < n; ++j) {
-      ok = ok && wait_s(j);  // (on a failure the loop goes on without waiting: the other half meets here)
+      wait_s(j);
       const uint32_t t_s = tmem + lanes + t * 128 + (j & 1) * 64;
       const int key0 = step_at(j) * kStep;
       float s[kPart];
@@ -453,7 +456,7 @@ __global__ void __launch_bounds__(Layout<NC>::kThreads, Layout<NC>::kCtas)
         if (grow) m = top;
         l *= f;
         if (j > 0) {  // PV(j - 1) has to be done; nothing writes O then until P(j) is handed over
-          ok = ok && wait_s(j + 1);
+          wait_s(j + 1);
           for (int c = half * 32; c < p.dim; c += 64) {
             float o[32];
             tmem_ld32(t_o + c, o);
@@ -488,7 +491,7 @@ __global__ void __launch_bounds__(Layout<NC>::kThreads, Layout<NC>::kCtas)
       l += sum[0].x + sum[0].y;
     }
     if (n > 0) {
-      ok = ok && wait_s(n + 1);  // PV(n - 1)
+      wait_s(n + 1);  // PV(n - 1)
       maxima[(n & 1) * kParity + half * kTile] = l;
       meet();
       l += maxima[(n & 1) * kParity + (half ^ 1) * kTile];

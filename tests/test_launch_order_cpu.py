@@ -35,3 +35,14 @@ def test_dependents_are_released_after_the_allocation(body):
     alloc, freed = body.index("tmem_alloc"), body.find("griddep_launch_dependents")
     assert freed > alloc
     assert "__syncthreads()" in body[alloc:freed]  # all of the block's warps are past it
+
+
+@pytest.mark.parametrize("name", ["attention_packed", "adapter_linear"])
+def test_warps_meet_between_a_wait_and_tensor_memory(name):
+    """``tcgen05.ld`` and ``.st`` are for a whole warp at once; a wait that each lane leaves by itself does not
+    bring the lanes back together, ``mbar_wait_warp`` does."""
+    text = re.sub(r"//[^\n]*", "", (CSRC / f"{name}.cu").read_text())
+    loads = [m.start() for m in re.finditer(r"tmem_ld(16|32)\(", text)]
+    assert len(loads) >= 3
+    for at in loads:
+        assert re.findall(r"mbar_wait_\w+", text[:at])[-1] == "mbar_wait_warp"
