@@ -18,6 +18,7 @@
 // Outputs as lanes: a warp stores 32 adjacent outputs of a row, and few rows (serving) use few
 // columns: the tensor core then streams W at the memory's rate.
 #include <atomic>
+#include <cmath>
 
 #include "capi_internal.cuh"
 #include "ctmr_b200.h"
@@ -875,20 +876,35 @@ int encode(CUtensorMap* map, const void* base, bool bf16, int rank, long long d0
 // inputs. CTA pairs of 256 x 256, which overlap a tile's stores with the next one's products: 8 in all and 0.62 per
 // block. (617 rows of 512 -> 1,536: tiles of 64 rows 6.0, of 128 8.2, of 32 9.1, pairs 10.6; 617 rows of
 // 4,096 -> 4,096: pairs 29, tiles of 128 41.)
+// Adapters, fitted to 64 to 8,192 rows in segments of 1 to 256 with ranks of 16 to 128: a block of one CTA's tile 0.45
+// (0.65 for two halves of rank), a pair's 0.27 (0.52), and 0.012 per CTA of the inner products, of which there are
+// tile / 16 to every block of t, most of them idle where segments are short. The best plan was taken within 5 %.
+// (4,096 one-row segments of rank 16: 4,096 -> 4,096 tiles of 64 rows 1,048, pairs 1,274; 512 -> 1,536 tiles of 16
+// rows 382, pairs 872. With rank 128 their t takes 68 and 17 MB where a pair's takes 270.)
 LinearPlan plan_linear(const LinearParams& p) {
   LinearPlan plan{};
   const int sms = device_sm_count(), kb = (p.in + kK - 1) / kK;
   auto waves = [](long long n, int at_once) { return static_cast<float>((n + at_once - 1) / at_once); };
+  const bool wide = p.rank > kHalf;
+  // Adapter blocks that a tile meets, if the segments' borders lie evenly; and what the inner products add.
+  auto blocks = [&](int tile) {
+    const float per = 1.f + static_cast<float>(p.segments - 1) / static_cast<float>((p.rows + tile - 1) / tile);
+    return p.segments > 0 ? fminf(per, static_cast<float>(tile)) : 0.f;
+  };
+  auto inner = [&](int tile) {
+    return p.segments > 0 ? 0.012f * (tile / 16) * static_cast<float>((p.rows + tile - 1) / tile + p.segments - 1) : 0.f;
+  };
   const long long pair_tiles = ((p.out + 255LL) / 256) * ((p.rows + 255LL) / 256);
-  float best = 8.f + waves(pair_tiles, sms / 2) * kb * 0.62f;
+  float best = 8.f + inner(256) + waves(pair_tiles, sms / 2) * (kb * 0.62f + blocks(256) * (wide ? 0.52f : 0.27f));
   plan.tile = kPairRows, plan.split = 0, plan.out_tiles = (p.out + 255) / 256;
   for (int tile = 16; tile <= 128; tile *= 2) {
     if (tile > 16 && tile / 2 >= p.rows) break;
     const long long tiles = ((p.out + 127LL) / 128) * ((p.rows + tile - 1LL) / tile);
     for (int split = 1; split <= 8 && split <= kb; split *= 2) {
+      const float adapters = p.segments > 0 ? fmaxf(blocks(tile) / split, 1.f) * (wide ? 0.65f : 0.45f) : 0.f;
       const float one = 2.8f + 0.032f * tile + (split > 1 ? 0.8f + 0.01f * tile : 0.f) +
-                        static_cast<float>(kb) / split * (0.32f + 0.0011f * tile);
-      const float t = waves(tiles * split, sms) * one;
+                        static_cast<float>(kb) / split * (0.32f + 0.0011f * tile) + adapters;
+      const float t = waves(tiles * split, sms) * one + inner(tile);
       if (t < best) best = t, plan.tile = tile, plan.split = split, plan.out_tiles = (p.out + 127) / 128;
     }
   }

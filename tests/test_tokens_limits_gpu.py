@@ -261,3 +261,15 @@ def test_adapter_linear_reports_every_bad_number(cuda, rows, more):
     assert call([0, rows, rows - 1], [0, -1]) == 32
     assert call([0, rows, rows], [0, 2]) == 32          # a segment without rows, an adapter that is not there
     assert call([0, rows, rows], [2, -1]) == 32
+
+
+@pytest.mark.parametrize(("inner", "outer", "rank", "lengths"), [
+    (512, 1536, 16, [1] * 4096), (4096, 520, 128, [1] * 1000), (256, 384, 72, [3] * 700), (72, 264, 8, [0, 1, 0] * 1500),
+])
+def test_adapter_linear_many_short_segments(cuda, inner, outer, rank, lengths):
+    """Hundreds to thousands of requests of a row or a few."""
+    from ctmr_b200 import ops
+
+    c = _linear_case(inner, lengths, [(5 * i) % 24 - 1 for i in range(len(lengths))], inner, outer, rank, 23, torch.bfloat16)
+    _within(ops.adapter_linear(**c), *_linear_ref(c))
+    _no_device_error()
