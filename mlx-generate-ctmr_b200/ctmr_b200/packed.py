@@ -65,6 +65,11 @@ def packed_self_attention_tokens(tokens: torch.Tensor, grid: PackedGrid, weights
     ``(inv_freq, sections)`` for three axes (``ops.axis_frequencies``).
     """
     dt = tokens.dtype
+    if tokens.dim() != 2 or tokens.shape[0] != grid.starts[-1]:
+        raise ValueError(f"tokens {tuple(tokens.shape)} where the grid has {grid.starts[-1]} rows")
+    used = ("qkv", "out_proj") if include_fc else ("qkv",)
+    if unknown := sorted(set(adapters or ()) - set(used)):
+        raise ValueError(f"adapters for {unknown}; this block has {', '.join(used)}")
     names = ("q", "k", "v")
     w_qkv = fast_b200._stacked_dense(tuple(weights[f"{prefix}.to_{n}.weight"] for n in names), dt)
     b_qkv = fast_b200._stacked_dense(tuple(weights[f"{prefix}.to_{n}.bias"] for n in names), dt) if qkv_bias else None

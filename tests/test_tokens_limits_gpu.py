@@ -273,3 +273,31 @@ def test_adapter_linear_many_short_segments(cuda, inner, outer, rank, lengths):
     c = _linear_case(inner, lengths, [(5 * i) % 24 - 1 for i in range(len(lengths))], inner, outer, rank, 23, torch.bfloat16)
     _within(ops.adapter_linear(**c), *_linear_ref(c))
     _no_device_error()
+
+
+# ---------------------------------------------------------------------------------------------- the packed block
+def test_packed_block_refuses_what_it_would_ignore(cuda):
+    """Adapters under names that the block does not have, and tokens that are not the grid's."""
+    from ctmr_b200 import ops, packed
+
+    gen, c = _gen(1), 32
+    weights = {f"attn.{n}.{part}": _randn(gen, *((c, c) if part == "weight" else (c,)))
+               for n in ("to_q", "to_k", "to_v", "out_proj") for part in ("weight", "bias")}
+    grid = packed.PackedGrid.of([(2, 2, 2), (1, 2, 3)])
+    tokens, index = _randn(gen, 14, c), torch.tensor([0, -1], device="cuda", dtype=torch.int32)
+
+    def stack(outputs):
+        return ops.stack_adapters([(_randn(gen, 8, c), _randn(gen, outputs, 8), 1.0)], dtype=torch.float16)
+
+    def run(tokens, include_fc=True, **adapters):
+        return packed.packed_self_attention_tokens(tokens, grid, weights, heads=2, scale=0.25, include_fc=include_fc,
+                                                   adapters=adapters, index=index)
+
+    assert run(tokens, qkv=stack(3 * c), out_proj=stack(c)).shape == (14, c)
+    assert run(tokens, include_fc=False, qkv=stack(3 * c)).shape == (14, c)
+    for bad in (dict(to_q=stack(c)), dict(qkv=stack(3 * c), proj=stack(c)), dict(include_fc=False, out_proj=stack(c))):
+        with pytest.raises(ValueError, match="adapters for"):
+            run(tokens, **bad)
+    for bad in (tokens[:13], torch.cat((tokens, tokens)), tokens[None]):
+        with pytest.raises(ValueError, match="rows"):
+            run(bad)
