@@ -301,3 +301,103 @@ def test_packed_block_refuses_what_it_would_ignore(cuda):
     for bad in (tokens[:13], torch.cat((tokens, tokens)), tokens[None]):
         with pytest.raises(ValueError, match="rows"):
             run(bad)
+
+
+# ---------------------------------------------------------------------------------------------- 17 to 128 rows
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("mode", ["plain", "causal", "all"])
+@pytest.mark.parametrize(("lq", "lk", "heads", "kv_heads", "dim"), [
+    (1, 4000, 17, 1, 64), (2, 4001, 16, 1, 32), (1, 3000, 20, 1, 80), (4, 4100, 16, 2, 128),  # one group of 17 to 32 rows
+    (1, 5000, 33, 1, 40), (11, 4000, 6, 2, 64), (8, 6000, 16, 2, 64),                         # two and more, heads to 64
+    (3, 4000, 11, 1, 128), (16, 5003, 4, 1, 72), (16, 9000, 8, 1, 128), (128, 6000, 1, 1, 96), (42, 8000, 3, 1, 104),
+])
+def test_attention_few_rows_of_a_key_head(cuda, lq, lk, heads, kv_heads, dim, mode, dtype):
+    """17 to 128 rows of a key head over long keys, in groups of 32: queries and heads that start inside a group."""
+    from ctmr_b200 import ops
+
+    q, k, v = _operands(lq + dim, lq, lk, heads, kv_heads, dim, dtype)
+    kw: dict = dict(causal=mode != "plain")
+    if mode == "all":
+        kw |= dict(cap=5.0, scale=2 * dim ** -0.5, slopes=torch.exp2(-torch.arange(heads, device="cuda") / 4.0) * 0.01)
+    pre = lk - lq + 3 if mode == "all" else 0
+    call = lambda: ops.attention(q, k, v, return_lse=True, **kw, prefix=torch.tensor(  # noqa: E731
+        [pre], device="cuda", dtype=torch.int32) if pre else None)
+    out, lse = call()
+    _check(out, lse, _rows_ref(q, k, v, **kw, prefix=pre), dtype)
+    assert "attention_few_kernel" in _kernels(call)
+    _no_device_error()
+
+
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("cap", [0.0, 20.0])
+@pytest.mark.parametrize(("batch", "lk", "heads", "kv_heads", "dim"), [
+    (200, 100, 4, 2, 64), (1, 2000, 8, 8, 128), (1, 2000, 16, 1, 72), (3, 1300, 24, 1, 40),
+])
+def test_attention_few_log_sum_exp_is_fp32(cuda, batch, lk, heads, kv_heads, dim, cap, dtype):
+    """One CTA to a request (200 of them), and keys split over a cluster."""
+    from ctmr_b200 import ops
+
+    gen = _gen(lk)
+    q = _randn(gen, batch, 1, heads, dim, dtype=dtype)
+    k, v = (_randn(gen, batch, lk, kv_heads, dim, dtype=dtype) for _ in range(2))
+    call = lambda: ops.attention(q, k, v, cap=cap, return_lse=True)  # noqa: E731
+    out, lse = call()
+    for b in range(0, batch, 37):
+        _check(out[b], lse[b], _rows_ref(q[b], k[b], v[b], cap=cap), dtype)
+    assert "attention_few_kernel" in _kernels(call)
+
+
+# ---------------------------------------------------------------------------------------------- layouts
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize(("lq", "lk", "heads", "kv_heads", "dim"), [
+    (150, 200, 4, 2, 64), (130, 131, 2, 2, 72), (1, 700, 8, 2, 128), (2, 4000, 16, 1, 40),
+])
+def test_attention_head_major_and_expanded(cuda, lq, lk, heads, kv_heads, dim, dtype):
+    """(batch, head, token, channel) tensors transposed, one context expanded over the batch, and one key head's
+    values expanded over the heads: the bits of the dense copies."""
+    from ctmr_b200 import ops
+
+    gen, batch = _gen(dim), 3
+    q = _randn(gen, batch, heads, lq, dim, dtype=dtype).transpose(1, 2)
+    k, v = (_randn(gen, batch, kv_heads, lk, dim, dtype=dtype).transpose(1, 2) for _ in range(2))
+    kw = dict(k_lengths=torch.tensor([lk, lk // 2, 1], device="cuda", dtype=torch.int32), return_lse=True)
+
+    def same(q, k, v):
+        out, lse = ops.attention(q, k, v, **kw)
+        dense, dense_lse = ops.attention(*(t.contiguous() for t in (q, k, v)), **kw)
+        assert torch.equal(out, dense) and torch.equal(lse, dense_lse)
+        for b, n in enumerate((lk, lk // 2, 1)):
+            _check(out[b], lse[b], _rows_ref(q[b], k[b, :n], v[b, :n]), dtype)
+
+    same(q, k, v)
+    same(q, k[:1].expand(batch, -1, -1, -1), v[1:2].expand(batch, -1, -1, -1))
+    same(q[:1].expand(batch, -1, -1, -1), k, v)
+    same(q, k, v[:, :, :1].expand(-1, -1, kv_heads, -1))
+    same(q[:, :, :1].expand(-1, -1, heads, -1), k[:, :, :1].expand(-1, -1, kv_heads, -1), v)
+    out = torch.full((batch, heads, lq, dim), 7.0, device="cuda", dtype=dtype).transpose(1, 2)
+    assert ops.attention(q, k, v, out=out, **kw)[0] is out
+    assert torch.equal(out, ops.attention(q, k, v, **kw)[0])
+    packed = [t.flatten(0, 1) for t in (q, k, v)]  # copies: token-major; then head-major packed rows
+    major = [t.transpose(0, 1).contiguous().transpose(0, 1) for t in packed]
+    offsets = dict(q_offsets=_offsets([lq] * batch), k_offsets=_offsets([lk] * batch))
+    assert torch.equal(ops.attention(*packed, **offsets), ops.attention(*major, **offsets))
+    _no_device_error()
+
+
+def test_adapter_linear_captured(cuda):
+    """Both launches in a graph, for the small and the pair kernel; replays on changed inputs follow them."""
+    from ctmr_b200 import ops
+
+    for rows, outer in ((40, 200), (2304, 2310)):
+        c = _linear_case(rows, [rows // 3, rows - rows // 3], [1, 0], 136, outer, 24, 2, torch.float16)
+        eager = ops.adapter_linear(**c)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            captured = ops.adapter_linear(**c)
+        for _ in range(2):
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(captured, eager)
+            c["x"].copy_(c["x"].flip(0))
+            eager = ops.adapter_linear(**c)
