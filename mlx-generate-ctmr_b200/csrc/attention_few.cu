@@ -18,6 +18,8 @@ namespace ctmr {
 namespace {
 
 constexpr int kWarps = 4, kThreads = kWarps * 32 + 32;  // four warps compute, one loads
+// P and its sum are held 2^15 larger: fp16 rounds numbers below 2^-14 ever more coarsely.
+constexpr float kLift = 15.f, kDrop = 1.f / 32768.f;
 constexpr int kKeys = 16, kStep = kWarps * kKeys;         // keys per warp and per step
 
 template <bool BF16>
@@ -225,7 +227,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         for (int n = 0; n < 2; ++n)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const float from = m[t][e] == -INFINITY ? 0.f : m[t][e];
+            const float from = m[t][e] == -INFINITY ? 0.f : m[t][e] - kLift;
             const float x0 = exp2_unit(s[n][2 * e] - from), x1 = exp2_unit(s[n][2 * e + 1] - from);
             l[t][e] = n == 0 ? fmaf(l[t][e], f[e], x0 + x1) : l[t][e] + (x0 + x1);
             a[n * 2 + e] = pack2<BF16>(x0, x1);
@@ -302,7 +304,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     *reinterpret_cast<uint2*>(out + d) =
         make_uint2(pack2<BF16>(sum.x * inv, sum.y * inv), pack2<BF16>(sum.z * inv, sum.w * inv));
     if (p.lse != nullptr && d == 0)
-      p.lse[(lse_at + i) * p.heads + h] = total == 0.f ? -INFINITY : (big + log2f(total)) * 0.6931471805599453f;
+      p.lse[(lse_at + i) * p.heads + h] = total == 0.f ? -INFINITY : (big + log2f(total * kDrop)) * 0.6931471805599453f;
   };
   const int quads = p.dim / 4, work = rows * quads;
   if (splits == 1) {

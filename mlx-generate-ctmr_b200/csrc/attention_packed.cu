@@ -15,8 +15,8 @@
 //   S(0) S(1) | PV(0) S(2) | PV(1) S(3) | ...
 // O stays in TMEM; it is
 // rescaled (by the softmax threads, which hold m) only where a row's maximum has grown by more than 2^8
-// since the last time: until then P may exceed one, up to 2^8, which neither 16-bit type minds, and
-// the sum of P is kept in fp32 with the same m.
+// since the last time: until then P may exceed one, up to 2^8 (2^15 as it is held), which neither 16-bit type
+// minds, and the sum of P is kept in fp32 with the same m.
 //
 // With a distance bias the steps are visited from the queries' own place outwards, first towards the first
 // key, then towards the last: in order of keys the maximum grew with every step that came nearer, and the
@@ -36,6 +36,9 @@ constexpr int kStep = 64;      // keys per step
 constexpr int kPart = 32;      // of them per softmax thread
 constexpr uint32_t kQChunk = kTile * 128, kKChunk = kStep * 128;  // rows of 64 16-bit channels
 constexpr float kRescale = 8.f;  // log2 of the growth that O and the sum are rescaled for
+// P and its sum are held 2^7 larger: fp16 rounds numbers below 2^-14 ever more coarsely (weights of 2^-20 to one
+// part in 32), and 2^(8 + 7) is the most that it holds.
+constexpr float kLift = 7.f, kDrop = 1.f / 128.f;
 
 // NC chunks of 64 channels per row (two above 64 channels), as many query tiles. V in a ring of four steps, K,
 // which runs two steps ahead, in one of five: K(j + 2) takes the place of K(j - 3), V(j) of V(j - 4); both are
@@ -69,7 +72,7 @@ __device__ __forceinline__ float max_or_nan(float a, float b) {
   return c;
 }
 
-// 2^x of a pair, x <= 8, on the FMA pipe: x = n + f with n the nearest integer (the low bits of x plus
+// 2^x of a pair, x <= 15, on the FMA pipe: x = n + f with n the nearest integer (the low bits of x plus
 // 1.5 * 2^23) and |f| <= 1/2, 2^f by a quartic (least maximum relative error on that interval, 2.6e-6, mean
 // error 4e-8: far below P's rounding, and small enough for the log-sum-exp, whose sum it enters; a cubic's
 // 7.5e-5 would show there), n added to the exponent. Zero below 2^-127, where that leaves no positive bits: a clamp
@@ -469,7 +472,7 @@ __global__ void __launch_bounds__(Layout<NC>::kThreads, Layout<NC>::kCtas)
           }
         }
       }
-      const float base = m == -INFINITY ? 0.f : -m;
+      const float base = m == -INFINITY ? 0.f : kLift - m;
       const float2 u2 = make_float2(unit, unit), b2 = make_float2(base, base);
       float2 sum[2] = {};
       uint32_t r[kPart / 2];
@@ -518,7 +521,7 @@ __global__ void __launch_bounds__(Layout<NC>::kThreads, Layout<NC>::kCtas)
       }
     }
     if (p.lse != nullptr && half == 0 && i < w.q_len)
-      p.lse[(w.row0 + i) * p.heads + h] = some ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY;
+      p.lse[(w.row0 + i) * p.heads + h] = some ? (m + log2f(l * kDrop)) * 0.6931471805599453f : -INFINITY;
   }
 
   tc_fence_before();

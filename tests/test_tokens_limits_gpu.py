@@ -401,3 +401,17 @@ def test_adapter_linear_captured(cuda):
             assert torch.equal(captured, eager)
             c["x"].copy_(c["x"].flip(0))
             eager = ops.adapter_linear(**c)
+
+
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize(("form", "case"), FORMS)
+def test_attention_small_weights_keep_their_bits(cuda, form, case, dtype):
+    """One key far above the others, whose values are zero: the output is what weights of 2^-18 to 2^-20 of it add up
+    to, and each of them is rounded to the type's relative precision (below 2^-14 fp16 by itself has fewer bits)."""
+    from ctmr_b200 import ops
+
+    q, k, v = _operands(9, *case, dtype)
+    q[..., 0], k[:, :, 0], k[:, :, 1:] = 1.0, 0.0, k[:, :, 1:] * 0.02
+    k[5, :, 0], v[5] = 19 * math.log(2), 0.0
+    out, lse = ops.attention(q, k, v, scale=1.0, return_lse=True)
+    _check(out, lse, _rows_ref(q, k, v, scale=1.0), dtype)
