@@ -10,7 +10,10 @@ logarithm's own 2^-22: ``3e-6 + (2^-22 + 2e-7) S + 2^-22 |lse|``.
 
 from __future__ import annotations
 
+import ctypes
 import math
+import tempfile
+from pathlib import Path
 
 import pytest
 import torch
@@ -50,15 +53,17 @@ def _check(out, lse, ref, dtype):
 
 
 def _kernels(call):
-    """Names of the kernels that a call launches."""
-    from torch.profiler import ProfilerActivity, profile
-
+    """What a call launches, by the driver's text of a graph that it is captured in."""
     call()
     torch.cuda.synchronize()
-    with profile(activities=[ProfilerActivity.CUDA]) as prof:
+    graph = torch.cuda.CUDAGraph(keep_graph=True)
+    with torch.cuda.graph(graph):
         call()
-        torch.cuda.synchronize()
-    return " ".join(e.key for e in prof.key_averages())
+    with tempfile.TemporaryDirectory() as where:
+        path = Path(where) / "graph.dot"
+        driver = ctypes.CDLL("libcuda.so.1")
+        assert driver.cuGraphDebugDotPrint(ctypes.c_void_p(graph.raw_cuda_graph()), str(path).encode(), 1) == 0
+        return path.read_text()
 
 
 # Each form's cases: query tokens, key tokens, heads, key heads, head size.
@@ -320,8 +325,8 @@ def test_attention_few_rows_of_a_key_head(cuda, lq, lk, heads, kv_heads, dim, mo
     if mode == "all":
         kw |= dict(cap=5.0, scale=2 * dim ** -0.5, slopes=torch.exp2(-torch.arange(heads, device="cuda") / 4.0) * 0.01)
     pre = lk - lq + 3 if mode == "all" else 0
-    call = lambda: ops.attention(q, k, v, return_lse=True, **kw, prefix=torch.tensor(  # noqa: E731
-        [pre], device="cuda", dtype=torch.int32) if pre else None)
+    prefix = torch.tensor([pre], device="cuda", dtype=torch.int32) if pre else None
+    call = lambda: ops.attention(q, k, v, return_lse=True, **kw, prefix=prefix)  # noqa: E731
     out, lse = call()
     _check(out, lse, _rows_ref(q, k, v, **kw, prefix=pre), dtype)
     assert "attention_few_kernel" in _kernels(call)
