@@ -49,15 +49,7 @@ struct LinearPlan {
 // ---------------------------------------------------------------- segments of a row tile
 // The last s with offsets[s] <= row (0 if none), by a warp.
 __device__ __forceinline__ int segment_at_row(const int* offsets, int segments, int row, int lane) {
-  int lo = 0, n = segments;
-  while (n > 1) {
-    const int step = (n + 31) / 32;
-    const bool ok = lane == 0 || (lane * step < n && offsets[lo + lane * step] <= row);
-    const int last = 31 - __clz(__ballot_sync(0xffffffffu, ok));
-    n = min(step, n - last * step);
-    lo += last * step;
-  }
-  return lo;
+  return last_segment(segments, lane, [&](int s) { return offsets[s] <= row; });
 }
 
 // The segments with an adapter that meet rows [r0, r1), in order; used by a whole warp. The first 32 are
@@ -104,20 +96,6 @@ struct AdapterScan {
 };
 
 // ---------------------------------------------------------------- inner products
-template <bool BF16>
-__device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  if constexpr (BF16)
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  else
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
 // One CTA: 16 rows of one block of t, all ranks (at most NT * 8). Its sixteen warps take the input in turn,
 // 32 inputs at a time, and add up in shared memory. Both operands come straight from memory, 16 bytes a
 // thread: a thread's eight inputs are dealt to two product steps, the same way for x and down, which
@@ -237,7 +215,8 @@ struct SmallSmem {
   static constexpr int kStages = 196608 / kStageBytes;
   static constexpr uint32_t kOffBar = kStages * kStageBytes;
   static constexpr uint32_t kBytes = kOffBar + 512 + 1024;  // + barriers + alignment slack
-  static_assert(BN * 512u <= kOffBar, "the partial sums fit in the stages");
+  // (A warp reads columns in batches that span BN / 4: at a split of eight the last share's reach past the tile.)
+  static_assert((BN + BN / 8) * 512u <= kOffBar, "the partial sums and what is read past them lie in the stages");
 };
 
 // A block as the producer hands it to the MMA thread beside its data: product steps (16 inputs each),
@@ -543,7 +522,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1)
           const uint32_t at = cluster_addr(smem, z) + (c * 128 + lane * 4) * 4;
 #pragma unroll
           for (int e = 0; e < kBatch; ++e) {
-            const float4 t = ld_cluster4(at + e * 4 * 512);  // past the share: still inside the tile
+            const float4 t = ld_cluster4(at + e * 4 * 512);  // past the share: anything, and not used
             v[e].x += t.x, v[e].y += t.y, v[e].z += t.z, v[e].w += t.w;
           }
         }
@@ -572,7 +551,8 @@ __global__ void __launch_bounds__(kSmallThreads, 1)
         if (p.segments > 0) {
           float z = 0.f;
 #pragma unroll
-          for (int e = 0; e < kBatch; ++e) z = fmaf(v[e].x, 0.f, fmaf(v[e].y, 0.f, fmaf(v[e].z, 0.f, fmaf(v[e].w, 0.f, z))));
+          for (int e = 0; e < kBatch; ++e)
+            if (c + 4 * e < c_end) z = fmaf(v[e].x, 0.f, fmaf(v[e].y, 0.f, fmaf(v[e].z, 0.f, fmaf(v[e].w, 0.f, z))));
           if (__any_sync(0xffffffffu, z != 0.f)) {
             unsigned bad = 0;
 #pragma unroll

@@ -22,20 +22,6 @@ constexpr int kWarps = 4, kThreads = kWarps * 32 + 32;  // four warps compute, o
 constexpr float kLift = 15.f, kDrop = 1.f / 32768.f;
 constexpr int kKeys = 16, kStep = kWarps * kKeys;         // keys per warp and per step
 
-template <bool BF16>
-__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  if constexpr (BF16)
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  else
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -195,8 +181,8 @@ __global__ void __launch_bounds__(kThreads, 2)
           for (int n = 0; n < 2; ++n) {
             uint32_t b[4];
             ldmatrix4(b, k_at + (w >> 1) * L::kChunk + n * 8 * 128 + (((w & 1) * 4 + mat) ^ in) * 16);
-            mma<BF16>(s[n], a0, b[0], b[1]);
-            mma<BF16>(s[n], a1, b[2], b[3]);
+            mma_16816<BF16>(s[n], a0, b[0], b[1]);
+            mma_16816<BF16>(s[n], a1, b[2], b[3]);
           }
         }
         if (capped) cap_scores(reinterpret_cast<float(&)[8]>(s), cap);
@@ -250,8 +236,8 @@ __global__ void __launch_bounds__(kThreads, 2)
               b[i] &= (key < k1 ? 0xffffu : 0u) | (key + 1 < k1 ? 0xffff0000u : 0u);
             }
           }
-          mma<BF16>(o[t][u], a, b[0], b[1]);
-          mma<BF16>(o[t][u + 1], a, b[2], b[3]);
+          mma_16816<BF16>(o[t][u], a, b[0], b[1]);
+          mma_16816<BF16>(o[t][u + 1], a, b[2], b[3]);
         }
       }
       __syncwarp();

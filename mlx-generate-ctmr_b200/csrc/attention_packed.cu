@@ -109,8 +109,9 @@ __device__ __forceinline__ int limit_of(const AttentionParams& p, const Place& w
 
 // Up to 32 documents: their tiles in order of falling key counts, each document's heads together, so that no
 // long one starts when the others are done (seven volumes of 105 to 2,048 tokens, 8 heads of 32: 61 us in order
-// of documents, 53 us so; four causal ones of 1 to 2,300 tokens, 16 heads of 128: 101 and 83 us). By a whole
-// warp; false where `id` is past the last tile.
+// of documents, 53 us so; four causal ones of 1 to 2,300 tokens, 16 heads of 128: 101 and 83 us). More documents
+// than a warp has lanes keep their order (four of 2,048 tokens and 28 of 64, and the same with an empty one more: 65
+// and 80 us with 8 heads of 32, 152 and 171 with 16 of 128). By a whole warp; false where `id` is past the last tile.
 template <int kBlock>
 __device__ __forceinline__ bool longest_first(const AttentionParams& p, int id, int lane, int& doc, int& head,
                                               int& tile) {

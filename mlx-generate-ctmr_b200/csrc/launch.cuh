@@ -7,9 +7,19 @@
 // returns once the preceding grid has completed and its writes are visible, so
 // the ordering of a plain launch is kept while the launch latency and the
 // set-up overlap the predecessor's tail. Each kernel signals
-// griddep_launch_dependents() right away: its successor may then be scheduled
-// as soon as this grid's last blocks are resident. Inside a CUDA-graph capture
-// the attribute becomes a programmatic edge. CTMR_DISABLE_PDL=1 turns it off.
+// griddep_launch_dependents() right away (one that takes tensor memory once its
+// block holds it): its successor may then be scheduled as soon as this grid's
+// last blocks are resident.
+//
+// One pair of kernels goes further: adapter_linear's product kernels, behind
+// their inner products, read x, the weight, the offsets and the bias before the
+// wait, and may write rows of y that no adapter meets. That is in order because
+// the inner kernel waits before it signals (so everything older is complete when
+// the product starts), reads x alone of these and writes none, and because every
+// block of the product waits before it ends.
+//
+// Inside a CUDA-graph capture the attribute becomes a programmatic edge.
+// CTMR_DISABLE_PDL=1 turns it off.
 #pragma once
 
 #include <cuda_runtime.h>

@@ -88,6 +88,21 @@ __device__ __forceinline__ void report_offsets(const int* offsets, int segments,
   }
 }
 
+// The last s in [0, n) that `holds` for, by a whole warp: it holds up to some s and not after (it is not asked for 0,
+// which is the answer where it holds for none). Log32(n) loads.
+template <typename Holds>
+__device__ __forceinline__ int last_segment(int n, int lane, Holds holds) {
+  int lo = 0;  // the answer lies in [lo, lo + n)
+  while (n > 1) {
+    const int step = (n + 31) / 32;
+    const bool ok = lane == 0 || (lane * step < n && holds(lo + lane * step));
+    const int last = 31 - __clz(__ballot_sync(0xffffffffu, ok));
+    n = min(step, n - last * step);
+    lo += last * step;
+  }
+  return lo;
+}
+
 // Tiles of `tile` rows that start afresh in each segment, without a table of them: segment s owns the
 // numbers [f(s), f(s + 1)), f(s) = offsets[s] / tile + s, which are at least as many as its tiles
 // (floor(b / t) - floor(a / t) + 1 >= ceil((b - a) / t)), so a grid of total / tile + segments + 1
@@ -95,16 +110,22 @@ __device__ __forceinline__ void report_offsets(const int* offsets, int segments,
 // f(s) <= id; f grows strictly, so a 32-way search by a warp finds it in log32(segments) loads.
 // Returns the segment, all lanes of the warp together.
 __device__ __forceinline__ int segment_of_tile(const int* offsets, int segments, int tile, int id, int lane) {
-  int lo = 0, n = segments;  // the answer lies in [lo, lo + n)
-  while (n > 1) {
-    const int step = (n + 31) / 32;
-    const int s = lo + lane * step;
-    const bool ok = lane == 0 || (lane * step < n && max(offsets[s], 0) / tile + s <= id);
-    const int last = 31 - __clz(__ballot_sync(0xffffffffu, ok));
-    n = min(step, n - last * step);
-    lo += last * step;
-  }
-  return lo;
+  return last_segment(segments, lane, [&](int s) { return max(offsets[s], 0) / tile + s <= id; });
+}
+
+// d += a b, 16 x 8 x 16, 16-bit operands, fp32 sums.
+template <bool BF16>
+__device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (BF16)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
 // ---------------------------------------------------------------- 16-bit values
