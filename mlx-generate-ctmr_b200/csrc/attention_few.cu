@@ -84,8 +84,8 @@ __global__ void __launch_bounds__(kThreads, 2)
     if (q_len > p.max_q) flag_error(kErrBadOffsets);
     q_at = qb * p.q_token, o_at = qb * p.o_token, lse_at = qb, k_row = kb;
     const long long block = (static_cast<long long>(blockIdx.z) * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x;
-    clear_outside(p, p.q_offsets[0], p.q_offsets[p.documents], block,
-                  static_cast<long long>(gridDim.x) * gridDim.y * gridDim.z);
+    if (warp == kWarps)  // the one that loads; the queries are loaded by all
+      clear_outside(p, block, static_cast<long long>(gridDim.x) * gridDim.y * gridDim.z, lane);
   } else {
     if (p.k_lengths != nullptr) {
       const int n = p.k_lengths[doc];

@@ -124,14 +124,14 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 }
 
 // Rows of a packed output before the first document and past the last (q_offsets' ends): zeros, and a log-sum-exp
-// of -infinity. Every block of the grid takes its share.
-__device__ __forceinline__ void clear_outside(const AttentionParams& p, int first, int last, long long block,
-                                              long long blocks) {
-  first = min(max(first, 0), p.q_tokens), last = min(max(last, 0), p.q_tokens);
+// of -infinity. One warp of every block of the grid takes its share.
+__device__ __forceinline__ void clear_outside(const AttentionParams& p, long long block, long long blocks, int lane) {
+  const int first = min(max(p.q_offsets[0], 0), p.q_tokens);
+  const int last = min(max(p.q_offsets[p.documents], 0), p.q_tokens);
   const int rows = first + p.q_tokens - last, units = p.heads * (p.dim / 8);
   if (rows == 0 || last < first) return;
-  const long long step = blocks * blockDim.x, n = static_cast<long long>(rows) * units;
-  for (long long i = block * blockDim.x + threadIdx.x; i < n; i += step) {
+  const long long step = blocks * 32, n = static_cast<long long>(rows) * units;
+  for (long long i = block * 32 + lane; i < n; i += step) {
     const int r = static_cast<int>(i / units), u = static_cast<int>(i - static_cast<long long>(r) * units);
     const int h = u / (p.dim / 8), d = u - h * (p.dim / 8);
     const long long row = r < first ? r : last + (r - first);
