@@ -243,7 +243,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
     bool ok = true;
     auto fold = [&](int i, float m_old, float m_new) -> bool {  // acc = acc * 2^(m_old - m_new) + PV_i
       const int s = i & 1;
-      if (!mbar_wait_bounded(&o_full[s], static_cast<uint32_t>(i >> 1) & 1u, kErrWaitAcc)) return false;
+      if (!mbar_wait_warp(&o_full[s], static_cast<uint32_t>(i >> 1) & 1u, kErrWaitAcc)) return false;
       tc_fence_after();
       uint32_t r[32];
       tmem_ld32_issue(tmem + lane_addr + (t_o - tmem) + static_cast<uint32_t>(s) * kHead, r);
@@ -256,7 +256,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
       return true;
     };
     for (int j = 0; j < n_tiles; ++j) {
-      ok = mbar_wait_bounded(s_full, static_cast<uint32_t>(j) & 1u, kErrWaitAcc) && !*abort_flag;
+      ok = mbar_wait_warp(s_full, static_cast<uint32_t>(j) & 1u, kErrWaitAcc) && __all_sync(0xffffffffu, !*abort_flag);
       if (!ok) break;
       tc_fence_after();
       // Pass 1: the row maximum over the tile (two 32-column loads in flight per wait), in eight

@@ -280,7 +280,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       for (int chunk = 0; chunk < nchunks && ok; ++chunk) {
         const int buf = chunk & 1;
-        ok = mbar_wait_bounded(&chunk_full[buf], static_cast<uint32_t>(chunk >> 1) & 1u, kErrWaitAcc);
+        ok = mbar_wait_warp(&chunk_full[buf], static_cast<uint32_t>(chunk >> 1) & 1u, kErrWaitAcc);
         tc_fence_after();
 #pragma unroll
         for (int cb = 0; cb < 8; ++cb) {
@@ -297,7 +297,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_arrive(&chunk_empty[buf]);
       }
     }
-    ok = mbar_wait_bounded(acc_full, 0, kErrWaitAcc) && ok;
+    ok = mbar_wait_warp(acc_full, 0, kErrWaitAcc) && ok;
     tc_fence_after();
     const int ww = row % g.tile_w;
     const int hh = (row / g.tile_w) % g.tile_h;

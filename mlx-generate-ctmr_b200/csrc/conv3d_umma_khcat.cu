@@ -557,8 +557,8 @@ __global__ void __launch_bounds__(FUSE ? kKhThreadsFused : kKhThreads, 1)
         stats_reset();
       }
       const int buf = nbuf == 2 ? (lt & 1) : 0;
-      const bool ok = mbar_wait_bounded(&tmem_full[buf], static_cast<uint32_t>(nbuf == 2 ? lt >> 1 : lt) & 1u,
-                                        kErrWaitAcc);
+      const bool ok = mbar_wait_warp(&tmem_full[buf], static_cast<uint32_t>(nbuf == 2 ? lt >> 1 : lt) & 1u,
+                                     kErrWaitAcc);
       if (!barrier_all(3, 256, ok && !*abort_flag)) {
         *abort_flag = 1;
         break;
@@ -955,7 +955,7 @@ __global__ void __launch_bounds__(kKhThreads, 1)
       const bool tile_ok = t < g.total_tiles;
       int w0, h0, d0, b;
       decode(min(t, g.total_tiles - 1), w0, h0, d0, b);
-      const bool ok = mbar_wait_bounded(&tmem_full[0], static_cast<uint32_t>(lt) & 1u, kErrWaitAcc);
+      const bool ok = mbar_wait_warp(&tmem_full[0], static_cast<uint32_t>(lt) & 1u, kErrWaitAcc);
       if (!barrier_all(3, 256, ok && !*abort_flag)) {
         *abort_flag = 1;
         break;

@@ -331,8 +331,7 @@ __global__ void __launch_bounds__(kThreadsV2, 1)
         for (int i = 0; i < 128; ++i) sum[i] = 0.f;
         for (int c = 0; c < nch && ok; ++c, ++chunk) {
           const int cbuf = chunk & 1;
-          ok = __all_sync(0xffffffffu,
-                          mbar_wait_bounded(&chunk_full[cbuf], static_cast<uint32_t>(chunk >> 1) & 1u, kErrWaitAcc));
+          ok = mbar_wait_warp(&chunk_full[cbuf], static_cast<uint32_t>(chunk >> 1) & 1u, kErrWaitAcc);
           tc_fence_after();
 #pragma unroll
           for (int cb = 0; cb < 8; ++cb) {
@@ -346,8 +345,7 @@ __global__ void __launch_bounds__(kThreadsV2, 1)
           tc_fence_before();
           mbar_arrive(&chunk_empty[cbuf]);
         }
-        ok = ok && __all_sync(0xffffffffu, mbar_wait_bounded(&tmem_full[lbuf], static_cast<uint32_t>(et >> 1) & 1u,
-                                                             kErrWaitAcc));
+        ok = ok && mbar_wait_warp(&tmem_full[lbuf], static_cast<uint32_t>(et >> 1) & 1u, kErrWaitAcc);
         tc_fence_after();
         bool valid;
         long long out_base, res_base;
@@ -444,7 +442,7 @@ __global__ void __launch_bounds__(kThreadsV2, 1)
       decode(t, n0, w0, h0, d0, b, phase);
       uint32_t ra[64], rb[64];
       issue(0, ra);
-      if (!mbar_wait_bounded(&tmem_full[buf], static_cast<uint32_t>(lt >> 1) & 1u, kErrWaitAcc)) {
+      if (!mbar_wait_warp(&tmem_full[buf], static_cast<uint32_t>(lt >> 1) & 1u, kErrWaitAcc)) {
         *abort_flag = 1;
         break;
       }

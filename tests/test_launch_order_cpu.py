@@ -46,3 +46,10 @@ def test_warps_meet_between_a_wait_and_tensor_memory(name):
     assert len(loads) >= 3
     for at in loads:
         assert re.findall(r"mbar_wait_\w+", text[:at])[-1] == "mbar_wait_warp"
+
+
+@pytest.mark.parametrize("path", [p for p in sorted(CSRC.glob("*.cu")) if "tmem_ld" in p.read_text()], ids=lambda p: p.stem)
+def test_accumulators_are_waited_for_by_whole_warps(path):
+    """The barriers that announce an accumulator are waited for by the warps that then read it."""
+    text = re.sub(r"//[^\n]*", "", path.read_text())
+    assert not re.findall(r"mbar_wait_bounded\(\s*&?(?:tmem_full|o_full|s_full|acc_full|chunk_full)\b", text)
