@@ -109,7 +109,7 @@ __device__ __forceinline__ int limit_of(const AttentionParams& p, const Place& w
 
 // Up to 32 documents: their tiles in order of falling key counts, each document's heads together, so that no
 // long one starts when the others are done (seven volumes of 105 to 2,048 tokens, 8 heads of 32: 61 us in order
-// of documents, 53 us so; four causal ones of 1 to 2,300 tokens, 16 heads of 128: 101 and 83 us). More documents
+// of documents, 55 us so; four causal ones of 1 to 2,300 tokens, 16 heads of 128: 101 and 83 us). More documents
 // than a warp has lanes keep their order (four of 2,048 tokens and 28 of 64, and the same with an empty one more: 65
 // and 80 us with 8 heads of 32, 152 and 171 with 16 of 128). By a whole warp; false where `id` is past the last tile.
 template <int kBlock>
@@ -407,7 +407,7 @@ __global__ void __launch_bounds__(Layout<NC>::kThreads, Layout<NC>::kCtas)
     bool ok = true;
     auto wait_s = [&](int j) {  // (after a failure without waiting: the other half meets here)
       // By the whole warp: tcgen05.ld wants its lanes together, and each would leave a wait by itself. (One try ahead
-      // of the loop, 8,192 tokens of 8 heads of 32 and 128: 224 and 233 us; the loop alone: 228 and 256.)
+      // of the loop, 8,192 tokens of 8 heads of 32, and of 128 causal: 222 and 171 us; the loop alone: 225 and 184.)
       uint64_t* bar = &s_full[t * 2 + (j & 1)];
       const uint32_t parity = static_cast<uint32_t>(j >> 1) & 1u;
       if (!__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) ok = ok && mbar_wait_warp(bar, parity, kErrWaitAcc);

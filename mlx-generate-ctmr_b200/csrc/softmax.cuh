@@ -62,8 +62,8 @@ __device__ __forceinline__ ScoreCap score_cap(float scale, float cap) {
 //                    of the exponential unit to a score. Its absolute error is 2e-7 c, which a small score under a
 //                    large cap would feel (a score of 1 under a cap of 1e6 by 0.1).
 // So a lane's scores may be capped by one polynomial or the other, 1e-7 apart, as its neighbours' are large or not.
-// (8 heads of 8,192 tokens of 128, cap 30: 376 us with the quartic, 341 us with the cubic; 248 us uncapped. With
-// the exponentials alone, four sequences of 1 to 2,300 tokens took 118 us where the quartic took 101.)
+// (Four sequences of 1 to 2,300 tokens, 16 heads of 128, cap 30: 75 us; without the cubic 81, with the last form alone
+// 103. 8 heads of 8,192 tokens: 350 to 370 us, 370 to 395 and 515, 545 under a cap of 3; 246 uncapped.)
 template <int N>
 __device__ __forceinline__ void cap_scores(float (&s)[N], const ScoreCap& cap) {
   float big = 0.f;
