@@ -11,6 +11,7 @@ Rows in 8 bits are e4m3 values times powers of two: the scale of 128 channels is
 and at least 2^-100, with which the largest of them is at most 448. A weight's scales may be any numbers.
 """
 
+import functools
 import math
 
 import torch
@@ -21,6 +22,7 @@ DTYPES = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
 BLOCK = 128
 
 
+@functools.cache  # imported once, as a program does
 def _ops():
     import sys
     from pathlib import Path
