@@ -394,6 +394,49 @@ typedef struct ctmr_attention_desc {
 } ctmr_attention_desc;
 CTMR_API int ctmr_attention(const ctmr_attention_desc* desc, void* stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * Rows in 8 bits: e4m3 values with a scale for every 128 channels, the last group maybe shorter. The
+ * scale of a group is the least power of two 2^k, k >= -100, with which its largest magnitude is at most
+ * 448, and value = e4m3(v / scale) to nearest, ties to even: the bytes of v's formula in 64 bits. A group that
+ * holds an infinity or a NaN becomes NaN as a whole. Strides in elements (bytes for 8-bit values). */
+
+/* Root-mean-square norm of rows: h = x + residual, y = h / sqrt(mean(h^2) + eps) * weight, and h itself,
+ * rounded to x's type, in `sum`. A row is (token, head): heads is 1 for (tokens, channels). y is of x's
+ * type, or in 8 bits where scale is not NULL (heads must then be 1). The norm is taken of the unrounded
+ * h; squares are added in 64 bits. sum may be x or residual, and y of x's type may be x or residual (not
+ * sum); other overlaps are not allowed. */
+typedef struct ctmr_rms_norm_desc {
+  const void* x;                   /* [token][head][channels], channels contiguous */
+  const void* residual;            /* like x, or NULL */
+  const void* weight;              /* (channels), dense, or NULL */
+  int dtype;                       /* CTMR_DTYPE_F32, _BF16 or _F16: x, residual, sum, and y without scale */
+  int weight_dtype;                /* CTMR_DTYPE_F32 or dtype */
+  int tokens, heads, channels;     /* channels: up to 32768 */
+  long long x_token_stride, x_head_stride, residual_token_stride, residual_head_stride;
+  float eps;                       /* positive */
+  void* y;
+  long long y_token_stride, y_head_stride;
+  void* sum;                       /* or NULL */
+  long long sum_token_stride, sum_head_stride;
+  float* scale;                    /* (tokens, groups), or NULL */
+  long long scale_token_stride, scale_group_stride;
+} ctmr_rms_norm_desc;
+CTMR_API int ctmr_rms_norm(const ctmr_rms_norm_desc* desc, void* stream);
+
+/* Rows to 8 bits: v = x, or with gate v = silu(a) * b, a the first `channels` of a row and b the next. */
+typedef struct ctmr_quantize_rows_desc {
+  const void* x;                   /* (rows, channels), (rows, 2 * channels) with gate */
+  int dtype;                       /* CTMR_DTYPE_F32, _BF16 or _F16 */
+  int rows, channels;
+  int gate;
+  long long x_stride;
+  void* values;                    /* (rows, channels) e4m3; not x */
+  long long values_stride;
+  float* scale;                    /* (rows, groups) */
+  long long scale_row_stride, scale_group_stride;
+} ctmr_quantize_rows_desc;
+CTMR_API int ctmr_quantize_rows(const ctmr_quantize_rows_desc* desc, void* stream);
+
 /* Device error word (bits 0-4 set when a bounded wait gave up or a launch was inconsistent, bit 5 when
  * offsets, lengths or adapter numbers in device memory were out of range); optionally cleared.
  * Synchronises the current device. */

@@ -62,6 +62,8 @@ EXPORTED_SYMBOLS = (
     "ctmr_adapter_linear_workspace_size",
     "ctmr_adapter_linear",
     "ctmr_attention",
+    "ctmr_rms_norm",
+    "ctmr_quantize_rows",
     "ctmr_get_device_error",
     "ctmr_status_string",
     "ctmr_last_error",
@@ -230,6 +232,53 @@ class AttentionDesc(ctypes.Structure):
     ]
 
 
+class RmsNormDesc(ctypes.Structure):
+    """``ctmr_rms_norm_desc``."""
+
+    _fields_ = [
+        ("x", ctypes.c_void_p),
+        ("residual", ctypes.c_void_p),
+        ("weight", ctypes.c_void_p),
+        ("dtype", ctypes.c_int),
+        ("weight_dtype", ctypes.c_int),
+        ("tokens", ctypes.c_int),
+        ("heads", ctypes.c_int),
+        ("channels", ctypes.c_int),
+        ("x_token_stride", ctypes.c_longlong),
+        ("x_head_stride", ctypes.c_longlong),
+        ("residual_token_stride", ctypes.c_longlong),
+        ("residual_head_stride", ctypes.c_longlong),
+        ("eps", ctypes.c_float),
+        ("y", ctypes.c_void_p),
+        ("y_token_stride", ctypes.c_longlong),
+        ("y_head_stride", ctypes.c_longlong),
+        ("sum", ctypes.c_void_p),
+        ("sum_token_stride", ctypes.c_longlong),
+        ("sum_head_stride", ctypes.c_longlong),
+        ("scale", ctypes.c_void_p),
+        ("scale_token_stride", ctypes.c_longlong),
+        ("scale_group_stride", ctypes.c_longlong),
+    ]
+
+
+class QuantizeRowsDesc(ctypes.Structure):
+    """``ctmr_quantize_rows_desc``."""
+
+    _fields_ = [
+        ("x", ctypes.c_void_p),
+        ("dtype", ctypes.c_int),
+        ("rows", ctypes.c_int),
+        ("channels", ctypes.c_int),
+        ("gate", ctypes.c_int),
+        ("x_stride", ctypes.c_longlong),
+        ("values", ctypes.c_void_p),
+        ("values_stride", ctypes.c_longlong),
+        ("scale", ctypes.c_void_p),
+        ("scale_row_stride", ctypes.c_longlong),
+        ("scale_group_stride", ctypes.c_longlong),
+    ]
+
+
 def _load() -> ctypes.CDLL:
     if not LIB_PATH.exists():
         raise ImportError(
@@ -266,6 +315,8 @@ def _load() -> ctypes.CDLL:
         "ctmr_adapter_linear_workspace_size": (sz, [ctypes.POINTER(AdapterLinearDesc)]),
         "ctmr_adapter_linear": (i, [ctypes.POINTER(AdapterLinearDesc), vp, sz, vp]),
         "ctmr_attention": (i, [ctypes.POINTER(AttentionDesc), vp]),
+        "ctmr_rms_norm": (i, [ctypes.POINTER(RmsNormDesc), vp]),
+        "ctmr_quantize_rows": (i, [ctypes.POINTER(QuantizeRowsDesc), vp]),
         "ctmr_get_device_error": (i, [ctypes.POINTER(ctypes.c_uint), i]),
         "ctmr_status_string": (ctypes.c_char_p, [i]),
         "ctmr_last_error": (ctypes.c_char_p, []),

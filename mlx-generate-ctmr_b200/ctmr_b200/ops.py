@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import ctypes
 from dataclasses import dataclass
+from typing import NamedTuple
 
 import torch
 
@@ -779,6 +780,122 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, q_offsets: t
     if status:
         check(status, "attention")
     return (out, lse) if return_lse else out
+
+
+E4M3 = torch.float8_e4m3fn
+SCALE_GROUP = 128  # channels that share a scale
+
+
+class ScaledRows(NamedTuple):
+    """Rows in 8 bits: ``values[i, c] * scale[i, c // 128]``."""
+
+    values: torch.Tensor  # (rows, channels) e4m3, rows a multiple of 16 bytes apart
+    scale: torch.Tensor   # (rows, ceil(channels / 128)) fp32
+
+    def float(self) -> torch.Tensor:
+        return self.values.float() * self.scale.repeat_interleave(SCALE_GROUP, dim=1)[:, :self.values.shape[1]]
+
+
+def _empty_rows8(like: torch.Tensor, rows: int, channels: int) -> ScaledRows:
+    """Uninitialised 8-bit rows; scales lie group by group, as the products read them."""
+    values = like.new_empty((rows, (channels + 15) // 16 * 16), dtype=E4M3)
+    if values.shape[1] != channels:
+        values = values[:, :channels]
+    return ScaledRows(values, like.new_empty(((channels + 127) // 128, rows), dtype=F32).t())
+
+
+def rms_norm(x: torch.Tensor, weight: torch.Tensor | None = None, *, residual: torch.Tensor | None = None,
+             eps: float = 1e-6, quantize: bool = False, out: torch.Tensor | None = None,
+             sum_out: torch.Tensor | None = None):
+    """Root-mean-square norm over the channels, after the residual's addition (``ctmr_rms_norm``).
+
+    ``h = x + residual``, ``y = h / sqrt(mean(h ** 2) + eps) * weight``. ``x`` is ``(rows, channels)`` or
+    ``(tokens, heads, channels)`` in fp32, bf16 or fp16, up to 32,768 channels, any strides over rows; ``weight``
+    ``(channels,)`` in fp32 or x's type. Returns ``y`` of x's type, or as ``ScaledRows`` with ``quantize`` (two
+    dimensions; the bytes that the formula in 64 bits rounds to); with a residual ``(y, h)``, h rounded to x's type.
+    The norm is taken of the unrounded sum. ``sum_out`` may be ``x`` or ``residual``, and so may ``out``.
+    """
+    dtype, dims, shape = x.dtype, x.dim(), x.shape
+    code = _FLOAT_CODES.get(dtype)
+    if dims not in (2, 3) or code is None:
+        raise ValueError(f"x must be a (rows, channels) or (tokens, heads, channels) fp32/bf16/fp16 tensor; got "
+                         f"{tuple(shape)} {dtype}")
+    dev, stream = _device_stream(x, "x")
+    tokens, channels, heads = shape[0], shape[-1], shape[1] if dims == 3 else 1
+    weight_at, weight_code = None, 0
+    if weight is not None:
+        if weight.shape != (channels,) or weight.dtype not in (F32, dtype) or weight.get_device() != dev:
+            raise ValueError(f"weight must be {channels} float32 or {dtype} values on cuda:{dev}")
+        weight = weight.contiguous()
+        weight_at, weight_code = weight.data_ptr(), _FLOAT_CODES[weight.dtype]
+
+    def place(t, name):
+        """Address and strides over tokens and heads."""
+        if t.shape != shape or t.dtype != dtype or t.get_device() != dev:
+            raise ValueError(f"{name} must be like x: {tuple(shape)} {dtype} on cuda:{dev}")
+        st = t.stride()
+        if channels > 1 and st[-1] != 1:
+            raise ValueError(f"the channels of x, residual and the outputs must be contiguous; {name} has strides {st}")
+        # a stride over an extent of one addresses nothing, whatever torch calls it
+        return t.data_ptr(), st[0] if tokens > 1 else 0, st[1] if heads > 1 else 0
+
+    x_at, r_at = place(x, "x"), (None, 0, 0)
+    s_at = (None, 0, 0)
+    if residual is not None:
+        r_at = place(residual, "residual")
+        if sum_out is None:
+            sum_out = x.new_empty(shape)
+        s_at = place(sum_out, "sum_out")
+    elif sum_out is not None:
+        raise ValueError("sum_out belongs to a residual")
+    if quantize:
+        if dims != 2 or out is not None:
+            raise ValueError("8-bit rows are made of (rows, channels) tensors, and allocated by the call")
+        out = _empty_rows8(x, tokens, channels)
+        values, scale = out
+        y_at = (values.data_ptr(), values.stride(0), 0, *s_at, scale.data_ptr(), 1, tokens)
+    else:
+        if out is None:
+            out = x.new_empty(shape)
+        y_at = (*place(out, "out"), *s_at, None, 0, 0)
+        if residual is not None and y_at[0] == s_at[0] and y_at[0]:
+            raise ValueError("out and sum_out must be two tensors")
+    desc = _lib.RmsNormDesc(x_at[0], r_at[0], weight_at, code, weight_code, tokens, heads, channels, *x_at[1:], *r_at[1:],
+                            eps, *y_at)
+    LAUNCHES[0] += 1
+    status = LIB.ctmr_rms_norm(ctypes.byref(desc), stream)
+    if status:
+        check(status, "rms_norm")
+    return (out, sum_out) if residual is not None else out
+
+
+def quantize_rows(x: torch.Tensor, *, gate: bool = False) -> ScaledRows:
+    """Rows in 8 bits with a scale for every 128 channels (``ctmr_quantize_rows``).
+
+    ``x`` is ``(rows, channels)`` in fp32, bf16 or fp16, any stride over rows; with ``gate`` ``(rows, 2 * channels)``,
+    and what is rounded is ``silu(x[:, :channels]) * x[:, channels:]``. The bytes are those that the formula in 64
+    bits rounds to. A group that holds an infinity or a NaN becomes NaN as a whole.
+    """
+    code = _FLOAT_CODES.get(x.dtype)
+    if x.dim() != 2 or code is None:
+        raise ValueError(f"x must be a (rows, channels) fp32/bf16/fp16 tensor; got {tuple(x.shape)} {x.dtype}")
+    dev, stream = _device_stream(x, "x")
+    rows, channels = x.shape
+    if channels > 1 and x.stride(1) != 1:
+        raise ValueError("the channels of x must be contiguous")
+    if gate:
+        if channels % 2:
+            raise ValueError(f"a gated pair has an even number of channels; got {channels}")
+        channels //= 2
+    out = _empty_rows8(x, rows, channels)
+    values, scale = out
+    desc = _lib.QuantizeRowsDesc(x.data_ptr(), code, rows, channels, gate, x.stride(0) if rows > 1 else 0,
+                                 values.data_ptr(), values.stride(0), scale.data_ptr(), 1, rows)
+    LAUNCHES[0] += 1
+    status = LIB.ctmr_quantize_rows(ctypes.byref(desc), stream)
+    if status:
+        check(status, "quantize_rows")
+    return out
 
 
 def transform(

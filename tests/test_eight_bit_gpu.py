@@ -1,0 +1,362 @@
+"""The 8-bit row operators (``rms_norm``, ``quantize_rows``, ``scaled_linear``) against plain implementations in 64 bits.
+
+Tolerances follow from the roundings. With u the half-ulp of the output's type (bf16 2^-8, fp16 2^-11, fp32 2^-24):
+
+* norm without 8 bits: one rounding of y, and the fp32 roundings of the sum, the factor and two products:
+  ``u |y| + 2^-21 |y|``; the sum is one fp32 addition rounded to the type, bit for bit;
+* 8-bit values: the nearest e4m3 of the 64-bit value over the group's scale, half a step of the value's binade. Where
+  the residual's addition rounds in fp32 the mean square carries its relative error, at most 2^-23, the factor
+  half of that: ``step / 2 + 2^-24 |v|``; without a residual 64 bits' own error, ``step / 2 + 2^-40 |v|``. Scales are
+  equal (no input's largest magnitude lies that near to 448 times a power of two, but where it is meant to).
+* product: one rounding of y, and fp32 sums of n products: ``u |y| + 2^-23 sqrt(n) sum |x||w|``.
+fp16 results below the smallest normal number round in steps of 2^-24, so 2^-25 is always allowed.
+"""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+U = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11, torch.float32: 2.0 ** -24}
+TYPES = [torch.bfloat16, torch.float16, torch.float32]
+E4M3 = torch.float8_e4m3fn
+
+
+def _gen(seed: int) -> torch.Generator:
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def _randn(gen, *shape, dtype=torch.float32, std=1.0):
+    return (torch.randn(shape, generator=gen, device="cuda") * std).to(dtype)
+
+
+def _within(got, ref, tol):
+    got = got.double()
+    assert got.shape == ref.shape
+    assert torch.isfinite(got).all()
+    over = ((got - ref).abs() - tol).max().item() if got.numel() else 0.0
+    assert over <= 0.0, f"{over:.3e} over the tolerance; error {(got - ref).abs().max().item():.3e}"
+
+
+def _no_device_error():
+    from ctmr_b200 import _lib
+
+    assert _lib.device_error(clear=True) == 0
+
+
+def _groups(v):
+    return torch.nn.functional.pad(v, (0, -v.shape[1] % 128)).unflatten(1, (-1, 128))
+
+
+def _scale_of(v):
+    """Scales of 64-bit rows: the least 2^k, k >= -100, that brings the largest magnitude to 448 or below."""
+    fraction, exponent = torch.frexp(_groups(v).abs().amax(dim=2))
+    k = torch.where(fraction == 0, -100, (exponent - 9 + (fraction > 0.875)).clamp(min=-100))
+    return torch.ldexp(torch.ones_like(fraction), k)
+
+
+def _check_rows(got, v, slack=2.0 ** -40):
+    """`got` are the ScaledRows of the 64-bit rows `v`."""
+    values, scale = got
+    assert values.dtype == E4M3 and scale.dtype == torch.float32 and values.shape == v.shape
+    ref = _scale_of(v)
+    assert torch.equal(scale.double(), ref)
+    u = v / ref.repeat_interleave(128, dim=1)[:, :v.shape[1]]
+    step = torch.exp2(torch.floor(torch.log2(u.abs().clamp(min=2.0 ** -6))) - 3.0)
+    _within(values, u, step / 2 + slack * u.abs())
+
+
+def _norm_ref(x, residual, weight, eps):
+    h = x.double() if residual is None else x.double() + residual.double()
+    y = h / torch.sqrt(h.square().mean(dim=-1, keepdim=True) + eps)
+    return y if weight is None else y * weight.double()
+
+
+def _check_norm(x, weight, residual, eps, quantize, **kw):
+    from ctmr_b200 import ops
+
+    ref = _norm_ref(x, residual, weight, eps)
+    total = None if residual is None else (x.float() + residual.float()).to(x.dtype)
+    y = ops.rms_norm(x, weight, residual=residual, eps=eps, quantize=quantize, **kw)
+    if residual is not None:
+        y, h = y
+        assert torch.equal(h, total)
+    if quantize:
+        assert x.shape[0] <= 1 or y.values.stride(0) % 16 == 0
+        _check_rows(y, ref, 2.0 ** -40 if residual is None else 2.0 ** -24)
+    else:
+        assert y.dtype == x.dtype
+        _within(y, ref, (U[x.dtype] + 2.0 ** -21) * ref.abs() + 2.0 ** -25)
+    _no_device_error()
+
+
+# ---------------------------------------------------------------------------------------------- norm
+@pytest.mark.parametrize("quantize", [False, True])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize(("rows", "channels"), [
+    (1, 1), (3, 7), (5, 8), (2, 127), (9, 128), (130, 129), (31, 256), (33, 260), (17, 512), (8, 1000), (7, 1024),
+    (5, 1025), (3, 1032), (40, 4096), (1, 5000), (2, 8200), (3, 16384), (2, 16390), (2, 32768), (1, 32761)])
+def test_norm(rows, channels, dtype, quantize):
+    gen = _gen(rows * 40000 + channels)
+    x = _randn(gen, rows, channels, dtype=dtype, std=3.0)
+    weight = 1.0 + _randn(gen, channels, std=0.2)
+    _check_norm(x, weight, _randn(gen, rows, channels, dtype=dtype), 1e-6, quantize)
+    _check_norm(x, weight.to(dtype), None, 1e-5, quantize)
+    _check_norm(x, None, None, 1e-3, quantize)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shift", [0, 1, 8])
+def test_norm_slices_and_in_place(dtype, shift):
+    """Columns of wider tensors, aligned or not; the sum over x or over the residual; y over x."""
+    from ctmr_b200 import ops
+
+    gen = _gen(5 + shift)
+    rows, channels = 37, 640
+    weight = 1.0 + _randn(gen, channels, std=0.2)
+    for quantize in (False, True):
+        for over in ("x", "residual", "y"):
+            if over == "y" and quantize:
+                continue
+            wide = _randn(gen, rows, channels + 24, dtype=dtype)
+            other = _randn(gen, rows, 2 * channels, dtype=dtype)
+            x, residual = wide[:, shift:shift + channels], other[:, :channels]
+            around = wide.clone()
+            ref = _norm_ref(x, residual, weight, 1e-6)
+            total = (x.float() + residual.float()).to(dtype)
+            kw = dict(out=x) if over == "y" else dict(sum_out=x if over == "x" else residual)
+            y, h = ops.rms_norm(x, weight, residual=residual, quantize=quantize, **kw)
+            assert torch.equal(h, total)
+            assert (y if over == "y" else h).data_ptr() == (residual if over == "residual" else x).data_ptr()
+            if quantize:
+                _check_rows(y, ref, 2.0 ** -24)
+            else:
+                _within(y, ref, (U[dtype] + 2.0 ** -21) * ref.abs() + 2.0 ** -25)
+            outside = torch.ones(channels + 24, dtype=torch.bool, device="cuda")
+            outside[shift:shift + channels] = False
+            assert torch.equal(wide[:, outside], around[:, outside])
+    _no_device_error()
+
+
+@pytest.mark.parametrize(("heads", "dim"), [(4, 64), (3, 72), (8, 128), (1, 40), (2, 2048), (5, 33)])
+def test_norm_of_heads(heads, dim):
+    """The query and key heads of a fused projection, in place."""
+    from ctmr_b200 import ops
+
+    gen = _gen(heads * dim)
+    qkv = _randn(gen, 50, 3 * heads, dim, dtype=torch.bfloat16)
+    before, weight = qkv.clone(), 1.0 + _randn(gen, dim, std=0.2)
+    view = qkv[:, :2 * heads]
+    ref = _norm_ref(view, None, weight, 1e-6)
+    assert ops.rms_norm(view, weight, out=view) is view
+    _within(view, ref, (2.0 ** -8 + 2.0 ** -21) * ref.abs())
+    assert torch.equal(qkv[:, 2 * heads:], before[:, 2 * heads:])
+    x, residual = before[:, heads:2 * heads], before[:, :heads]
+    _check_norm(x, weight, residual, 1e-6, False)
+
+
+def test_norm_zero_rows_large_small_and_not_finite():
+    from ctmr_b200 import ops
+
+    gen = _gen(11)
+    x = _randn(gen, 9, 384, dtype=torch.float32)
+    x[1] = 0.0
+    x[2] *= 1e30     # squares past 32 bits
+    x[3] *= 1e-30    # below eps: v = x / sqrt(eps)
+    x[5, 200] = float("inf")
+    x[7, 3] = float("nan")
+    for quantize in (False, True):
+        y = ops.rms_norm(x, quantize=quantize)
+        ref = _norm_ref(x, None, None, 1e-6)
+        keep = [0, 1, 2, 3, 4, 6, 8]
+        if quantize:
+            _check_rows(ops.ScaledRows(y.values[keep], y.scale[keep]), ref[keep])
+            got = y.float()
+        else:
+            _within(y[keep], ref[keep], 2.0 ** -20 * ref[keep].abs())
+            got = y
+        # An infinity's own group is NaN (infinity times zero), the rest of its row zero; a NaN's row is NaN.
+        assert torch.isnan(got[5, 200]) and (got[5, :128] == 0).all() and (got[5, 256:] == 0).all()
+        assert torch.isnan(got[5, 128:256]).all() == quantize
+        assert torch.isnan(got[7]).all()
+    _no_device_error()
+
+
+def test_norm_of_no_rows():
+    from ctmr_b200 import ops
+
+    x = torch.empty((0, 256), dtype=torch.bfloat16, device="cuda")
+    assert ops.rms_norm(x).shape == (0, 256)
+    y, h = ops.rms_norm(x, residual=x, quantize=True)
+    assert y.values.shape == (0, 256) and y.scale.shape == (0, 2) and h.shape == (0, 256)
+    assert ops.quantize_rows(x, gate=True).values.shape == (0, 128)
+
+
+# ---------------------------------------------------------------------------------------------- quantiser
+def _gate_ref(x):
+    a, b = x.double().chunk(2, dim=1)
+    return a / (1.0 + torch.exp(-a)) * b
+
+
+@pytest.mark.parametrize("gate", [False, True])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize(("rows", "channels"), [
+    (1, 1), (3, 7), (5, 8), (2, 127), (9, 128), (700, 129), (617, 256), (33, 260), (1, 4096), (8, 1000), (300, 11264),
+    (4000, 136), (2, 100000)])
+def test_quantize(rows, channels, dtype, gate):
+    from ctmr_b200 import ops
+
+    gen = _gen(rows * 40000 + channels)
+    x = _randn(gen, rows, channels * (2 if gate else 1), dtype=dtype, std=4.0)
+    _check_rows(ops.quantize_rows(x, gate=gate), _gate_ref(x) if gate else x.double())
+    wide = _randn(gen, rows, x.shape[1] + 5, dtype=dtype, std=0.1)
+    x = wide[:, 3:3 + x.shape[1]]
+    _check_rows(ops.quantize_rows(x, gate=gate), _gate_ref(x) if gate else x.double())
+    _no_device_error()
+
+
+def test_quantize_ties_and_borders():
+    """Every e4m3 value, the ties between them (to even) and the numbers beside the ties; groups whose largest
+    magnitude is 448 times a power of two, and the next number above."""
+    from ctmr_b200 import ops
+
+    codes = torch.arange(127, dtype=torch.uint8, device="cuda").view(E4M3).float()  # 0 .. 448
+    ties = (codes[1:] + codes[:-1]) / 2
+    x = torch.cat([codes, ties, ties * (1 + 2.0 ** -23), ties * (1 - 2.0 ** -23)])
+    x = torch.cat([x, -x])
+    x = torch.nn.functional.pad(x, (0, -x.numel() % 127)).view(-1, 127)
+    x = torch.cat([x, torch.full((x.shape[0], 1), 448.0, device="cuda")], dim=1)
+    got = ops.quantize_rows(x)
+    assert (got.scale == 1).all()
+    assert torch.equal(got.values.view(torch.uint8), x.to(E4M3).view(torch.uint8))
+    for k in (-90, -20, 0, 60):
+        top = torch.tensor([448.0, 448.0 * (1 + 2.0 ** -23), 448.0 * (1 - 2.0 ** -24), 449.0], device="cuda") * 2.0 ** k
+        rows = torch.zeros((4, 128), device="cuda")
+        rows[:, 77] = top
+        assert ops.quantize_rows(rows).scale.flatten().tolist() == [2.0 ** k, 2.0 ** (k + 1), 2.0 ** k, 2.0 ** (k + 1)]
+    _no_device_error()
+
+
+def test_gate_borders():
+    """Gated values that lie on a tie or on a scale's border but for their last bits: 64 bits decide."""
+    from ctmr_b200 import ops
+
+    gen = _gen(3)
+    a = _randn(gen, 64, 128, std=2.0)
+    silu = a.double() / (1 + torch.exp(-a.double()))
+    # b brings silu(a) b as near to (odd / 16) or to 448 as 32 bits allow.
+    target = (torch.randint(8, 16, a.shape, generator=gen, device="cuda") * 2 + 1).double() / 16
+    b = (target / silu).float()
+    a[:, 5], b[:, 5] = 30.0, 448.0 / 30.0
+    x = torch.cat([a, b], dim=1)
+    x[::2, 128 + 5] = torch.nextafter(x[::2, 128 + 5], torch.tensor(0.0, device="cuda"))
+    _check_rows(ops.quantize_rows(x, gate=True), _gate_ref(x))
+
+
+def test_quantize_extremes_and_not_finite():
+    from ctmr_b200 import ops
+
+    x = _randn(_gen(1), 6, 300, dtype=torch.bfloat16)
+    x[0] = 0.0
+    x[1] *= 1e37
+    x[2] *= 1e-37   # below the least scale: zeros
+    x[3, 130] = float("-inf")
+    x[4, 299] = float("nan")
+    got = ops.quantize_rows(x)
+    keep = torch.tensor([0, 1, 2, 5], device="cuda")
+    _check_rows(ops.ScaledRows(got.values[keep], got.scale[keep]), x[keep].double())
+    back = got.float()
+    assert (back[0] == 0).all() and torch.isfinite(back[1]).all()
+    assert torch.isnan(back[3, 128:256]).all() and torch.isfinite(back[3, :128]).all() and torch.isfinite(back[3, 256:]).all()
+    assert torch.isnan(back[4, 256:]).all() and torch.isfinite(back[4, :256]).all()
+    a = torch.tensor([-200.0, -90.0, -88.0, -30.0, 0.0, 30.0, 90.0, 3e38] * 16, device="cuda")
+    pair = torch.cat([a, torch.full_like(a, 0.5)])[None]
+    _check_rows(ops.quantize_rows(pair, gate=True), _gate_ref(pair))
+    pair[0, 7] = 1.0  # the small ones decide the scale
+    pair = torch.where(pair[:, :128].repeat(1, 2).abs() > 1e30, 0.0, pair)
+    _check_rows(ops.quantize_rows(pair, gate=True), _gate_ref(pair))
+
+
+# ---------------------------------------------------------------------------------------------- both
+def test_rows_past_32_bits():
+    """Rows whose elements lie more than 2^31 apart."""
+    from ctmr_b200 import ops
+
+    pitch = 2 ** 31 + 64
+    room = torch.empty(pitch + 1024, dtype=torch.float16, device="cuda")
+    x = room.as_strided((2, 512), (pitch, 1))
+    x.copy_(_randn(_gen(2), 2, 512))
+    _check_norm(x, None, None, 1e-6, True)
+    _check_norm(x, None, None, 1e-6, False)
+    _check_rows(ops.quantize_rows(x), x.double())
+    _check_rows(ops.quantize_rows(x, gate=True), _gate_ref(x))
+
+
+def test_graphs_and_streams():
+    """Captured and replayed on other inputs, and called on a stream of its own, with the eager call's bits."""
+    from ctmr_b200 import ops
+
+    gen = _gen(8)
+    x, residual = _randn(gen, 70, 1536, dtype=torch.bfloat16), _randn(gen, 70, 1536, dtype=torch.bfloat16)
+    weight = 1.0 + _randn(gen, 1536, std=0.2)
+
+    def both():
+        y, h = ops.rms_norm(x, weight, residual=residual, quantize=True)
+        z = ops.quantize_rows(h, gate=True)
+        return y.values.view(torch.uint8), y.scale, h, z.values.view(torch.uint8), z.scale
+
+    both()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        kept = both()
+    for seed in (1, 2):
+        x.copy_(_randn(_gen(seed), 70, 1536))
+        graph.replay()
+        eager = both()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(kept, eager))
+    other = torch.cuda.Stream()
+    other.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(other):
+        apart = both()
+    other.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(apart, eager))
+    _no_device_error()
+
+
+def test_refusals():
+    from ctmr_b200 import ops
+
+    x = torch.zeros((4, 256), dtype=torch.bfloat16, device="cuda")
+    bad = [
+        lambda: ops.rms_norm(x.cpu()),
+        lambda: ops.rms_norm(x.double()),
+        lambda: ops.rms_norm(x[0]),
+        lambda: ops.rms_norm(x[:, ::2]),
+        lambda: ops.rms_norm(x, torch.ones(255, device="cuda")),
+        lambda: ops.rms_norm(x, torch.ones(256, device="cuda", dtype=torch.float16)),
+        lambda: ops.rms_norm(x, torch.ones(256)),
+        lambda: ops.rms_norm(x, residual=x.float()),
+        lambda: ops.rms_norm(x, residual=x[:2]),
+        lambda: ops.rms_norm(x, sum_out=torch.empty_like(x)),
+        lambda: ops.rms_norm(x, eps=0.0),
+        lambda: ops.rms_norm(x, eps=float("nan")),
+        lambda: ops.rms_norm(x, residual=x, out=x, sum_out=x),
+        lambda: ops.rms_norm(x, quantize=True, out=torch.empty_like(x)),
+        lambda: ops.rms_norm(x.view(4, 2, 128), quantize=True),
+        lambda: ops.rms_norm(torch.zeros((1, 32769), device="cuda")),
+        lambda: ops.rms_norm(torch.zeros((2, 0), device="cuda")),
+        lambda: ops.quantize_rows(x.view(4, 2, 128)),
+        lambda: ops.quantize_rows(x.to(torch.int8)),
+        lambda: ops.quantize_rows(x.t()),
+        lambda: ops.quantize_rows(x[:, :255], gate=True),
+        lambda: ops.quantize_rows(x.cpu()),
+    ]
+    for call in bad:
+        with pytest.raises(ValueError):
+            call()
+    _no_device_error()
