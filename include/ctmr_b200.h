@@ -437,6 +437,29 @@ typedef struct ctmr_quantize_rows_desc {
 } ctmr_quantize_rows_desc;
 CTMR_API int ctmr_quantize_rows(const ctmr_quantize_rows_desc* desc, void* stream);
 
+/* The product of 8-bit rows with an 8-bit weight, fp32 sums:
+ *   y_mn = sum_b x_scale[m][b] weight_scale[n / 128][b] (sum of x_mk weight_nk over block b of 128 inputs) + bias_n,
+ * scales of any value; the product of a row's and a weight's scale must be in fp32's range. What is NaN or
+ * not finite in a row, or in an output's weights, stays in that row, or output. Values and weights are e4m3,
+ * 16-byte aligned, rows a multiple of 16 bytes apart; inputs, outputs and rows of any number. */
+typedef struct ctmr_scaled_linear_desc {
+  const void* x;                   /* (rows, in_features) e4m3 */
+  long long x_stride;
+  const float* x_scale;            /* (rows, in blocks), strides in elements */
+  long long x_scale_row_stride, x_scale_block_stride;
+  int rows, in_features, out_features;
+  const void* weight;              /* (out_features, in_features) e4m3 */
+  long long weight_stride;
+  const float* weight_scale;       /* (out blocks, in blocks) */
+  long long weight_scale_row_stride, weight_scale_block_stride;
+  const void* bias;                /* (out_features) or NULL */
+  int bias_dtype;                  /* CTMR_DTYPE_F32 or y_dtype */
+  void* y;                         /* (rows, out_features), rows y_stride elements apart */
+  int y_dtype;                     /* CTMR_DTYPE_F32, _BF16 or _F16 */
+  long long y_stride;
+} ctmr_scaled_linear_desc;
+CTMR_API int ctmr_scaled_linear(const ctmr_scaled_linear_desc* desc, void* stream);
+
 /* Device error word (bits 0-4 set when a bounded wait gave up or a launch was inconsistent, bit 5 when
  * offsets, lengths or adapter numbers in device memory were out of range); optionally cleared.
  * Synchronises the current device. */

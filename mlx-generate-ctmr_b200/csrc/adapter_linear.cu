@@ -17,7 +17,6 @@
 //
 // Outputs as lanes: a warp stores 32 adjacent outputs of a row, and few rows (serving) use few
 // columns: the tensor core then streams W at the memory's rate.
-#include <atomic>
 #include <cmath>
 
 #include "capi_internal.cuh"
@@ -806,33 +805,10 @@ __global__ void __launch_bounds__(kPairThreads, 1)
 }
 
 // ---------------------------------------------------------------- host
-// CTA pairs that are resident at once (a GPC with an odd number of SMs leaves one idle), queried once per
-// device: one pair more would run alone after all the others.
+// CTA pairs that are resident at once: one pair more would run alone after all the others.
 int resident_pairs() {
-  static std::atomic<int> cached[64];
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = 0;
-  int n = cached[dev].load(std::memory_order_relaxed);
-  if (n > 0) return n;
-  auto kern = linear_pair_kernel<true>;
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = 2;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.gridDim = dim3(2 * (device_sm_count() / 2));
-  cfg.blockDim = dim3(kPairThreads);
-  cfg.dynamicSmemBytes = kPairBytes;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kPairBytes)) !=
-          cudaSuccess ||
-      cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess || n < 1) {
-    (void)cudaGetLastError();
-    n = device_sm_count() / 2;
-  }
-  cached[dev].store(n, std::memory_order_relaxed);
-  return n;
+  static ResidentClusters resident;
+  return resident.count(linear_pair_kernel<true>, 2, kPairThreads, kPairBytes);
 }
 
 int encode(CUtensorMap* map, const void* base, bool bf16, int rank, long long d0, long long d1, long long d2,
@@ -898,27 +874,6 @@ template <bool BF16, int NT>
 cudaError_t launch_inner(const LinearParams& p, const LinearPlan& plan, cudaStream_t stream) {
   return launch_kernel(adapter_inner_kernel<BF16, NT>, dim3(plan.blocks + 1, plan.tile / 16), dim3(kInnerWarps * 32),
                        0, stream, p, plan);
-}
-
-template <typename... KArgs, typename... Args>
-cudaError_t launch_cluster(SharedMemoryGrant& grant, void (*kern)(KArgs...), unsigned grid, int threads, size_t smem,
-                           int cluster, cudaStream_t stream, Args&&... args) {
-  cudaError_t e = grant.ensure(kern, smem);
-  if (e != cudaSuccess) return e;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = static_cast<unsigned>(cluster);
-  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = cluster > 1 ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...);
 }
 
 template <int BN, bool BF16>

@@ -82,4 +82,38 @@ int ctmr_quantize_rows(const ctmr_quantize_rows_desc* d, void* stream) {
   return finish(ctmr::launch_quantize(p, d->dtype, static_cast<cudaStream_t>(stream)), "quantize_rows launch");
 }
 
+int ctmr_scaled_linear(const ctmr_scaled_linear_desc* d, void* stream) {
+  if (d == nullptr) return api_fail(CTMR_ERR_INVALID, "null descriptor");
+  if (!float_type(d->y_dtype)) return api_fail(CTMR_ERR_INVALID, "scaled_linear output type");
+  if (d->bias != nullptr && d->bias_dtype != CTMR_DTYPE_F32 && d->bias_dtype != d->y_dtype)
+    return api_fail(CTMR_ERR_INVALID, "bias must be fp32 or of the output's type");
+  if (d->rows < 0 || d->in_features <= 0 || d->out_features <= 0)
+    return api_fail(CTMR_ERR_INVALID, "scaled_linear extents");
+  if (d->rows > 0x3fffffff || d->in_features > 0x3fffffff || d->out_features > 0x3fffffff)
+    return api_fail(CTMR_ERR_UNSUPPORTED, "scaled_linear extents above 2^30 - 1");
+  if (d->x_stride < d->in_features || d->weight_stride < d->in_features || d->x_stride % 16 != 0 ||
+      d->weight_stride % 16 != 0 || d->x_stride >= (1LL << 38) || d->weight_stride >= (1LL << 38))
+    return api_fail(CTMR_ERR_INVALID, "rows of x and weight cover a row and lie a multiple of 16 bytes apart");
+  if (d->y_stride < d->out_features || !stride_ok(d->y_stride) || !stride_ok(d->x_scale_row_stride) ||
+      !stride_ok(d->x_scale_block_stride) || !stride_ok(d->weight_scale_row_stride) ||
+      !stride_ok(d->weight_scale_block_stride))
+    return api_fail(CTMR_ERR_INVALID, "strides must not be negative, and rows of y must cover a row");
+  if (d->rows == 0) return CTMR_OK;
+  if (d->x == nullptr || d->weight == nullptr || d->x_scale == nullptr || d->weight_scale == nullptr || d->y == nullptr)
+    return api_fail(CTMR_ERR_INVALID, "null x, weight, scale or y");
+  if (reinterpret_cast<uintptr_t>(d->x) % 16 != 0 || reinterpret_cast<uintptr_t>(d->weight) % 16 != 0)
+    return api_fail(CTMR_ERR_INVALID, "x and weight must be 16-byte aligned");
+  if (!aligned_to(d->x_scale, CTMR_DTYPE_F32) || !aligned_to(d->weight_scale, CTMR_DTYPE_F32) ||
+      !aligned_to(d->y, d->y_dtype) || !aligned_to(d->bias, d->bias_dtype))
+    return api_fail(CTMR_ERR_INVALID, "tensors must be aligned to their elements");
+  ctmr::ScaledLinearParams p{};
+  p.x = d->x, p.weight = d->weight, p.bias = d->bias, p.x_scale = d->x_scale, p.w_scale = d->weight_scale, p.y = d->y;
+  p.x_stride = d->x_stride, p.weight_stride = d->weight_stride, p.y_stride = d->y_stride;
+  p.xs_row = d->x_scale_row_stride, p.xs_block = d->x_scale_block_stride;
+  p.ws_row = d->weight_scale_row_stride, p.ws_block = d->weight_scale_block_stride;
+  p.rows = d->rows, p.in = d->in_features, p.out = d->out_features;
+  p.bias_f32 = d->bias_dtype == CTMR_DTYPE_F32;
+  return ctmr::launch_scaled_linear(p, d->y_dtype, static_cast<cudaStream_t>(stream));
+}
+
 }  // extern "C"

@@ -40,8 +40,17 @@ struct QuantizeParams {
   int rows, channels, gate;
 };
 
+struct ScaledLinearParams {
+  const void *x, *weight, *bias;       // e4m3 rows; bias: fp32 or y's type, or null
+  const float *x_scale, *w_scale;      // (rows, blocks of 128 inputs), (blocks of 128 outputs, blocks of 128 inputs)
+  void* y;
+  long long x_stride, weight_stride, y_stride, xs_row, xs_block, ws_row, ws_block;
+  int rows, in, out, bias_f32;
+};
+
 cudaError_t launch_row_norm(const RowNormParams& p, int dtype, cudaStream_t stream);
 cudaError_t launch_quantize(const QuantizeParams& p, int dtype, cudaStream_t stream);
+int launch_scaled_linear(const ScaledLinearParams& p, int y_dtype, cudaStream_t stream);  // a CTMR_ status
 
 // ---------------------------------------------------------------- eight values of a row
 // 8 consecutive elements of a row from memory, zeros past `left` of them. WIDE: the row's address, stride and

@@ -225,6 +225,18 @@ __device__ __forceinline__ void umma_tf32(uint32_t d_tmem, uint64_t a_desc, uint
       : "memory");
 }
 
+// D[tmem] (+)= A[smem desc] * B[smem desc]^T, kind::f8f6f4 with e4m3 operands, one byte a value (32 values of K a
+// product), fp32 accumulate.
+__device__ __forceinline__ void umma_f8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                        uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
 // The 16-bit or the TF32 product of the same operand bytes, chosen at compile time: the single
 // issuing thread's instruction stream is on the MMA critical path, so it carries no branch.
 template <bool TF32>
@@ -254,6 +266,15 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, float (&v)[16]) {
   for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
 }
 
+// The same, started only: the registers hold them after tmem_ld_wait and tmem_ld_fence16.
+__device__ __forceinline__ void tmem_ld16_start(uint32_t taddr, float (&v)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]),
+        "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
+      : "r"(taddr));
+}
+
 // 32 consecutive 32-bit columns of this warp's 32 TMEM lanes (one lane per thread), started only: the
 // registers hold them after tmem_ld_wait.
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float* v) {
@@ -268,6 +289,12 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float* v) {
 }
 
 __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+
+// Ties 16 registers that tmem_ld16_start filled to this point: their uses stay after the wait before it.
+__device__ __forceinline__ void tmem_ld_fence16(float* v) {
+  asm volatile("" : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]),
+        "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15]));
+}
 
 // Ties 32 registers that tmem_ld32 filled to this point: their uses stay after the wait before it.
 __device__ __forceinline__ void tmem_ld_fence(float* v) {
@@ -419,6 +446,16 @@ __device__ __forceinline__ void umma_f16_pair(uint32_t d_tmem, uint64_t a_desc, 
       : "memory");
 }
 
+__device__ __forceinline__ void umma_f8_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                             uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
 // Arrive on the mbarrier at this shared-memory offset in both CTAs of the pair (CTA mask 0b11) once
 // every product this thread issued before has completed.
 __device__ __forceinline__ void umma_commit_pair(uint64_t* bar) {
@@ -436,6 +473,11 @@ __host__ __device__ constexpr uint32_t idesc_f16(bool bf16, uint32_t m, uint32_t
          | ((tf32 ? 2u : (bf16 ? 1u : 0u)) << 7)             // A format
          | ((tf32 ? 2u : (bf16 ? 1u : 0u)) << 10)            // B format
          | ((n >> 3) << 17) | ((m >> 4) << 24);
+}
+
+// The same for kind::f8f6f4 with both operands e4m3 (format 0).
+__host__ __device__ constexpr uint32_t idesc_e4m3(uint32_t m, uint32_t n) {
+  return (1u << 4) | ((n >> 3) << 17) | ((m >> 4) << 24);
 }
 
 }  // namespace ctmr

@@ -1,0 +1,613 @@
+// The product of 8-bit rows with an 8-bit weight, both with scales along blocks of 128 inputs:
+//   y[m, n] = sum_b xs[m, b] ws[n / 128, b] (sum_{k in block b} x[m, k] w[n, k]) + bias[n].
+//
+// tcgen05 products of kind::f8f6f4 make each block's sum in TMEM; a block is one 128-byte swizzled row of shared memory
+// and four products. The scales change with every block, so the epilogue's warps take each block's sums out of
+// TMEM and add them, scaled, to sums that they keep in fp32 registers, while the next blocks' products run. That also
+// bounds how long a sum stays inside the tensor core.
+//
+// Two forms. Pairs of CTAs take 256 rows x 256 outputs, rows as TMEM lanes: a thread then has one row scale and one
+// weight scale a block, and one multiplication and 128 additions. Few rows take tiles of 128 outputs as lanes by 16 to
+// 128 rows as columns, with the inputs split over a cluster: all SMs stream the weight at the memory's rate, and the
+// partial sums meet through distributed shared memory, in the order of the ranks.
+#include "capi_internal.cuh"
+#include "ctmr_b200.h"
+#include "eight_bit.cuh"
+#include "launch.cuh"
+
+namespace ctmr {
+namespace {
+
+constexpr int kK = kScaleGroup;
+constexpr uint32_t kHalfTile = 128 * 128;  // 128 rows of 128 bytes
+
+struct ScaledMaps {
+  CUtensorMap x, w;
+};
+
+struct ScaledPlan {
+  int tile, row_tiles, out_tiles;
+  int split;  // CTAs (a cluster) that share a tile's blocks; 0: CTA pairs
+};
+
+template <typename T>
+__device__ __forceinline__ float bias_at(const ScaledLinearParams& p, int o) {
+  if (p.bias == nullptr || o >= p.out) return 0.f;
+  return p.bias_f32 ? static_cast<const float*>(p.bias)[o] : to_float(static_cast<const T*>(p.bias)[o]);
+}
+
+__device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"  // volatile: in order with the barriers
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr));
+  return v;
+}
+
+// N values of a row from output o on; WIDE: the address allows 16-byte accesses and all of them are the row's.
+template <typename T, int N>
+__device__ __forceinline__ void store_outputs(T* at, const float* v, bool wide, int left) {
+  if (wide && left >= N) {
+    constexpr int kEach = 16 / sizeof(T) < N ? 16 / sizeof(T) : N;
+    struct alignas(kEach * sizeof(T)) Pack {
+      T e[kEach];
+    };
+#pragma unroll
+    for (int i = 0; i < N; i += kEach) {
+      Pack pack;
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) pack.e[e] = from_float<T>(v[i + e]);
+      *reinterpret_cast<Pack*>(at + i) = pack;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (i < left) at[i] = from_float<T>(v[i]);
+  }
+}
+
+// ---------------------------------------------------------------- few rows
+constexpr int kFewThreads = 224;  // warp 0 TMA, warp 1 MMA, warps 2-5 sums, warp 6 scales
+
+template <int BN>
+struct FewSmem {
+  static constexpr uint32_t kStageBytes = kHalfTile + BN * 128;
+  static constexpr int kStages = 180224 / kStageBytes;
+  static constexpr int kAcc = 4;      // blocks whose sums are in TMEM
+  static constexpr int kFactors = 8;  // blocks whose scales are in shared memory
+  static constexpr uint32_t kCols = kAcc * BN < 32 ? 32 : kAcc * BN;
+  static constexpr uint32_t kOffFactors = kStages * kStageBytes;
+  static constexpr uint32_t kOffBar = kOffFactors + kFactors * BN * 4;
+  static constexpr uint32_t kBytes = kOffBar + 512 + 1024;  // + barriers + alignment slack
+  static_assert(BN * 512u <= kOffFactors, "the partial sums lie in the stages");
+  static_assert((2 * kStages + 2 * kAcc + 2 * kFactors) * 8 + 16 <= 512, "barriers");
+};
+
+// blockIdx.x = (row tile * out tiles + out tile) * split + rank.
+template <int BN, typename T>
+__global__ void __launch_bounds__(kFewThreads, 1)
+    scaled_few_kernel(const __grid_constant__ ScaledMaps maps, const __grid_constant__ ScaledLinearParams p,
+                      const __grid_constant__ ScaledPlan plan) {
+  using L = FewSmem<BN>;
+  constexpr int S = L::kStages, A = L::kAcc, F = L::kFactors;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  float* factors = reinterpret_cast<float*>(smem + L::kOffFactors);  // [F][BN]
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::kOffBar);
+  uint64_t* empty = full + S;
+  uint64_t* acc_full = empty + S;
+  uint64_t* acc_empty = acc_full + A;
+  uint64_t* factor_full = acc_empty + A;
+  uint64_t* factor_empty = factor_full + F;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(factor_empty + F);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = static_cast<int>(blockIdx.x) % plan.split, unit = static_cast<int>(blockIdx.x) / plan.split;
+  const int row_tile = unit / plan.out_tiles, m0 = (unit - row_tile * plan.out_tiles) * 128, r0 = row_tile * BN;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < S; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < A; ++i) {
+      mbar_init(&acc_full[i], 1);
+      mbar_init(&acc_empty[i], 4);
+    }
+    for (int i = 0; i < F; ++i) {
+      mbar_init(&factor_full[i], 1);
+      mbar_init(&factor_empty[i], 4);
+    }
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, L::kCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  griddep_wait();
+  griddep_launch_dependents();
+
+  const int kb = (p.in + kK - 1) / kK, k_begin = rank * kb / plan.split, k_end = (rank + 1) * kb / plan.split;
+  const int n = k_end - k_begin;
+  if (warp == 0) {
+    // ------------------------------------------------------------ TMA producer
+    bool ok = true;
+    int it = 0;
+    for (; ok && it < n; ++it) {
+      const int s = it % S;
+      if (it >= S) ok = mbar_wait_warp(&empty[s], static_cast<uint32_t>(it / S - 1) & 1u, kErrWaitEmpty);
+      if (!ok) break;
+      if (lane == 0) {
+        uint8_t* at = smem + s * L::kStageBytes;
+        mbar_arrive_expect_tx(&full[s], L::kStageBytes);
+        tma_load_2d(at, &maps.w, &full[s], (k_begin + it) * kK, m0);
+        tma_load_2d(at + kHalfTile, &maps.x, &full[s], (k_begin + it) * kK, r0);
+      }
+      __syncwarp();
+    }
+    if (lane == 0) {
+      if (!ok) *abort_flag = 1;
+      for (int i = max(0, it - S); i < it; ++i)  // every issued load lands before the CTA goes on
+        mbar_wait_bounded(&full[i % S], static_cast<uint32_t>(i / S) & 1u, kErrWaitDrain);
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA issuer: a warp that stays together
+    const uint32_t tm = warp_value(tmem), base = warp_value(smem_u32(smem));
+    const uint64_t d0 = smem_desc_kmajor(base, 128);
+    constexpr uint32_t id = idesc_e4m3(128, BN);
+    bool ok = true;
+    for (int it = 0; it < n; ++it) {
+      const int s = it % S, a = it % A;
+      if (it >= A) ok = mbar_wait_warp(&acc_empty[a], static_cast<uint32_t>(it / A - 1) & 1u, kErrWaitAcc);
+      ok = ok && mbar_wait_warp(&full[s], static_cast<uint32_t>(it / S) & 1u, kErrWaitFull);
+      if (!ok) break;
+      tc_fence_after();
+      const uint64_t ad = desc_advance(d0, static_cast<uint32_t>(s) * L::kStageBytes), bd = desc_advance(ad, kHalfTile);
+      if (elect_one()) {
+#pragma unroll
+        for (uint32_t k = 0; k < 4; ++k)
+          umma_f8(tm + a * BN, desc_advance(ad, k * 32u), desc_advance(bd, k * 32u), id, k > 0 ? 1u : 0u);
+        umma_commit(&empty[s]);
+        umma_commit(&acc_full[a]);
+      }
+      __syncwarp();
+    }
+    if (!ok) *abort_flag = 1;
+    __syncwarp();
+  } else if (warp == 6) {
+    // ------------------------------------------------------------ scales, four blocks' loads at a time
+    constexpr int kEach = (BN + 31) / 32;
+    const float* xs[kEach];
+    bool in[kEach];
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+      const int c = j * 32 + lane;
+      in[j] = c < BN && r0 + c < p.rows;
+      xs[j] = p.x_scale + (in[j] ? (r0 + c) * p.xs_row : 0);
+    }
+    const float* ws = p.w_scale + (m0 / kScaleGroup) * p.ws_row;
+    bool ok = true;
+    for (int it = 0; ok && it < n; it += 4) {
+      float v[4][kEach], w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int k = k_begin + it + i;
+        w[i] = it + i < n ? ws[k * p.ws_block] : 0.f;
+#pragma unroll
+        for (int j = 0; j < kEach; ++j) v[i][j] = it + i < n && in[j] ? xs[j][k * p.xs_block] : 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int at = it + i, f = at % F;
+        if (at >= n) break;
+        if (at >= F) ok = mbar_wait_warp(&factor_empty[f], static_cast<uint32_t>(at / F - 1) & 1u, kErrWaitEmpty);
+        if (!ok) break;
+#pragma unroll
+        for (int j = 0; j < kEach; ++j)
+          if (j * 32 + lane < BN) factors[f * BN + j * 32 + lane] = v[i][j] * w[i];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&factor_full[f]);
+      }
+    }
+    if (!ok) *abort_flag = 1;
+    __syncwarp();
+  } else {
+    // ------------------------------------------------------------ sums
+    const int quarter = warp & 3;
+    const uint32_t lanes = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
+    float sum[BN];
+#pragma unroll
+    for (int c = 0; c < BN; ++c) sum[c] = 0.f;
+    bool ok = true;
+    for (int it = 0; it < n; ++it) {
+      const int a = it % A, f = it % F;
+      ok = mbar_wait_warp(&factor_full[f], static_cast<uint32_t>(it / F) & 1u, kErrWaitFull) &&
+           mbar_wait_warp(&acc_full[a], static_cast<uint32_t>(it / A) & 1u, kErrWaitAcc);
+      if (!ok) break;
+      tc_fence_after();
+      const float4* by = reinterpret_cast<const float4*>(factors + f * BN);
+      float v[2][16];
+      tmem_ld16_start(lanes + a * BN, v[0]);
+#pragma unroll
+      for (int c = 0; c < BN; c += 16) {
+        float(&now)[16] = v[(c / 16) & 1];
+        tmem_ld_wait();
+        tmem_ld_fence16(now);
+        if (c + 16 < BN) {
+          tmem_ld16_start(lanes + a * BN + c + 16, v[(c / 16 + 1) & 1]);
+        } else {  // all read
+          tc_fence_before();
+          if (lane == 0) mbar_arrive(&acc_empty[a]);
+        }
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+          const float4 s = by[(c + e) / 4];
+          sum[c + e] = fmaf(now[e], s.x, sum[c + e]);
+          sum[c + e + 1] = fmaf(now[e + 1], s.y, sum[c + e + 1]);
+          sum[c + e + 2] = fmaf(now[e + 2], s.z, sum[c + e + 2]);
+          sum[c + e + 3] = fmaf(now[e + 3], s.w, sum[c + e + 3]);
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&factor_empty[f]);
+    }
+    if (!ok) *abort_flag = 1;
+    const int o = m0 + quarter * 32 + lane;
+    if (plan.split > 1) {
+      // The stages' data are consumed: they hold the partial tile now, [column][output].
+      float* part = reinterpret_cast<float*>(smem);
+#pragma unroll
+      for (int c = 0; c < BN; ++c) part[c * 128 + quarter * 32 + lane] = sum[c];
+    } else if (ok && o < p.out) {
+      const float bias = bias_at<T>(p, o);
+      T* y = static_cast<T*>(p.y) + r0 * p.y_stride + o;
+#pragma unroll
+      for (int c = 0; c < BN; ++c)
+        if (r0 + c < p.rows) y[c * p.y_stride] = from_float<T>(sum[c] + bias);
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (plan.split > 1) {
+    cluster_sync();
+    if (!*abort_flag) {
+      // Each CTA adds up its share of the columns: four outputs a thread, a column a warp.
+      const int o = m0 + lane * 4;
+      float bias[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) bias[e] = bias_at<T>(p, o + e);
+      const bool wide = p.y_stride % 4 == 0 && reinterpret_cast<uintptr_t>(p.y) % (4 * sizeof(T)) == 0;
+      const int c_begin = rank * BN / plan.split, c_end = min((rank + 1) * BN / plan.split, p.rows - r0);
+      constexpr int kBatch = 4, kWarps = kFewThreads / 32;
+      for (int c = c_begin + warp; c < c_end; c += kWarps * kBatch) {
+        float v[kBatch][4];
+#pragma unroll
+        for (int e = 0; e < kBatch; ++e)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) v[e][i] = 0.f;
+#pragma unroll 2
+        for (int z = 0; z < plan.split; ++z) {
+          const uint32_t at = cluster_addr(smem, z) + lane * 16;
+#pragma unroll
+          for (int e = 0; e < kBatch; ++e) {
+            const float4 t = ld_cluster4(at + min(c + e * kWarps, c_end - 1) * 512);
+            v[e][0] += t.x, v[e][1] += t.y, v[e][2] += t.z, v[e][3] += t.w;
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < kBatch; ++e) {
+          const int column = c + e * kWarps;
+          if (column >= c_end) break;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) v[e][i] += bias[i];
+          store_outputs<T, 4>(static_cast<T*>(p.y) + (r0 + column) * p.y_stride + o, v[e], wide, p.out - o);
+        }
+      }
+    }
+    cluster_sync();  // no CTA leaves while another reads its partial tile
+  }
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, L::kCols);
+  }
+}
+
+// ---------------------------------------------------------------- CTA pairs
+constexpr int kPairThreads = 320;  // warp 0 TMA, warp 1 MMA (first CTA), warps 2-9 sums
+constexpr int kPairTile = 256;
+constexpr int kPairStages = 6;
+constexpr uint32_t kPairStageBytes = 2 * kHalfTile;  // this CTA's 128 rows and 128 outputs
+constexpr uint32_t kPairOffBar = kPairStages * kPairStageBytes;
+constexpr uint32_t kPairBytes = kPairOffBar + 512 + 1024;
+constexpr int kRaster = 8;  // row tiles that are walked together, so that the weight's and x's tiles meet in L2
+
+// 256 rows x 256 outputs per pair (tcgen05.mma.cta_group::2), persistent. A CTA's 128 x 256 sums of a block are
+// half its TMEM: the products of one block run while the other's sums are taken out, 128 of a row to a thread.
+template <typename T>
+__global__ void __launch_bounds__(kPairThreads, 1)
+    scaled_pair_kernel(const __grid_constant__ ScaledMaps maps, const __grid_constant__ ScaledLinearParams p,
+                       const __grid_constant__ ScaledPlan plan) {
+  constexpr int S = kPairStages;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + kPairOffBar);
+  uint64_t* empty = full + S;
+  uint64_t* acc_full = empty + S;      // [2]
+  uint64_t* acc_empty = acc_full + 2;  // [2] read out by both CTAs (first CTA's barriers)
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const int pair = static_cast<int>(blockIdx.x >> 1), pairs = static_cast<int>(gridDim.x >> 1);
+  const int tiles = plan.row_tiles * plan.out_tiles;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < S; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&acc_full[i], 1);
+      mbar_init(&acc_empty[i], 16);
+    }
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(tmem_slot, 512);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();  // both CTAs' barriers exist before anything crosses the pair
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  griddep_wait();
+  griddep_launch_dependents();
+
+  auto place = [&](int t, int& r0, int& n0) {
+    const int per = kRaster * plan.out_tiles, group = t / per, in_group = t - group * per;
+    const int height = min(kRaster, plan.row_tiles - group * kRaster);
+    r0 = (group * kRaster + in_group % height) * kPairTile + static_cast<int>(rank) * 128;  // this CTA's rows
+    n0 = in_group / height * kPairTile;
+  };
+
+  const int kb = (p.in + kK - 1) / kK;
+  if (warp == 0) {
+    // ------------------------------------------------------------ TMA producer (both CTAs)
+    const uint32_t full0 = cluster_addr(full, 0);
+    int it = 0;
+    bool ok = true;
+    for (int t = pair; ok && t < tiles; t += pairs) {
+      int r0, n0;
+      place(t, r0, n0);
+      for (int k = 0; k < kb; ++k, ++it) {
+        const int s = it % S;
+        if (it >= S) ok = mbar_wait_warp(&empty[s], static_cast<uint32_t>(it / S - 1) & 1u, kErrWaitEmpty);
+        if (!ok) break;
+        if (lane == 0) {
+          uint8_t* at = smem + s * kPairStageBytes;
+          if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * kPairStageBytes);
+          tma_load_2d_pair(at, &maps.x, full0 + 8u * s, k * kK, r0);
+          tma_load_2d_pair(at + kHalfTile, &maps.w, full0 + 8u * s, k * kK, n0 + static_cast<int>(rank) * 128);
+        }
+        __syncwarp();
+      }
+    }
+    if (lane == 0) {
+      if (!ok) *abort_flag = 1;
+      // The first CTA's barriers count both CTAs' bytes: all land before the closing cluster barrier.
+      if (rank == 0)
+        for (int i = max(0, it - S); i < it; ++i)
+          if (!mbar_wait_bounded(&full[i % S], static_cast<uint32_t>(i / S) & 1u, kErrWaitDrain)) break;
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA issuer (first CTA): a warp that stays together
+    if (rank == 0) {
+      constexpr uint32_t id = idesc_e4m3(256, kPairTile);
+      const uint32_t tm = warp_value(tmem), base = warp_value(smem_u32(smem));
+      const uint64_t d0 = smem_desc_kmajor(base, 128);
+      const int my_tiles = warp_value(pair < tiles ? (tiles - pair + pairs - 1) / pairs : 0), blocks = my_tiles * kb;
+      bool ok = true;
+      for (int it = 0; it < blocks; ++it) {
+        const int s = it % S, a = it & 1;
+        if (it >= 2) ok = mbar_wait_warp(&acc_empty[a], static_cast<uint32_t>((it >> 1) - 1) & 1u, kErrWaitAcc);
+        ok = ok && mbar_wait_warp(&full[s], static_cast<uint32_t>(it / S) & 1u, kErrWaitFull);
+        if (!ok) break;
+        tc_fence_after();
+        const uint64_t ad = desc_advance(d0, static_cast<uint32_t>(s) * kPairStageBytes), bd = desc_advance(ad, kHalfTile);
+        if (elect_one()) {
+#pragma unroll
+          for (uint32_t k = 0; k < 4; ++k)
+            umma_f8_pair(tm + a * 256, desc_advance(ad, k * 32u), desc_advance(bd, k * 32u), id, k > 0 ? 1u : 0u);
+          umma_commit_pair(&empty[s]);
+          umma_commit_pair(&acc_full[a]);
+        }
+        __syncwarp();
+      }
+      if (!ok) *abort_flag = 1;
+    }
+    __syncwarp();
+  } else {
+    // ------------------------------------------------------------ sums (both CTAs)
+    const int quarter = warp & 3, half = (warp - 2) >> 2;
+    const uint32_t lanes = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + half * 128;
+    const uint32_t release0 = cluster_addr(acc_empty, 0);
+    // Scales four blocks ahead of their use, across tiles.
+    float xs[4], ws[4];
+    auto fetch = [&](int t, int k0) {
+      int r0, n0;
+      place(min(t, tiles - 1), r0, n0);
+      const int row = r0 + quarter * 32 + lane, column = n0 + half * 128;
+      const bool in = t < tiles && row < p.rows && column < p.out;
+      const float* x = p.x_scale + (in ? row * p.xs_row : 0);
+      const float* w = p.w_scale + (in ? column / kScaleGroup * p.ws_row : 0);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        xs[i] = in && k0 + i < kb ? x[(k0 + i) * p.xs_block] : 0.f;
+        ws[i] = in && k0 + i < kb ? w[(k0 + i) * p.ws_block] : 0.f;
+      }
+    };
+    if (pair < tiles) fetch(pair, 0);
+    int it = 0;
+    bool ok = true;
+    for (int t = pair; ok && t < tiles; t += pairs) {
+      float sum[128];
+#pragma unroll
+      for (int c = 0; c < 128; ++c) sum[c] = 0.f;
+      for (int k0 = 0; ok && k0 < kb; k0 += 4) {
+        float by[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) by[i] = xs[i] * ws[i];
+        const bool more = k0 + 4 < kb;
+        fetch(more ? t : t + pairs, more ? k0 + 4 : 0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (k0 + i >= kb) break;
+          const int a = it & 1;
+          ok = mbar_wait_warp(&acc_full[a], static_cast<uint32_t>(it >> 1) & 1u, kErrWaitAcc);
+          if (!ok) break;
+          ++it;
+          tc_fence_after();
+          float v[2][16];
+          tmem_ld16_start(lanes + a * 256, v[0]);
+#pragma unroll
+          for (int c = 0; c < 128; c += 16) {
+            float(&now)[16] = v[(c / 16) & 1];
+            tmem_ld_wait();
+            tmem_ld_fence16(now);
+            if (c + 16 < 128) {
+              tmem_ld16_start(lanes + a * 256 + c + 16, v[(c / 16 + 1) & 1]);
+            } else {  // all read: the next block but one may overwrite it
+              tc_fence_before();
+              if (lane == 0) mbar_arrive_cluster(release0 + 8u * a);
+            }
+#pragma unroll
+            for (int e = 0; e < 16; ++e) sum[c + e] = fmaf(now[e], by[i], sum[c + e]);
+          }
+        }
+      }
+      ok = ok && __all_sync(0xffffffffu, !*abort_flag);
+      if (!ok) break;
+      int r0, n0;
+      place(t, r0, n0);
+      const int row = r0 + quarter * 32 + lane, column = n0 + half * 128;
+      if (row < p.rows) {
+        const bool wide = p.y_stride % (16 / static_cast<int>(sizeof(T))) == 0 && reinterpret_cast<uintptr_t>(p.y) % 16 == 0;
+        T* y = static_cast<T*>(p.y) + row * p.y_stride + column;
+#pragma unroll
+        for (int c = 0; c < 128; c += 8) {
+          if (column + c >= p.out) break;
+          if (p.bias != nullptr)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) sum[c + e] += bias_at<T>(p, column + c + e);
+          store_outputs<T, 8>(y + c, sum + c, wide, p.out - column - c);
+        }
+      }
+      __syncwarp();
+    }
+    if (!ok) *abort_flag = 1;
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();  // neither CTA exits while the other's products, copies or arrivals may reach it
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem, 512);
+  }
+}
+
+// ---------------------------------------------------------------- host
+int encode(CUtensorMap* map, const void* base, long long in, long long rows, long long stride, int box_rows,
+           const char* what) {
+  auto enc = api_tensor_map_encoder();
+  if (enc == nullptr) return api_fail(CTMR_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(in), static_cast<cuuint64_t>(rows)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(stride)};
+  const cuuint32_t box[2] = {kK, static_cast<cuuint32_t>(box_rows)}, step[2] = {1, 1};
+  const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, step,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return api_fail(CTMR_ERR_INVALID, "%s: tensor map rejected (CUresult %d)", what, int(r));
+  return CTMR_OK;
+}
+
+// Which form, tile and split: the least of these estimates (microseconds).
+ScaledPlan plan_scaled(const ScaledLinearParams& p) {
+  ScaledPlan plan{};
+  const int sms = device_sm_count(), kb = (p.in + kK - 1) / kK;
+  auto waves = [](long long n, int at_once) { return static_cast<float>((n + at_once - 1) / at_once); };
+  const long long pair_tiles = ((p.out + 255LL) / 256) * ((p.rows + 255LL) / 256);
+  float best = 6.f + waves(pair_tiles, sms / 2) * kb * 0.35f;
+  plan.tile = kPairTile, plan.split = 0, plan.out_tiles = (p.out + 255) / 256;
+  for (int tile = 16; tile <= 128; tile *= 2) {
+    if (tile > 16 && tile / 2 >= p.rows) break;
+    const long long tiles = ((p.out + 127LL) / 128) * ((p.rows + tile - 1LL) / tile);
+    for (int split = 1; split <= 8 && split <= kb; split *= 2) {
+      const float one = 2.8f + 0.02f * tile + (split > 1 ? 0.8f + 0.01f * tile : 0.f) +
+                        static_cast<float>(kb) / split * (0.25f + 0.001f * tile);
+      const float t = waves(tiles * split, sms) * one;
+      if (t < best) best = t, plan.tile = tile, plan.split = split, plan.out_tiles = (p.out + 127) / 128;
+    }
+  }
+  plan.row_tiles = (p.rows + plan.tile - 1) / plan.tile;
+  return plan;
+}
+
+template <int BN, typename T>
+cudaError_t launch_few(const ScaledMaps& maps, const ScaledLinearParams& p, const ScaledPlan& plan, unsigned grid,
+                       cudaStream_t stream) {
+  static SharedMemoryGrant grant;
+  return launch_cluster(grant, scaled_few_kernel<BN, T>, grid, kFewThreads, FewSmem<BN>::kBytes, plan.split, stream, maps,
+                        p, plan);
+}
+
+template <typename T>
+int launch(const ScaledLinearParams& p, cudaStream_t stream) {
+  const ScaledPlan plan = plan_scaled(p);
+  ScaledMaps maps;
+  int st = encode(&maps.x, p.x, p.in, p.rows, p.x_stride, plan.split == 0 ? 128 : plan.tile, "x");
+  if (st == CTMR_OK) st = encode(&maps.w, p.weight, p.in, p.out, p.weight_stride, 128, "weight");
+  if (st != CTMR_OK) return st;
+  const long long tiles = static_cast<long long>(plan.row_tiles) * plan.out_tiles;
+  if (tiles * (plan.split > 0 ? plan.split : 1) > 0x7fffffffLL)
+    return api_fail(CTMR_ERR_UNSUPPORTED, "scaled_linear: too many tiles");
+  cudaError_t e;
+  if (plan.split == 0) {
+    static ResidentClusters resident;
+    static SharedMemoryGrant grant;
+    const long long pairs = resident.count(scaled_pair_kernel<T>, 2, kPairThreads, kPairBytes);
+    e = launch_cluster(grant, scaled_pair_kernel<T>, static_cast<unsigned>(2 * (tiles < pairs ? tiles : pairs)),
+                       kPairThreads, kPairBytes, 2, stream, maps, p, plan);
+  } else {
+    const unsigned grid = static_cast<unsigned>(tiles * plan.split);
+    if (plan.tile == 16) e = launch_few<16, T>(maps, p, plan, grid, stream);
+    else if (plan.tile == 32) e = launch_few<32, T>(maps, p, plan, grid, stream);
+    else if (plan.tile == 64) e = launch_few<64, T>(maps, p, plan, grid, stream);
+    else e = launch_few<128, T>(maps, p, plan, grid, stream);
+  }
+  return e == cudaSuccess ? CTMR_OK : api_fail(CTMR_ERR_CUDA, "scaled_linear launch: %s", cudaGetErrorString(e));
+}
+
+}  // namespace
+
+int launch_scaled_linear(const ScaledLinearParams& p, int y_dtype, cudaStream_t stream) {
+  switch (y_dtype) {
+    case CTMR_DTYPE_F32: return launch<float>(p, stream);
+    case CTMR_DTYPE_BF16: return launch<__nv_bfloat16>(p, stream);
+    default: return launch<__half>(p, stream);
+  }
+}
+
+}  // namespace ctmr

@@ -64,6 +64,7 @@ EXPORTED_SYMBOLS = (
     "ctmr_attention",
     "ctmr_rms_norm",
     "ctmr_quantize_rows",
+    "ctmr_scaled_linear",
     "ctmr_get_device_error",
     "ctmr_status_string",
     "ctmr_last_error",
@@ -279,6 +280,31 @@ class QuantizeRowsDesc(ctypes.Structure):
     ]
 
 
+class ScaledLinearDesc(ctypes.Structure):
+    """``ctmr_scaled_linear_desc``."""
+
+    _fields_ = [
+        ("x", ctypes.c_void_p),
+        ("x_stride", ctypes.c_longlong),
+        ("x_scale", ctypes.c_void_p),
+        ("x_scale_row_stride", ctypes.c_longlong),
+        ("x_scale_block_stride", ctypes.c_longlong),
+        ("rows", ctypes.c_int),
+        ("in_features", ctypes.c_int),
+        ("out_features", ctypes.c_int),
+        ("weight", ctypes.c_void_p),
+        ("weight_stride", ctypes.c_longlong),
+        ("weight_scale", ctypes.c_void_p),
+        ("weight_scale_row_stride", ctypes.c_longlong),
+        ("weight_scale_block_stride", ctypes.c_longlong),
+        ("bias", ctypes.c_void_p),
+        ("bias_dtype", ctypes.c_int),
+        ("y", ctypes.c_void_p),
+        ("y_dtype", ctypes.c_int),
+        ("y_stride", ctypes.c_longlong),
+    ]
+
+
 def _load() -> ctypes.CDLL:
     if not LIB_PATH.exists():
         raise ImportError(
@@ -317,6 +343,7 @@ def _load() -> ctypes.CDLL:
         "ctmr_attention": (i, [ctypes.POINTER(AttentionDesc), vp]),
         "ctmr_rms_norm": (i, [ctypes.POINTER(RmsNormDesc), vp]),
         "ctmr_quantize_rows": (i, [ctypes.POINTER(QuantizeRowsDesc), vp]),
+        "ctmr_scaled_linear": (i, [ctypes.POINTER(ScaledLinearDesc), vp]),
         "ctmr_get_device_error": (i, [ctypes.POINTER(ctypes.c_uint), i]),
         "ctmr_status_string": (ctypes.c_char_p, [i]),
         "ctmr_last_error": (ctypes.c_char_p, []),

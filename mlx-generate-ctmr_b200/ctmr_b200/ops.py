@@ -796,6 +796,38 @@ class ScaledRows(NamedTuple):
         return self.values.float() * self.scale.repeat_interleave(SCALE_GROUP, dim=1)[:, :self.values.shape[1]]
 
 
+class ScaledWeight(NamedTuple):
+    """A projection's weight in 8 bits: ``values[o, i] * scale[o // 128, i // 128]``."""
+
+    values: torch.Tensor  # (out, in) e4m3, rows a multiple of 16 bytes apart
+    scale: torch.Tensor   # (ceil(out / 128), ceil(in / 128)) fp32, any values
+
+    def float(self) -> torch.Tensor:
+        out, inner = self.values.shape
+        scale = self.scale.repeat_interleave(SCALE_GROUP, dim=0)[:out]
+        return self.values.float() * scale.repeat_interleave(SCALE_GROUP, dim=1)[:, :inner]
+
+
+def scale_weight(weight: torch.Tensor) -> ScaledWeight:
+    """A ``(out, in)`` weight in 8 bits, for ``scaled_linear``: for every block of 128 x 128 the least power of two,
+    at least 2^-100, with which its largest magnitude is at most 448. Done once, where the weight is loaded; one that
+    is stored in 8 bits already is ``ScaledWeight(values, scale)``."""
+    if weight.dim() != 2 or not weight.is_floating_point() or min(weight.shape) < 1:
+        raise ValueError(f"weight must be a (out, in) tensor; got {tuple(weight.shape)} {weight.dtype}")
+    out, inner = weight.shape
+    if not torch.isfinite(weight).all():
+        raise ValueError("weight holds values that are not finite")
+    w = torch.nn.functional.pad(weight.detach().to(F32), (0, -inner % SCALE_GROUP, 0, -out % SCALE_GROUP))
+    blocks = w.unflatten(1, (-1, SCALE_GROUP)).unflatten(0, (-1, SCALE_GROUP))
+    top = blocks.abs().amax(dim=(1, 3))
+    fraction, exponent = torch.frexp(top)  # 448 is 0.875 * 2^9
+    power = torch.where(top == 0, -100, (exponent - 9 + (fraction > 0.875)).clamp(min=-100))
+    scale = ((power.to(torch.int32) + 127) << 23).view(F32)
+    values = (blocks / scale[:, None, :, None]).flatten(2).flatten(0, 1)[:out]
+    room = (inner + 15) // 16 * 16
+    return ScaledWeight(values[:, :room].to(E4M3).contiguous()[:, :inner], scale)
+
+
 def _empty_rows8(like: torch.Tensor, rows: int, channels: int) -> ScaledRows:
     """Uninitialised 8-bit rows; scales lie group by group, as the products read them."""
     values = like.new_empty((rows, (channels + 15) // 16 * 16), dtype=E4M3)
@@ -895,6 +927,61 @@ def quantize_rows(x: torch.Tensor, *, gate: bool = False) -> ScaledRows:
     status = LIB.ctmr_quantize_rows(ctypes.byref(desc), stream)
     if status:
         check(status, "quantize_rows")
+    return out
+
+
+def scaled_linear(x: ScaledRows, weight: ScaledWeight, bias: torch.Tensor | None = None, *,
+                  out_dtype: torch.dtype = BF16, out: torch.Tensor | None = None) -> torch.Tensor:
+    """A projection of 8-bit rows by an 8-bit weight, both with scales along blocks of 128 inputs
+    (``ctmr_scaled_linear``): ``y = x weight^T + bias`` of the values that they stand for, fp32 sums, rounded once to
+    ``out_dtype`` (bf16, fp16 or fp32).
+
+    ``x`` comes from ``quantize_rows`` or ``rms_norm``, ``weight`` from ``scale_weight`` or a checkpoint; both scales
+    may be any numbers, in any strides. Any number of rows, inputs and outputs. ``bias`` is fp32 or of the output's type.
+    What is not finite in a row, or in an output's weights, stays in that row, or output.
+    """
+    values, x_scale = x
+    w, w_scale = weight
+    if values.dtype != E4M3 or w.dtype != E4M3 or values.dim() != 2 or w.dim() != 2 or w.shape[1] != values.shape[1]:
+        raise ValueError(f"x and weight must be (rows, in) and (out, in) e4m3 tensors; got {tuple(values.shape)} "
+                         f"{values.dtype} and {tuple(w.shape)} {w.dtype}")
+    dev, stream = _device_stream(values, "x")
+    rows, inner = values.shape
+    outer = w.shape[0]
+    blocks = (inner + 127) // 128
+    if (x_scale.dtype != F32 or w_scale.dtype != F32 or x_scale.shape != (rows, blocks)
+            or w_scale.shape != ((outer + 127) // 128, blocks)):
+        raise ValueError(f"scales must be ({rows}, {blocks}) and ({(outer + 127) // 128}, {blocks}) float32; got "
+                         f"{tuple(x_scale.shape)} {x_scale.dtype} and {tuple(w_scale.shape)} {w_scale.dtype}")
+    if w.get_device() != dev or x_scale.get_device() != dev or w_scale.get_device() != dev:
+        raise ValueError(f"weight and scales must be on cuda:{dev}")
+    bias_at, bias_code = None, 0
+    if out is not None:
+        out_dtype = out.dtype
+    code = _FLOAT_CODES.get(out_dtype)
+    if code is None:
+        raise ValueError(f"the output is bf16, fp16 or fp32; got {out_dtype}")
+    if bias is not None:
+        if bias.shape != (outer,) or bias.dtype not in (F32, out_dtype) or bias.get_device() != dev:
+            raise ValueError(f"bias must be {outer} float32 or {out_dtype} values on cuda:{dev}")
+        bias = bias.contiguous()
+        bias_at, bias_code = bias.data_ptr(), _FLOAT_CODES[bias.dtype]
+    if out is None:
+        out = x_scale.new_empty((rows, outer), dtype=out_dtype)
+    elif out.shape != (rows, outer) or out.get_device() != dev:
+        raise ValueError(f"out must be ({rows}, {outer}) on cuda:{dev}")
+    (xs, xc), (ws, wc), (ys, yc) = values.stride(), w.stride(), out.stride()
+    if (inner > 1 and (xc != 1 or wc != 1)) or (outer > 1 and yc != 1):
+        raise ValueError("the columns of x, weight and out must be contiguous")
+    room = (inner + 15) // 16 * 16  # a stride over an extent of one addresses nothing
+    desc = _lib.ScaledLinearDesc(
+        values.data_ptr(), xs if rows > 1 else room, x_scale.data_ptr(), *x_scale.stride(), rows, inner, outer,
+        w.data_ptr(), ws if outer > 1 else room, w_scale.data_ptr(), *w_scale.stride(), bias_at, bias_code,
+        out.data_ptr(), code, ys if rows > 1 else outer)
+    LAUNCHES[0] += 1
+    status = LIB.ctmr_scaled_linear(ctypes.byref(desc), stream)
+    if status:
+        check(status, "scaled_linear")
     return out
 
 

@@ -77,3 +77,37 @@ def _quantize(**kw):
 def test_quantize_validation(change, status):
     assert LIB.ctmr_quantize_rows(_quantize(**change), None) == status
     assert LIB.ctmr_quantize_rows(None, None) == INVALID
+
+
+def _linear(**kw):
+    return _changed(_lib.ScaledLinearDesc(0x1000, 256, 0x2000, 1, 10, 10, 250, 300, 0x3000, 256, 0x4000, 2, 1, 0x5000,
+                                          _lib.DTYPE_F32, 0x6000, _lib.DTYPE_BF16, 300), kw)
+
+
+@pytest.mark.parametrize(("change", "status"), [
+    (dict(y_dtype=3), INVALID),
+    (dict(bias_dtype=_lib.DTYPE_F16), INVALID),
+    (dict(rows=-1), INVALID),
+    (dict(in_features=0), INVALID),
+    (dict(out_features=0), INVALID),
+    (dict(rows=2 ** 30), UNSUPPORTED),
+    (dict(x_stride=248), INVALID),
+    (dict(x_stride=264), INVALID),
+    (dict(weight_stride=240), INVALID),
+    (dict(y_stride=299), INVALID),
+    (dict(x_scale_row_stride=-1), INVALID),
+    (dict(weight_scale_block_stride=-1), INVALID),
+    (dict(x=0x1008), INVALID),
+    (dict(weight=0x3008), INVALID),
+    (dict(x=None), INVALID),
+    (dict(x_scale=None), INVALID),
+    (dict(weight_scale=None), INVALID),
+    (dict(y=None), INVALID),
+    (dict(y=0x6001), INVALID),
+    (dict(bias=0x5002), INVALID),
+    (dict(x_scale=0x2002), INVALID),
+    (dict(rows=0, x=None), OK),
+])
+def test_linear_validation(change, status):
+    assert LIB.ctmr_scaled_linear(_linear(**change), None) == status
+    assert LIB.ctmr_scaled_linear(None, None) == INVALID

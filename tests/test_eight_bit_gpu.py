@@ -279,7 +279,136 @@ def test_quantize_extremes_and_not_finite():
     _check_rows(ops.quantize_rows(pair, gate=True), _gate_ref(pair))
 
 
-# ---------------------------------------------------------------------------------------------- both
+# ---------------------------------------------------------------------------------------------- product
+def _rows8(gen, rows, channels, std=1.0):
+    """8-bit rows with scales of any value, not only powers of two."""
+    from ctmr_b200 import ops
+
+    x = ops.quantize_rows(_randn(gen, rows, channels, std=std))
+    return ops.ScaledRows(x.values, x.scale * (0.5 + torch.rand(x.scale.shape, generator=gen, device="cuda")))
+
+
+def _weight8(gen, out, inner):
+    from ctmr_b200 import ops
+
+    w = ops.scale_weight(_randn(gen, out, inner, std=inner ** -0.5))
+    return ops.ScaledWeight(w.values, w.scale * (0.5 + torch.rand(w.scale.shape, generator=gen, device="cuda")))
+
+
+def _spread(scale, dim, n):
+    return scale.double().repeat_interleave(128, dim=dim).narrow(dim, 0, n)
+
+
+def _linear_ref(x, weight, bias):
+    """(y, sum |x||w|) in 64 bits."""
+    out, inner = weight.values.shape
+    a = x.values.double() * _spread(x.scale, 1, inner)
+    w = weight.values.double() * _spread(_spread(weight.scale, 0, out), 1, inner)
+    y = a @ w.T
+    return (y if bias is None else y + bias.double()), a.abs() @ w.abs().T
+
+
+def _check_linear(got, x, weight, bias):
+    ref, size = _linear_ref(x, weight, bias)
+    inner = weight.values.shape[1]
+    _within(got, ref, U[got.dtype] * ref.abs() + 2.0 ** -23 * inner ** 0.5 * size + 2.0 ** -25)
+    _no_device_error()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize(("rows", "inner", "outer"), [
+    (1, 1, 1), (1, 64, 7), (3, 100, 128), (1, 4096, 1000), (16, 128, 129), (17, 1024, 256), (32, 4096, 512),
+    (33, 1000, 1000), (64, 2000, 130), (65, 640, 384), (100, 129, 77), (128, 512, 1536), (129, 2048, 4096),
+    (300, 256, 2000), (617, 512, 1536), (1000, 4096, 512), (2049, 1032, 520), (1300, 333, 4097), (5000, 128, 256),
+    (4096, 2048, 2048), (1, 20000, 300)])
+def test_linear(rows, inner, outer, dtype):
+    from ctmr_b200 import ops
+
+    gen = _gen(rows * 7 + inner + outer)
+    x, w = _rows8(gen, rows, inner), _weight8(gen, outer, inner)
+    bias = _randn(gen, outer, std=0.5)
+    _check_linear(ops.scaled_linear(x, w, out_dtype=dtype), x, w, None)
+    _check_linear(ops.scaled_linear(x, w, bias, out_dtype=dtype), x, w, bias)
+    _check_linear(ops.scaled_linear(x, w, bias.to(dtype), out_dtype=dtype), x, w, bias.to(dtype))
+
+
+@pytest.mark.parametrize("rows", [5, 90, 700])
+def test_linear_strides(rows):
+    """Rows, weights and outputs inside wider tensors, scales in either order; what lies around stays."""
+    from ctmr_b200 import ops
+
+    gen = _gen(rows)
+    inner, outer = 384, 650
+    x, w = _rows8(gen, rows, inner + 128), _weight8(gen, outer + 128, inner + 256)
+    part = ops.ScaledRows(x.values[:, 128:], x.scale[:, 1:].contiguous())
+    wide = ops.ScaledWeight(w.values[128:, 128:128 + inner], w.scale[1:, 1:4].t().contiguous().t())
+    for dtype in TYPES:
+        room = torch.full((rows, outer + 9), 7.0, dtype=dtype, device="cuda")
+        out = room[:, 3:3 + outer]
+        assert ops.scaled_linear(part, wide, out=out) is out
+        _check_linear(out, part, wide, None)
+        assert (room[:, :3] == 7).all() and (room[:, 3 + outer:] == 7).all()
+
+
+@pytest.mark.parametrize("rows", [1, 40, 200, 1500])
+def test_linear_not_finite(rows):
+    """A NaN or an infinity in a row or in an output's weights stays there; rows' padding is never read."""
+    from ctmr_b200 import ops
+
+    gen = _gen(rows)
+    inner, outer = 520, 300
+    x, w = _rows8(gen, rows, inner), _weight8(gen, outer, inner)
+    good = ops.scaled_linear(x, w, out_dtype=torch.float32)
+    room = torch.full((rows, 528), 0x7f, dtype=torch.uint8, device="cuda")  # NaN in the padding
+    room[:, :inner] = x.values.view(torch.uint8)
+    assert torch.equal(ops.scaled_linear(ops.ScaledRows(room.view(E4M3)[:, :inner], x.scale), w, out_dtype=torch.float32), good)
+    scale = x.scale.clone()
+    scale[rows // 2, 1] = float("nan")
+    got = ops.scaled_linear(ops.ScaledRows(x.values, scale), w, out_dtype=torch.float32)
+    assert torch.isnan(got[rows // 2]).all()
+    keep = torch.arange(rows, device="cuda") != rows // 2
+    assert torch.equal(got[keep], good[keep])
+    room = torch.zeros((outer, 528), dtype=torch.uint8, device="cuda")
+    room[:, :inner] = w.values.view(torch.uint8)
+    room[77, 400] = 0x7f
+    got = ops.scaled_linear(x, ops.ScaledWeight(room.view(E4M3)[:, :inner], w.scale), out_dtype=torch.float32)
+    assert torch.isnan(got[:, 77]).all()
+    keep = torch.arange(outer, device="cuda") != 77
+    assert torch.equal(got[:, keep], good[:, keep])
+    _no_device_error()
+
+
+def test_linear_same_bits_again():
+    """The order of the sums is the same in every call."""
+    from ctmr_b200 import ops
+
+    for rows, inner, outer in ((1, 8192, 512), (48, 4096, 1024), (700, 2048, 768)):
+        gen = _gen(rows)
+        x, w = _rows8(gen, rows, inner), _weight8(gen, outer, inner)
+        first = ops.scaled_linear(x, w, out_dtype=torch.float32)
+        for _ in range(5):
+            assert torch.equal(ops.scaled_linear(x, w, out_dtype=torch.float32), first)
+
+
+def test_scale_weight():
+    from ctmr_b200 import ops
+
+    gen = _gen(4)
+    for out, inner in ((1, 1), (128, 128), (300, 200), (129, 1000)):
+        weight = _randn(gen, out, inner, dtype=torch.bfloat16)
+        got = ops.scale_weight(weight)
+        assert got.values.shape == (out, inner) and (out == 1 or got.values.stride(0) % 16 == 0)
+        top = weight.double().abs()[:128, :128].max()
+        assert torch.frexp(got.scale)[0].eq(0.5).all()  # powers of two
+        assert top <= 448 * got.scale[0, 0] and top > 224 * got.scale[0, 0]
+        _within(got.float(), weight.double(), 2.0 ** -4 * weight.double().abs() + 2.0 ** -10 * got.scale.max().double())
+    assert (ops.scale_weight(torch.zeros((3, 5), device="cuda")).float() == 0).all()
+    for bad in (torch.zeros(5), torch.zeros((2, 2), dtype=torch.int32), torch.full((2, 2), float("inf"))):
+        with pytest.raises(ValueError):
+            ops.scale_weight(bad)
+
+
+# ---------------------------------------------------------------------------------------------- all
 def test_rows_past_32_bits():
     """Rows whose elements lie more than 2^31 apart."""
     from ctmr_b200 import ops
@@ -301,11 +430,13 @@ def test_graphs_and_streams():
     gen = _gen(8)
     x, residual = _randn(gen, 70, 1536, dtype=torch.bfloat16), _randn(gen, 70, 1536, dtype=torch.bfloat16)
     weight = 1.0 + _randn(gen, 1536, std=0.2)
+    w = _weight8(gen, 3000, 1536)
 
     def both():
         y, h = ops.rms_norm(x, weight, residual=residual, quantize=True)
         z = ops.quantize_rows(h, gate=True)
-        return y.values.view(torch.uint8), y.scale, h, z.values.view(torch.uint8), z.scale
+        return y.values.view(torch.uint8), y.scale, h, z.values.view(torch.uint8), z.scale, ops.scaled_linear(y, w), \
+            ops.scaled_linear(ops.ScaledRows(y.values[:5], y.scale[:5]), w)
 
     both()
     side = torch.cuda.Stream()
@@ -355,6 +486,26 @@ def test_refusals():
         lambda: ops.quantize_rows(x.t()),
         lambda: ops.quantize_rows(x[:, :255], gate=True),
         lambda: ops.quantize_rows(x.cpu()),
+    ]
+    a, w = ops.quantize_rows(x), ops.scale_weight(torch.ones((300, 256), device="cuda"))
+    bad += [
+        lambda: ops.scaled_linear(ops.ScaledRows(x, a.scale), w),
+        lambda: ops.scaled_linear(ops.ScaledRows(a.values.cpu(), a.scale), w),
+        lambda: ops.scaled_linear(ops.ScaledRows(a.values, a.scale[:3]), w),
+        lambda: ops.scaled_linear(ops.ScaledRows(a.values, a.scale.double()), w),
+        lambda: ops.scaled_linear(ops.ScaledRows(a.values[:, :128], a.scale[:, :1]), w),
+        lambda: ops.scaled_linear(ops.ScaledRows(a.values[:, 8:136], a.scale), ops.scale_weight(torch.ones((3, 128), device="cuda"))),
+        lambda: ops.scaled_linear(ops.ScaledRows(a.values[:, 8:136], a.scale[:, :1]),
+                                  ops.scale_weight(torch.ones((3, 128), device="cuda"))),  # not 16-byte aligned
+        lambda: ops.scaled_linear(a, ops.ScaledWeight(w.values, w.scale[:2])),
+        lambda: ops.scaled_linear(a, ops.ScaledWeight(w.values, w.scale.cpu())),
+        lambda: ops.scaled_linear(a, w, out_dtype=torch.float64),
+        lambda: ops.scaled_linear(a, w, torch.ones(299, device="cuda")),
+        lambda: ops.scaled_linear(a, w, torch.ones(300, device="cuda", dtype=torch.float16)),
+        lambda: ops.scaled_linear(a, w, out=torch.empty((4, 299), device="cuda")),
+        lambda: ops.scaled_linear(a, w, out=torch.empty((300, 4), device="cuda").t()),
+        lambda: ops.scaled_linear(ops.ScaledRows(torch.zeros((4, 250), device="cuda").to(E4M3), a.scale),
+                                  ops.scale_weight(torch.ones((3, 250), device="cuda"))),  # rows 250 bytes apart
     ]
     for call in bad:
         with pytest.raises(ValueError):
