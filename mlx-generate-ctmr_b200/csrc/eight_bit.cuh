@@ -5,15 +5,16 @@
 // dividing by it is exact, so the rounding to e4m3 is the only one, and e4m3's relative step does not depend on
 // the scale's mantissa. A group that holds an infinity or a NaN becomes NaN as a whole, scale and values.
 //
-// The bytes are those that the formula in 64 bits rounds to. Values are computed in 32 bits with an error below
-// kNear of themselves; where both ends of that interval round to the same byte, so does everything between. Where
-// they do not (one value in some 2^16), that value is computed again in 64 bits. The scale likewise, where the
+// The bytes are those that the formula in 64 bits rounds to. Values are computed in 32 bits and stay within a few
+// units of 2^-24 of themselves; where both ends of that interval round to the same byte, so does everything between.
+// Where they do not (one value in some 2^17), that value is computed again in 64 bits. The scale likewise, where the
 // largest magnitude is as near to 448 times a power of two.
 #pragma once
 
 #include <cuda_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
 
 #include "tokens.cuh"
 
@@ -30,14 +31,16 @@ struct RowNormParams {
   long long x_token, x_head, r_token, r_head, y_token, y_head, s_token, s_head, scale_token, scale_group;
   int tokens, heads, channels, weight_f32;
   float eps;
+  double per_channel;  // 1 / channels, set by the launcher
 };
 
-struct QuantizeParams {
+struct QuantizeParams {  // the last three: set by the launcher
   const void* x;  // (rows, channels), or (rows, 2 channels) where gated
   void* values;
   float* scale;
   long long x_stride, values_stride, scale_row, scale_group;
   int rows, channels, gate;
+  uint32_t per_row, skip_rows, skip_groups;
 };
 
 struct ScaledLinearParams {
@@ -52,47 +55,194 @@ cudaError_t launch_row_norm(const RowNormParams& p, int dtype, cudaStream_t stre
 cudaError_t launch_quantize(const QuantizeParams& p, int dtype, cudaStream_t stream);
 int launch_scaled_linear(const ScaledLinearParams& p, int y_dtype, cudaStream_t stream);  // a CTMR_ status
 
-// ---------------------------------------------------------------- eight values of a row
-// 8 consecutive elements of a row from memory, zeros past `left` of them. WIDE: the row's address, stride and
-// length allow 16-byte accesses.
+// ---------------------------------------------------------------- a group of a row
+// Eight lanes hold a group of 128 channels, 16 each: consecutive ones where the row's address, stride and length allow
+// 32-byte accesses (WIDE), every eighth one otherwise, so that the lanes' single accesses still lie side by side.
+constexpr int kEach = 16, kGroupLanes = kScaleGroup / kEach;
+
+template <bool WIDE>
+__device__ __forceinline__ int channel_of(int group, int lane8, int e) {
+  return group * kScaleGroup + (WIDE ? lane8 * kEach + e : lane8 + kGroupLanes * e);
+}
+
+__device__ __forceinline__ void load32(const void* at, uint32_t (&r)[8]) {
+  asm volatile("ld.global.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"  // volatile: before the stores over the same row
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "l"(at)
+               : "memory");
+}
+
+__device__ __forceinline__ void store32(void* at, const uint32_t (&r)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(at), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]),
+               "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+
+// v[at] of registers.
+__device__ __forceinline__ float pick(const float (&v)[kEach], int at) {
+  float r = v[0];
+#pragma unroll
+  for (int i = 1; i < kEach; ++i) r = at == i ? v[i] : r;
+  return r;
+}
+
+// A lane's 16 channels of a row as they lie in memory. Past the row's end `values`, by whole warps, gives zeros.
 template <typename T, bool WIDE>
-__device__ __forceinline__ void load8(const T* at, int left, float (&v)[8]) {
-  if constexpr (WIDE) {
-    uint4 raw[sizeof(T) == 4 ? 2 : 1];
-    const bool in = left > 0;
+struct Loaded {
+  uint32_t raw[WIDE ? kEach * sizeof(T) / 4 : 1];
+  T each[WIDE ? 1 : kEach];
+
+  __device__ __forceinline__ void load(const T* row, int channels, int group, int lane8) {
+    if constexpr (WIDE) {
+      const int c = channel_of<true>(group, lane8, 0);
+      if (c < channels) {
+        load32(row + c, *reinterpret_cast<uint32_t(*)[8]>(raw));
+        if constexpr (sizeof(T) == 4) load32(row + c + 8, *reinterpret_cast<uint32_t(*)[8]>(raw + 8));
+      }
+    } else {
 #pragma unroll
-    for (uint32_t i = 0; i < sizeof(raw) / 16; ++i)
-      raw[i] = in ? reinterpret_cast<const uint4*>(at)[i] : make_uint4(0, 0, 0, 0);
-    const T* e = reinterpret_cast<const T*>(raw);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = to_float(e[i]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = i < left ? to_float(at[i]) : 0.f;
+      for (int i = 0; i < kEach; ++i) {
+        const int c = channel_of<false>(group, lane8, i);
+        each[i] = c < channels ? row[c] : from_float<T>(0.f);
+      }
+    }
   }
+
+  __device__ __forceinline__ void values(float (&v)[kEach], bool inside) const {
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      if constexpr (!WIDE) {
+        v[i] = to_float(each[i]);
+      } else if constexpr (sizeof(T) == 4) {
+        v[i] = __uint_as_float(raw[i]);
+      } else if constexpr (std::is_same<T, __half>::value) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&raw[i / 2]));
+        v[i] = i % 2 ? f.y : f.x;
+      } else {
+        v[i] = __uint_as_float(i % 2 ? raw[i / 2] & 0xffff0000u : raw[i / 2] << 16);
+      }
+    }
+    if (WIDE && __any_sync(0xffffffffu, !inside))  // (a branch: selects, or zeros ahead of the load, would cost every warp)
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) v[i] = inside ? v[i] : 0.f;
+  }
+};
+
+template <typename T, bool WIDE>
+__device__ __forceinline__ void load16(const T* row, int channels, int group, int lane8, float (&v)[kEach]) {
+  Loaded<T, WIDE> in;
+  in.load(row, channels, group, lane8);
+  in.values(v, channel_of<WIDE>(group, lane8, 0) < channels);
+}
+
+// Two values to the 16-bit type, the first in the low half.
+__device__ __forceinline__ uint32_t pack2(float a, float b, __half) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b, __nv_bfloat16) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
 }
 
 template <typename T, bool WIDE>
-__device__ __forceinline__ void store8(T* at, int left, const float (&v)[8]) {
+__device__ __forceinline__ void store16(T* row, int channels, int group, int lane8, const float (&v)[kEach]) {
   if constexpr (WIDE) {
-    if (left <= 0) return;
-    uint4 raw[sizeof(T) == 4 ? 2 : 1];
-    T* e = reinterpret_cast<T*>(raw);
+    const int c = channel_of<true>(group, lane8, 0);
+    if (c >= channels) return;
+    uint32_t raw[8];
+    if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) e[i] = from_float<T>(v[i]);
+      for (int j = 0; j < 2; ++j) {
 #pragma unroll
-    for (uint32_t i = 0; i < sizeof(raw) / 16; ++i) reinterpret_cast<uint4*>(at)[i] = raw[i];
+        for (int i = 0; i < 8; ++i) raw[i] = __float_as_uint(v[8 * j + i]);
+        store32(row + c + 8 * j, raw);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) raw[i] = pack2(v[2 * i], v[2 * i + 1], T());
+      store32(row + c, raw);
+    }
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (i < left) at[i] = from_float<T>(v[i]);
+    for (int i = 0; i < kEach; ++i) {
+      const int c = channel_of<false>(group, lane8, i);
+      if (c < channels) row[c] = from_float<T>(v[i]);
+    }
   }
+}
+
+template <bool WIDE>
+__device__ __forceinline__ void store_bytes(uint8_t* row, int channels, int group, int lane8, const uint32_t (&q)[4]) {
+  if constexpr (WIDE) {
+    const int c = channel_of<true>(group, lane8, 0);
+    if (c < channels) *reinterpret_cast<uint4*>(row + c) = make_uint4(q[0], q[1], q[2], q[3]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const int c = channel_of<false>(group, lane8, i);
+      if (c < channels) row[c] = static_cast<uint8_t>(q[i / 4] >> (i % 4 * 8));
+    }
+  }
+}
+
+// Products and sums at two to an instruction.
+__device__ __forceinline__ void mul16(float (&v)[kEach], const float (&a)[kEach], const float (&b)[kEach]) {
+#pragma unroll
+  for (int i = 0; i < kEach; i += 2)
+    asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmul.rn.f32x2 z, x, y;\n\t"
+        "mov.b64 {%0, %1}, z;\n\t}"
+        : "=f"(v[i]), "=f"(v[i + 1])
+        : "f"(a[i]), "f"(a[i + 1]), "f"(b[i]), "f"(b[i + 1]));
+}
+
+__device__ __forceinline__ void mul16(float (&v)[kEach], const float (&a)[kEach], float b) {
+#pragma unroll
+  for (int i = 0; i < kEach; i += 2)
+    asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %4};\n\tmul.rn.f32x2 z, x, y;\n\t"
+        "mov.b64 {%0, %1}, z;\n\t}"
+        : "=f"(v[i]), "=f"(v[i + 1])
+        : "f"(a[i]), "f"(a[i + 1]), "f"(b));
+}
+
+// a b + c.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y, z, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
+      "fma.rn.f32x2 w, x, y, z;\n\tmov.b64 {%0, %1}, w;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+      "mul.rn.f32x2 w, x, y;\n\tmov.b64 {%0, %1}, w;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+
+__device__ __forceinline__ void add16(float (&v)[kEach], const float (&a)[kEach]) {
+#pragma unroll
+  for (int i = 0; i < kEach; i += 2)
+    asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%0, %1};\n\tmov.b64 y, {%2, %3};\n\tadd.rn.f32x2 z, x, y;\n\t"
+        "mov.b64 {%0, %1}, z;\n\t}"
+        : "+f"(v[i]), "+f"(v[i + 1])
+        : "f"(a[i]), "f"(a[i + 1]));
 }
 
 // ---------------------------------------------------------------- rounding to e4m3
-constexpr float kNear = 0x1p-20f;  // what the 32-bit formulas stay within, several times over
+constexpr float kUnit = 0x1p-24f;  // one rounding of a 32-bit value
 
-// The larger magnitude; NaN if either is.
+__device__ __forceinline__ bool is_finite(float v) { return fabsf(v) <= 3.402823466e38f; }
+
+// The largest of three magnitudes, or of two numbers; NaN if any is.
+__device__ __forceinline__ float max_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 __device__ __forceinline__ float max_nan(float a, float b) {
   float r;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
@@ -106,9 +256,11 @@ __device__ __forceinline__ uint32_t e4m3x2(float a, float b) {
   return r;
 }
 
-__device__ __forceinline__ uint2 e4m3x8(const float (&v)[8], float by) {
-  return make_uint2(e4m3x2(v[0] * by, v[1] * by) | e4m3x2(v[2] * by, v[3] * by) << 16,
-                    e4m3x2(v[4] * by, v[5] * by) | e4m3x2(v[6] * by, v[7] * by) << 16);
+__device__ __forceinline__ void e4m3x16(uint32_t (&q)[4], const float (&v)[kEach], float by) {
+  float u[kEach];
+  mul16(u, v, by);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) q[i] = e4m3x2(u[4 * i], u[4 * i + 1]) | e4m3x2(u[4 * i + 2], u[4 * i + 3]) << 16;
 }
 
 // The byte of a 64-bit value, rounded once: to 32 bits first, with the last bit set where that cut something off, so
@@ -119,68 +271,55 @@ __device__ __forceinline__ uint32_t e4m3_exact(double v) {
   return e4m3x2(f, 0.f) & 0xffu;
 }
 
-// k of the scale 2^k for a finite largest magnitude: 448 is 1.75 * 2^8, so a mantissa above 1.75 carries.
+// k of the scale 2^k for a largest magnitude (any k if it is not finite): 448 is 1.75 * 2^8, so a mantissa above 1.75
+// carries.
 __device__ __forceinline__ int scale_power(float top) {
   return max(static_cast<int>((__float_as_uint(top) + 0x1fffffu) >> 23) - 135, -100);
 }
 
 __device__ __forceinline__ float power_of_two(int k) { return __uint_as_float(static_cast<uint32_t>(k + 127) << 23); }
 
-// Rounds a group of 128 channels, 8 to each of the 16 lanes of half a warp, all of which call this. `exact(i)` gives
-// value i in 64 bits; without EXACT the values are as they are meant. Returns the 8 bytes, and the scale.
-template <bool EXACT, typename Exact>
-__device__ __forceinline__ uint2 quantize_group(const float (&v)[8], Exact exact, float& scale) {
-  float top = 0.f;
+// Rounds a group of channels, held by eight lanes of a warp all of whose lanes call this. UNITS: how many roundings
+// the values are off by at most, the one of scaling them here included; 0: they are as they are meant. `top64()` gives
+// the largest magnitude of the lane's values in 64 bits. Gives the 16 bytes, the scale and its inverse, and returns (bit
+// i: value i) which values 64 bits have to decide.
+template <int UNITS, typename Top>
+__device__ __forceinline__ uint32_t quantize_group(const float (&v)[kEach], Top top64, uint32_t (&q)[4], float& scale,
+                                                   float& by) {
+  constexpr float kLow = 1.f - UNITS * kUnit, kHigh = 1.f + 2 * ((UNITS + 1) / 2) * kUnit;
+  float top = max_nan(v[0], v[1], v[2]);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) top = max_nan(top, fabsf(v[i]));
+  for (int i = 3; i + 1 < kEach; i += 2) top = max_nan(top, v[i], v[i + 1]);
+  top = max_nan(top, v[kEach - 1], 0.f);
 #pragma unroll
-  for (int i = 8; i > 0; i /= 2) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, i));
-  const bool finite = top <= 3.402823466e38f;
-  int k = finite ? scale_power(top) : 0;
-  if constexpr (EXACT) {
-    const int low = finite ? scale_power(top * (1.f - kNear)) : 0;
-    if (finite && scale_power(fminf(top * (1.f + kNear), 3.402823466e38f)) != low) {
-      double most = 0.0;
-#pragma unroll 1
-      for (int i = 0; i < 8; ++i) most = fmax(most, fabs(exact(i)));
+  for (int i = kGroupLanes / 2; i > 0; i /= 2) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, i));
+  int k = scale_power(top);
+  if constexpr (UNITS > 0) {
+    const int low = scale_power(top * kLow);
+    k = scale_power(top * kHigh);
+    if (k != low && is_finite(top)) {
+      double most = top64();
 #pragma unroll
-      for (int i = 8; i > 0; i /= 2) most = fmax(most, __shfl_xor_sync(0xffffu << (threadIdx.x & 16), most, i));
-      k = most <= ldexp(448.0, low) ? low : low + 1;
+      for (int i = kGroupLanes / 2; i > 0; i /= 2)
+        most = fmax(most, __shfl_xor_sync(0xffu << (threadIdx.x & 24), most, i));
+      if (most <= ldexp(448.0, low)) k = low;
     }
   }
-  scale = finite ? power_of_two(k) : __int_as_float(0x7fc00000);
-  const float by = finite ? power_of_two(-k) : scale;
-  if constexpr (EXACT) {
-    uint2 q = e4m3x8(v, by * (1.f - kNear));
-    const uint2 other = e4m3x8(v, by * (1.f + kNear));
-    if (q.x != other.x || q.y != other.y) {
-#pragma unroll 1
-      for (int i = 0; i < 8; ++i) {
-        const uint32_t at = (i & 3) * 8, diff = i < 4 ? q.x ^ other.x : q.y ^ other.y;
-        if (!(diff >> at & 0xffu)) continue;
-        const uint32_t byte = e4m3_exact(ldexp(exact(i), -k)) << at, keep = ~(0xffu << at);
-        if (i < 4) q.x = (q.x & keep) | byte;
-        else q.y = (q.y & keep) | byte;
-      }
-    }
-    return q;
-  } else {
-    return e4m3x8(v, by);
-  }
-}
-
-// Stores 8 bytes, `left` of which are the row's.
-template <bool WIDE>
-__device__ __forceinline__ void store_bytes(uint8_t* at, int left, uint2 q) {
-  if constexpr (WIDE) {
-    if (left > 0) *reinterpret_cast<uint2*>(at) = q;
-  } else if (left >= 8 && (reinterpret_cast<uintptr_t>(at) & 7) == 0) {
-    *reinterpret_cast<uint2*>(at) = q;
-  } else {
+  const float nan = __int_as_float(0x7fc00000);
+  scale = is_finite(top) ? power_of_two(k) : nan;
+  by = is_finite(top) ? power_of_two(-k) : nan;
+  uint32_t differ = 0;
+  if constexpr (UNITS > 0) {
+    uint32_t other[4];
+    e4m3x16(q, v, by * kLow);
+    e4m3x16(other, v, by * kHigh);
+    if ((q[0] ^ other[0]) | (q[1] ^ other[1]) | (q[2] ^ other[2]) | (q[3] ^ other[3]))
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (i < left) at[i] = static_cast<uint8_t>((i < 4 ? q.x : q.y) >> ((i & 3) * 8));
+      for (int i = 0; i < kEach; ++i) differ |= ((q[i / 4] ^ other[i / 4]) >> (i % 4 * 8) & 0xffu) != 0 ? 1u << i : 0u;
+  } else {
+    e4m3x16(q, v, by);
   }
+  return differ;
 }
 
 }  // namespace ctmr

@@ -13,75 +13,109 @@
 namespace ctmr {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 256, kBlocks = 3, kGroups = kThreads / kGroupLanes;
 
-// silu(a) b. e^-a is infinite below -88, and the product then zero: below what any scale keeps.
-__device__ __forceinline__ float gated(float a, float b) {
+// silu(a) b, two at a time. e^-a is infinite below -88, and the product then zero: below what any scale keeps.
+__device__ __forceinline__ float2 gated2(float2 a, float2 b) {
   constexpr float kLog2E = 1.44269504f, kRest = 1.92596299e-8f;
-  const float n = fminf(fmaxf(-a, -128.f), 128.f);  // further out nothing changes, but the product would overflow
-  const float t = n * kLog2E, rest = fmaf(n, kRest, fmaf(n, kLog2E, -t));
-  float e, r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
-  e = fmaf(e, rest * 0.693147181f, e);
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
-  return a * r * b;
+  // Further out nothing changes, but the product would overflow.
+  const float2 n = make_float2(fminf(fmaxf(-a.x, -128.f), 128.f), fminf(fmaxf(-a.y, -128.f), 128.f));
+  const float2 log2e = make_float2(kLog2E, kLog2E), minus = make_float2(-kLog2E, -kLog2E);
+  const float2 t = mul2(n, log2e);
+  // What t's rounding cut off, with the other sign, times ln 2: e^n = 2^t (1 - rest).
+  const float2 rest = mul2(fma2(n, make_float2(-kRest, -kRest), fma2(n, minus, t)), make_float2(0.693147181f, 0.693147181f));
+  float2 e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(t.x));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(t.y));
+  // 1 + e (1 - rest)
+  const float2 one = make_float2(1.f, 1.f), less = fma2(rest, make_float2(-1.f, -1.f), one);
+  const float2 d = fma2(e, less, one);
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.x) : "f"(d.x));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.y) : "f"(d.y));
+  return mul2(mul2(a, r), b);
 }
 
-__device__ __noinline__ double gated64(double a, double b) { return a / (1.0 + exp(-a)) * b; }
+// In units of 2^-24: the exponential's approximation 4 and its correction 1, the sum 1, the reciprocal 2, the three
+// products 3.
+constexpr int kGatedUnits = 12;
 
-// U eights of channels to a thread.
-template <typename T, int U, bool GATE, bool WIDE>
-__global__ void __launch_bounds__(kThreads) quantize_kernel(const __grid_constant__ QuantizeParams p) {
-  const uint32_t per_row = (p.channels + kScaleGroup - 1) / kScaleGroup * (kScaleGroup / 8);
-  // The block's first eight; 32-bit arithmetic from there on.
-  const unsigned long long first = static_cast<unsigned long long>(blockIdx.x) * (kThreads * U);
-  const unsigned long long row0 = first / per_row;
-  const uint32_t col0 = static_cast<uint32_t>(first - row0 * per_row);
+__device__ __forceinline__ double gated64(double a, double b) { return a / (1.0 + exp(-a)) * b; }
+
+// What 64 bits decide, by single lanes: calls, so that the kernel's registers are not laid out for it.
+template <typename T, bool WIDE>
+__device__ __noinline__ double gated_top(const T* x, int channels, int group, int lane8) {
+  double most = 0.0;
+  for (int i = 0; i < kEach; ++i) {
+    const int c = channel_of<WIDE>(group, lane8, i);
+    if (c < channels) most = fmax(most, fabs(gated64(to_float(x[c]), to_float(x[channels + c]))));
+  }
+  return most;
+}
+
+template <typename T, bool WIDE>
+__device__ __noinline__ void gated_patch(const T* x, uint8_t* values, int channels, int group, int lane8, uint32_t differ,
+                                         float by) {
+  for (; differ != 0; differ &= differ - 1) {
+    const int c = channel_of<WIDE>(group, lane8, __ffs(differ) - 1);
+    values[c] = static_cast<uint8_t>(e4m3_exact(gated64(to_float(x[c]), to_float(x[channels + c])) * by));
+  }
+}
+
+// A block takes 32 groups of channels at a time, eight lanes each, then those p.skip_rows rows and p.skip_groups
+// groups further: no division but the first. (Two groups to a lane, 8,192 x 11,264 gated: 108 us for 100.)
+template <typename T, bool GATE, bool WIDE>
+__global__ void __launch_bounds__(kThreads, kBlocks) quantize_kernel(const __grid_constant__ QuantizeParams p) {
+  const int lane8 = threadIdx.x % kGroupLanes;
+  const uint32_t start = blockIdx.x * kGroups + threadIdx.x / kGroupLanes, rows = static_cast<uint32_t>(p.rows);
+  uint32_t row = start / p.per_row, group = start - row * p.per_row;
   griddep_wait();
   griddep_launch_dependents();
-  float v[U][8], b[U][8];
-  int row[U], c[U], left[U];
+  while (__any_sync(0xffffffffu, row < rows)) {  // whole warps, for the shuffles
+    const bool in = row < rows;
+    const int channels = in ? p.channels : 0;
+    const T* x = static_cast<const T*>(p.x) + (in ? row * p.x_stride : 0);
+    uint8_t* values = static_cast<uint8_t*>(p.values) + (in ? row * p.values_stride : 0);
+    Loaded<T, WIDE> a, b;
+    a.load(x, channels, group, lane8);
+    if constexpr (GATE) b.load(x + p.channels, channels, group, lane8);
+    const bool inside = channel_of<WIDE>(group, lane8, 0) < channels;
+    float v[kEach];
+    a.values(v, inside);
+    if constexpr (GATE) {
+      float other[kEach];
+      b.values(other, inside);
 #pragma unroll
-  for (int i = 0; i < U; ++i) {
-    const uint32_t at = col0 + i * kThreads + threadIdx.x, down = at / per_row;
-    const unsigned long long r = row0 + down;
-    const bool in = r < static_cast<unsigned long long>(p.rows);
-    row[i] = in ? static_cast<int>(r) : 0;
-    c[i] = static_cast<int>(at - down * per_row) * 8;
-    left[i] = in ? p.channels - c[i] : 0;
-    const T* x = static_cast<const T*>(p.x) + row[i] * p.x_stride + c[i];
-    load8<T, WIDE>(x, left[i], v[i]);
-    if constexpr (GATE) load8<T, WIDE>(x + p.channels, left[i], b[i]);
-  }
-#pragma unroll
-  for (int i = 0; i < U; ++i) {
-    if constexpr (GATE)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[i][e] = gated(v[i][e], b[i][e]);
-    float scale;
-    const T* x = static_cast<const T*>(p.x) + row[i] * p.x_stride + c[i];
-    auto exact = [&](int e) { return e < left[i] ? gated64(to_float(x[e]), to_float(x[p.channels + e])) : 0.0; };
-    const uint2 q = quantize_group<GATE>(v[i], exact, scale);
-    store_bytes<WIDE>(static_cast<uint8_t*>(p.values) + row[i] * p.values_stride + c[i], left[i], q);
-    if ((threadIdx.x & 15) == 0 && left[i] > 0)
-      p.scale[row[i] * p.scale_row + (c[i] / kScaleGroup) * p.scale_group] = scale;
+      for (int e = 0; e < kEach; e += 2) {
+        const float2 g = gated2(make_float2(v[e], v[e + 1]), make_float2(other[e], other[e + 1]));
+        v[e] = g.x, v[e + 1] = g.y;
+      }
+    }
+    uint32_t q[4];
+    float scale, by;
+    const uint32_t differ = quantize_group<GATE ? kGatedUnits : 0>(
+        v, [&]() { return gated_top<T, WIDE>(x, p.channels, group, lane8); }, q, scale, by);
+    store_bytes<WIDE>(values, channels, group, lane8, q);
+    if (differ != 0) gated_patch<T, WIDE>(x, values, p.channels, group, lane8, differ, by);
+    if (lane8 == 0 && in) p.scale[row * p.scale_row + group * p.scale_group] = scale;
+    if (!in) continue;  // a row past the end stays where it is
+    row += p.skip_rows, group += p.skip_groups;
+    if (group >= p.per_row) group -= p.per_row, ++row;
   }
 }
 
 template <typename T, bool GATE>
-cudaError_t launch(const QuantizeParams& p, cudaStream_t stream) {
-  const bool wide = p.channels % 8 == 0 && p.x_stride % (16 / static_cast<int>(sizeof(T))) == 0 &&
-                    reinterpret_cast<uintptr_t>(p.x) % 16 == 0 && p.values_stride % 8 == 0 &&
-                    reinterpret_cast<uintptr_t>(p.values) % 8 == 0;
-  const unsigned long long per_row = (p.channels + kScaleGroup - 1) / kScaleGroup * (kScaleGroup / 8);
-  const unsigned long long eights = per_row * p.rows;
-  const bool small = eights <= 4ull * kThreads * device_sm_count();  // fewer than four blocks an SM: no second eight
-  const int each = kThreads * (small ? 1 : 2);
-  const unsigned long long grid = (eights + each - 1) / each;
-  if (grid > 0x7fffffffull) return cudaErrorInvalidConfiguration;
-  auto go = [&](auto kern) { return launch_kernel(kern, dim3(static_cast<unsigned>(grid)), dim3(kThreads), 0, stream, p); };
-  if (small) return wide ? go(quantize_kernel<T, 1, GATE, true>) : go(quantize_kernel<T, 1, GATE, false>);
-  return wide ? go(quantize_kernel<T, 2, GATE, true>) : go(quantize_kernel<T, 2, GATE, false>);
+cudaError_t launch(QuantizeParams p, cudaStream_t stream) {
+  const bool wide = p.channels % kEach == 0 && p.x_stride % (32 / static_cast<int>(sizeof(T))) == 0 &&
+                    reinterpret_cast<uintptr_t>(p.x) % 32 == 0 && p.values_stride % 16 == 0 &&
+                    reinterpret_cast<uintptr_t>(p.values) % 16 == 0;
+  p.per_row = (static_cast<uint32_t>(p.channels) + kScaleGroup - 1) / kScaleGroup;
+  const unsigned long long groups = static_cast<unsigned long long>(p.per_row) * p.rows;
+  const unsigned long long blocks = (groups + kGroups - 1) / kGroups;
+  const uint32_t resident = kBlocks * device_sm_count();
+  const uint32_t grid = blocks < resident ? static_cast<uint32_t>(blocks) : resident;
+  p.skip_rows = grid * kGroups / p.per_row, p.skip_groups = grid * kGroups % p.per_row;
+  auto go = [&](auto kern) { return launch_kernel(kern, dim3(grid), dim3(kThreads), 0, stream, p); };
+  return wide ? go(quantize_kernel<T, GATE, true>) : go(quantize_kernel<T, GATE, false>);
 }
 
 template <typename T>

@@ -16,134 +16,202 @@
 namespace ctmr {
 namespace {
 
-// BLOCK: a block to a row; otherwise a warp. V: eights of channels to a thread.
-template <typename T, int V, bool BLOCK, bool EIGHT, bool WIDE>
-__global__ void __launch_bounds__(BLOCK ? 1024 : 256) row_norm_kernel(const __grid_constant__ RowNormParams p) {
-  __shared__ double part[BLOCK ? 32 : 1];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int span = BLOCK ? blockDim.x : 32, mine = BLOCK ? threadIdx.x : lane;
-  const long long row = BLOCK ? blockIdx.x : static_cast<long long>(blockIdx.x) * (blockDim.x >> 5) + warp;
+// In units of 2^-24: the sum, the factor, two products and the scaling.
+constexpr int kNormUnits = 6;
+
+// LANES lanes to a row: 8, 16 or 32 of a warp, or (0) a block. V: groups of channels to eight lanes. LOOP (of blocks):
+// a block goes on to another row, whose loads it starts before this row's sum is known, with the weight in registers.
+template <typename T, int V, int LANES, bool LOOP, bool EIGHT, bool WIDE>
+__global__ void __launch_bounds__(LANES ? 256 : LOOP ? 512 : 1024, 1) row_norm_kernel(const __grid_constant__ RowNormParams p) {
+  constexpr bool BLOCK = LANES == 0;
+  // Sums of 16-bit numbers are exact in 32 bits but where one is 2^13 times the other; 32-bit ones keep the rest.
+  constexpr bool kLow = EIGHT && sizeof(T) == 4;
+  __shared__ double part[2][BLOCK ? 32 : 1];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, lane8 = lane & 7;
+  const int span = BLOCK ? blockDim.x : LANES;
+  // A thread's first group; the next is span / 8 further.
+  const int first = (BLOCK ? threadIdx.x : threadIdx.x & (span - 1)) / kGroupLanes, step = span / kGroupLanes;
+  const long long rows = static_cast<long long>(p.tokens) * p.heads;
+  long long row = BLOCK ? blockIdx.x : (static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x) / LANES;
   griddep_wait();
   griddep_launch_dependents();
-  if (!BLOCK && row >= static_cast<long long>(p.tokens) * p.heads) return;  // whole warps
-  const int token = p.heads == 1 ? static_cast<int>(row) : static_cast<int>(row / p.heads);
-  const int head = p.heads == 1 ? 0 : static_cast<int>(row - static_cast<long long>(token) * p.heads);
-  const T* x = static_cast<const T*>(p.x) + token * p.x_token + head * p.x_head;
-  const T* r = static_cast<const T*>(p.residual) + (p.residual ? token * p.r_token + head * p.r_head : 0);
+  const bool idle = row >= rows;  // part of a warp may be: it stays for the shuffles
+  if (idle) row = rows - 1;
+  const int channels = idle ? 0 : p.channels;
 
-  float h[V][8];
-  double total = 0.0;
+  int token, head;
+  const T *x, *r;
+  float h[V][kEach], w[V][kEach], low[kLow ? V : 1][kEach];
+  auto at_row = [&](long long i) {
+    token = p.heads == 1 ? static_cast<int>(i) : static_cast<int>(i / p.heads);
+    head = p.heads == 1 ? 0 : static_cast<int>(i - static_cast<long long>(token) * p.heads);
+    x = static_cast<const T*>(p.x) + token * p.x_token + head * p.x_head;
+    r = static_cast<const T*>(p.residual) + (p.residual ? token * p.r_token + head * p.r_head : 0);
+  };
+  auto load_row = [&](Loaded<T, WIDE>(&a)[V], Loaded<T, WIDE>(&b)[V]) {
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    const int c = (mine + i * span) * 8;
-    load8<T, WIDE>(x + c, p.channels - c, h[i]);
-  }
-  if (p.residual != nullptr) {
-    float add[V][8];
+    for (int i = 0; i < V; ++i) a[i].load(x, channels, first + i * step, lane8);
+    if (p.residual != nullptr)
+#pragma unroll
+      for (int i = 0; i < V; ++i) b[i].load(r, channels, first + i * step, lane8);
+  };
+  auto load_weight = [&](int i) {
+    if (p.weight_f32) load16<float, WIDE>(static_cast<const float*>(p.weight), channels, first + i * step, lane8, w[i]);
+    else load16<T, WIDE>(static_cast<const T*>(p.weight), channels, first + i * step, lane8, w[i]);
+  };
+
+  Loaded<T, WIDE> x_in[V], r_in[V];
+  at_row(row);
+  load_row(x_in, r_in);
+  if (LOOP && p.weight != nullptr)
+#pragma unroll
+    for (int i = 0; i < V; ++i) load_weight(i);
+  for (int turn = 0;; turn ^= 1) {
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      const int c = (mine + i * span) * 8;
-      load8<T, WIDE>(r + c, p.channels - c, add[i]);
+      const bool inside = channel_of<WIDE>(first + i * step, lane8, 0) < channels;
+      x_in[i].values(h[i], inside);
+      if (p.residual != nullptr) {
+        float add[kEach];
+        r_in[i].values(add, inside);
+        if constexpr (kLow) {  // what the sum's rounding cuts off, exactly
+#pragma unroll
+          for (int e = 0; e < kEach; ++e) {
+            const float sum = h[i][e] + add[e], back = sum - h[i][e];
+            low[i][e] = (h[i][e] - (sum - back)) + (add[e] - back);
+          }
+        }
+        add16(h[i], add);
+      } else if constexpr (kLow) {
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) low[i][e] = 0.f;
+      }
     }
+    const int token_now = token, head_now = head;
+    const bool more = LOOP && row + gridDim.x < rows;
+    if (more) {
+      row += gridDim.x;
+      at_row(row);
+      load_row(x_in, r_in);
+    }
+    double sums[4] = {0.0, 0.0, 0.0, 0.0};  // four chains
 #pragma unroll
     for (int i = 0; i < V; ++i)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) h[i][e] += add[i][e];
-  }
+      for (int e = 0; e < kEach; ++e)
+        sums[e % 4] = fma(static_cast<double>(h[i][e]), static_cast<double>(h[i][e]), sums[e % 4]);
+    double total = (sums[0] + sums[1]) + (sums[2] + sums[3]);
 #pragma unroll
-  for (int i = 0; i < V; ++i)
-#pragma unroll
-    for (int e = 0; e < 8; ++e) total = fma(static_cast<double>(h[i][e]), static_cast<double>(h[i][e]), total);
-#pragma unroll
-  for (int i = 16; i > 0; i /= 2) total += __shfl_xor_sync(0xffffffffu, total, i);
-  if constexpr (BLOCK) {
-    if (lane == 0) part[warp] = total;
-    __syncthreads();
-    const int warps = blockDim.x >> 5;
-    total = lane < warps ? part[lane] : 0.0;
-#pragma unroll
-    for (int i = 16; i > 0; i /= 2) total += __shfl_xor_sync(0xffffffffu, total, i);
-  }
-  const double by64 = 1.0 / sqrt(total / p.channels + static_cast<double>(p.eps));
-  const float by = static_cast<float>(by64);
+    for (int i = (BLOCK ? 32 : LANES) / 2; i > 0; i /= 2) total += __shfl_xor_sync(0xffffffffu, total, i);
+    if constexpr (BLOCK) {
+      if (lane == 0) part[turn][warp] = total;
+      __syncthreads();
+      const int warps = blockDim.x >> 5;
+      total = part[turn][0];
+      for (int i = 1; i < warps; ++i) total += part[turn][i];
+    }
+    // 1 / sqrt(mean + eps): 32 bits' root and a step of Newton's in 64, good to 2^-43.
+    const double mean = fma(total, p.per_channel, static_cast<double>(p.eps));
+    double by64;
+    if (mean < 0x1p120) {
+      by64 = static_cast<double>(rsqrtf(static_cast<float>(mean)));
+      by64 = fma(0.5 * by64, fma(-mean * by64, by64, 1.0), by64);
+    } else {
+      by64 = 1.0 / sqrt(mean);
+    }
+    const float by = static_cast<float>(by64);
 
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    const int c = (mine + i * span) * 8, left = p.channels - c;
-    float w[8], s[8];
-    if (p.weight == nullptr) {
+    for (int i = 0; i < V; ++i) {
+      const int group = first + i * step;
+      float s[kEach];
+      mul16(s, h[i], by);
+      if (p.weight != nullptr) {
+        if (!LOOP) load_weight(i);
+        mul16(s, s, w[i]);
+      }
+      if constexpr (EIGHT) {
+        if (__any_sync(0xffffffffu, channel_of<WIDE>(group, lane8, kEach - 1) >= channels))  // nothing past the row's end, whatever the factor
 #pragma unroll
-      for (int e = 0; e < 8; ++e) w[e] = 1.f;
-    } else if (p.weight_f32) {
-      load8<float, WIDE>(static_cast<const float*>(p.weight) + c, left, w);
-    } else {
-      load8<T, WIDE>(static_cast<const T*>(p.weight) + c, left, w);
+          for (int e = 0; e < kEach; ++e) s[e] = channel_of<WIDE>(group, lane8, e) < channels ? s[e] : 0.f;
+        uint32_t q[4];
+        float scale, by8;
+        auto exact = [&](int e) {
+          double v = static_cast<double>(pick(h[i], e));
+          if (kLow) v += static_cast<double>(pick(low[i], e));
+          if (p.weight != nullptr) v *= static_cast<double>(pick(w[i], e));
+          return v * by64;
+        };
+        auto top64 = [&]() {
+          double most = 0.0;
+#pragma unroll 1
+          for (int e = 0; e < kEach; ++e) most = fmax(most, fabs(exact(e)));
+          return most;
+        };
+        // From registers: a reload would keep the warp, and the block that waits for it, some microseconds.
+        uint32_t differ = quantize_group<kNormUnits>(s, top64, q, scale, by8);
+#pragma unroll 1
+        for (; differ != 0; differ &= differ - 1) {
+          const int e = __ffs(differ) - 1, bit = (e & 3) * 8;
+          const uint32_t byte = e4m3_exact(exact(e) * by8);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (j == e >> 2) q[j] = (q[j] & ~(0xffu << bit)) | byte << bit;
+        }
+        store_bytes<WIDE>(static_cast<uint8_t*>(p.y) + token_now * p.y_token, channels, group, lane8, q);
+        if (lane8 == 0 && group * kScaleGroup < channels)
+          p.scale[token_now * p.scale_token + group * p.scale_group] = scale;
+      } else {
+        store16<T, WIDE>(static_cast<T*>(p.y) + token_now * p.y_token + head_now * p.y_head, channels, group, lane8, s);
+      }
+      // Last, as it may lie where x or r did.
+      if (p.sum != nullptr)
+        store16<T, WIDE>(static_cast<T*>(p.sum) + token_now * p.s_token + head_now * p.s_head, channels, group, lane8,
+                         h[i]);
     }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) s[e] = left > 0 ? h[i][e] * by * w[e] : 0.f;
-    if constexpr (EIGHT) {
-      if (!WIDE)  // what lies past the row's end in a half-filled eight
-#pragma unroll
-        for (int e = 0; e < 8; ++e) s[e] = e < left ? s[e] : 0.f;
-      float scale;
-      // Read again: the sum in 32 bits may have been rounded.
-      auto exact = [&](int e) {
-        if (e >= left) return 0.0;
-        double v = static_cast<double>(to_float(x[c + e]));
-        if (p.residual != nullptr) v += static_cast<double>(to_float(r[c + e]));
-        if (p.weight != nullptr)
-          v *= static_cast<double>(p.weight_f32 ? static_cast<const float*>(p.weight)[c + e]
-                                                : to_float(static_cast<const T*>(p.weight)[c + e]));
-        return v * by64;
-      };
-      const uint2 q = quantize_group<true>(s, exact, scale);
-      store_bytes<WIDE>(static_cast<uint8_t*>(p.y) + token * p.y_token + c, left, q);
-      if ((lane & 15) == 0 && left > 0) p.scale[token * p.scale_token + (c / kScaleGroup) * p.scale_group] = scale;
-    } else {
-      store8<T, WIDE>(static_cast<T*>(p.y) + token * p.y_token + head * p.y_head + c, left, s);
-    }
-    // Last, as it may lie where x or r did.
-    if (p.sum != nullptr) store8<T, WIDE>(static_cast<T*>(p.sum) + token * p.s_token + head * p.s_head + c, left, h[i]);
+    if (!more) break;
   }
 }
 
-template <typename T, int V, bool BLOCK, bool EIGHT>
-cudaError_t launch(const RowNormParams& p, bool wide, unsigned grid, int threads, cudaStream_t stream) {
-  return wide ? launch_kernel(row_norm_kernel<T, V, BLOCK, EIGHT, true>, dim3(grid), dim3(threads), 0, stream, p)
-              : launch_kernel(row_norm_kernel<T, V, BLOCK, EIGHT, false>, dim3(grid), dim3(threads), 0, stream, p);
+template <typename T, int V, int LANES, bool LOOP, bool EIGHT>
+cudaError_t launch(const RowNormParams& p, bool wide, long long grid, int threads, cudaStream_t stream) {
+  auto go = [&](auto kern) {
+    return launch_kernel(kern, dim3(static_cast<unsigned>(grid)), dim3(threads), 0, stream, p);
+  };
+  return wide ? go(row_norm_kernel<T, V, LANES, LOOP, EIGHT, true>) : go(row_norm_kernel<T, V, LANES, LOOP, EIGHT, false>);
 }
 
 template <typename T, bool EIGHT>
 cudaError_t launch_rows(const RowNormParams& p, cudaStream_t stream) {
-  // 16-byte accesses where every row allows them.
-  constexpr int kEach = 16 / sizeof(T);
-  auto row_ok = [](const void* at, long long token, long long head, int each) {
-    return at == nullptr || (reinterpret_cast<uintptr_t>(at) % 16 == 0 && token % each == 0 && head % each == 0);
+  // 32-byte accesses where every row allows them.
+  constexpr int kAlign = 32 / sizeof(T);
+  auto row_ok = [](const void* at, long long token, long long head) {
+    return at == nullptr || (reinterpret_cast<uintptr_t>(at) % 32 == 0 && token % kAlign == 0 && head % kAlign == 0);
   };
-  const bool wide = p.channels % 8 == 0 && row_ok(p.x, p.x_token, p.x_head, kEach) &&
-                    row_ok(p.residual, p.r_token, p.r_head, kEach) && row_ok(p.sum, p.s_token, p.s_head, kEach) &&
-                    (EIGHT ? reinterpret_cast<uintptr_t>(p.y) % 8 == 0 && p.y_token % 8 == 0
-                           : row_ok(p.y, p.y_token, p.y_head, kEach)) &&
-                    (p.weight == nullptr || reinterpret_cast<uintptr_t>(p.weight) % 16 == 0);
+  const bool wide = p.channels % kEach == 0 && row_ok(p.x, p.x_token, p.x_head) &&
+                    row_ok(p.residual, p.r_token, p.r_head) && row_ok(p.sum, p.s_token, p.s_head) &&
+                    (EIGHT ? reinterpret_cast<uintptr_t>(p.y) % 16 == 0 && p.y_token % 16 == 0
+                           : row_ok(p.y, p.y_token, p.y_head)) &&
+                    (p.weight == nullptr || reinterpret_cast<uintptr_t>(p.weight) % 32 == 0);
   const long long rows = static_cast<long long>(p.tokens) * p.heads;
-  const int eights = (p.channels + 7) / 8;
-  if (eights <= 128) {
-    const int warps = 8;
-    const unsigned grid = static_cast<unsigned>((rows + warps - 1) / warps);
-    if (eights <= 32) return launch<T, 1, false, EIGHT>(p, wide, grid, warps * 32, stream);
-    if (eights <= 64) return launch<T, 2, false, EIGHT>(p, wide, grid, warps * 32, stream);
-    return launch<T, 4, false, EIGHT>(p, wide, grid, warps * 32, stream);
-  }
-  auto threads = [&](int v) { return ((eights + v - 1) / v + 31) / 32 * 32; };
-  const unsigned grid = static_cast<unsigned>(rows);
-  if (threads(1) <= 512) return launch<T, 1, true, EIGHT>(p, wide, grid, threads(1), stream);
-  if (threads(2) <= 1024) return launch<T, 2, true, EIGHT>(p, wide, grid, threads(2), stream);
-  return launch<T, 4, true, EIGHT>(p, wide, grid, threads(4), stream);
+  const int groups = (p.channels + kScaleGroup - 1) / kScaleGroup;
+  auto grid = [&](int lanes) { return (rows * lanes + 255) / 256; };
+  if (groups == 1) return launch<T, 1, 8, false, EIGHT>(p, wide, grid(8), 256, stream);
+  if (groups == 2) return launch<T, 1, 16, false, EIGHT>(p, wide, grid(16), 256, stream);
+  if (groups <= 4) return launch<T, 1, 32, false, EIGHT>(p, wide, grid(32), 256, stream);
+  if (groups <= 8) return launch<T, 2, 32, false, EIGHT>(p, wide, grid(32), 256, stream);
+  auto threads = [&](int v) { return (groups + 4 * v - 1) / (4 * v) * 32; };
+  const long long resident = static_cast<long long>(device_sm_count()) * (512 / threads(1));  // at 128 registers
+  if (threads(1) <= 512 && rows > resident) return launch<T, 1, 0, true, EIGHT>(p, wide, resident, threads(1), stream);
+  if (threads(1) <= 512) return launch<T, 1, 0, false, EIGHT>(p, wide, rows, threads(1), stream);
+  return launch<T, 2, 0, false, EIGHT>(p, wide, rows, threads(2), stream);
 }
 
 }  // namespace
 
-cudaError_t launch_row_norm(const RowNormParams& p, int dtype, cudaStream_t stream) {
+cudaError_t launch_row_norm(const RowNormParams& p_, int dtype, cudaStream_t stream) {
+  RowNormParams p = p_;
+  p.per_channel = 1.0 / p.channels;
   const bool eight = p.scale != nullptr;
   switch (dtype) {
     case CTMR_DTYPE_F32: return eight ? launch_rows<float, true>(p, stream) : launch_rows<float, false>(p, stream);
