@@ -389,6 +389,12 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar_cluster) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar_cluster) : "memory");
 }
 
+// The same without cluster scope, for a barrier that hands over tensor memory alone (read out before a
+// tcgen05.fence): the cluster-wide release waits for the thread's memory accesses, some 2,000 clocks.
+__device__ __forceinline__ void mbar_arrive_remote(uint32_t bar_cluster) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar_cluster) : "memory");
+}
+
 // Tiled 5-D load into this CTA's shared memory whose completion bytes count on an mbarrier of
 // either CTA of the pair (`bar_cluster`, a shared::cluster address): both CTAs' halves of a stage
 // complete on the first CTA's barrier, which its MMA-issuing thread waits on.

@@ -320,12 +320,24 @@ __global__ void __launch_bounds__(kFewThreads, 1)
   }
 }
 
+// sum += v by, 16 of them, two to an instruction.
+__device__ __forceinline__ void add_scaled(float* sum, const float (&v)[16], float by) {
+#pragma unroll
+  for (int i = 0; i < 16; i += 2)
+    asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %4};\n\tmov.b64 z, {%0, %1};\n\t"
+        "fma.rn.f32x2 z, x, y, z;\n\tmov.b64 {%0, %1}, z;\n\t}"
+        : "+f"(sum[i]), "+f"(sum[i + 1])
+        : "f"(v[i]), "f"(v[i + 1]), "f"(by));
+}
+
 // ---------------------------------------------------------------- CTA pairs
-constexpr int kPairThreads = 320;  // warp 0 TMA, warp 1 MMA (first CTA), warps 2-9 sums
+constexpr int kPairThreads = 352;  // warp 0 TMA, warp 1 MMA (first CTA), warp 2 scales, warps 3-10 sums
 constexpr int kPairTile = 256;
 constexpr int kPairStages = 6;
 constexpr uint32_t kPairStageBytes = 2 * kHalfTile;  // this CTA's 128 rows and 128 outputs
-constexpr uint32_t kPairOffBar = kPairStages * kPairStageBytes;
+constexpr int kPairFactors = 8;  // blocks whose scales are in shared memory: [half of the outputs][row]
+constexpr uint32_t kPairOffFactors = kPairStages * kPairStageBytes;
+constexpr uint32_t kPairOffBar = kPairOffFactors + kPairFactors * 256 * 4;
 constexpr uint32_t kPairBytes = kPairOffBar + 512 + 1024;
 constexpr int kRaster = 8;  // row tiles that are walked together, so that the weight's and x's tiles meet in L2
 
@@ -342,7 +354,10 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   uint64_t* empty = full + S;
   uint64_t* acc_full = empty + S;      // [2]
   uint64_t* acc_empty = acc_full + 2;  // [2] read out by both CTAs (first CTA's barriers)
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+  uint64_t* factor_full = acc_empty + 2;
+  uint64_t* factor_empty = factor_full + kPairFactors;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(factor_empty + kPairFactors);
+  float* factors = reinterpret_cast<float*>(smem + kPairOffFactors);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -358,6 +373,10 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     for (int i = 0; i < 2; ++i) {
       mbar_init(&acc_full[i], 1);
       mbar_init(&acc_empty[i], 16);
+    }
+    for (int i = 0; i < kPairFactors; ++i) {
+      mbar_init(&factor_full[i], 1);
+      mbar_init(&factor_empty[i], 8);
     }
     *abort_flag = 0;
     fence_barrier_init();
@@ -438,63 +457,80 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       if (!ok) *abort_flag = 1;
     }
     __syncwarp();
+  } else if (warp == 2) {
+    // ------------------------------------------------------------ scales (both CTAs), four blocks' loads at a time.
+    // (In the registers of the warps that use them there is no room to have them loaded ahead.)
+    int it = 0;
+    bool ok = true;
+    for (int t = pair; ok && t < tiles; t += pairs) {
+      int r0, n0;
+      place(t, r0, n0);
+      const float* xs[4];
+      const float* ws[2];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) xs[j] = r0 + j * 32 + lane < p.rows ? p.x_scale + (r0 + j * 32 + lane) * p.xs_row : nullptr;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) ws[j] = n0 + j * 128 < p.out ? p.w_scale + (n0 / kScaleGroup + j) * p.ws_row : nullptr;
+      for (int k0 = 0; ok && k0 < kb; k0 += 4) {
+        float x[4][4], w[4][2];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const bool in = k0 + i < kb;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) x[i][j] = in && xs[j] != nullptr ? xs[j][(k0 + i) * p.xs_block] : 0.f;
+#pragma unroll
+          for (int j = 0; j < 2; ++j) w[i][j] = in && ws[j] != nullptr ? ws[j][(k0 + i) * p.ws_block] : 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (k0 + i >= kb) break;
+          const int f = it % kPairFactors;
+          if (it >= kPairFactors)
+            ok = mbar_wait_warp(&factor_empty[f], static_cast<uint32_t>(it / kPairFactors - 1) & 1u, kErrWaitEmpty);
+          if (!ok) break;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) factors[f * 256 + j * 32 + lane] = x[i][j & 3] * w[i][j >> 2];
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&factor_full[f]);
+          ++it;
+        }
+      }
+    }
+    if (!ok) *abort_flag = 1;
+    __syncwarp();
   } else {
     // ------------------------------------------------------------ sums (both CTAs)
-    const int quarter = warp & 3, half = (warp - 2) >> 2;
+    const int quarter = warp & 3, half = (warp - 3) >> 2;
     const uint32_t lanes = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + half * 128;
     const uint32_t release0 = cluster_addr(acc_empty, 0);
-    // Scales four blocks ahead of their use, across tiles.
-    float xs[4], ws[4];
-    auto fetch = [&](int t, int k0) {
-      int r0, n0;
-      place(min(t, tiles - 1), r0, n0);
-      const int row = r0 + quarter * 32 + lane, column = n0 + half * 128;
-      const bool in = t < tiles && row < p.rows && column < p.out;
-      const float* x = p.x_scale + (in ? row * p.xs_row : 0);
-      const float* w = p.w_scale + (in ? column / kScaleGroup * p.ws_row : 0);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        xs[i] = in && k0 + i < kb ? x[(k0 + i) * p.xs_block] : 0.f;
-        ws[i] = in && k0 + i < kb ? w[(k0 + i) * p.ws_block] : 0.f;
-      }
-    };
-    if (pair < tiles) fetch(pair, 0);
+    const float* my_factor = factors + half * 128 + quarter * 32 + lane;
     int it = 0;
     bool ok = true;
     for (int t = pair; ok && t < tiles; t += pairs) {
       float sum[128];
 #pragma unroll
       for (int c = 0; c < 128; ++c) sum[c] = 0.f;
-      for (int k0 = 0; ok && k0 < kb; k0 += 4) {
-        float by[4];
+      for (int k = 0; k < kb; ++k, ++it) {
+        const int a = it & 1, f = it % kPairFactors;
+        ok = mbar_wait_warp(&factor_full[f], static_cast<uint32_t>(it / kPairFactors) & 1u, kErrWaitFull);
+        const float by = my_factor[f * 256];
+        ok = ok && mbar_wait_warp(&acc_full[a], static_cast<uint32_t>(it >> 1) & 1u, kErrWaitAcc);
+        if (!ok) break;
+        tc_fence_after();
 #pragma unroll
-        for (int i = 0; i < 4; ++i) by[i] = xs[i] * ws[i];
-        const bool more = k0 + 4 < kb;
-        fetch(more ? t : t + pairs, more ? k0 + 4 : 0);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if (k0 + i >= kb) break;
-          const int a = it & 1;
-          ok = mbar_wait_warp(&acc_full[a], static_cast<uint32_t>(it >> 1) & 1u, kErrWaitAcc);
-          if (!ok) break;
-          ++it;
-          tc_fence_after();
-          float v[2][16];
-          tmem_ld16_start(lanes + a * 256, v[0]);
-#pragma unroll
-          for (int c = 0; c < 128; c += 16) {
-            float(&now)[16] = v[(c / 16) & 1];
-            tmem_ld_wait();
-            tmem_ld_fence16(now);
-            if (c + 16 < 128) {
-              tmem_ld16_start(lanes + a * 256 + c + 16, v[(c / 16 + 1) & 1]);
-            } else {  // all read: the next block but one may overwrite it
-              tc_fence_before();
-              if (lane == 0) mbar_arrive_cluster(release0 + 8u * a);
+        for (int c = 0; c < 128; c += 16) {
+          float v[16];
+          tmem_ld16_start(lanes + a * 256 + c, v);
+          tmem_ld_wait();
+          tmem_ld_fence16(v);
+          if (c + 16 == 128) {  // all read: the next block but one may overwrite it
+            tc_fence_before();
+            if (lane == 0) {
+              mbar_arrive_remote(release0 + 8u * a);
+              mbar_arrive(&factor_empty[f]);
             }
-#pragma unroll
-            for (int e = 0; e < 16; ++e) sum[c + e] = fmaf(now[e], by[i], sum[c + e]);
           }
+          add_scaled(sum + c, v, by);
         }
       }
       ok = ok && __all_sync(0xffffffffu, !*abort_flag);
