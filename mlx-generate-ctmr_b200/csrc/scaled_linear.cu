@@ -330,14 +330,57 @@ __device__ __forceinline__ void add_scaled(float* sum, const float (&v)[16], flo
         : "f"(v[i]), "f"(v[i + 1]), "f"(by));
 }
 
+// By a warp: 32 rows (a lane's sums are one) of COLUMNS outputs, 64 bytes of each row at a time by way of shared memory, so
+// that four lanes write side by side. (A lane that writes its own row's 16 bytes, 32 rows to an access, kept the
+// warps 8,600 clocks a tile.)
+template <typename T, int COLUMNS>
+__device__ __forceinline__ void write_rows(const ScaledLinearParams& p, uint8_t* store, const float* sum, int row0, int o0,
+                                           int lane) {
+  constexpr int kPer = 16 / sizeof(T), kWide = 4 * kPer;  // outputs in 16 bytes, in 64
+  const bool wide = p.y_stride % kPer == 0 && reinterpret_cast<uintptr_t>(p.y) % 16 == 0;
+#pragma unroll
+  for (int c = 0; c < COLUMNS; c += kWide) {
+    if (o0 + c >= p.out) break;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {  // 16 bytes each, in an order by which neither side meets a bank twice
+      alignas(16) T e[kPer];
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        e[i] = from_float<T>(sum[c + j * kPer + i]);
+      }
+      *reinterpret_cast<uint4*>(store + lane * 64 + (j ^ (lane >> 1 & 3)) * 16) = *reinterpret_cast<const uint4*>(e);
+    }
+    __syncwarp();
+    const int chunk = lane & 3, o = o0 + c + chunk * kPer;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = i * 8 + lane / 4;
+      const uint4 v = *reinterpret_cast<const uint4*>(store + r * 64 + (chunk ^ (r >> 1 & 3)) * 16);
+      if (row0 + r >= p.rows) continue;
+      T* y = static_cast<T*>(p.y) + (row0 + r) * p.y_stride + o;
+      if (wide && o + kPer <= p.out) {
+        *reinterpret_cast<uint4*>(y) = v;
+      } else {
+        const T* e = reinterpret_cast<const T*>(&v);
+#pragma unroll
+        for (int x = 0; x < kPer; ++x)
+          if (o + x < p.out) y[x] = e[x];
+      }
+    }
+    __syncwarp();
+  }
+}
+
 // ---------------------------------------------------------------- CTA pairs
-constexpr int kPairThreads = 352;  // warp 0 TMA, warp 1 MMA (first CTA), warp 2 scales, warps 3-10 sums
+constexpr int kSumWarps = 8, kColumns = 1024 / kSumWarps;
+constexpr int kPairThreads = 96 + 32 * kSumWarps;  // warp 0 TMA, warp 1 MMA (first CTA), warp 2 scales, the others sums
 constexpr int kPairTile = 256;
 constexpr int kPairStages = 6;
 constexpr uint32_t kPairStageBytes = 2 * kHalfTile;  // this CTA's 128 rows and 128 outputs
-constexpr int kPairFactors = 8;  // blocks whose scales are in shared memory: [half of the outputs][row]
+constexpr int kPairFactors = 3;  // fours of blocks whose scales are in shared memory: [block][half of the outputs][row]
 constexpr uint32_t kPairOffFactors = kPairStages * kPairStageBytes;
-constexpr uint32_t kPairOffBar = kPairOffFactors + kPairFactors * 256 * 4;
+constexpr uint32_t kPairOffStore = kPairOffFactors + kPairFactors * 4 * 256 * 4;  // 32 rows of 64 bytes a warp
+constexpr uint32_t kPairOffBar = kPairOffStore + kSumWarps * 2048;
 constexpr uint32_t kPairBytes = kPairOffBar + 512 + 1024;
 constexpr int kRaster = 8;  // row tiles that are walked together, so that the weight's and x's tiles meet in L2
 
@@ -372,11 +415,11 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&acc_full[i], 1);
-      mbar_init(&acc_empty[i], 16);
+      mbar_init(&acc_empty[i], 2 * kSumWarps);
     }
     for (int i = 0; i < kPairFactors; ++i) {
       mbar_init(&factor_full[i], 1);
-      mbar_init(&factor_empty[i], 8);
+      mbar_init(&factor_empty[i], kSumWarps);
     }
     *abort_flag = 0;
     fence_barrier_init();
@@ -440,8 +483,9 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       bool ok = true;
       for (int it = 0; it < blocks; ++it) {
         const int s = it % S, a = it & 1;
-        if (it >= 2) ok = mbar_wait_warp(&acc_empty[a], static_cast<uint32_t>((it >> 1) - 1) & 1u, kErrWaitAcc);
-        ok = ok && mbar_wait_warp(&full[s], static_cast<uint32_t>(it / S) & 1u, kErrWaitFull);
+        ok = mbar_wait_warp(&full[s], static_cast<uint32_t>(it / S) & 1u, kErrWaitFull);
+        // Last, as it is the one that others wait behind.
+        if (it >= 2) ok = ok && mbar_wait_warp(&acc_empty[a], static_cast<uint32_t>((it >> 1) - 1) & 1u, kErrWaitAcc);
         if (!ok) break;
         tc_fence_after();
         const uint64_t ad = desc_advance(d0, static_cast<uint32_t>(s) * kPairStageBytes), bd = desc_advance(ad, kHalfTile);
@@ -481,76 +525,71 @@ __global__ void __launch_bounds__(kPairThreads, 1)
 #pragma unroll
           for (int j = 0; j < 2; ++j) w[i][j] = in && ws[j] != nullptr ? ws[j][(k0 + i) * p.ws_block] : 0.f;
         }
+        const int f = it % kPairFactors;
+        if (it >= kPairFactors)
+          ok = mbar_wait_warp(&factor_empty[f], static_cast<uint32_t>(it / kPairFactors - 1) & 1u, kErrWaitEmpty);
+        if (!ok) break;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if (k0 + i >= kb) break;
-          const int f = it % kPairFactors;
-          if (it >= kPairFactors)
-            ok = mbar_wait_warp(&factor_empty[f], static_cast<uint32_t>(it / kPairFactors - 1) & 1u, kErrWaitEmpty);
-          if (!ok) break;
+        for (int i = 0; i < 4; ++i)
 #pragma unroll
-          for (int j = 0; j < 8; ++j) factors[f * 256 + j * 32 + lane] = x[i][j & 3] * w[i][j >> 2];
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&factor_full[f]);
-          ++it;
-        }
+          for (int j = 0; j < 8; ++j) factors[(f * 4 + i) * 256 + j * 32 + lane] = x[i][j & 3] * w[i][j >> 2];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&factor_full[f]);
+        ++it;
       }
     }
     if (!ok) *abort_flag = 1;
     __syncwarp();
   } else {
     // ------------------------------------------------------------ sums (both CTAs)
-    const int quarter = warp & 3, half = (warp - 3) >> 2;
-    const uint32_t lanes = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + half * 128;
+    const int quarter = warp & 3, columns = (warp - 3) / 4 * kColumns;
+    const uint32_t lanes = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + columns;
     const uint32_t release0 = cluster_addr(acc_empty, 0);
-    const float* my_factor = factors + half * 128 + quarter * 32 + lane;
-    int it = 0;
+    const float* my_factor = factors + columns / 128 * 128 + quarter * 32 + lane;
+    uint8_t* store = smem + kPairOffStore + (warp - 3) * 2048;
+    int it = 0, group = 0;
     bool ok = true;
     for (int t = pair; ok && t < tiles; t += pairs) {
-      float sum[128];
+      int r0, n0;
+      place(t, r0, n0);
+      float sum[kColumns];
 #pragma unroll
-      for (int c = 0; c < 128; ++c) sum[c] = 0.f;
+      for (int c = 0; c < kColumns; ++c) sum[c] = 0.f;
+      if (p.bias != nullptr)
+#pragma unroll
+        for (int c = 0; c < kColumns; ++c) sum[c] = bias_at<T>(p, n0 + columns + c);
       for (int k = 0; k < kb; ++k, ++it) {
-        const int a = it & 1, f = it % kPairFactors;
-        ok = mbar_wait_warp(&factor_full[f], static_cast<uint32_t>(it / kPairFactors) & 1u, kErrWaitFull);
-        const float by = my_factor[f * 256];
+        const int a = it & 1, f = group % kPairFactors;
+        if ((k & 3) == 0) ok = mbar_wait_warp(&factor_full[f], static_cast<uint32_t>(group / kPairFactors) & 1u, kErrWaitFull);
+        const float by = my_factor[(f * 4 + (k & 3)) * 256];
         ok = ok && mbar_wait_warp(&acc_full[a], static_cast<uint32_t>(it >> 1) & 1u, kErrWaitAcc);
         if (!ok) break;
         tc_fence_after();
+        const bool last = (k & 3) == 3 || k + 1 == kb;
+        // The next 16 on their way while these are added.
+        float v[2][16];
+        tmem_ld16_start(lanes + a * 256, v[0]);
 #pragma unroll
-        for (int c = 0; c < 128; c += 16) {
-          float v[16];
-          tmem_ld16_start(lanes + a * 256 + c, v);
+        for (int c = 0; c < kColumns; c += 16) {
+          float(&now)[16] = v[c / 16 & 1];
           tmem_ld_wait();
-          tmem_ld_fence16(v);
-          if (c + 16 == 128) {  // all read: the next block but one may overwrite it
+          tmem_ld_fence16(now);
+          if (c + 16 < kColumns) {
+            tmem_ld16_start(lanes + a * 256 + c + 16, v[c / 16 + 1 & 1]);
+          } else {  // all read: the next block but one may overwrite it
             tc_fence_before();
             if (lane == 0) {
               mbar_arrive_remote(release0 + 8u * a);
-              mbar_arrive(&factor_empty[f]);
+              if (last) mbar_arrive(&factor_empty[f]);
             }
           }
-          add_scaled(sum + c, v, by);
+          add_scaled(sum + c, now, by);
         }
+        group += last;
       }
       ok = ok && __all_sync(0xffffffffu, !*abort_flag);
       if (!ok) break;
-      int r0, n0;
-      place(t, r0, n0);
-      const int row = r0 + quarter * 32 + lane, column = n0 + half * 128;
-      if (row < p.rows) {
-        const bool wide = p.y_stride % (16 / static_cast<int>(sizeof(T))) == 0 && reinterpret_cast<uintptr_t>(p.y) % 16 == 0;
-        T* y = static_cast<T*>(p.y) + row * p.y_stride + column;
-#pragma unroll
-        for (int c = 0; c < 128; c += 8) {
-          if (column + c >= p.out) break;
-          if (p.bias != nullptr)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) sum[c + e] += bias_at<T>(p, column + c + e);
-          store_outputs<T, 8>(y + c, sum + c, wide, p.out - column - c);
-        }
-      }
-      __syncwarp();
+      write_rows<T, kColumns>(p, store, sum, r0 + quarter * 32, n0 + columns, lane);
     }
     if (!ok) *abort_flag = 1;
   }
