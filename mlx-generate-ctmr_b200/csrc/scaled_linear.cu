@@ -69,23 +69,27 @@ __device__ __forceinline__ void store_outputs(T* at, const float* v, bool wide, 
 // ---------------------------------------------------------------- few rows
 constexpr int kFewThreads = 224;  // warp 0 TMA, warp 1 MMA, warps 2-5 sums, warp 6 scales
 
+// A stage holds two blocks: waiting for a barrier costs a warp some 100 clocks, the products of a block of few rows less.
+// A tile of 16 rows leaves room for two CTAs on an SM. (Of 32 rows only with two stages each, which is slower.)
 template <int BN>
 struct FewSmem {
-  static constexpr uint32_t kStageBytes = kHalfTile + BN * 128;
-  static constexpr int kStages = 180224 / kStageBytes;
-  static constexpr int kAcc = 4;      // blocks whose sums are in TMEM
-  static constexpr int kFactors = 8;  // blocks whose scales are in shared memory
-  static constexpr uint32_t kCols = kAcc * BN < 32 ? 32 : kAcc * BN;
+  static constexpr int kCtas = BN <= 16 ? 2 : 1;
+  static constexpr uint32_t kBlockBytes = kHalfTile + BN * 128, kStageBytes = 2 * kBlockBytes;
+  static constexpr int kStages = (kCtas == 2 ? 112640 : 200704) / kStageBytes;
+  static constexpr int kAcc = 2;      // stages whose sums are in TMEM
+  static constexpr int kFactors = 2;  // fours of blocks whose scales are in shared memory
+  static constexpr uint32_t kCols = 2 * kAcc * BN;
   static constexpr uint32_t kOffFactors = kStages * kStageBytes;
-  static constexpr uint32_t kOffBar = kOffFactors + kFactors * BN * 4;
-  static constexpr uint32_t kBytes = kOffBar + 512 + 1024;  // + barriers + alignment slack
+  static constexpr uint32_t kOffBar = kOffFactors + kFactors * 4 * BN * 4;
+  static constexpr uint32_t kBytes = kOffBar + 256 + 1024;  // + barriers + alignment slack
   static_assert(BN * 512u <= kOffFactors, "the partial sums lie in the stages");
-  static_assert((2 * kStages + 2 * kAcc + 2 * kFactors) * 8 + 16 <= 512, "barriers");
+  static_assert((2 * kStages + 2 * kAcc + 2 * kFactors) * 8 + 16 <= 256, "barriers");
+  static_assert(kCtas * (kBytes + 1024) <= 228 * 1024, "shared memory of an SM");
 };
 
 // blockIdx.x = (row tile * out tiles + out tile) * split + rank.
 template <int BN, typename T>
-__global__ void __launch_bounds__(kFewThreads, 1)
+__global__ void __launch_bounds__(kFewThreads, FewSmem<BN>::kCtas)
     scaled_few_kernel(const __grid_constant__ ScaledMaps maps, const __grid_constant__ ScaledLinearParams p,
                       const __grid_constant__ ScaledPlan plan) {
   using L = FewSmem<BN>;
@@ -130,24 +134,26 @@ __global__ void __launch_bounds__(kFewThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  const int kb = (p.in + kK - 1) / kK, k_begin = rank * kb / plan.split, k_end = (rank + 1) * kb / plan.split;
   griddep_wait();
   griddep_launch_dependents();
 
-  const int kb = (p.in + kK - 1) / kK, k_begin = rank * kb / plan.split, k_end = (rank + 1) * kb / plan.split;
-  const int n = k_end - k_begin;
+  const int n = k_end - k_begin, stages = (n + 1) / 2;
   if (warp == 0) {
     // ------------------------------------------------------------ TMA producer
     bool ok = true;
     int it = 0;
-    for (; ok && it < n; ++it) {
-      const int s = it % S;
+    for (; ok && it < stages; ++it) {
+      const int s = it % S, blocks = min(2, n - 2 * it);
       if (it >= S) ok = mbar_wait_warp(&empty[s], static_cast<uint32_t>(it / S - 1) & 1u, kErrWaitEmpty);
       if (!ok) break;
       if (lane == 0) {
-        uint8_t* at = smem + s * L::kStageBytes;
-        mbar_arrive_expect_tx(&full[s], L::kStageBytes);
-        tma_load_2d(at, &maps.w, &full[s], (k_begin + it) * kK, m0);
-        tma_load_2d(at + kHalfTile, &maps.x, &full[s], (k_begin + it) * kK, r0);
+        mbar_arrive_expect_tx(&full[s], blocks * L::kBlockBytes);
+        for (int h = 0; h < blocks; ++h) {
+          uint8_t* at = smem + s * L::kStageBytes + h * L::kBlockBytes;
+          tma_load_2d(at, &maps.w, &full[s], (k_begin + 2 * it + h) * kK, m0);
+          tma_load_2d(at + kHalfTile, &maps.x, &full[s], (k_begin + 2 * it + h) * kK, r0);
+        }
       }
       __syncwarp();
     }
@@ -163,17 +169,22 @@ __global__ void __launch_bounds__(kFewThreads, 1)
     const uint64_t d0 = smem_desc_kmajor(base, 128);
     constexpr uint32_t id = idesc_e4m3(128, BN);
     bool ok = true;
-    for (int it = 0; it < n; ++it) {
+    for (int it = 0; it < stages; ++it) {
       const int s = it % S, a = it % A;
-      if (it >= A) ok = mbar_wait_warp(&acc_empty[a], static_cast<uint32_t>(it / A - 1) & 1u, kErrWaitAcc);
-      ok = ok && mbar_wait_warp(&full[s], static_cast<uint32_t>(it / S) & 1u, kErrWaitFull);
+      ok = mbar_wait_warp(&full[s], static_cast<uint32_t>(it / S) & 1u, kErrWaitFull);
+      if (it >= A) ok = ok && mbar_wait_warp(&acc_empty[a], static_cast<uint32_t>(it / A - 1) & 1u, kErrWaitAcc);
       if (!ok) break;
       tc_fence_after();
-      const uint64_t ad = desc_advance(d0, static_cast<uint32_t>(s) * L::kStageBytes), bd = desc_advance(ad, kHalfTile);
+      const uint64_t ad = desc_advance(d0, static_cast<uint32_t>(s) * L::kStageBytes);
+      const bool both = 2 * it + 1 < n;
       if (elect_one()) {
 #pragma unroll
-        for (uint32_t k = 0; k < 4; ++k)
-          umma_f8(tm + a * BN, desc_advance(ad, k * 32u), desc_advance(bd, k * 32u), id, k > 0 ? 1u : 0u);
+        for (uint32_t h = 0; h < 2; ++h)
+          if (h == 0 || both)
+#pragma unroll
+            for (uint32_t k = 0; k < 4; ++k)
+              umma_f8(tm + (2 * a + h) * BN, desc_advance(ad, h * L::kBlockBytes + k * 32u),
+                      desc_advance(ad, h * L::kBlockBytes + kHalfTile + k * 32u), id, k > 0 ? 1u : 0u);
         umma_commit(&empty[s]);
         umma_commit(&acc_full[a]);
       }
@@ -182,7 +193,7 @@ __global__ void __launch_bounds__(kFewThreads, 1)
     if (!ok) *abort_flag = 1;
     __syncwarp();
   } else if (warp == 6) {
-    // ------------------------------------------------------------ scales, four blocks' loads at a time
+    // ------------------------------------------------------------ scales, four blocks at a time
     constexpr int kEach = (BN + 31) / 32;
     const float* xs[kEach];
     bool in[kEach];
@@ -194,27 +205,25 @@ __global__ void __launch_bounds__(kFewThreads, 1)
     }
     const float* ws = p.w_scale + (m0 / kScaleGroup) * p.ws_row;
     bool ok = true;
-    for (int it = 0; ok && it < n; it += 4) {
+    for (int it = 0; ok && 4 * it < n; ++it) {
       float v[4][kEach], w[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int k = k_begin + it + i;
-        w[i] = it + i < n ? ws[k * p.ws_block] : 0.f;
+        const int k = k_begin + 4 * it + i;
+        w[i] = 4 * it + i < n ? ws[k * p.ws_block] : 0.f;
 #pragma unroll
-        for (int j = 0; j < kEach; ++j) v[i][j] = it + i < n && in[j] ? xs[j][k * p.xs_block] : 0.f;
+        for (int j = 0; j < kEach; ++j) v[i][j] = 4 * it + i < n && in[j] ? xs[j][k * p.xs_block] : 0.f;
       }
+      const int f = it % F;
+      if (it >= F) ok = mbar_wait_warp(&factor_empty[f], static_cast<uint32_t>(it / F - 1) & 1u, kErrWaitEmpty);
+      if (!ok) break;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int at = it + i, f = at % F;
-        if (at >= n) break;
-        if (at >= F) ok = mbar_wait_warp(&factor_empty[f], static_cast<uint32_t>(at / F - 1) & 1u, kErrWaitEmpty);
-        if (!ok) break;
+      for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int j = 0; j < kEach; ++j)
-          if (j * 32 + lane < BN) factors[f * BN + j * 32 + lane] = v[i][j] * w[i];
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&factor_full[f]);
-      }
+          if (j * 32 + lane < BN) factors[(f * 4 + i) * BN + j * 32 + lane] = v[i][j] * w[i];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&factor_full[f]);
     }
     if (!ok) *abort_flag = 1;
     __syncwarp();
@@ -226,37 +235,43 @@ __global__ void __launch_bounds__(kFewThreads, 1)
 #pragma unroll
     for (int c = 0; c < BN; ++c) sum[c] = 0.f;
     bool ok = true;
-    for (int it = 0; it < n; ++it) {
-      const int a = it % A, f = it % F;
-      ok = mbar_wait_warp(&factor_full[f], static_cast<uint32_t>(it / F) & 1u, kErrWaitFull) &&
-           mbar_wait_warp(&acc_full[a], static_cast<uint32_t>(it / A) & 1u, kErrWaitAcc);
+    for (int it = 0; it < stages; ++it) {
+      const int a = it % A, f = it / 2 % F;
+      if (it % 2 == 0) ok = mbar_wait_warp(&factor_full[f], static_cast<uint32_t>(it / 2 / F) & 1u, kErrWaitFull);
+      ok = ok && mbar_wait_warp(&acc_full[a], static_cast<uint32_t>(it / A) & 1u, kErrWaitAcc);
       if (!ok) break;
       tc_fence_after();
-      const float4* by = reinterpret_cast<const float4*>(factors + f * BN);
-      float v[2][16];
-      tmem_ld16_start(lanes + a * BN, v[0]);
+      const int blocks = min(2, n - 2 * it);
 #pragma unroll
-      for (int c = 0; c < BN; c += 16) {
-        float(&now)[16] = v[(c / 16) & 1];
-        tmem_ld_wait();
-        tmem_ld_fence16(now);
-        if (c + 16 < BN) {
-          tmem_ld16_start(lanes + a * BN + c + 16, v[(c / 16 + 1) & 1]);
-        } else {  // all read
-          tc_fence_before();
-          if (lane == 0) mbar_arrive(&acc_empty[a]);
-        }
+      for (int h = 0; h < 2; ++h) {
+        if (h == blocks) break;
+        const float4* by = reinterpret_cast<const float4*>(factors + (f * 4 + it % 2 * 2 + h) * BN);
+        const uint32_t at = lanes + (2 * a + h) * BN;
+        float v[2][16];
+        tmem_ld16_start(at, v[0]);
 #pragma unroll
-        for (int e = 0; e < 16; e += 4) {
-          const float4 s = by[(c + e) / 4];
-          sum[c + e] = fmaf(now[e], s.x, sum[c + e]);
-          sum[c + e + 1] = fmaf(now[e + 1], s.y, sum[c + e + 1]);
-          sum[c + e + 2] = fmaf(now[e + 2], s.z, sum[c + e + 2]);
-          sum[c + e + 3] = fmaf(now[e + 3], s.w, sum[c + e + 3]);
+        for (int c = 0; c < BN; c += 16) {
+          float(&now)[16] = v[(c / 16) & 1];
+          tmem_ld_wait();
+          tmem_ld_fence16(now);
+          if (c + 16 < BN) {
+            tmem_ld16_start(at + c + 16, v[(c / 16 + 1) & 1]);
+          } else if (h + 1 == blocks) {  // all read
+            tc_fence_before();
+            if (lane == 0) mbar_arrive(&acc_empty[a]);
+          }
+#pragma unroll
+          for (int e = 0; e < 16; e += 4) {
+            const float4 s = by[(c + e) / 4];
+            sum[c + e] = fmaf(now[e], s.x, sum[c + e]);
+            sum[c + e + 1] = fmaf(now[e + 1], s.y, sum[c + e + 1]);
+            sum[c + e + 2] = fmaf(now[e + 2], s.z, sum[c + e + 2]);
+            sum[c + e + 3] = fmaf(now[e + 3], s.w, sum[c + e + 3]);
+          }
         }
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive(&factor_empty[f]);
+      if (lane == 0 && (it % 2 == 1 || it + 1 == stages)) mbar_arrive(&factor_empty[f]);
     }
     if (!ok) *abort_flag = 1;
     const int o = m0 + quarter * 32 + lane;
@@ -618,21 +633,33 @@ int encode(CUtensorMap* map, const void* base, long long in, long long rows, lon
   return CTMR_OK;
 }
 
-// Which form, tile and split: the least of these estimates (microseconds).
+// Which form, tile and split: the least of these estimates (microseconds), fitted to runs of 1 to 1,000 rows with 512
+// to 11,264 inputs and 512 to 4,096 outputs, which they meet within some 15 %. One CTA to a tile: 2.2 + 0.052 tile for
+// the start, the first loads and the stores, 0.185 + 0.001 tile a block of 128 inputs. Split over a cluster, the partial
+// sums' way takes longer the more columns there are. CTA pairs: 4.5, and 0.53 a block and 0.6 a tile, whose stores fall
+// between the next one's products. (1 row of 4,096 -> 4,096: tiles of 16 rows split four ways 6.5, two ways 7.5, not
+// 9.4; 32 rows: tiles of 32 split two ways 8.0, four ways 9.0; 128 rows: of 64 split two ways 10.6, of 128 four ways
+// 11.6; 300 rows: of 128 19.7, pairs 20.7; 1,000 rows: pairs 22.3, tiles of 128 38.5.)
 ScaledPlan plan_scaled(const ScaledLinearParams& p) {
   ScaledPlan plan{};
   const int sms = device_sm_count(), kb = (p.in + kK - 1) / kK;
   auto waves = [](long long n, int at_once) { return static_cast<float>((n + at_once - 1) / at_once); };
   const long long pair_tiles = ((p.out + 255LL) / 256) * ((p.rows + 255LL) / 256);
-  float best = 6.f + waves(pair_tiles, sms / 2) * kb * 0.35f;
+  float best = 4.5f + waves(pair_tiles, sms / 2) * (0.6f + kb * 0.53f);
   plan.tile = kPairTile, plan.split = 0, plan.out_tiles = (p.out + 255) / 256;
   for (int tile = 16; tile <= 128; tile *= 2) {
     if (tile > 16 && tile / 2 >= p.rows) break;
     const long long tiles = ((p.out + 127LL) / 128) * ((p.rows + tile - 1LL) / tile);
+    const float columns = static_cast<float>(tile < p.rows ? tile : p.rows);
     for (int split = 1; split <= 8 && split <= kb; split *= 2) {
-      const float one = 2.8f + 0.02f * tile + (split > 1 ? 0.8f + 0.01f * tile : 0.f) +
-                        static_cast<float>(kb) / split * (0.25f + 0.001f * tile);
-      const float t = waves(tiles * split, sms) * one;
+      const float start = split == 1 ? 2.2f + 0.052f * tile
+                          : split == 2 ? 4.2f + 0.027f * tile : 4.2f + 0.1f * split + 0.08f * columns;
+      // (Clusters that are resident at once: of the 148 SMs, four's take 132 and eight's 120.)
+      const int clusters = split <= 2 ? sms / split : split == 4 ? sms * 33 / 148 : sms * 15 / 148;
+      // A tile of 16 rows shares its SM with another, which then takes half as long again.
+      const float rounds = waves(tiles, clusters), t =
+          (tile == 16 ? 0.55f + 0.45f * rounds : rounds) *
+          (start + static_cast<float>(kb) / split * (0.185f + 0.001f * tile));
       if (t < best) best = t, plan.tile = tile, plan.split = split, plan.out_tiles = (p.out + 127) / 128;
     }
   }

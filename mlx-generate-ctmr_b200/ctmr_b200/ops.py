@@ -830,10 +830,20 @@ def scale_weight(weight: torch.Tensor) -> ScaledWeight:
 
 def _empty_rows8(like: torch.Tensor, rows: int, channels: int) -> ScaledRows:
     """Uninitialised 8-bit rows; scales lie group by group, as the products read them."""
-    values = like.new_empty((rows, (channels + 15) // 16 * 16), dtype=E4M3)
-    if values.shape[1] != channels:
-        values = values[:, :channels]
-    return ScaledRows(values, like.new_empty(((channels + 127) // 128, rows), dtype=F32).t())
+    return ScaledRows(like.new_empty_strided((rows, channels), ((channels + 15) & ~15, 1), dtype=E4M3),
+                      like.new_empty_strided((rows, (channels + 127) >> 7), (1, rows), dtype=F32))
+
+
+def _row_place(t: torch.Tensor, like: torch.Tensor, dev: int, name: str) -> tuple[int, int, int]:
+    """Address of rows like another tensor's, and their strides over tokens and heads."""
+    shape = like.shape
+    if t is not like and (t.shape != shape or t.dtype != like.dtype or t.get_device() != dev):
+        raise ValueError(f"{name} must be like x: {tuple(shape)} {like.dtype} on cuda:{dev}")
+    st = t.stride()
+    if st[-1] != 1 and shape[-1] > 1:
+        raise ValueError(f"the channels of x, residual and the outputs must be contiguous; {name} has strides {st}")
+    # a stride over an extent of one addresses nothing, whatever torch calls it
+    return t.data_ptr(), st[0] if shape[0] > 1 else 0, st[1] if len(shape) == 3 and shape[1] > 1 else 0
 
 
 def rms_norm(x: torch.Tensor, weight: torch.Tensor | None = None, *, residual: torch.Tensor | None = None,
@@ -861,36 +871,28 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor | None = None, *, residual: t
         weight = weight.contiguous()
         weight_at, weight_code = weight.data_ptr(), _FLOAT_CODES[weight.dtype]
 
-    def place(t, name):
-        """Address and strides over tokens and heads."""
-        if t.shape != shape or t.dtype != dtype or t.get_device() != dev:
-            raise ValueError(f"{name} must be like x: {tuple(shape)} {dtype} on cuda:{dev}")
-        st = t.stride()
-        if channels > 1 and st[-1] != 1:
-            raise ValueError(f"the channels of x, residual and the outputs must be contiguous; {name} has strides {st}")
-        # a stride over an extent of one addresses nothing, whatever torch calls it
-        return t.data_ptr(), st[0] if tokens > 1 else 0, st[1] if heads > 1 else 0
-
-    x_at, r_at = place(x, "x"), (None, 0, 0)
-    s_at = (None, 0, 0)
+    dense = channels * heads, channels if heads > 1 else 0  # strides of what this call allocates
+    x_at, r_at, s_at = _row_place(x, x, dev, "x"), (None, 0, 0), (None, 0, 0)
     if residual is not None:
-        r_at = place(residual, "residual")
+        r_at = _row_place(residual, x, dev, "residual")
         if sum_out is None:
             sum_out = x.new_empty(shape)
-        s_at = place(sum_out, "sum_out")
+            s_at = (sum_out.data_ptr(), *dense)
+        else:
+            s_at = _row_place(sum_out, x, dev, "sum_out")
     elif sum_out is not None:
         raise ValueError("sum_out belongs to a residual")
     if quantize:
         if dims != 2 or out is not None:
             raise ValueError("8-bit rows are made of (rows, channels) tensors, and allocated by the call")
         out = _empty_rows8(x, tokens, channels)
-        values, scale = out
-        y_at = (values.data_ptr(), values.stride(0), 0, *s_at, scale.data_ptr(), 1, tokens)
+        y_at = (out[0].data_ptr(), (channels + 15) & ~15, 0, *s_at, out[1].data_ptr(), 1, tokens)
+    elif out is None:
+        out = x.new_empty(shape)
+        y_at = (out.data_ptr(), *dense, *s_at, None, 0, 0)
     else:
-        if out is None:
-            out = x.new_empty(shape)
-        y_at = (*place(out, "out"), *s_at, None, 0, 0)
-        if residual is not None and y_at[0] == s_at[0] and y_at[0]:
+        y_at = (*_row_place(out, x, dev, "out"), *s_at, None, 0, 0)
+        if y_at[0] == s_at[0] and y_at[0]:
             raise ValueError("out and sum_out must be two tensors")
     desc = _lib.RmsNormDesc(x_at[0], r_at[0], weight_at, code, weight_code, tokens, heads, channels, *x_at[1:], *r_at[1:],
                             eps, *y_at)
@@ -920,9 +922,8 @@ def quantize_rows(x: torch.Tensor, *, gate: bool = False) -> ScaledRows:
             raise ValueError(f"a gated pair has an even number of channels; got {channels}")
         channels //= 2
     out = _empty_rows8(x, rows, channels)
-    values, scale = out
     desc = _lib.QuantizeRowsDesc(x.data_ptr(), code, rows, channels, gate, x.stride(0) if rows > 1 else 0,
-                                 values.data_ptr(), values.stride(0), scale.data_ptr(), 1, rows)
+                                 out[0].data_ptr(), (channels + 15) & ~15, out[1].data_ptr(), 1, rows)
     LAUNCHES[0] += 1
     status = LIB.ctmr_quantize_rows(ctypes.byref(desc), stream)
     if status:
