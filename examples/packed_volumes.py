@@ -77,6 +77,15 @@ def main() -> None:
         print(f"{len(volumes)} volumes, {grid.starts[-1]} tokens: packed with adapters and rotary positions "
               f"{milliseconds(together):.3f} ms, one by one without either {milliseconds(apart):.3f} ms; "
               f"without either the two differ by {far:.1e} (relative)")
+        scaled = packed.scaled_projections(weights, include_fc=True)
+
+        def eight():
+            return packed.packed_spatial_attention_ncdhw(volumes, grid, weights, scaled=scaled, rotary=rotary, **kw)
+
+        turned = packed.packed_spatial_attention_ncdhw(volumes, grid, weights, rotary=rotary, **kw)
+        far = max(((a - b).norm() / (b - x).norm()).item() for a, b, x in zip(eight(), turned, volumes))
+        print(f"projections in 8 bits, with rotary positions {milliseconds(eight):.3f} ms; what the block adds "
+              f"differs by {far:.1e} from the 16-bit projections'")
 
 
 if __name__ == "__main__":

@@ -7,6 +7,10 @@ Q/K/V projection carries each volume's low-rank adapter beside it (``ops.adapter
 heads optionally get rotary positions along depth, height and width (``ops.rotary_axes``), attention stays
 inside each volume (``ops.attention``), and the output projection again carries the adapters. Without adapters
 and positions the result is that of ``spatial_attention_ncdhw`` volume by volume (``attention.py:92-160``).
+
+The projections may run in 8 bits instead (``scaled_projections``): rows are quantised as they are made
+(``ops.quantize_rows``, ``ops.rms_norm``) and multiplied by 8-bit weights (``ops.scaled_linear``).
+``packed_transformer_tokens`` runs pre-norm blocks (norm, attention, norm, gated hidden channels) that way.
 """
 
 from __future__ import annotations
@@ -53,16 +57,39 @@ def _project(tokens, weight, bias, grid, adapters, index):
     return ops.adapter_linear(tokens, weight, bias, **adapters, offsets=grid.offsets, index=index)
 
 
+def _attend(qkv: torch.Tensor, grid: PackedGrid, heads: int, scale: float, rotary: tuple | None) -> torch.Tensor:
+    """Attention inside each volume, of the stacked projection's rows ``(rows, 3 C)``; gives ``(rows, C)``."""
+    rows, c = qkv.shape[0], qkv.shape[1] // 3
+    qkv = qkv.view(rows, 3 * heads, c // heads)
+    if rotary is not None:  # query and key heads lie side by side: one call, in place
+        inv_freq, sections = rotary
+        turned = qkv[:, :2 * heads]
+        ops.rotary_axes(turned, grid.positions, inv_freq, sections, out=turned)
+    q, k, v = qkv.split(heads, dim=1)
+    return ops.attention(q, k, v, q_offsets=grid.offsets, scale=scale).view(rows, c)
+
+
+def scaled_projections(weights: Mapping[str, torch.Tensor], *, include_fc: bool,
+                       prefix: str = "attn") -> dict[str, ops.ScaledWeight]:
+    """The 8-bit weights of an attention block's projections, made once, where the block is loaded."""
+    scaled = {"qkv": ops.scale_weight(torch.cat([weights[f"{prefix}.to_{n}.weight"] for n in ("q", "k", "v")]))}
+    if include_fc:
+        scaled["out_proj"] = ops.scale_weight(weights[f"{prefix}.out_proj.weight"])
+    return scaled
+
+
 def packed_self_attention_tokens(tokens: torch.Tensor, grid: PackedGrid, weights: Mapping[str, torch.Tensor], *,
                                  heads: int, scale: float, include_fc: bool,
                                  adapters: Mapping[str, Mapping[str, torch.Tensor]] | None = None,
                                  index: torch.Tensor | None = None, rotary: tuple | None = None, prefix: str = "attn",
-                                 qkv_bias: bool = True) -> torch.Tensor:
+                                 qkv_bias: bool = True,
+                                 scaled: Mapping[str, ops.ScaledWeight] | None = None) -> torch.Tensor:
     """``fast_b200.self_attention_tokens`` on the packed rows ``(rows, C)`` of a grid's volumes, 16-bit.
 
     ``adapters`` may hold stacks (``ops.stack_adapters``) under ``"qkv"`` (C -> 3C) and ``"out_proj"``
     (C -> C); ``index`` (int32 on the device) names each volume's, negative for none. ``rotary`` is
-    ``(inv_freq, sections)`` for three axes (``ops.axis_frequencies``).
+    ``(inv_freq, sections)`` for three axes (``ops.axis_frequencies``). ``scaled`` (``scaled_projections``) runs the
+    projections in 8 bits, without adapters.
     """
     dt = tokens.dtype
     if tokens.dim() != 2 or tokens.shape[0] != grid.starts[-1]:
@@ -70,20 +97,21 @@ def packed_self_attention_tokens(tokens: torch.Tensor, grid: PackedGrid, weights
     used = ("qkv", "out_proj") if include_fc else ("qkv",)
     if unknown := sorted(set(adapters or ()) - set(used)):
         raise ValueError(f"adapters for {unknown}; this block has {', '.join(used)}")
+    if scaled is not None and (adapters or set(scaled) != set(used)):
+        raise ValueError(f"8-bit projections take no adapters and are {', '.join(used)}; got {', '.join(sorted(scaled))}")
     names = ("q", "k", "v")
-    w_qkv = fast_b200._stacked_dense(tuple(weights[f"{prefix}.to_{n}.weight"] for n in names), dt)
     b_qkv = fast_b200._stacked_dense(tuple(weights[f"{prefix}.to_{n}.bias"] for n in names), dt) if qkv_bias else None
     adapters = adapters or {}
-    qkv = _project(tokens, w_qkv, b_qkv, grid, adapters.get("qkv"), index)
-    rows, c = tokens.shape
-    qkv = qkv.view(rows, 3 * heads, c // heads)
-    if rotary is not None:  # query and key heads lie side by side: one call, in place
-        inv_freq, sections = rotary
-        turned = qkv[:, :2 * heads]
-        ops.rotary_axes(turned, grid.positions, inv_freq, sections, out=turned)
-    q, k, v = qkv.split(heads, dim=1)
-    merged = ops.attention(q, k, v, q_offsets=grid.offsets, scale=scale).view(rows, c)
-    if include_fc:
+    if scaled is not None:
+        qkv = ops.scaled_linear(ops.quantize_rows(tokens), scaled["qkv"], b_qkv, out_dtype=dt)
+    else:
+        w_qkv = fast_b200._stacked_dense(tuple(weights[f"{prefix}.to_{n}.weight"] for n in names), dt)
+        qkv = _project(tokens, w_qkv, b_qkv, grid, adapters.get("qkv"), index)
+    merged = _attend(qkv, grid, heads, scale, rotary)
+    if include_fc and scaled is not None:
+        merged = ops.scaled_linear(ops.quantize_rows(merged), scaled["out_proj"],
+                                   fast_b200._dense_weight(weights[f"{prefix}.out_proj.bias"], dt), out_dtype=dt)
+    elif include_fc:
         merged = _project(merged, fast_b200._dense_weight(weights[f"{prefix}.out_proj.weight"], dt),
                           fast_b200._dense_weight(weights[f"{prefix}.out_proj.bias"], dt), grid,
                           adapters.get("out_proj"), index)
@@ -93,7 +121,8 @@ def packed_self_attention_tokens(tokens: torch.Tensor, grid: PackedGrid, weights
 def packed_spatial_attention_ncdhw(volumes: Sequence[torch.Tensor], grid: PackedGrid, weights: Mapping[str, torch.Tensor],
                                    *, num_groups: int, eps: float, num_head_channels: int, include_fc: bool,
                                    adapters: Mapping[str, Mapping[str, torch.Tensor]] | None = None,
-                                   index: torch.Tensor | None = None, rotary: tuple | None = None) -> list[torch.Tensor]:
+                                   index: torch.Tensor | None = None, rotary: tuple | None = None,
+                                   scaled: Mapping[str, ops.ScaledWeight] | None = None) -> list[torch.Tensor]:
     """``fast_b200.spatial_attention_ncdhw`` of several ``(1, C, D, H, W)`` volumes at once; see the module's
     head. Needs a 16-bit arithmetic precision (``fast_b200.arithmetic_precision("fp16" | "bf16")``)."""
     dt = fast_b200.dense_dtype()
@@ -116,6 +145,30 @@ def packed_spatial_attention_ncdhw(volumes: Sequence[torch.Tensor], grid: Packed
         kept.append(x)
     heads, scale = c // num_head_channels, float(num_head_channels) ** -0.5
     merged = packed_self_attention_tokens(tokens, grid, weights, heads=heads, scale=scale, include_fc=include_fc,
-                                          adapters=adapters, index=index, rotary=rotary)
+                                          adapters=adapters, index=index, rotary=rotary, scaled=scaled)
     return [torch.add(x, merged[start:start + d * h * w].view(1, d, h, w, c).permute(0, 4, 1, 2, 3))
             for x, (d, h, w), start in zip(kept, grid.extents, grid.starts)]
+
+
+def packed_transformer_tokens(tokens: torch.Tensor, grid: PackedGrid, blocks: Sequence[Mapping[str, object]], *, heads: int,
+                              eps: float = 1e-6, rotary: tuple | None = None) -> torch.Tensor:
+    """Pre-norm transformer blocks on a grid's packed rows ``(rows, C)`` in 16 bits, projections in 8.
+
+    A block holds ``norm1`` and ``norm2`` (``(C,)``), and ``ops.ScaledWeight``s ``qkv`` (C -> 3C), ``out_proj``
+    (C -> C), ``gate_up`` (C -> 2F: what is gated by silu, then what it multiplies) and ``down`` (F -> C). Each norm
+    adds the branch before it to the residual stream and gives 8-bit rows in the same pass."""
+    if tokens.dim() != 2 or tokens.shape[0] != grid.starts[-1] or tokens.shape[1] % heads:
+        raise ValueError(f"tokens {tuple(tokens.shape)} where the grid has {grid.starts[-1]} rows, in {heads} heads")
+    dt, scale = tokens.dtype, (tokens.shape[1] // heads) ** -0.5
+    stream, branch = tokens, None
+    for block in blocks:
+        if branch is None:
+            rows = ops.rms_norm(stream, block["norm1"], eps=eps, quantize=True)
+        else:
+            rows, stream = ops.rms_norm(branch, block["norm1"], residual=stream, eps=eps, quantize=True)
+        merged = _attend(ops.scaled_linear(rows, block["qkv"], out_dtype=dt), grid, heads, scale, rotary)
+        branch = ops.scaled_linear(ops.quantize_rows(merged), block["out_proj"], out_dtype=dt)
+        rows, stream = ops.rms_norm(branch, block["norm2"], residual=stream, eps=eps, quantize=True)
+        hidden = ops.quantize_rows(ops.scaled_linear(rows, block["gate_up"], out_dtype=dt), gate=True)
+        branch = ops.scaled_linear(hidden, block["down"], out_dtype=dt)
+    return stream if branch is None else torch.add(stream, branch)
