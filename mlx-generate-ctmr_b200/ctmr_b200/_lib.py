@@ -8,6 +8,7 @@ raises ``ImportError``, so no caller can silently run on another backend.
 from __future__ import annotations
 
 import ctypes
+import struct
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "lib" / "libctmr_b200.so"
@@ -305,6 +306,20 @@ class ScaledLinearDesc(ctypes.Structure):
     ]
 
 
+def _packer(desc: type[ctypes.Structure]):
+    """``pack(*fields)``: the bytes of a descriptor (null pointers as 0), in a quarter of the time that the structure
+    takes: these calls are over before it is filled in."""
+    codes = {ctypes.c_void_p: "P", ctypes.c_int: "i", ctypes.c_longlong: "q", ctypes.c_float: "f"}
+    packer = struct.Struct("@" + "".join(codes[t] for _, t in desc._fields_) + "0P")
+    assert packer.size == ctypes.sizeof(desc)
+    return packer.pack
+
+
+pack_rms_norm = _packer(RmsNormDesc)
+pack_quantize_rows = _packer(QuantizeRowsDesc)
+pack_scaled_linear = _packer(ScaledLinearDesc)
+
+
 def _load() -> ctypes.CDLL:
     if not LIB_PATH.exists():
         raise ImportError(
@@ -341,9 +356,9 @@ def _load() -> ctypes.CDLL:
         "ctmr_adapter_linear_workspace_size": (sz, [ctypes.POINTER(AdapterLinearDesc)]),
         "ctmr_adapter_linear": (i, [ctypes.POINTER(AdapterLinearDesc), vp, sz, vp]),
         "ctmr_attention": (i, [ctypes.POINTER(AttentionDesc), vp]),
-        "ctmr_rms_norm": (i, [ctypes.POINTER(RmsNormDesc), vp]),
-        "ctmr_quantize_rows": (i, [ctypes.POINTER(QuantizeRowsDesc), vp]),
-        "ctmr_scaled_linear": (i, [ctypes.POINTER(ScaledLinearDesc), vp]),
+        "ctmr_rms_norm": (i, [vp, vp]),  # descriptors by reference or as bytes
+        "ctmr_quantize_rows": (i, [vp, vp]),
+        "ctmr_scaled_linear": (i, [vp, vp]),
         "ctmr_get_device_error": (i, [ctypes.POINTER(ctypes.c_uint), i]),
         "ctmr_status_string": (ctypes.c_char_p, [i]),
         "ctmr_last_error": (ctypes.c_char_p, []),

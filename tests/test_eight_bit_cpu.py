@@ -19,6 +19,14 @@ def _changed(d, kw):
     return ctypes.byref(d)
 
 
+@pytest.mark.parametrize(("pack", "desc"), [
+    (_lib.pack_rms_norm, _lib.RmsNormDesc), (_lib.pack_quantize_rows, _lib.QuantizeRowsDesc),
+    (_lib.pack_scaled_linear, _lib.ScaledLinearDesc)])
+def test_packed_descriptors_are_the_structures(pack, desc):
+    values = [0.5 if t is ctypes.c_float else 3 + 2 * i for i, (_, t) in enumerate(desc._fields_)]
+    assert pack(*values) == bytes(desc(*values))
+
+
 def _norm(**kw):
     return _changed(_lib.RmsNormDesc(0x1000, 0x2000, 0x3000, _lib.DTYPE_BF16, _lib.DTYPE_F32, 10, 1, 256, 256, 0, 256, 0,
                                      1e-6, 0x4000, 256, 0, 0x5000, 256, 0, 0x6000, 1, 10), kw)
