@@ -70,14 +70,18 @@ __global__ void __launch_bounds__(kThreads, kBlocks) quantize_kernel(const __gri
   uint32_t row = start / p.per_row, group = start - row * p.per_row;
   griddep_wait();
   griddep_launch_dependents();
+  Loaded<T, WIDE> a, b;
+  auto load = [&]() {
+    const bool in = row < rows;
+    const T* x = static_cast<const T*>(p.x) + (in ? row * p.x_stride : 0);
+    a.load(x, in ? p.channels : 0, group, lane8);
+    if constexpr (GATE) b.load(x + p.channels, in ? p.channels : 0, group, lane8);
+  };
+  load();
   while (__any_sync(0xffffffffu, row < rows)) {  // whole warps, for the shuffles
     const bool in = row < rows;
+    const uint32_t row_now = in ? row : 0, group_now = group;
     const int channels = in ? p.channels : 0;
-    const T* x = static_cast<const T*>(p.x) + (in ? row * p.x_stride : 0);
-    uint8_t* values = static_cast<uint8_t*>(p.values) + (in ? row * p.values_stride : 0);
-    Loaded<T, WIDE> a, b;
-    a.load(x, channels, group, lane8);
-    if constexpr (GATE) b.load(x + p.channels, channels, group, lane8);
     const bool inside = channel_of<WIDE>(group, lane8, 0) < channels;
     float v[kEach];
     a.values(v, inside);
@@ -90,16 +94,20 @@ __global__ void __launch_bounds__(kThreads, kBlocks) quantize_kernel(const __gri
         v[e] = g.x, v[e + 1] = g.y;
       }
     }
+    if (in) {  // (a row past the end stays where it is)
+      row += p.skip_rows, group += p.skip_groups;
+      if (group >= p.per_row) group -= p.per_row, ++row;
+    }
+    load();  // the next group, on its way while this one is rounded
     uint32_t q[4];
     float scale, by;
+    const T* x = static_cast<const T*>(p.x) + row_now * p.x_stride;
+    uint8_t* values = static_cast<uint8_t*>(p.values) + row_now * p.values_stride;
     const uint32_t differ = quantize_group<GATE ? kGatedUnits : 0>(
-        v, [&]() { return gated_top<T, WIDE>(x, p.channels, group, lane8); }, q, scale, by);
-    store_bytes<WIDE>(values, channels, group, lane8, q);
-    if (differ != 0) gated_patch<T, WIDE>(x, values, p.channels, group, lane8, differ, by);
-    if (lane8 == 0 && in) p.scale[row * p.scale_row + group * p.scale_group] = scale;
-    if (!in) continue;  // a row past the end stays where it is
-    row += p.skip_rows, group += p.skip_groups;
-    if (group >= p.per_row) group -= p.per_row, ++row;
+        v, [&]() { return gated_top<T, WIDE>(x, p.channels, group_now, lane8); }, q, scale, by);
+    store_bytes<WIDE>(values, channels, group_now, lane8, q);
+    if (differ != 0) gated_patch<T, WIDE>(x, values, p.channels, group_now, lane8, differ, by);
+    if (lane8 == 0 && in) p.scale[row_now * p.scale_row + group_now * p.scale_group] = scale;
   }
 }
 
