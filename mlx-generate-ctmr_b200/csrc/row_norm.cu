@@ -113,7 +113,7 @@ __global__ void __launch_bounds__(LANES ? 256 : LOOP ? 512 : 1024, 1) row_norm_k
     // 1 / sqrt(mean + eps): 32 bits' root and a step of Newton's in 64, good to 2^-43.
     const double mean = fma(total, p.per_channel, static_cast<double>(p.eps));
     double by64;
-    if (mean < 0x1p120) {
+    if (mean < 0x1p120 && mean > 0x1p-120) {
       by64 = static_cast<double>(rsqrtf(static_cast<float>(mean)));
       by64 = fma(0.5 * by64, fma(-mean * by64, by64, 1.0), by64);
     } else {

@@ -7,7 +7,7 @@
 // bounds how long a sum stays inside the tensor core.
 //
 // Two forms. Pairs of CTAs take 256 rows x 256 outputs, rows as TMEM lanes: a thread then has one row scale and one
-// weight scale a block, and one multiplication and 128 additions. Few rows take tiles of 128 outputs as lanes by 16 to
+// weight scale a block, and 128 products and additions. Few rows take tiles of 128 outputs as lanes by 16 to
 // 128 rows as columns, with the inputs split over a cluster: all SMs stream the weight at the memory's rate, and the
 // partial sums meet through distributed shared memory, in the order of the ranks.
 #include "capi_internal.cuh"
@@ -22,12 +22,13 @@ constexpr int kK = kScaleGroup;
 constexpr uint32_t kHalfTile = 128 * 128;  // 128 rows of 128 bytes
 
 struct ScaledMaps {
-  CUtensorMap x, w;
+  CUtensorMap x, w, y;  // y: CTA pairs only, and where rows of y allow it
 };
 
 struct ScaledPlan {
   int tile, row_tiles, out_tiles;
-  int split;  // CTAs (a cluster) that share a tile's blocks; 0: CTA pairs
+  int split;   // CTAs (a cluster) that share a tile's blocks; 0: CTA pairs
+  int copied;  // y's map is there
 };
 
 template <typename T>
@@ -335,24 +336,12 @@ __global__ void __launch_bounds__(kFewThreads, FewSmem<BN>::kCtas)
   }
 }
 
-// sum += v by, 16 of them, two to an instruction.
-__device__ __forceinline__ void add_scaled(float* sum, const float (&v)[16], float by) {
-#pragma unroll
-  for (int i = 0; i < 16; i += 2)
-    asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %4};\n\tmov.b64 z, {%0, %1};\n\t"
-        "fma.rn.f32x2 z, x, y, z;\n\tmov.b64 {%0, %1}, z;\n\t}"
-        : "+f"(sum[i]), "+f"(sum[i + 1])
-        : "f"(v[i]), "f"(v[i + 1]), "f"(by));
-}
-
-// By a warp: 32 rows (a lane's sums are one) of COLUMNS outputs, 64 bytes of each row at a time by way of shared memory, so
-// that four lanes write side by side. (A lane that writes its own row's 16 bytes, 32 rows to an access, kept the
-// warps 8,600 clocks a tile.)
+// By a warp: 32 rows (a lane's sums are one) of COLUMNS outputs, 64 bytes of each row at a time by way of shared memory,
+// so that lanes write side by side; for rows of y that TMA does not take (not 16-byte aligned).
 template <typename T, int COLUMNS>
 __device__ __forceinline__ void write_rows(const ScaledLinearParams& p, uint8_t* store, const float* sum, int row0, int o0,
                                            int lane) {
   constexpr int kPer = 16 / sizeof(T), kWide = 4 * kPer;  // outputs in 16 bytes, in 64
-  const bool wide = p.y_stride % kPer == 0 && reinterpret_cast<uintptr_t>(p.y) % 16 == 0;
 #pragma unroll
   for (int c = 0; c < COLUMNS; c += kWide) {
     if (o0 + c >= p.out) break;
@@ -360,9 +349,7 @@ __device__ __forceinline__ void write_rows(const ScaledLinearParams& p, uint8_t*
     for (int j = 0; j < 4; ++j) {  // 16 bytes each, in an order by which neither side meets a bank twice
       alignas(16) T e[kPer];
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        e[i] = from_float<T>(sum[c + j * kPer + i]);
-      }
+      for (int i = 0; i < kPer; ++i) e[i] = from_float<T>(sum[c + j * kPer + i]);
       *reinterpret_cast<uint4*>(store + lane * 64 + (j ^ (lane >> 1 & 3)) * 16) = *reinterpret_cast<const uint4*>(e);
     }
     __syncwarp();
@@ -373,29 +360,64 @@ __device__ __forceinline__ void write_rows(const ScaledLinearParams& p, uint8_t*
       const uint4 v = *reinterpret_cast<const uint4*>(store + r * 64 + (chunk ^ (r >> 1 & 3)) * 16);
       if (row0 + r >= p.rows) continue;
       T* y = static_cast<T*>(p.y) + (row0 + r) * p.y_stride + o;
-      if (wide && o + kPer <= p.out) {
-        *reinterpret_cast<uint4*>(y) = v;
-      } else {
-        const T* e = reinterpret_cast<const T*>(&v);
+      const T* e = reinterpret_cast<const T*>(&v);
 #pragma unroll
-        for (int x = 0; x < kPer; ++x)
-          if (o + x < p.out) y[x] = e[x];
-      }
+      for (int x = 0; x < kPer; ++x)
+        if (o + x < p.out) y[x] = e[x];
     }
     __syncwarp();
   }
+}
+
+// The same by TMA, 128 bytes of each row at a time from two boxes in turn: the warp goes on to the next tile while they
+// are written. (8,191 x 4,096 -> 12,288: 473 us with stores by the warps, 13 % of them waiting for the stores of
+// all SMs at once.)
+template <typename T, int COLUMNS>
+__device__ __forceinline__ void copy_rows(const CUtensorMap& map, const ScaledLinearParams& p, uint8_t* store,
+                                          const float* sum, int row0, int o0, int lane) {
+  constexpr int kPer = 16 / sizeof(T), kBox = 8 * kPer;  // outputs in 16 bytes, in 128
+#pragma unroll
+  for (int c = 0; c < COLUMNS; c += kBox) {
+    uint8_t* box = store + (c / kBox & 1) * 4096;
+    if (lane == 0) bulk_groups_read<1>();  // the box's last copy, two groups ago, has read it
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      alignas(16) T e[kPer];
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) e[i] = from_float<T>(sum[c + j * kPer + i]);
+      *reinterpret_cast<uint4*>(box + lane * 128 + (j ^ (lane & 7)) * 16) = *reinterpret_cast<const uint4*>(e);
+    }
+    fence_proxy_async_shared();
+    __syncwarp();
+    if (lane == 0) {
+      if (row0 < p.rows && o0 + c < p.out) tma_store_2d(&map, box, o0 + c, row0);
+      bulk_group_end();
+    }
+  }
+}
+
+// sum += v by, 16 of them, two to an instruction.
+__device__ __forceinline__ void add_scaled(float* sum, const float (&v)[16], float by) {
+#pragma unroll
+  for (int i = 0; i < 16; i += 2)
+    asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %4};\n\tmov.b64 z, {%0, %1};\n\t"
+        "fma.rn.f32x2 z, x, y, z;\n\tmov.b64 {%0, %1}, z;\n\t}"
+        : "+f"(sum[i]), "+f"(sum[i + 1])
+        : "f"(v[i]), "f"(v[i + 1]), "f"(by));
 }
 
 // ---------------------------------------------------------------- CTA pairs
 constexpr int kSumWarps = 8, kColumns = 1024 / kSumWarps;
 constexpr int kPairThreads = 96 + 32 * kSumWarps;  // warp 0 TMA, warp 1 MMA (first CTA), warp 2 scales, the others sums
 constexpr int kPairTile = 256;
-constexpr int kPairStages = 6;
+constexpr int kPairStages = 4;
 constexpr uint32_t kPairStageBytes = 2 * kHalfTile;  // this CTA's 128 rows and 128 outputs
 constexpr int kPairFactors = 3;  // fours of blocks whose scales are in shared memory: [block][half of the outputs][row]
-constexpr uint32_t kPairOffFactors = kPairStages * kPairStageBytes;
-constexpr uint32_t kPairOffStore = kPairOffFactors + kPairFactors * 4 * 256 * 4;  // 32 rows of 64 bytes a warp
-constexpr uint32_t kPairOffBar = kPairOffStore + kSumWarps * 2048;
+constexpr uint32_t kStoreBytes = 2 * 4096;  // a warp's two boxes of 32 rows of 128 bytes
+constexpr uint32_t kPairOffStore = kPairStages * kPairStageBytes;
+constexpr uint32_t kPairOffFactors = kPairOffStore + kSumWarps * kStoreBytes;
+constexpr uint32_t kPairOffBar = kPairOffFactors + kPairFactors * 4 * 256 * 4;
 constexpr uint32_t kPairBytes = kPairOffBar + 512 + 1024;
 constexpr int kRaster = 8;  // row tiles that are walked together, so that the weight's and x's tiles meet in L2
 
@@ -561,18 +583,18 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     const uint32_t lanes = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + columns;
     const uint32_t release0 = cluster_addr(acc_empty, 0);
     const float* my_factor = factors + columns / 128 * 128 + quarter * 32 + lane;
-    uint8_t* store = smem + kPairOffStore + (warp - 3) * 2048;
     int it = 0, group = 0;
     bool ok = true;
     for (int t = pair; ok && t < tiles; t += pairs) {
       int r0, n0;
-      place(t, r0, n0);
       float sum[kColumns];
 #pragma unroll
       for (int c = 0; c < kColumns; ++c) sum[c] = 0.f;
-      if (p.bias != nullptr)
+      if (p.bias != nullptr) {
+        place(t, r0, n0);
 #pragma unroll
         for (int c = 0; c < kColumns; ++c) sum[c] = bias_at<T>(p, n0 + columns + c);
+      }
       for (int k = 0; k < kb; ++k, ++it) {
         const int a = it & 1, f = group % kPairFactors;
         if ((k & 3) == 0) ok = mbar_wait_warp(&factor_full[f], static_cast<uint32_t>(group / kPairFactors) & 1u, kErrWaitFull);
@@ -582,30 +604,37 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         tc_fence_after();
         const bool last = (k & 3) == 3 || k + 1 == kb;
         // The next 16 on their way while these are added.
-        float v[2][16];
-        tmem_ld16_start(lanes + a * 256, v[0]);
+        float v[16];
 #pragma unroll
         for (int c = 0; c < kColumns; c += 16) {
-          float(&now)[16] = v[c / 16 & 1];
+          tmem_ld16_start(lanes + a * 256 + c, v);
           tmem_ld_wait();
-          tmem_ld_fence16(now);
-          if (c + 16 < kColumns) {
-            tmem_ld16_start(lanes + a * 256 + c + 16, v[c / 16 + 1 & 1]);
-          } else {  // all read: the next block but one may overwrite it
+          tmem_ld_fence16(v);
+          if (c + 16 == kColumns) {  // all read: the next block but one may overwrite it
             tc_fence_before();
             if (lane == 0) {
               mbar_arrive_remote(release0 + 8u * a);
               if (last) mbar_arrive(&factor_empty[f]);
             }
           }
-          add_scaled(sum + c, now, by);
+          add_scaled(sum + c, v, by);
         }
         group += last;
       }
       ok = ok && __all_sync(0xffffffffu, !*abort_flag);
       if (!ok) break;
-      write_rows<T, kColumns>(p, store, sum, r0 + quarter * 32, n0 + columns, lane);
+      // The tile's place once more: kept over the loop it would cost registers that the sums need.
+      int tile = t, thread = threadIdx.x;
+      asm volatile("" : "+r"(tile), "+r"(thread));
+      place(tile, r0, n0);
+      const int at_lane = thread & 31, at_warp = thread >> 5;
+      r0 += (at_warp & 3) * 32, n0 += (at_warp - 3) / 4 * kColumns;
+      uint8_t* store = smem + kPairOffStore + (at_warp - 3) * kStoreBytes;
+      if (plan.copied) copy_rows<T, kColumns>(maps.y, p, store, sum, r0, n0, at_lane);
+      else write_rows<T, kColumns>(p, store, sum, r0, n0, at_lane);
     }
+    if (lane == 0) bulk_groups_done();
+    __syncwarp();
     if (!ok) *abort_flag = 1;
   }
 
@@ -619,15 +648,15 @@ __global__ void __launch_bounds__(kPairThreads, 1)
 }
 
 // ---------------------------------------------------------------- host
-int encode(CUtensorMap* map, const void* base, long long in, long long rows, long long stride, int box_rows,
-           const char* what) {
+int encode(CUtensorMap* map, CUtensorMapDataType type, const void* base, long long columns, long long rows,
+           long long row_bytes, int box_columns, int box_rows, const char* what) {
   auto enc = api_tensor_map_encoder();
   if (enc == nullptr) return api_fail(CTMR_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
-  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(in), static_cast<cuuint64_t>(rows)};
-  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(stride)};
-  const cuuint32_t box[2] = {kK, static_cast<cuuint32_t>(box_rows)}, step[2] = {1, 1};
-  const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, step,
-                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(columns), static_cast<cuuint64_t>(rows)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(row_bytes)};
+  const cuuint32_t box[2] = {static_cast<cuuint32_t>(box_columns), static_cast<cuuint32_t>(box_rows)}, step[2] = {1, 1};
+  const CUresult r = enc(map, type, 2, const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return api_fail(CTMR_ERR_INVALID, "%s: tensor map rejected (CUresult %d)", what, int(r));
   return CTMR_OK;
@@ -639,7 +668,7 @@ int encode(CUtensorMap* map, const void* base, long long in, long long rows, lon
 // sums' way takes longer the more columns there are. CTA pairs: 4.5, and 0.53 a block and 0.6 a tile, whose stores fall
 // between the next one's products. (1 row of 4,096 -> 4,096: tiles of 16 rows split four ways 6.5, two ways 7.5, not
 // 9.4; 32 rows: tiles of 32 split two ways 8.0, four ways 9.0; 128 rows: of 64 split two ways 10.6, of 128 four ways
-// 11.6; 300 rows: of 128 19.7, pairs 20.7; 1,000 rows: pairs 22.3, tiles of 128 38.5.)
+// 11.7; 300 rows: of 128 19.8, pairs 19.4; 1,000 rows: pairs 20.6, tiles of 128 38.5.)
 ScaledPlan plan_scaled(const ScaledLinearParams& p) {
   ScaledPlan plan{};
   const int sms = device_sm_count(), kb = (p.in + kK - 1) / kK;
@@ -677,13 +706,20 @@ cudaError_t launch_few(const ScaledMaps& maps, const ScaledLinearParams& p, cons
 
 template <typename T>
 int launch(const ScaledLinearParams& p, cudaStream_t stream) {
-  const ScaledPlan plan = plan_scaled(p);
+  ScaledPlan plan = plan_scaled(p);
   ScaledMaps maps;
-  int st = encode(&maps.x, p.x, p.in, p.rows, p.x_stride, plan.split == 0 ? 128 : plan.tile, "x");
-  if (st == CTMR_OK) st = encode(&maps.w, p.weight, p.in, p.out, p.weight_stride, 128, "weight");
+  constexpr CUtensorMapDataType kByte = CU_TENSOR_MAP_DATA_TYPE_UINT8;
+  int st = encode(&maps.x, kByte, p.x, p.in, p.rows, p.x_stride, kK, plan.split == 0 ? 128 : plan.tile, "x");
+  if (st == CTMR_OK) st = encode(&maps.w, kByte, p.weight, p.in, p.out, p.weight_stride, kK, 128, "weight");
+  const long long y_bytes = p.y_stride * static_cast<long long>(sizeof(T));
+  plan.copied = plan.split == 0 && y_bytes % 16 == 0 && reinterpret_cast<uintptr_t>(p.y) % 16 == 0;
+  maps.y = maps.w;  // not read otherwise
+  if (st == CTMR_OK && plan.copied)
+    st = encode(&maps.y, sizeof(T) == 4 ? CU_TENSOR_MAP_DATA_TYPE_UINT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, p.y, p.out,
+                p.rows, y_bytes, 128 / sizeof(T), 32, "y");
   if (st != CTMR_OK) return st;
   const long long tiles = static_cast<long long>(plan.row_tiles) * plan.out_tiles;
-  if (tiles * (plan.split > 0 ? plan.split : 1) > 0x7fffffffLL)
+  if (tiles * (plan.split > 0 ? plan.split : 1) > 0x3fffffffLL)
     return api_fail(CTMR_ERR_UNSUPPORTED, "scaled_linear: too many tiles");
   cudaError_t e;
   if (plan.split == 0) {

@@ -423,6 +423,36 @@ def test_rows_past_32_bits():
     _check_rows(ops.quantize_rows(x, gate=True), _gate_ref(x))
 
 
+@pytest.mark.parametrize(("rows", "inner", "outer", "pitch"), [(3, 256, 5, 2 ** 30 + 16), (700, 256, 2000, 2 ** 22)])
+def test_linear_past_32_bits(rows, inner, outer, pitch):
+    """Rows of x and of y, and their scales, more than 2^31 elements from the first, in either form."""
+    from ctmr_b200 import ops
+
+    gen = _gen(rows)
+    x, w = _rows8(gen, rows, inner), _weight8(gen, outer, inner)
+    far = torch.empty((rows - 1) * pitch + inner, dtype=torch.uint8, device="cuda").view(E4M3).as_strided((rows, inner), (pitch, 1))
+    far.copy_(x.values)
+    out = torch.empty((rows - 1) * pitch + outer, dtype=torch.float16, device="cuda").as_strided((rows, outer), (pitch, 1))
+    scale = torch.empty((rows - 1) * pitch + 2, dtype=torch.float32, device="cuda").as_strided((rows, 2), (pitch, 1))
+    scale.copy_(x.scale)
+    x = ops.ScaledRows(far, scale)
+    ops.scaled_linear(x, w, out=out)
+    _check_linear(out, x, w, None)
+
+
+def test_norm_with_the_least_eps():
+    """Rows near or at zero, where the mean square and eps lie below 32 bits' normal numbers."""
+    from ctmr_b200 import ops
+
+    x = _randn(_gen(4), 6, 512, std=1e-21)
+    x[2] = 0.0
+    for eps in (1e-38, 1e-40, 1e-44):
+        eps = torch.tensor(eps, dtype=torch.float32).item()
+        ref = _norm_ref(x, None, None, eps)
+        _within(ops.rms_norm(x, eps=eps), ref, 2.0 ** -20 * ref.abs())
+        _check_rows(ops.rms_norm(x, eps=eps, quantize=True), ref)
+
+
 def test_graphs_and_streams():
     """Captured and replayed on other inputs, and called on a stream of its own, with the eager call's bits."""
     from ctmr_b200 import ops
@@ -430,13 +460,13 @@ def test_graphs_and_streams():
     gen = _gen(8)
     x, residual = _randn(gen, 70, 1536, dtype=torch.bfloat16), _randn(gen, 70, 1536, dtype=torch.bfloat16)
     weight = 1.0 + _randn(gen, 1536, std=0.2)
-    w = _weight8(gen, 3000, 1536)
+    w, many = _weight8(gen, 3000, 1536), _rows8(gen, 1000, 1536)
 
     def both():
         y, h = ops.rms_norm(x, weight, residual=residual, quantize=True)
         z = ops.quantize_rows(h, gate=True)
         return y.values.view(torch.uint8), y.scale, h, z.values.view(torch.uint8), z.scale, ops.scaled_linear(y, w), \
-            ops.scaled_linear(ops.ScaledRows(y.values[:5], y.scale[:5]), w)
+            ops.scaled_linear(ops.ScaledRows(y.values[:5], y.scale[:5]), w), ops.scaled_linear(many, w)
 
     both()
     side = torch.cuda.Stream()
