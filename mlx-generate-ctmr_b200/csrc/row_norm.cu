@@ -199,7 +199,7 @@ cudaError_t launch_rows(const RowNormParams& p, cudaStream_t stream) {
   if (groups == 1) return launch<T, 1, 8, false, EIGHT>(p, wide, grid(8), 256, stream);
   if (groups == 2) return launch<T, 1, 16, false, EIGHT>(p, wide, grid(16), 256, stream);
   if (groups <= 4) return launch<T, 1, 32, false, EIGHT>(p, wide, grid(32), 256, stream);
-  if (groups <= 8) return launch<T, 2, 32, false, EIGHT>(p, wide, grid(32), 256, stream);
+  if (groups <= 8 && rows > 16 * device_sm_count()) return launch<T, 2, 32, false, EIGHT>(p, wide, grid(32), 256, stream);
   auto threads = [&](int v) { return (groups + 4 * v - 1) / (4 * v) * 32; };
   const long long resident = static_cast<long long>(device_sm_count()) * (512 / threads(1));  // at 128 registers
   if (threads(1) <= 512 && rows > resident) return launch<T, 1, 0, true, EIGHT>(p, wide, resident, threads(1), stream);

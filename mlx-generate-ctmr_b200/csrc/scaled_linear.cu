@@ -597,12 +597,15 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       }
       for (int k = 0; k < kb; ++k, ++it) {
         const int a = it & 1, f = group % kPairFactors;
-        if ((k & 3) == 0) ok = mbar_wait_warp(&factor_full[f], static_cast<uint32_t>(group / kPairFactors) & 1u, kErrWaitFull);
+        if ((k & 3) == 0) {
+          ok = mbar_wait_warp(&factor_full[f], static_cast<uint32_t>(group / kPairFactors) & 1u, kErrWaitFull);
+          // All lanes are past the four before.
+          if (lane == 0 && group > 0) mbar_arrive(&factor_empty[(group - 1) % kPairFactors]);
+        }
         const float by = my_factor[(f * 4 + (k & 3)) * 256];
         ok = ok && mbar_wait_warp(&acc_full[a], static_cast<uint32_t>(it >> 1) & 1u, kErrWaitAcc);
         if (!ok) break;
         tc_fence_after();
-        const bool last = (k & 3) == 3 || k + 1 == kb;
         // The next 16 on their way while these are added.
         float v[16];
 #pragma unroll
@@ -612,14 +615,11 @@ __global__ void __launch_bounds__(kPairThreads, 1)
           tmem_ld_fence16(v);
           if (c + 16 == kColumns) {  // all read: the next block but one may overwrite it
             tc_fence_before();
-            if (lane == 0) {
-              mbar_arrive_remote(release0 + 8u * a);
-              if (last) mbar_arrive(&factor_empty[f]);
-            }
+            if (lane == 0) mbar_arrive_remote(release0 + 8u * a);
           }
           add_scaled(sum + c, v, by);
         }
-        group += last;
+        group += (k & 3) == 3 || k + 1 == kb;
       }
       ok = ok && __all_sync(0xffffffffu, !*abort_flag);
       if (!ok) break;
