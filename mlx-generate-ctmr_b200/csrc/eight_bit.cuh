@@ -56,26 +56,20 @@ cudaError_t launch_quantize(const QuantizeParams& p, int dtype, cudaStream_t str
 int launch_scaled_linear(const ScaledLinearParams& p, int y_dtype, cudaStream_t stream);  // a CTMR_ status
 
 // ---------------------------------------------------------------- a group of a row
-// Eight lanes hold a group of 128 channels, 16 each: consecutive ones where the row's address, stride and length allow
-// 32-byte accesses (WIDE), every eighth one otherwise, so that the lanes' single accesses still lie side by side.
+// Eight lanes hold a group of 128 channels, 16 each: eight consecutive ones of either half where the row's address, stride
+// and length allow 16-byte accesses (WIDE), every eighth one otherwise: a warp's accesses lie side by side either way.
 constexpr int kEach = 16, kGroupLanes = kScaleGroup / kEach;
 
 template <bool WIDE>
 __device__ __forceinline__ int channel_of(int group, int lane8, int e) {
-  return group * kScaleGroup + (WIDE ? lane8 * kEach + e : lane8 + kGroupLanes * e);
+  return group * kScaleGroup + (WIDE ? e / 8 * 64 + lane8 * 8 + e % 8 : lane8 + kGroupLanes * e);
 }
 
-__device__ __forceinline__ void load32(const void* at, uint32_t (&r)[8]) {
-  asm volatile("ld.global.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"  // volatile: before the stores over the same row
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
-               : "l"(at)
-               : "memory");
-}
-
-__device__ __forceinline__ void store32(void* at, const uint32_t (&r)[8]) {
-  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(at), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]),
-               "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
-               : "memory");
+// 16 bytes, kept in order with the stores over the same row.
+__device__ __forceinline__ uint4 load_bytes16(const void* at) {
+  uint4 r;
+  asm volatile("ld.global.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(at) : "memory");
+  return r;
 }
 
 // v[at] of registers.
@@ -89,15 +83,23 @@ __device__ __forceinline__ float pick(const float (&v)[kEach], int at) {
 // A lane's 16 channels of a row as they lie in memory. Past the row's end `values`, by whole warps, gives zeros.
 template <typename T, bool WIDE>
 struct Loaded {
-  uint32_t raw[WIDE ? kEach * sizeof(T) / 4 : 1];
+  static constexpr uint32_t kWords = kEach * sizeof(T) / 4;
+  uint32_t raw[WIDE ? kWords : 1];
   T each[WIDE ? 1 : kEach];
 
   __device__ __forceinline__ void load(const T* row, int channels, int group, int lane8) {
     if constexpr (WIDE) {
-      const int c = channel_of<true>(group, lane8, 0);
-      if (c < channels) {
-        load32(row + c, *reinterpret_cast<uint32_t(*)[8]>(raw));
-        if constexpr (sizeof(T) == 4) load32(row + c + 8, *reinterpret_cast<uint32_t(*)[8]>(raw + 8));
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int c = channel_of<true>(group, lane8, 8 * half);
+        if (c < channels) {
+#pragma unroll
+          for (uint32_t i = 0; i < kWords / 8; ++i) {
+            const uint4 r = load_bytes16(row + c + 4 * i);
+            const uint32_t to = half * (kWords / 2) + 4 * i;
+            raw[to] = r.x, raw[to + 1] = r.y, raw[to + 2] = r.z, raw[to + 3] = r.w;
+          }
+        }
       }
     } else {
 #pragma unroll
@@ -108,7 +110,7 @@ struct Loaded {
     }
   }
 
-  __device__ __forceinline__ void values(float (&v)[kEach], bool inside) const {
+  __device__ __forceinline__ void values(float (&v)[kEach], int channels, int group, int lane8) const {
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
       if constexpr (!WIDE) {
@@ -122,9 +124,10 @@ struct Loaded {
         v[i] = __uint_as_float(i % 2 ? raw[i / 2] & 0xffff0000u : raw[i / 2] << 16);
       }
     }
-    if (WIDE && __any_sync(0xffffffffu, !inside))  // (a branch: selects, or zeros ahead of the load, would cost every warp)
+    // (A branch: selects, or zeros ahead of the load, would cost every warp.)
+    if (WIDE && __any_sync(0xffffffffu, channel_of<WIDE>(group, lane8, kEach - 1) >= channels))
 #pragma unroll
-      for (int i = 0; i < kEach; ++i) v[i] = inside ? v[i] : 0.f;
+      for (int i = 0; i < kEach; ++i) v[i] = channel_of<WIDE>(group, lane8, i / 8 * 8) < channels ? v[i] : 0.f;
   }
 };
 
@@ -132,7 +135,7 @@ template <typename T, bool WIDE>
 __device__ __forceinline__ void load16(const T* row, int channels, int group, int lane8, float (&v)[kEach]) {
   Loaded<T, WIDE> in;
   in.load(row, channels, group, lane8);
-  in.values(v, channel_of<WIDE>(group, lane8, 0) < channels);
+  in.values(v, channels, group, lane8);
 }
 
 // Two values to the 16-bit type, the first in the low half.
@@ -148,20 +151,18 @@ __device__ __forceinline__ uint32_t pack2(float a, float b, __nv_bfloat16) {
 template <typename T, bool WIDE>
 __device__ __forceinline__ void store16(T* row, int channels, int group, int lane8, const float (&v)[kEach]) {
   if constexpr (WIDE) {
-    const int c = channel_of<true>(group, lane8, 0);
-    if (c >= channels) return;
-    uint32_t raw[8];
-    if constexpr (sizeof(T) == 4) {
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) raw[i] = __float_as_uint(v[8 * j + i]);
-        store32(row + c + 8 * j, raw);
+    for (int half = 0; half < 2; ++half) {
+      const int c = channel_of<true>(group, lane8, 8 * half);
+      const float* w = v + 8 * half;
+      if (c >= channels) continue;
+      if constexpr (sizeof(T) == 4) {
+        reinterpret_cast<float4*>(row + c)[0] = make_float4(w[0], w[1], w[2], w[3]);
+        reinterpret_cast<float4*>(row + c)[1] = make_float4(w[4], w[5], w[6], w[7]);
+      } else {
+        *reinterpret_cast<uint4*>(row + c) =
+            make_uint4(pack2(w[0], w[1], T()), pack2(w[2], w[3], T()), pack2(w[4], w[5], T()), pack2(w[6], w[7], T()));
       }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) raw[i] = pack2(v[2 * i], v[2 * i + 1], T());
-      store32(row + c, raw);
     }
   } else {
 #pragma unroll
@@ -175,8 +176,11 @@ __device__ __forceinline__ void store16(T* row, int channels, int group, int lan
 template <bool WIDE>
 __device__ __forceinline__ void store_bytes(uint8_t* row, int channels, int group, int lane8, const uint32_t (&q)[4]) {
   if constexpr (WIDE) {
-    const int c = channel_of<true>(group, lane8, 0);
-    if (c < channels) *reinterpret_cast<uint4*>(row + c) = make_uint4(q[0], q[1], q[2], q[3]);
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const int c = channel_of<true>(group, lane8, 8 * half);
+      if (c < channels) *reinterpret_cast<uint2*>(row + c) = make_uint2(q[2 * half], q[2 * half + 1]);
+    }
   } else {
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {

@@ -82,12 +82,11 @@ __global__ void __launch_bounds__(kThreads, kBlocks) quantize_kernel(const __gri
     const bool in = row < rows;
     const uint32_t row_now = in ? row : 0, group_now = group;
     const int channels = in ? p.channels : 0;
-    const bool inside = channel_of<WIDE>(group, lane8, 0) < channels;
     float v[kEach];
-    a.values(v, inside);
+    a.values(v, channels, group, lane8);
     if constexpr (GATE) {
       float other[kEach];
-      b.values(other, inside);
+      b.values(other, channels, group, lane8);
 #pragma unroll
       for (int e = 0; e < kEach; e += 2) {
         const float2 g = gated2(make_float2(v[e], v[e + 1]), make_float2(other[e], other[e + 1]));
@@ -113,9 +112,9 @@ __global__ void __launch_bounds__(kThreads, kBlocks) quantize_kernel(const __gri
 
 template <typename T, bool GATE>
 cudaError_t launch(QuantizeParams p, cudaStream_t stream) {
-  const bool wide = p.channels % kEach == 0 && p.x_stride % (32 / static_cast<int>(sizeof(T))) == 0 &&
-                    reinterpret_cast<uintptr_t>(p.x) % 32 == 0 && p.values_stride % 16 == 0 &&
-                    reinterpret_cast<uintptr_t>(p.values) % 16 == 0;
+  const bool wide = p.channels % 8 == 0 && p.x_stride % (16 / static_cast<int>(sizeof(T))) == 0 &&
+                    reinterpret_cast<uintptr_t>(p.x) % 16 == 0 && p.values_stride % 8 == 0 &&
+                    reinterpret_cast<uintptr_t>(p.values) % 8 == 0;
   p.per_row = (static_cast<uint32_t>(p.channels) + kScaleGroup - 1) / kScaleGroup;
   const unsigned long long groups = static_cast<unsigned long long>(p.per_row) * p.rows;
   const unsigned long long blocks = (groups + kGroups - 1) / kGroups;

@@ -69,11 +69,10 @@ __global__ void __launch_bounds__(LANES ? 256 : LOOP ? 512 : 1024, 1) row_norm_k
   for (int turn = 0;; turn ^= 1) {
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      const bool inside = channel_of<WIDE>(first + i * step, lane8, 0) < channels;
-      x_in[i].values(h[i], inside);
+      x_in[i].values(h[i], channels, first + i * step, lane8);
       if (p.residual != nullptr) {
         float add[kEach];
-        r_in[i].values(add, inside);
+        r_in[i].values(add, channels, first + i * step, lane8);
         if constexpr (kLow) {  // what the sum's rounding cuts off, exactly
 #pragma unroll
           for (int e = 0; e < kEach; ++e) {
@@ -183,16 +182,16 @@ cudaError_t launch(const RowNormParams& p, bool wide, long long grid, int thread
 
 template <typename T, bool EIGHT>
 cudaError_t launch_rows(const RowNormParams& p, cudaStream_t stream) {
-  // 32-byte accesses where every row allows them.
-  constexpr int kAlign = 32 / sizeof(T);
+  // 16-byte accesses where every row allows them.
+  constexpr int kAlign = 16 / sizeof(T);
   auto row_ok = [](const void* at, long long token, long long head) {
-    return at == nullptr || (reinterpret_cast<uintptr_t>(at) % 32 == 0 && token % kAlign == 0 && head % kAlign == 0);
+    return at == nullptr || (reinterpret_cast<uintptr_t>(at) % 16 == 0 && token % kAlign == 0 && head % kAlign == 0);
   };
-  const bool wide = p.channels % kEach == 0 && row_ok(p.x, p.x_token, p.x_head) &&
-                    row_ok(p.residual, p.r_token, p.r_head) && row_ok(p.sum, p.s_token, p.s_head) &&
-                    (EIGHT ? reinterpret_cast<uintptr_t>(p.y) % 16 == 0 && p.y_token % 16 == 0
+  const bool wide = p.channels % 8 == 0 && row_ok(p.x, p.x_token, p.x_head) && row_ok(p.residual, p.r_token, p.r_head) &&
+                    row_ok(p.sum, p.s_token, p.s_head) &&
+                    (EIGHT ? reinterpret_cast<uintptr_t>(p.y) % 8 == 0 && p.y_token % 8 == 0
                            : row_ok(p.y, p.y_token, p.y_head)) &&
-                    (p.weight == nullptr || reinterpret_cast<uintptr_t>(p.weight) % 32 == 0);
+                    (p.weight == nullptr || reinterpret_cast<uintptr_t>(p.weight) % 16 == 0);
   const long long rows = static_cast<long long>(p.tokens) * p.heads;
   const int groups = (p.channels + kScaleGroup - 1) / kScaleGroup;
   auto grid = [&](int lanes) { return (rows * lanes + 255) / 256; };
