@@ -3,8 +3,9 @@
 //
 // Bound by memory (5 bytes a channel of a gated 16-bit row, 3 of a plain one) as long as the arithmetic stays below
 // some 25 instructions a channel: silu is one exponential and one reciprocal, with the exponent's product taken
-// in two parts so that the error stays near 2^-22 for any size of a. Groups of 128 channels, 16 threads each, follow one
-// another over the rows without regard to where a row ends, so that no size leaves threads idle.
+// in two parts so that the error stays near 2^-22 for any size of a. Groups of 128 channels, eight lanes each, follow one
+// another over the rows without regard to where a row ends, so that no size leaves threads idle. 8,192 gated rows of
+// 11,264: 87 us, 5.3 TB/s (84 without the 64-bit decisions); what is left are instructions, 24 a channel.
 #include "capi_internal.cuh"
 #include "ctmr_b200.h"
 #include "eight_bit.cuh"
@@ -62,7 +63,7 @@ __device__ __noinline__ void gated_patch(const T* x, uint8_t* values, int channe
 }
 
 // A block takes 32 groups of channels at a time, eight lanes each, then those p.skip_rows rows and p.skip_groups
-// groups further: no division but the first. (Two groups to a lane, 8,192 x 11,264 gated: 108 us for 100.)
+// groups further: no division but the first.
 template <typename T, bool GATE, bool WIDE>
 __global__ void __launch_bounds__(kThreads, kBlocks) quantize_kernel(const __grid_constant__ QuantizeParams p) {
   const int lane8 = threadIdx.x % kGroupLanes;

@@ -10,6 +10,13 @@
 // weight scale a block, and 128 products and additions. Few rows take tiles of 128 outputs as lanes by 16 to
 // 128 rows as columns, with the inputs split over a cluster: all SMs stream the weight at the memory's rate, and the
 // partial sums meet through distributed shared memory, in the order of the ranks.
+//
+// 8,191 rows of 4,096 -> 12,288: 394 us in short runs (2,090 TFLOP/s), 427 to 436 back to back, where the power cap
+// holds the clock near 1.48 GHz. A block takes a pair some 930 clocks, its products 512: the way from the products' end
+// to the sums' warps, through their loads and back is longer than the other buffer's products, and two buffers fill TMEM.
+// (Halves of 128 outputs with four buffers, one CTA to a tile of 128 x 256, and sixteen warps for the sums were slower.)
+// 32 rows of 4,096 -> 4,096: 8.1 us, one of 11,264 -> 4,096 11.7 (3.9 TB/s of weight): a launch, the first loads and the
+// exchange take 4 to 5 us of both.
 #include "capi_internal.cuh"
 #include "ctmr_b200.h"
 #include "eight_bit.cuh"
