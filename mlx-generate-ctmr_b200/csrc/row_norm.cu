@@ -196,16 +196,20 @@ cudaError_t launch_rows(const RowNormParams& p, cudaStream_t stream) {
   const int groups = (p.channels + kScaleGroup - 1) / kScaleGroup;
   // Lanes to a row: 8, 16 or 32 of a warp, two groups to eight lanes up to 1,024 channels; with few rows a block of one
   // group to eight lanes even there (1,777 rows of 1,001 fp32 channels 7.4 us, by warps 10.7; 300 of 1,024 in bf16 2.8
-  // and 3.6; 20,000 rows keep all warps busy either way). Longer rows: blocks that go on from row to row once there
-  // are more rows than resident blocks (8,192 rows of 4,096: 49 us; a block to each row 57).
+  // and 3.6; 20,000 rows keep all warps busy either way). Longer rows: blocks that go on from row to row, of up
+  // to 128 registers, where these fill their SMs and accesses are wide (8,192 rows of 4,096: 49 us, a block of 64
+  // registers to each row 57; of 4,224, whose 288 threads fit once: 90 and 68; of 4,097: 190 and 146), or where there
+  // are few rows and a row's own time counts (1,777 rows of 1,001: 7.4 and 10.5; 600 of 2,048: 4.0 and 4.4).
   auto grid = [&](int lanes) { return (rows * lanes + 255) / 256; };
   if (groups == 1) return launch<T, 1, 8, false, EIGHT>(p, wide, grid(8), 256, stream);
   if (groups == 2) return launch<T, 1, 16, false, EIGHT>(p, wide, grid(16), 256, stream);
   if (groups <= 4) return launch<T, 1, 32, false, EIGHT>(p, wide, grid(32), 256, stream);
   if (groups <= 8 && rows > 16 * device_sm_count()) return launch<T, 2, 32, false, EIGHT>(p, wide, grid(32), 256, stream);
   auto threads = [&](int v) { return (groups + 4 * v - 1) / (4 * v) * 32; };
-  const long long resident = static_cast<long long>(device_sm_count()) * (512 / threads(1));  // at 128 registers
-  if (threads(1) <= 512 && rows > resident) return launch<T, 1, 0, true, EIGHT>(p, wide, resident, threads(1), stream);
+  const int at_once = 512 / threads(1);  // blocks on an SM at 128 registers
+  const long long resident = static_cast<long long>(device_sm_count()) * at_once;
+  if (threads(1) <= 512 && (rows <= 2 * resident || (wide && at_once * threads(1) >= 448)))
+    return launch<T, 1, 0, true, EIGHT>(p, wide, rows < resident ? rows : resident, threads(1), stream);
   if (threads(1) <= 512) return launch<T, 1, 0, false, EIGHT>(p, wide, rows, threads(1), stream);
   return launch<T, 2, 0, false, EIGHT>(p, wide, rows, threads(2), stream);
 }

@@ -350,6 +350,42 @@ def test_linear_strides(rows):
         assert (room[:, :3] == 7).all() and (room[:, 3 + outer:] == 7).all()
 
 
+@pytest.mark.parametrize("rows", [3, 700])
+def test_linear_one_scale_for_all(rows):
+    """A scale for a whole tensor, or for a whole row, expanded."""
+    from ctmr_b200 import ops
+
+    gen = _gen(rows)
+    x, w = _rows8(gen, rows, 640), _weight8(gen, 300, 640)
+    x = ops.ScaledRows(x.values, x.scale[:, :1].expand(rows, 5))
+    w = ops.ScaledWeight(w.values, w.scale[:1, :1].expand(3, 5))
+    _check_linear(ops.scaled_linear(x, w, out_dtype=torch.float32), x, w, None)
+
+
+def test_calls_on_two_streams_at_once():
+    """Each call by itself: nothing is shared between them."""
+    from ctmr_b200 import ops
+
+    gen = _gen(21)
+    cases = [(_randn(gen, 600, 2048, dtype=torch.bfloat16), _weight8(gen, 1000, 2048)) for _ in range(2)]
+
+    def chain(x, w):
+        y, h = ops.rms_norm(x, residual=x, quantize=True)
+        return ops.scaled_linear(y, w), ops.scaled_linear(ops.ScaledRows(y.values[:9], y.scale[:9]), w), h
+
+    alone = [chain(*c) for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        both = []
+        for s, c in zip(streams, cases):
+            with torch.cuda.stream(s):
+                both.append(chain(*c))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for p, q in zip(alone, both) for a, b in zip(p, q))
+    _no_device_error()
+
+
 @pytest.mark.parametrize("rows", [1, 40, 200, 1500])
 def test_linear_not_finite(rows):
     """A NaN or an infinity in a row or in an output's weights stays there; rows' padding is never read."""
