@@ -252,6 +252,14 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
+__device__ __forceinline__ double max_nan(double a, double b) { return a >= b || a != a ? a : b; }
+
+// The least of three numbers; NaN is none.
+__device__ __forceinline__ float min3(float a, float b, float c) {
+  float r;
+  asm("min.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 
 // Two values as e4m3 bytes, to nearest, ties to even, at most 448; the first in the low byte.
 __device__ __forceinline__ uint32_t e4m3x2(float a, float b) {
@@ -286,30 +294,41 @@ __device__ __forceinline__ float power_of_two(int k) { return __uint_as_float(st
 // Rounds a group of channels, held by eight lanes of a warp all of whose lanes call this. UNITS: how many roundings
 // the values are off by at most, the one of scaling them here included; 0: they are as they are meant. `top64()` gives
 // the largest magnitude of the lane's values in 64 bits. Gives the 16 bytes, the scale and its inverse, and returns (bit
-// i: value i) which values 64 bits have to decide.
-template <int UNITS, typename Top>
-__device__ __forceinline__ uint32_t quantize_group(const float (&v)[kEach], Top top64, uint32_t (&q)[4], float& scale,
+// i: value i) which values 64 bits have to decide. FAR: a lane that is `far` does not have its values; 64 bits decide its
+// whole group, and one whose values left 32 bits' range.
+template <int UNITS, bool FAR, typename Top>
+__device__ __forceinline__ uint32_t quantize_group(const float (&v)[kEach], bool far, Top top64, uint32_t (&q)[4], float& scale,
                                                    float& by) {
   constexpr float kLow = 1.f - UNITS * kUnit, kHigh = 1.f + 2 * ((UNITS + 1) / 2) * kUnit;
+  const float nan = __int_as_float(0x7fc00000);
   float top = max_nan(v[0], v[1], v[2]);
 #pragma unroll
   for (int i = 3; i + 1 < kEach; i += 2) top = max_nan(top, v[i], v[i + 1]);
   top = max_nan(top, v[kEach - 1], 0.f);
+  if (FAR && far) top = nan;
 #pragma unroll
   for (int i = kGroupLanes / 2; i > 0; i /= 2) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, i));
   int k = scale_power(top);
   if constexpr (UNITS > 0) {
     const int low = scale_power(top * kLow);
     k = scale_power(top * kHigh);
-    if (k != low && is_finite(top)) {
+    if (FAR ? k != low || !is_finite(top) : k != low && is_finite(top)) {
       double most = top64();
 #pragma unroll
       for (int i = kGroupLanes / 2; i > 0; i /= 2)
-        most = fmax(most, __shfl_xor_sync(0xffu << (threadIdx.x & 24), most, i));
-      if (most <= ldexp(448.0, low)) k = low;
+        most = max_nan(most, __shfl_xor_sync(0xffu << (threadIdx.x & 24), most, i));
+      if (!FAR || is_finite(top)) {
+        if (most <= ldexp(448.0, low)) k = low;
+      } else if (most <= 448.0 * 0x1p127) {  // (an infinity's or a NaN's group stays as it is)
+        int exponent;
+        const double fraction = frexp(most, &exponent);  // 448 is 0.875 * 2^9
+        k = max(most == 0.0 ? -100 : exponent - 9 + (fraction > 0.875), -100);
+        scale = power_of_two(k), by = ldexpf(1.f, -k);
+        e4m3x16(q, v, 0.f);
+        return 0xffffu;
+      }
     }
   }
-  const float nan = __int_as_float(0x7fc00000);
   scale = is_finite(top) ? power_of_two(k) : nan;
   by = is_finite(top) ? power_of_two(-k) : nan;
   uint32_t differ = 0;

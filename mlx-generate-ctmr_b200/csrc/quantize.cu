@@ -5,7 +5,7 @@
 // some 25 instructions a channel: silu is one exponential and one reciprocal, with the exponent's product taken
 // in two parts so that the error stays near 2^-22 for any size of a. Groups of 128 channels, eight lanes each, follow one
 // another over the rows without regard to where a row ends, so that no size leaves threads idle. 8,192 gated rows of
-// 11,264: 87 us, 5.3 TB/s (84 without the 64-bit decisions); what is left are instructions, 24 a channel.
+// 11,264: 87 to 90 us, 5.2 TB/s (3 less without the 64-bit decisions); what is left are instructions, 24 a channel.
 #include "capi_internal.cuh"
 #include "ctmr_b200.h"
 #include "eight_bit.cuh"
@@ -16,11 +16,15 @@ namespace {
 
 constexpr int kThreads = 256, kBlocks = 3, kGroups = kThreads / kGroupLanes;
 
-// silu(a) b, two at a time. e^-a is infinite below -88, and the product then zero: below what any scale keeps.
+// Below this silu(a) nears the end of 32 bits' normal numbers, from where a large b can bring it back: groups that hold
+// such an a are computed in 64 bits. (Activations hardly ever do.)
+constexpr float kFarGate = -86.f;
+
+// silu(a) b, two at a time, for a from kFarGate on. The reciprocal meets b first: a may be subnormal, and then b large.
 __device__ __forceinline__ float2 gated2(float2 a, float2 b) {
   constexpr float kLog2E = 1.44269504f, kRest = 1.92596299e-8f;
   // Further out nothing changes, but the product would overflow.
-  const float2 n = make_float2(fminf(fmaxf(-a.x, -128.f), 128.f), fminf(fmaxf(-a.y, -128.f), 128.f));
+  const float2 n = make_float2(fmaxf(-a.x, -128.f), fmaxf(-a.y, -128.f));
   const float2 log2e = make_float2(kLog2E, kLog2E), minus = make_float2(-kLog2E, -kLog2E);
   const float2 t = mul2(n, log2e);
   // What t's rounding cut off, with the other sign, times ln 2: e^n = 2^t (1 - rest).
@@ -33,7 +37,7 @@ __device__ __forceinline__ float2 gated2(float2 a, float2 b) {
   const float2 d = fma2(e, less, one);
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.x) : "f"(d.x));
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.y) : "f"(d.y));
-  return mul2(mul2(a, r), b);
+  return mul2(mul2(b, r), a);
 }
 
 // In units of 2^-24: the exponential's approximation 4 and its correction 1, the sum 1, the reciprocal 2, the three
@@ -48,7 +52,7 @@ __device__ __noinline__ double gated_top(const T* x, int channels, int group, in
   double most = 0.0;
   for (int i = 0; i < kEach; ++i) {
     const int c = channel_of<WIDE>(group, lane8, i);
-    if (c < channels) most = fmax(most, fabs(gated64(to_float(x[c]), to_float(x[channels + c]))));
+    if (c < channels) most = max_nan(most, fabs(gated64(to_float(x[c]), to_float(x[channels + c]))));
   }
   return most;
 }
@@ -58,7 +62,7 @@ __device__ __noinline__ void gated_patch(const T* x, uint8_t* values, int channe
                                          float by) {
   for (; differ != 0; differ &= differ - 1) {
     const int c = channel_of<WIDE>(group, lane8, __ffs(differ) - 1);
-    values[c] = static_cast<uint8_t>(e4m3_exact(gated64(to_float(x[c]), to_float(x[channels + c])) * by));
+    if (c < channels) values[c] = static_cast<uint8_t>(e4m3_exact(gated64(to_float(x[c]), to_float(x[channels + c])) * by));
   }
 }
 
@@ -83,16 +87,20 @@ __global__ void __launch_bounds__(kThreads, kBlocks) quantize_kernel(const __gri
     const bool in = row < rows;
     const uint32_t row_now = in ? row : 0, group_now = group;
     const int channels = in ? p.channels : 0;
+    const T* x = static_cast<const T*>(p.x) + row_now * p.x_stride;
     float v[kEach];
+    bool far = false;
     a.values(v, channels, group, lane8);
     if constexpr (GATE) {
-      float other[kEach];
+      float other[kEach], least = 0.f;
       b.values(other, channels, group, lane8);
 #pragma unroll
       for (int e = 0; e < kEach; e += 2) {
+        least = min3(least, v[e], v[e + 1]);
         const float2 g = gated2(make_float2(v[e], v[e + 1]), make_float2(other[e], other[e + 1]));
         v[e] = g.x, v[e + 1] = g.y;
       }
+      far = least < kFarGate;
     }
     if (in) {  // (a row past the end stays where it is)
       row += p.skip_rows, group += p.skip_groups;
@@ -101,12 +109,11 @@ __global__ void __launch_bounds__(kThreads, kBlocks) quantize_kernel(const __gri
     load();  // the next group, on its way while this one is rounded
     uint32_t q[4];
     float scale, by;
-    const T* x = static_cast<const T*>(p.x) + row_now * p.x_stride;
     uint8_t* values = static_cast<uint8_t*>(p.values) + row_now * p.values_stride;
-    const uint32_t differ = quantize_group<GATE ? kGatedUnits : 0>(
-        v, [&]() { return gated_top<T, WIDE>(x, p.channels, group_now, lane8); }, q, scale, by);
+    const uint32_t differ = quantize_group<GATE ? kGatedUnits : 0, GATE>(
+        v, far, [&]() { return gated_top<T, WIDE>(x, channels, group_now, lane8); }, q, scale, by);
     store_bytes<WIDE>(values, channels, group_now, lane8, q);
-    if (differ != 0) gated_patch<T, WIDE>(x, values, p.channels, group_now, lane8, differ, by);
+    if (differ != 0) gated_patch<T, WIDE>(x, values, channels, group_now, lane8, differ, by);
     if (lane8 == 0 && in) p.scale[row_now * p.scale_row + group_now * p.scale_group] = scale;
   }
 }

@@ -148,7 +148,7 @@ __global__ void __launch_bounds__(LANES ? 256 : LOOP ? 512 : 1024, 1) row_norm_k
           return most;
         };
         // From registers: a reload would keep the warp, and the block that waits for it, some microseconds.
-        uint32_t differ = quantize_group<kNormUnits>(s, top64, q, scale, by8);
+        uint32_t differ = quantize_group<kNormUnits, false>(s, false, top64, q, scale, by8);
 #pragma unroll 1
         for (; differ != 0; differ &= differ - 1) {
           const int e = __ffs(differ) - 1, bit = (e & 3) * 8;

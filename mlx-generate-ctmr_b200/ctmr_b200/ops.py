@@ -914,7 +914,7 @@ def quantize_rows(x: torch.Tensor, *, gate: bool = False) -> ScaledRows:
 
     ``x`` is ``(rows, channels)`` in fp32, bf16 or fp16, any stride over rows; with ``gate`` ``(rows, 2 * channels)``,
     and what is rounded is ``silu(x[:, :channels]) * x[:, channels:]``. The bytes are those that the formula in 64
-    bits rounds to. A group that holds an infinity or a NaN becomes NaN as a whole.
+    bits rounds to. A group that holds an infinity, a NaN or a product past 448 * 2^127 becomes NaN as a whole.
     """
     code = _FLOAT_CODES.get(x.dtype)
     if x.dim() != 2 or code is None:
