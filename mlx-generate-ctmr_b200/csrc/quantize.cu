@@ -16,9 +16,9 @@ namespace {
 
 constexpr int kThreads = 256, kBlocks = 3, kGroups = kThreads / kGroupLanes;
 
-// Below this silu(a) nears the end of 32 bits' normal numbers, from where a large b can bring it back: groups that hold
-// such an a are computed in 64 bits. (Activations hardly ever do.)
-constexpr float kFarGate = -86.f;
+// Below this silu(a) nears the end of 32 bits' normal numbers, from where a large b can bring it back: groups that hold both
+// at once are computed in 64 bits. (Up to 128, b leaves less than 2^-110, half the least step of the least scale.)
+constexpr float kFarGate = -86.f, kFarOther = 128.f;
 
 // silu(a) b, two at a time, for a from kFarGate on. The reciprocal meets b first: a may be subnormal, and then b large.
 __device__ __forceinline__ float2 gated2(float2 a, float2 b) {
@@ -95,12 +95,18 @@ __global__ void __launch_bounds__(kThreads, kBlocks) quantize_kernel(const __gri
       float other[kEach], least = 0.f;
       b.values(other, channels, group, lane8);
 #pragma unroll
+      for (int e = 0; e < kEach; e += 2) least = min3(least, v[e], v[e + 1]);
+      if (__any_sync(0xffffffffu, least < kFarGate)) {  // (ahead of the products, after which b would have to be kept)
+        float most = 0.f;
+#pragma unroll
+        for (int e = 0; e < kEach; e += 2) most = max_nan(most, other[e], other[e + 1]);
+        far = least < kFarGate && !(most <= kFarOther);
+      }
+#pragma unroll
       for (int e = 0; e < kEach; e += 2) {
-        least = min3(least, v[e], v[e + 1]);
         const float2 g = gated2(make_float2(v[e], v[e + 1]), make_float2(other[e], other[e + 1]));
         v[e] = g.x, v[e + 1] = g.y;
       }
-      far = least < kFarGate;
     }
     if (in) {  // (a row past the end stays where it is)
       row += p.skip_rows, group += p.skip_groups;
