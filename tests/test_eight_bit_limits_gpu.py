@@ -1,15 +1,22 @@
 """The 8-bit row operators at the edges of what they accept and in every form that their launchers choose, against plain
 implementations in 64 bits.
 
-Tolerances. 8-bit rows as in test_eight_bit_gpu, the bytes those of the 64-bit formula everywhere:
+Tolerances. Norms and 8-bit rows as in test_eight_bit_gpu, the bytes those of the 64-bit formula everywhere:
 ``step / 2 + 2^-40 |v|``.
+
+Products, in the 2-norm: sums in TMEM take four instructions a block of 128 inputs, each off by at most 2^-23 of the
+running sum (a truncation), and after b of B blocks the sum in registers is rounded by 2^-24 of itself. With operands of
+random signs a running sum grows as the square root of its terms and the errors of different blocks are independent, so
+the squares add up: (B / 2) 2^-48 from the registers and (1 + 2 + 3 + 4) / 4 * 2^-46 from TMEM:
+``2^-24 sqrt(B / 2 + 10) ||y||``. fp32's bias addition adds 2^-24 |y| at most. A single row or column: twice that.
 """
 
 from __future__ import annotations
 
 import pytest
 import torch
-from test_eight_bit_gpu import TYPES, _check_rows, _gate_ref, _gen, _no_device_error, _randn
+from test_eight_bit_gpu import (TYPES, U, _check_rows, _gate_ref, _gen, _linear_ref, _no_device_error, _norm_ref, _randn,
+                                _rows8, _weight8, _within)
 
 pytestmark = pytest.mark.gpu
 
@@ -78,3 +85,109 @@ def test_gates_past_32_bits(dtype):
         bad = torch.isnan(back[row])
         assert bad[group * 128:(group + 1) * 128].all() and bad.sum() == min(128, 600 - group * 128)
         assert torch.isnan(got.scale[row]).sum() == 1
+
+
+# ---------------------------------------------------------------------------------------------- norm
+def _check(x, weight, residual, quantize, **kw):
+    from ctmr_b200 import ops
+
+    ref = _norm_ref(x, residual, weight, 1e-6)
+    total = None if residual is None else (x.float() + residual.float()).to(x.dtype)
+    y = ops.rms_norm(x, weight, residual=residual, quantize=quantize, **kw)
+    if residual is not None:
+        y, h = y
+        assert torch.equal(h, total)
+    if quantize:
+        _check_rows(y, ref)
+    else:
+        _within(y, ref, (U[x.dtype] + 2.0 ** -21) * ref.abs() + 2.0 ** -25)
+    _no_device_error()
+
+
+def _resident(channels):
+    """Blocks of a row that are resident at once: 512 threads to an SM, 32 to 512 channels of the row each warp."""
+    threads = ((channels + 127) // 128 + 3) // 4 * 32
+    return torch.cuda.get_device_properties(0).multi_processor_count * (512 // threads)
+
+
+# Blocks that go on from row to row (over several turns, the last one not full; with few rows of an odd width), two groups
+# of channels to eight lanes of a warp, and a block to each row.
+FORMS = [(2048, "3 turns"), (4096, "3 turns"), (1001, "1.5 turns"), (1000, "warps"), (1024, "warps"), (4097, "2 turns"),
+         (4224, "2 turns")]
+
+
+def _rows(channels, form):
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    if form == "warps":
+        return 16 * sms + 301
+    return int(float(form.split()[0]) * _resident(channels)) + 77 * (form != "1.5 turns")
+
+
+@pytest.mark.parametrize("quantize", [False, True])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize(("channels", "form"), FORMS)
+def test_norm_of_many_rows(channels, form, dtype, quantize):
+    gen = _gen(channels)
+    rows = _rows(channels, form)
+    x, residual = _randn(gen, rows, channels, dtype=dtype, std=3.0), _randn(gen, rows, channels, dtype=dtype)
+    weight = 1.0 + _randn(gen, channels, std=0.2)
+    _check(x, weight, residual, quantize)
+    _check(x, weight.to(dtype), None, quantize)
+    _check(x, None, None, quantize)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("over", ["x", "residual", "y"])
+def test_norm_of_many_rows_in_place(dtype, over):
+    """The next row's loads are ahead of this row's stores: they are another row's."""
+    gen = _gen(41)
+    rows, channels = _rows(2048, "3 turns"), 2048
+    weight = 1.0 + _randn(gen, channels, std=0.2)
+    for quantize in (False, True):
+        if over == "y" and quantize:
+            continue
+        x, residual = _randn(gen, rows, channels, dtype=dtype), _randn(gen, rows, channels, dtype=dtype)
+        # (the reference is taken before the call)
+        _check(x, weight, residual, quantize, **(dict(out=x) if over == "y" else dict(sum_out=x if over == "x" else residual)))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_norm_of_many_heads(dtype):
+    """Heads of a fused projection, more than are resident at once, in both orders of rows."""
+    from ctmr_b200 import ops
+
+    gen = _gen(42)
+    dim, heads = 2048, 5
+    tokens = _resident(dim) * 2 // heads + 13
+    weight = 1.0 + _randn(gen, dim, std=0.2)
+    wide = _randn(gen, tokens, heads + 2, dim, dtype=dtype)
+    before = wide.clone()
+    view = wide[:, 1:1 + heads]
+    ref = _norm_ref(view, None, weight, 1e-6)
+    assert ops.rms_norm(view, weight, out=view) is view
+    _within(view, ref, (U[dtype] + 2.0 ** -21) * ref.abs() + 2.0 ** -25)
+    assert torch.equal(wide[:, :1], before[:, :1]) and torch.equal(wide[:, 1 + heads:], before[:, 1 + heads:])
+    x, residual = _randn(gen, heads, tokens, dim, dtype=dtype).transpose(0, 1), before[:, :heads]
+    _check(x, weight, residual, False)
+
+
+# ---------------------------------------------------------------------------------------------- product
+@pytest.mark.parametrize(("rows", "inner", "outer"), [(1, 11264, 512), (16, 4096, 300), (32, 1024, 1536), (100, 2000, 512),
+                                                      (128, 4096, 384), (617, 512, 1536), (1500, 4096, 777), (2300, 11264, 512)])
+@pytest.mark.parametrize("bias", [False, True])
+def test_products_are_summed_in_32_bits(rows, inner, outer, bias):
+    from ctmr_b200 import ops
+
+    gen = _gen(rows + inner + outer)
+    x, w = _rows8(gen, rows, inner), _weight8(gen, outer, inner)
+    bias = _randn(gen, outer, std=0.5) if bias else None
+    ref, _ = _linear_ref(x, w, bias)
+    err = ops.scaled_linear(x, w, bias, out_dtype=torch.float32).double() - ref
+    bound = 2.0 ** -24 * (((inner + 127) // 128 / 2 + 10) ** 0.5 + (bias is not None))
+    assert err.norm() <= bound * ref.norm()
+    for dim in (0, 1):
+        # (a line's products are as large as x's and w's; its sums may have come out small)
+        size = torch.linalg.vector_norm(ref, dim=dim)
+        usual = ref.norm() / ref.numel() ** 0.5 * ref.shape[dim] ** 0.5
+        assert (torch.linalg.vector_norm(err, dim=dim) <= 2 * bound * torch.maximum(size, usual)).all()
+    _no_device_error()
