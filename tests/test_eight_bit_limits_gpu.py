@@ -88,12 +88,12 @@ def test_gates_past_32_bits(dtype):
 
 
 # ---------------------------------------------------------------------------------------------- norm
-def _check(x, weight, residual, quantize, **kw):
+def _check(x, weight, residual, quantize, eps=1e-6, **kw):
     from ctmr_b200 import ops
 
-    ref = _norm_ref(x, residual, weight, 1e-6)
+    ref = _norm_ref(x, residual, weight, eps)
     total = None if residual is None else (x.float() + residual.float()).to(x.dtype)
-    y = ops.rms_norm(x, weight, residual=residual, quantize=quantize, **kw)
+    y = ops.rms_norm(x, weight, residual=residual, eps=eps, quantize=quantize, **kw)
     if residual is not None:
         y, h = y
         assert torch.equal(h, total)
@@ -169,6 +169,51 @@ def test_norm_of_many_heads(dtype):
     assert torch.equal(wide[:, :1], before[:, :1]) and torch.equal(wide[:, 1 + heads:], before[:, 1 + heads:])
     x, residual = _randn(gen, heads, tokens, dim, dtype=dtype).transpose(0, 1), before[:, :heads]
     _check(x, weight, residual, False)
+
+
+def _near_ties(h, width, eps):
+    """Weights that bring h / sqrt(mean(h^2) + eps) as near to ties between e4m3 values as 32 bits allow."""
+    y = h / torch.sqrt(h.square().mean() + eps)
+    return (((torch.arange(width, device="cuda") % 8 * 2 + 17) / 16).double() / y).float()
+
+
+@pytest.mark.parametrize("channels", [128, 512, 1001, 2048, 9000])
+def test_norm_keeps_what_the_sum_in_32_bits_cuts_off(channels):
+    """fp32: a residual that the 32-bit sum loses, the same way in every channel: 64 bits of x + residual decide."""
+    gen = _gen(51)
+    eps = 2.0 ** -20  # (a number of fp32: it decides some of these rows alone)
+
+    def check(x, residual):
+        weight = _near_ties(x[0].double() + residual[0].double(), channels, eps)
+        _check(x.expand(3, -1).contiguous(), weight, residual.expand(3, -1).contiguous(), True, eps)
+
+    x = 1 + torch.randint(120, (1, channels), generator=gen, device="cuda") / 128
+    for factor in (1.0, -1.0, 2.0 ** 60, 2.0 ** 120, 2.0 ** -18):
+        check(x * abs(factor), torch.full_like(x, factor * 0.7 * 2.0 ** -24))
+    # one such channel among ordinary ones, and the two tensors the other way round
+    residual = _randn(gen, 1, channels)
+    residual[0, channels // 3] = 2.0 ** -24
+    check(x, residual)
+    check(residual, x)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_norm_of_not_finite_sums(dtype):
+    """An infinity's own group is NaN, the rest of its row zero, whichever tensor it is in; a NaN's row is NaN."""
+    from ctmr_b200 import ops
+
+    gen = _gen(52)
+    x, residual = _randn(gen, 6, 700, dtype=dtype), _randn(gen, 6, 700, dtype=dtype)
+    good = ops.rms_norm(x, residual=residual, quantize=True)[0].float()
+    x[1, 300], residual[2, 300], x[3, 5], residual[3, 5] = float("inf"), -float("inf"), float("inf"), 1.0
+    x[4, 9] = float("nan")
+    got = ops.rms_norm(x, residual=residual, quantize=True)[0].float()
+    for row, start in ((1, 256), (2, 256), (3, 0)):
+        inside = torch.zeros(700, dtype=torch.bool, device="cuda")
+        inside[start:start + 128] = True
+        assert torch.isnan(got[row, inside]).all() and (got[row, ~inside] == 0).all()
+    assert torch.isnan(got[4]).all()
+    assert torch.equal(got[[0, 5]], good[[0, 5]])
 
 
 # ---------------------------------------------------------------------------------------------- product
