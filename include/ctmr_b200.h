@@ -403,9 +403,12 @@ CTMR_API int ctmr_attention(const ctmr_attention_desc* desc, void* stream);
 
 /* Root-mean-square norm of rows: h = x + residual, y = h / sqrt(mean(h^2) + eps) * weight, and h itself,
  * rounded to x's type, in `sum`. A row is (token, head): heads is 1 for (tokens, channels). y is of x's
- * type, or in 8 bits where scale is not NULL (heads must then be 1). The norm is taken of the unrounded
- * h; squares are added in 64 bits. sum may be x or residual, and y of x's type may be x or residual (not
- * sum); other overlaps are not allowed. */
+ * type, or in 8 bits where scale is not NULL (heads must then be 1). The norm is taken of h before it is
+ * rounded to x's type; squares are added in 64 bits. Of 16-bit x, h is the sum in fp32, exact unless one term is
+ * 2^13 times the other; past fp32's range it is an infinity. The bytes are exact for rows of a root mean square
+ * up to 2^126 and weights up to 2^15; beyond, values within 2^-20 of a tie may fall to either side, and what
+ * h / sqrt(...) has below 2^-126 is lost. sum may be x or residual, and y of x's type may be x or residual
+ * (not sum); other overlaps are not allowed. */
 typedef struct ctmr_rms_norm_desc {
   const void* x;                   /* [token][head][channels], channels contiguous */
   const void* residual;            /* like x, or NULL */

@@ -16,7 +16,8 @@
 namespace ctmr {
 namespace {
 
-// In units of 2^-24: the sum, the factor, two products and the scaling.
+// In units of 2^-24: the sum, the factor, two products and the scaling. (The factor is a normal number for rows of a root
+// mean square up to 2^126; h times it may be none, but only weights above 2^15 bring such a value back to what is kept.)
 constexpr int kNormUnits = 6;
 
 // What the squares of h lack of those of h + low, but for 2^-44 of them. In 32 bits, which cost a row of 4,096 fp32
@@ -47,7 +48,8 @@ __device__ __forceinline__ double squares_rest(const float (&h)[V][kEach], const
 template <typename T, int V, int LANES, bool LOOP, bool EIGHT, bool WIDE>
 __global__ void __launch_bounds__(LANES ? 256 : LOOP ? 512 : 1024, 1) row_norm_kernel(const __grid_constant__ RowNormParams p) {
   constexpr bool BLOCK = LANES == 0;
-  // Sums of 16-bit numbers are exact in 32 bits but where one is 2^13 times the other; 32-bit ones keep the rest.
+  // Sums of 16-bit numbers are exact in 32 bits but where one is 2^13 times the other, and h is then that sum; 32-bit
+  // ones keep the rest.
   constexpr bool kLow = EIGHT && sizeof(T) == 4;
   __shared__ double part[2][BLOCK ? 32 : 1];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, lane8 = lane & 7;

@@ -861,7 +861,9 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor | None = None, *, residual: t
     ``(tokens, heads, channels)`` in fp32, bf16 or fp16, up to 32,768 channels, any strides over rows; ``weight``
     ``(channels,)`` in fp32 or x's type. Returns ``y`` of x's type, or as ``ScaledRows`` with ``quantize`` (two
     dimensions; the bytes that the formula in 64 bits rounds to); with a residual ``(y, h)``, h rounded to x's type.
-    The norm is taken of the unrounded sum; ``eps`` is an fp32 number. ``sum_out`` may be ``x`` or ``residual``, and so may ``out``.
+    The norm is taken of the unrounded sum (of 16-bit x: the sum in fp32, exact unless one term is 2^13 times the
+    other); ``eps`` is an fp32 number. The bytes are exact for rows of a root mean square up to 2^126 and weights up
+    to 2^15. ``sum_out`` may be ``x`` or ``residual``, and so may ``out``.
     """
     dtype, dims, shape = x.dtype, x.dim(), x.shape
     code = _FLOAT_CODES.get(dtype)

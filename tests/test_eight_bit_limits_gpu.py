@@ -174,7 +174,7 @@ def test_norm_of_many_heads(dtype):
 def _near_ties(h, width, eps):
     """Weights that bring h / sqrt(mean(h^2) + eps) as near to ties between e4m3 values as 32 bits allow."""
     y = h / torch.sqrt(h.square().mean() + eps)
-    return (((torch.arange(width, device="cuda") % 8 * 2 + 17) / 16).double() / y).float()
+    return (((torch.arange(width, device="cuda") % 8 * 2 + 17) / 16).double() / torch.where(y == 0, 1.0, y)).float()
 
 
 @pytest.mark.parametrize("channels", [128, 512, 1001, 2048, 9000])
@@ -214,6 +214,52 @@ def test_norm_of_not_finite_sums(dtype):
         assert torch.isnan(got[row, inside]).all() and (got[row, ~inside] == 0).all()
     assert torch.isnan(got[4]).all()
     assert torch.equal(got[[0, 5]], good[[0, 5]])
+
+
+@pytest.mark.parametrize("channels", [128, 512, 1001, 2048, 9000])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_norm_of_16_bit_rows_is_of_the_sum_in_32_bits(dtype, channels):
+    from ctmr_b200 import ops
+
+    gen = _gen(53)
+    eps = 2.0 ** -20
+    x = (1 + torch.randint(120, (1, channels), generator=gen, device="cuda") / 128).to(dtype)
+    one = _randn(gen, 1, channels, dtype=dtype)
+    one[0, channels // 3] = 2.0 ** -24
+    for residual in (torch.full_like(x, 2.0 ** -24), torch.full_like(x, -(2.0 ** -24)), one):
+        h = (x.float() + residual.float()).double()
+        weight = _near_ties(h[0], channels, eps)
+        y, total = ops.rms_norm(x.expand(3, -1), weight, residual=residual.expand(3, -1), eps=eps, quantize=True)
+        assert torch.equal(total, h.to(dtype).expand(3, -1))
+        _check_rows(y, _norm_ref(h.expand(3, -1), None, weight, eps))
+
+
+@pytest.mark.parametrize("quantize", [False, True])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("channels", [96, 512, 2048])
+def test_norm_of_rows_near_the_largest_number(channels, dtype, quantize):
+    """One over the root is below 32 bits' normal numbers, off by up to 2^-22: bytes are right but within 2^-20 of a tie."""
+    from ctmr_b200 import ops
+
+    x = ((torch.rand((3, channels), generator=_gen(61), device="cuda") * 2 - 1) * 3.3e38).to(dtype)
+    ref = _norm_ref(x, None, None, 1e-6)
+    y = ops.rms_norm(x, quantize=quantize)
+    if quantize:
+        _check_rows(y, ref, 2.0 ** -20)
+    else:
+        _within(y, ref, (U[dtype] + 2.0 ** -20) * ref.abs())
+    _no_device_error()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_norm_of_small_values_under_large_weights(dtype):
+    """Groups far below their row's size, brought back by weights of 2^15."""
+    gen = _gen(62)
+    x = _randn(gen, 20, 640)
+    x[:, 128:] *= torch.exp2(torch.linspace(-90.0, -132.0, 20, device="cuda"))[:, None]
+    weight = torch.where(_randn(gen, 640) > 0, 2.0 ** 15, -(2.0 ** 15))
+    _check(x.to(dtype), weight, None, True)
+    _check(x.to(dtype), weight, torch.zeros_like(x, dtype=dtype), True)
 
 
 # ---------------------------------------------------------------------------------------------- product
