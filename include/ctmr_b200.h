@@ -399,7 +399,7 @@ CTMR_API int ctmr_attention(const ctmr_attention_desc* desc, void* stream);
  * scale of a group is the least power of two 2^k, k >= -100, with which its largest magnitude is at most
  * 448, and value = e4m3(v / scale) to nearest, ties to even: the bytes of v's formula in 64 bits. A group that
  * holds an infinity, a NaN or a value past 448 * 2^127 (no scale of fp32 reaches further) becomes NaN as a whole.
- * Strides in elements (bytes for 8-bit values). */
+ * Strides in elements (bytes for 8-bit values); rows of inputs may overlap one another, rows of outputs not. */
 
 /* Root-mean-square norm of rows: h = x + residual, y = h / sqrt(mean(h^2) + eps) * weight, and h itself,
  * rounded to x's type, in `sum`. A row is (token, head): heads is 1 for (tokens, channels). y is of x's

@@ -18,7 +18,26 @@ bool aligned_to(const void* p, int dtype) {
   return reinterpret_cast<uintptr_t>(p) % (dtype == CTMR_DTYPE_F32 ? 4 : 2) == 0;
 }
 
+long long scale_groups(int channels) { return (channels + ctmr::kScaleGroup - 1LL) / ctmr::kScaleGroup; }
+
 bool stride_ok(long long s) { return s >= 0 && s < (1LL << 38); }
+
+// Whether rows of `width` elements at i a + j b, i < na and j < nb, lie apart from one another.
+bool rows_apart(long long na, long long a, long long nb, long long b, long long width) {
+  if (na > 1 && nb > 1 && a > b) return rows_apart(nb, b, na, a, width);
+  if (na > 1 && a < width) return false;
+  if (nb > 1 && b < width) return false;
+  if (na <= 1 || nb <= 1) return true;
+  const __int128 end = static_cast<__int128>(a) * (na - 1) + width;  // of j = 0
+  // Where rows of different j lie between one another, each j's start against its neighbours of j = 0.
+  __int128 at = b;
+  for (long long j = 1; j < nb && at < end; ++j, at += b) {
+    const __int128 i = at / a, after = (i + 1) * a - at;
+    if (i < na && at - i * a < width) return false;
+    if (i + 1 < na && after < width) return false;
+  }
+  return true;
+}
 
 int finish(cudaError_t e, const char* what) {
   return e == cudaSuccess ? CTMR_OK : api_fail(CTMR_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
@@ -51,6 +70,12 @@ int ctmr_rms_norm(const ctmr_rms_norm_desc* d, void* stream) {
       !aligned_to(d->weight, d->weight_dtype) || (d->scale == nullptr && !aligned_to(d->y, d->dtype)) ||
       !aligned_to(d->scale, CTMR_DTYPE_F32))
     return api_fail(CTMR_ERR_INVALID, "tensors must be aligned to their elements");
+  if (!rows_apart(d->tokens, d->y_token_stride, d->heads, d->y_head_stride, d->channels) ||
+      (d->sum != nullptr && !rows_apart(d->tokens, d->sum_token_stride, d->heads, d->sum_head_stride, d->channels)) ||
+      (d->scale != nullptr &&
+       !rows_apart(d->tokens, d->scale_token_stride, scale_groups(d->channels), d->scale_group_stride, 1)))
+    return api_fail(CTMR_ERR_INVALID, "rows of y, of sum or of scale overlap one another");
+  if (d->sum == d->y) return api_fail(CTMR_ERR_INVALID, "y and sum must be two tensors");
   ctmr::RowNormParams p{};
   p.x = d->x, p.residual = d->residual, p.weight = d->weight, p.y = d->y, p.sum = d->sum, p.scale = d->scale;
   p.x_token = strides[0], p.x_head = strides[1], p.r_token = strides[2], p.r_head = strides[3];
@@ -74,6 +99,9 @@ int ctmr_quantize_rows(const ctmr_quantize_rows_desc* d, void* stream) {
     return api_fail(CTMR_ERR_INVALID, "null x, values or scale");
   if (!aligned_to(d->x, d->dtype) || !aligned_to(d->scale, CTMR_DTYPE_F32))
     return api_fail(CTMR_ERR_INVALID, "tensors must be aligned to their elements");
+  if (!rows_apart(d->rows, d->values_stride, 1, 0, d->channels) ||
+      !rows_apart(d->rows, d->scale_row_stride, scale_groups(d->channels), d->scale_group_stride, 1))
+    return api_fail(CTMR_ERR_INVALID, "rows of values or of scale overlap one another");
   ctmr::QuantizeParams p{};
   p.x = d->x, p.values = d->values, p.scale = d->scale;
   p.x_stride = d->x_stride, p.values_stride = d->values_stride;

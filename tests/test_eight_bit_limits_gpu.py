@@ -262,6 +262,27 @@ def test_norm_of_small_values_under_large_weights(dtype):
     _check(x.to(dtype), weight, torch.zeros_like(x, dtype=dtype), True)
 
 
+def test_outputs_over_themselves_are_refused():
+    """Expanded tensors as outputs: x or residual itself, or one of the caller's."""
+    from ctmr_b200 import ops
+
+    gen = _gen(71)
+    x, one = _randn(gen, 6, 256), _randn(gen, 1, 256).expand(6, -1)
+    heads = _randn(gen, 6, 1, 256).expand(-1, 4, -1)
+    for call in (lambda: ops.rms_norm(x, residual=one, sum_out=one),
+                 lambda: ops.rms_norm(one, residual=x, sum_out=one),
+                 lambda: ops.rms_norm(one, out=one),
+                 lambda: ops.rms_norm(x, out=torch.empty(128 * 5 + 256, device="cuda").as_strided((6, 256), (128, 1))),
+                 lambda: ops.rms_norm(heads, out=heads)):
+        with pytest.raises(ValueError, match="overlap"):
+            call()
+    # as inputs they are fine, and one row or head may have any stride
+    _check(one, None, one, True)
+    _check(heads, None, heads, False)
+    y = torch.empty((1, 256), device="cuda").expand(1, -1)
+    assert ops.rms_norm(one[:1], out=y) is y
+
+
 # ---------------------------------------------------------------------------------------------- product
 @pytest.mark.parametrize(("rows", "inner", "outer"), [(1, 11264, 512), (16, 4096, 300), (32, 1024, 1536), (100, 2000, 512),
                                                       (128, 4096, 384), (617, 512, 1536), (1500, 4096, 777), (2300, 11264, 512)])
