@@ -815,9 +815,10 @@ def scale_weight(weight: torch.Tensor) -> ScaledWeight:
     if weight.dim() != 2 or not weight.is_floating_point() or min(weight.shape) < 1:
         raise ValueError(f"weight must be a (out, in) tensor; got {tuple(weight.shape)} {weight.dtype}")
     out, inner = weight.shape
-    if not torch.isfinite(weight).all():
-        raise ValueError("weight holds values that are not finite")
-    w = torch.nn.functional.pad(weight.detach().to(F32), (0, -inner % SCALE_GROUP, 0, -out % SCALE_GROUP))
+    w = weight.detach().to(F32)
+    if not torch.isfinite(w).all():
+        raise ValueError("weight holds values that are not finite in fp32")
+    w = torch.nn.functional.pad(w, (0, -inner % SCALE_GROUP, 0, -out % SCALE_GROUP))
     blocks = w.unflatten(1, (-1, SCALE_GROUP)).unflatten(0, (-1, SCALE_GROUP))
     top = blocks.abs().amax(dim=(1, 3))
     fraction, exponent = torch.frexp(top)  # 448 is 0.875 * 2^9

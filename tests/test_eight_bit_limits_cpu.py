@@ -1,13 +1,14 @@
-"""What the 8-bit row operators of the C ABI refuse about their outputs' rows: status codes, no CUDA call."""
+"""What the 8-bit row operators refuse about outputs, numbers and weights, without a CUDA call."""
 
 from __future__ import annotations
 
 import itertools
 
 import pytest
+import torch
 from test_eight_bit_cpu import INVALID, LIB, OK, _norm, _quantize
 
-from ctmr_b200 import _lib
+from ctmr_b200 import _lib, ops
 
 # A descriptor with rows that reaches every check, refused at its last one if at no other.
 REFUSED_LAST = dict(sum=0x4000, y=0x4000)
@@ -66,3 +67,23 @@ def test_no_rows_have_no_overlap():
     assert LIB.ctmr_rms_norm(_norm(tokens=0, y_token_stride=0), None) == OK
     assert LIB.ctmr_quantize_rows(_quantize(rows=0, values_stride=0), None) == OK
     assert _lib.LIB is LIB
+
+
+@pytest.mark.parametrize("value", [1e300, -3.5e38, float("nan"), float("inf")])
+def test_weights_past_fp32_are_refused(value):
+    weight = torch.ones((3, 5), dtype=torch.float64)
+    weight[1, 2] = value
+    with pytest.raises(ValueError):
+        ops.scale_weight(weight)
+
+
+def test_weights_of_every_type():
+    """A weight is taken in fp32: the largest numbers, e4m3's own, and none but zeros."""
+    big = torch.tensor([[3.4e38, 1.0, -3.4e38]], dtype=torch.float64)
+    got = ops.scale_weight(big)
+    assert got.scale.item() == 2.0 ** 120 and torch.equal(got.values.float(), torch.tensor([[256.0, 0.0, -256.0]]))
+    codes = torch.arange(256, dtype=torch.uint8).view(torch.float8_e4m3fn)
+    codes = codes[codes.float().isfinite()].view(2, 127)
+    got = ops.scale_weight(codes)
+    assert got.scale.item() == 1.0 and torch.equal(got.values.float(), codes.float())
+    assert (ops.scale_weight(torch.zeros((2, 300), dtype=torch.float16)).scale == 2.0 ** -100).all()
