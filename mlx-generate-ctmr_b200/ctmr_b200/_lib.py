@@ -308,11 +308,18 @@ class ScaledLinearDesc(ctypes.Structure):
 
 def _packer(desc: type[ctypes.Structure]):
     """``pack(*fields)``: the bytes of a descriptor (null pointers as 0), in a quarter of the time that the structure
-    takes: these calls are over before it is filled in."""
+    takes: these calls are over before it is filled in. Numbers that their fields do not hold are a ``ValueError``."""
     codes = {ctypes.c_void_p: "P", ctypes.c_int: "i", ctypes.c_longlong: "q", ctypes.c_float: "f"}
     packer = struct.Struct("@" + "".join(codes[t] for _, t in desc._fields_) + "0P")
     assert packer.size == ctypes.sizeof(desc)
-    return packer.pack
+
+    def pack(*fields) -> bytes:
+        try:
+            return packer.pack(*fields)
+        except (struct.error, OverflowError) as e:
+            raise ValueError(f"{desc.__name__}: {e}") from None
+
+    return pack
 
 
 pack_rms_norm = _packer(RmsNormDesc)

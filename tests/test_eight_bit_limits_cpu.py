@@ -2,6 +2,7 @@
 
 from __future__ import annotations
 
+import ctypes
 import itertools
 
 import pytest
@@ -87,3 +88,12 @@ def test_weights_of_every_type():
     got = ops.scale_weight(codes)
     assert got.scale.item() == 1.0 and torch.equal(got.values.float(), codes.float())
     assert (ops.scale_weight(torch.zeros((2, 300), dtype=torch.float16)).scale == 2.0 ** -100).all()
+
+
+@pytest.mark.parametrize(("field", "value"), [("tokens", 2 ** 31), ("channels", 2 ** 40), ("eps", 1e39), ("eps", "1"),
+                                              ("x_token_stride", 2 ** 63), ("heads", 1.5)])
+def test_numbers_that_a_descriptor_does_not_hold_are_refused(field, value):
+    fields = [0.5 if t is ctypes.c_float else 3 for _, t in _lib.RmsNormDesc._fields_]
+    fields[[n for n, _ in _lib.RmsNormDesc._fields_].index(field)] = value
+    with pytest.raises(ValueError, match="RmsNormDesc"):
+        _lib.pack_rms_norm(*fields)
