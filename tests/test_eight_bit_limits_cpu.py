@@ -90,10 +90,18 @@ def test_weights_of_every_type():
     assert (ops.scale_weight(torch.zeros((2, 300), dtype=torch.float16)).scale == 2.0 ** -100).all()
 
 
-@pytest.mark.parametrize(("field", "value"), [("tokens", 2 ** 31), ("channels", 2 ** 40), ("eps", 1e39), ("eps", "1"),
+@pytest.mark.parametrize(("field", "value"), [("tokens", 2 ** 31), ("channels", 2 ** 40), ("eps", "1"),
                                               ("x_token_stride", 2 ** 63), ("heads", 1.5)])
 def test_numbers_that_a_descriptor_does_not_hold_are_refused(field, value):
     fields = [0.5 if t is ctypes.c_float else 3 for _, t in _lib.RmsNormDesc._fields_]
     fields[[n for n, _ in _lib.RmsNormDesc._fields_].index(field)] = value
     with pytest.raises(ValueError, match="RmsNormDesc"):
         _lib.pack_rms_norm(*fields)
+
+
+def test_an_eps_past_fp32_is_refused():
+    """It is packed as an infinity, which the entry refuses."""
+    fields = [getattr(_norm()._obj, n) or 0 for n, _ in _lib.RmsNormDesc._fields_]
+    names = [n for n, _ in _lib.RmsNormDesc._fields_]
+    fields[names.index("eps")] = 1e39
+    assert LIB.ctmr_rms_norm(_lib.pack_rms_norm(*fields), None) == INVALID and b"eps" in LIB.ctmr_last_error()
