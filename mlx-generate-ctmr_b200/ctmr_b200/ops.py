@@ -829,10 +829,15 @@ def scale_weight(weight: torch.Tensor) -> ScaledWeight:
     return ScaledWeight(values[:, :room].to(E4M3).contiguous()[:, :inner], scale)
 
 
-# Uninitialised memory of a shape, strides and type on the current device, from torch's caching allocator: the entry
-# that compiled programs use, at a fifth of ``new_empty``'s 3 us.
-_empty = getattr(torch._C._dynamo.guards, "_empty_strided_cuda", None) or (
-    lambda size, stride, dtype: torch.empty_strided(size, stride, dtype=dtype, device="cuda"))
+def _allocator(root=torch._C):
+    """Uninitialised memory of a shape, strides and type on the current device, from torch's caching allocator: by the
+    entry that compiled programs use where this torch has it, at a fifth of ``new_empty``'s 3 us."""
+    for name in ("_dynamo", "guards", "_empty_strided_cuda"):
+        root = getattr(root, name, None)
+    return root or (lambda size, stride, dtype: torch.empty_strided(size, stride, dtype=dtype, device="cuda"))
+
+
+_empty = _allocator()
 
 
 def _empty_rows8(rows: int, channels: int) -> ScaledRows:

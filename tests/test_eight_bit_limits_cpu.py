@@ -4,6 +4,7 @@ from __future__ import annotations
 
 import ctypes
 import itertools
+from types import SimpleNamespace
 
 import pytest
 import torch
@@ -105,3 +106,12 @@ def test_an_eps_past_fp32_is_refused():
     names = [n for n, _ in _lib.RmsNormDesc._fields_]
     fields[names.index("eps")] = 1e39
     assert LIB.ctmr_rms_norm(_lib.pack_rms_norm(*fields), None) == INVALID and b"eps" in LIB.ctmr_last_error()
+
+
+@pytest.mark.parametrize("root", [SimpleNamespace(), SimpleNamespace(_dynamo=None),
+                                  SimpleNamespace(_dynamo=SimpleNamespace(guards=SimpleNamespace()))])
+def test_outputs_are_allocated_where_torch_lacks_its_direct_entry(root, monkeypatch):
+    got = {}
+    monkeypatch.setattr(torch, "empty_strided", lambda size, stride, **kw: got.update(size=size, stride=stride, **kw))
+    ops._allocator(root)((2, 3), (4, 1), torch.float32)
+    assert got == dict(size=(2, 3), stride=(4, 1), dtype=torch.float32, device="cuda")
