@@ -53,3 +53,14 @@ def test_accumulators_are_waited_for_by_whole_warps(path):
     """The barriers that announce an accumulator are waited for by the warps that then read it."""
     text = re.sub(r"//[^\n]*", "", path.read_text())
     assert not re.findall(r"mbar_wait_bounded\(\s*&?(?:tmem_full|o_full|s_full|acc_full|chunk_full)\b", text)
+
+
+def test_warps_meet_before_sums_are_read_out():
+    """The same for loads that are started and waited for apart (``tmem_ld16_start``)."""
+    text = re.sub(r"//[^\n]*", "", (CSRC / "scaled_linear.cu").read_text())
+    loads = [m.start() for m in re.finditer(r"tmem_ld16_start\(", text)]
+    assert len(loads) >= 3
+    for at in loads:
+        assert re.findall(r"mbar_wait_\w+", text[:at])[-1] == "mbar_wait_warp"
+        # What a load gives is read after a wait for it, tied to that place.
+        assert re.search(r"tmem_ld_wait\(\);\s*tmem_ld_fence16\(", text[at:])
