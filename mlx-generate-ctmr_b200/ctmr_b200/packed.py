@@ -157,7 +157,7 @@ def packed_transformer_tokens(tokens: torch.Tensor, grid: PackedGrid, blocks: Se
     A block holds ``norm1`` and ``norm2`` (``(C,)``), and ``ops.ScaledWeight``s ``qkv`` (C -> 3C), ``out_proj``
     (C -> C), ``gate_up`` (C -> 2F: what is gated by silu, then what it multiplies) and ``down`` (F -> C). Each norm
     adds the branch before it to the residual stream and gives 8-bit rows in the same pass."""
-    if tokens.dim() != 2 or tokens.shape[0] != grid.starts[-1] or tokens.shape[1] % heads:
+    if tokens.dim() != 2 or tokens.shape[0] != grid.starts[-1] or heads < 1 or tokens.shape[1] % heads:
         raise ValueError(f"tokens {tuple(tokens.shape)} where the grid has {grid.starts[-1]} rows, in {heads} heads")
     dt, scale = tokens.dtype, (tokens.shape[1] // heads) ** -0.5
     stream, branch = tokens, None

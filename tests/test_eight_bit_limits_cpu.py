@@ -10,7 +10,7 @@ import pytest
 import torch
 from test_eight_bit_cpu import INVALID, LIB, OK, _norm, _quantize
 
-from ctmr_b200 import _lib, ops
+from ctmr_b200 import _lib, ops, packed
 
 # A descriptor with rows that reaches every check, refused at its last one if at no other.
 REFUSED_LAST = dict(sum=0x4000, y=0x4000)
@@ -115,3 +115,9 @@ def test_outputs_are_allocated_where_torch_lacks_its_direct_entry(root, monkeypa
     monkeypatch.setattr(torch, "empty_strided", lambda size, stride, **kw: got.update(size=size, stride=stride, **kw))
     ops._allocator(root)((2, 3), (4, 1), torch.float32)
     assert got == dict(size=(2, 3), stride=(4, 1), dtype=torch.float32, device="cuda")
+
+
+@pytest.mark.parametrize("heads", [0, -2, 3])
+def test_blocks_of_no_heads_are_refused(heads):
+    with pytest.raises(ValueError, match="heads"):
+        packed.packed_transformer_tokens(torch.zeros((8, 64)), SimpleNamespace(starts=[0, 8]), [], heads=heads)
