@@ -443,7 +443,7 @@ CTMR_API int ctmr_quantize_rows(const ctmr_quantize_rows_desc* desc, void* strea
 
 /* The product of 8-bit rows with an 8-bit weight, fp32 sums:
  *   y_mn = sum_b x_scale[m][b] weight_scale[n / 128][b] (sum of x_mk weight_nk over block b of 128 inputs) + bias_n,
- * scales of any value; the product of a row's and a weight's scale must be in fp32's range. What is NaN or
+ * scales of any value; the product of a row's and a weight's scale must be in fp32's normal range. What is NaN or
  * not finite in a row, or in an output's weights, stays in that row, or output. Values and weights are e4m3,
  * 16-byte aligned, rows a multiple of 16 bytes apart; inputs, outputs and rows of any number. */
 typedef struct ctmr_scaled_linear_desc {

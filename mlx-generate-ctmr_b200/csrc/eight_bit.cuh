@@ -57,7 +57,9 @@ int launch_scaled_linear(const ScaledLinearParams& p, int y_dtype, cudaStream_t 
 
 // ---------------------------------------------------------------- a group of a row
 // Eight lanes hold a group of 128 channels, 16 each: eight consecutive ones of either half where the row's address, stride
-// and length allow 16-byte accesses (WIDE), every eighth one otherwise: a warp's accesses lie side by side either way.
+// and length allow 16-byte accesses (WIDE), every eighth one otherwise: the eight lanes' accesses lie side by side then, but
+// are 8 elements, half a sector of 16-bit ones, and a warp's four groups lie apart (rows of 4,097 take two to three times
+// those of 4,096).
 constexpr int kEach = 16, kGroupLanes = kScaleGroup / kEach;
 
 template <bool WIDE>

@@ -5,7 +5,8 @@
 // some 25 instructions a channel: silu is one exponential and one reciprocal, with the exponent's product taken
 // in two parts so that the error stays near 2^-22 for any size of a. Groups of 128 channels, eight lanes each, follow one
 // another over the rows without regard to where a row ends, so that no size leaves threads idle. 8,192 gated rows of
-// 11,264: 87 to 90 us, 5.2 TB/s (3 less without the 64-bit decisions); what is left are instructions, 24 a channel.
+// 11,264: 88 us, 5.3 TB/s, where one output is written over and over (part of its 92 MB then stays in L2), 94 to 96 with
+// outputs of their own; what is left are instructions, 24 a channel.
 #include "capi_internal.cuh"
 #include "ctmr_b200.h"
 #include "eight_bit.cuh"
@@ -16,8 +17,8 @@ namespace {
 
 constexpr int kThreads = 256, kBlocks = 3, kGroups = kThreads / kGroupLanes;
 
-// Below this silu(a) nears the end of 32 bits' normal numbers, from where a large b can bring it back: groups that hold both
-// at once are computed in 64 bits. (Up to 128, b leaves less than 2^-110, half the least step of the least scale.)
+// Below this silu(a) nears the end of 32 bits' normal numbers, from where a large b can bring it back: groups that hold
+// both at once are computed in 64 bits. (Up to 128, b leaves less than 2^-110, half the least step of the least scale.)
 constexpr float kFarGate = -86.f, kFarOther = 128.f;
 
 // silu(a) b, two at a time, for a from kFarGate on. The reciprocal meets b first: a may be subnormal, and then b large.

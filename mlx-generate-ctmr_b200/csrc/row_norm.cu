@@ -3,8 +3,9 @@
 // h rounded to x's type beside it, where it is kept (the residual stream of a block).
 //
 // One pass over memory: a row's values stay in registers between the sum and the scaling. What bounds it is memory, 7
-// bytes a channel for 16-bit rows with a residual and an 8-bit output: 8,192 rows of 4,096 take 49 us, 4.8 TB/s
-// (without the 64-bit decisions 46, without the weight 38, which is the memory's own rate). The squares are added in 64
+// bytes a channel for 16-bit rows with a residual and an 8-bit output: 8,192 rows of 4,096 take 50 us, 4.7 TB/s
+// (without a weight 49, with a 16-bit output, which is 32 MB more to write, 46). Between that and the memory's 36 stand
+// latencies: a quarter of an SM's warps, which issue 0.53 instructions a clock and scheduler. The squares are added in 64
 // bits: at 3 channels a clock and SM the conversions take a fifth of their unit's time, and the 8-bit rounding gets a
 // mean that its 64-bit recomputation can rely on. The norm is taken of the unrounded sum h, so that it does not see
 // the stream's rounding.
@@ -226,7 +227,10 @@ cudaError_t launch_rows(const RowNormParams& p, cudaStream_t stream) {
   // and 3.6; 20,000 rows keep all warps busy either way). Longer rows: blocks that go on from row to row, of up
   // to 128 registers, where these fill their SMs and accesses are wide (8,192 rows of 4,096: 49 us, a block of 64
   // registers to each row 57; of 4,224, whose 288 threads fit once: 90 and 68; of 4,097: 190 and 146), or where there
-  // are few rows and a row's own time counts (1,777 rows of 1,001: 7.4 and 10.5; 600 of 2,048: 4.0 and 4.4).
+  // are few rows and a row's own time counts (1,777 rows of 1,001: 7.4 and 10.5; 600 of 2,048: 4.0 and 4.4). The blocks
+  // of 64 registers, to which that leaves many rows of 4,097 to 7,040 channels, and all rows above 8,192, are far from
+  // the memory's rate and spill: 8,192 rows of 5,120 take 72 us (bytes: 45), of 6,144 100
+  // (54), 2,000 of 16,384 97 (35).
   auto grid = [&](int lanes) { return (rows * lanes + 255) / 256; };
   if (groups == 1) return launch<T, 1, 8, false, EIGHT>(p, wide, grid(8), 256, stream);
   if (groups == 2) return launch<T, 1, 16, false, EIGHT>(p, wide, grid(16), 256, stream);

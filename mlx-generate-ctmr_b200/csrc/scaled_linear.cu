@@ -12,9 +12,10 @@
 // partial sums meet through distributed shared memory, in the order of the ranks.
 //
 // 8,191 rows of 4,096 -> 12,288: 394 us in short runs (2,090 TFLOP/s), 427 to 436 back to back, where the power cap
-// holds the clock near 1.48 GHz. A block takes a pair some 930 clocks, its products 512: the way from the products' end
-// to the sums' warps, through their loads and back is longer than the other buffer's products, and two buffers fill TMEM.
-// (Halves of 128 outputs with four buffers, one CTA to a tile of 128 x 256, and sixteen warps for the sums were slower.)
+// holds the clock near 1.48 GHz. A block takes a pair some 930 clocks, its products 512. The way from the products' end
+// to the sums' warps (250), through their loads (320) and back (300) is longer than the other buffer's products, and two
+// buffers fill TMEM; but by these figures two blocks would take 512 + 870 clocks, 691 each: the other 240 are not
+// accounted for. (Halves of 128 outputs with four buffers, one CTA to a tile of 128 x 256, and sixteen warps for the sums were slower.)
 // 32 rows of 4,096 -> 4,096: 8.1 us, one of 11,264 -> 4,096 11.7 (3.9 TB/s of weight): a launch, the first loads and the
 // exchange take 4 to 5 us of both.
 #include "capi_internal.cuh"
@@ -343,8 +344,10 @@ __global__ void __launch_bounds__(kFewThreads, FewSmem<BN>::kCtas)
   }
 }
 
-// By a warp: 32 rows (a lane's sums are one) of COLUMNS outputs, 64 bytes of each row at a time by way of shared memory,
-// so that lanes write side by side; for rows of y that TMA does not take (not 16-byte aligned).
+// By a warp: 32 rows (a lane's sums are one) of COLUMNS outputs, 64 bytes of each row at a time by way of shared memory;
+// for rows of y that TMA does not take (not 16-byte aligned). A lane then holds 16 bytes of a row and stores them element
+// by element, 16 bytes from its neighbour's: slow where the outputs are many and the products few (8,191 x 4,096 ->
+// 12,287: 747 us, 12,288: 378 to 423; 16,000 x 64 -> 12,289: 890, 12,288: 72; 8,968 x 512 -> 1,537: 117, 1,536: 35).
 template <typename T, int COLUMNS>
 __device__ __forceinline__ void write_rows(const ScaledLinearParams& p, uint8_t* store, const float* sum, int row0, int o0,
                                            int lane) {
@@ -613,7 +616,8 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         ok = ok && mbar_wait_warp(&acc_full[a], static_cast<uint32_t>(it >> 1) & 1u, kErrWaitAcc);
         if (!ok) break;
         tc_fence_after();
-        // The next 16 on their way while these are added.
+        // 16 sums at a time, waited for and then added: a second array, for loads ahead, would be 16 registers more, which
+        // the sums do not leave.
         float v[16];
 #pragma unroll
         for (int c = 0; c < kColumns; c += 16) {
@@ -670,7 +674,9 @@ int encode(CUtensorMap* map, CUtensorMapDataType type, const void* base, long lo
 }
 
 // Which form, tile and split: the least of these estimates (microseconds), fitted to runs of 1 to 1,000 rows with 512
-// to 11,264 inputs and 512 to 4,096 outputs, which they meet within some 15 %. One CTA to a tile: 2.2 + 0.052 tile for
+// to 11,264 inputs and 512 to 4,096 outputs, which they meet within some 15 %. The output's bytes are not in them, nor
+// whether TMA writes its rows: wide outputs of few inputs take longer (16,000 x 64 -> 12,288: 51 estimated, 72 measured;
+// 8,968 x 512 -> 1,536: 13 and 34). One CTA to a tile: 2.2 + 0.052 tile for
 // the start, the first loads and the stores, 0.185 + 0.001 tile a block of 128 inputs. Split over a cluster, the partial
 // sums' way takes longer the more columns there are. CTA pairs: 4.5, and 0.53 a block and 0.6 a tile, whose stores fall
 // between the next one's products. (1 row of 4,096 -> 4,096: tiles of 16 rows split four ways 6.5, two ways 7.5, not

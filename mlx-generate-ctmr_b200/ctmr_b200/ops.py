@@ -952,7 +952,7 @@ def scaled_linear(x: ScaledRows, weight: ScaledWeight, bias: torch.Tensor | None
     ``out_dtype`` (bf16, fp16 or fp32).
 
     ``x`` comes from ``quantize_rows`` or ``rms_norm``, ``weight`` from ``scale_weight`` or a checkpoint; both scales
-    may be any numbers, in any strides. Any number of rows, inputs and outputs. ``bias`` is fp32 or of the output's type.
+    may be any numbers whose products fp32 holds as normal ones, in any strides. Any number of rows, inputs and outputs. ``bias`` is fp32 or of the output's type.
     What is not finite in a row, or in an output's weights, stays in that row, or output.
     """
     values, x_scale = x
