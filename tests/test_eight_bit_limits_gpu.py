@@ -48,6 +48,23 @@ def test_gates_of_very_negative_values(dtype):
     _no_device_error()
 
 
+@pytest.mark.parametrize("low", [-88.0, -20.0])
+def test_gates_beside_ties_over_the_whole_range(low):
+    """silu(a) b as near to ties between e4m3 values as b's 32 bits allow, for a of every size: the interval that sends a
+    value to 64 bits has to hold what 32 bits get wrong anywhere."""
+    from ctmr_b200 import ops
+
+    gen = _gen(34)
+    for _ in range(4):
+        a = low + (30.0 - low) * torch.rand((4000, 256), generator=gen, device="cuda")
+        a = torch.where(a.abs() < 1e-3, 1.0, a)
+        target = (torch.randint(8, 16, a.shape, generator=gen, device="cuda") * 2 + 1).double() / 16
+        b = (target * (1.0 + torch.exp(-a.double())) / a.double()).float()
+        x = torch.cat([a, b], dim=1)
+        _check_rows(ops.quantize_rows(x, gate=True), _gate_ref(x))
+    _no_device_error()
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_gates_below_the_normal_numbers(dtype):
     """Subnormal a or b, times a large other half."""
